@@ -179,6 +179,11 @@ _SIGNATURES = {
     "aiosb_linear_stat_norm": (
         [_p, _p, _i64, _i64, _p, _f32, _i64, _i64, _p, _i64, _p, _i64, _i32, _p, _i64, _p, _p], _i32
     ),
+    "aiosb_quantize_fp8": ([_p, _i64, _i64, _i64, _p, _p, _p], _i32),
+    "aiosb_quantize_weight_fp8": ([_p, _i64, _i64, _i64, _p, _p, _p], _i32),
+    "aiosb_rmsnorm_fp8": ([_p, _i64, _i64, _i64, _p, _p, _p, _f32, _p, _p, _p], _i32),
+    "aiosb_silu_mul_fp8": ([_p, _i64, _i64, _i64, _p, _p, _p], _i32),
+    "aiosb_linear_fp8": ([_p, _i64, _p, _i64, _i64, _p, _p, _i64, _p, _i64, _i32, _p, _i64, _p, _p], _i32),
     "aiosb_attention_decode": (
         [_p, _i64, _p, _i64, _p, _p, _f32, _p, _p, _i64, _p, _p, _p, _p, _i64, _p, _i64, _p, _p, _p, _p, _i32,
          _i64, _i64, _i64, _i64, _i64, _f32, _p, _i64, _p, _p],

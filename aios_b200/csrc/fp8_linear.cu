@@ -1,0 +1,432 @@
+// Linear with 8-bit operands: y[t, c] = [residual +] sum_b sx[t, b] sw[c / 128, b]
+// sum_{k in block b} xq[t, k] wq[c, k] on e4m3 values with one fp32 scale for each
+// 128 columns of an x row and for each 128 x 128 block of the weight.
+//
+// The tensor cores (tcgen05 kind::f8f6f4) form the sum over one 128-wide block of k
+// at a time; its two scales belong to no operand, so each block's product is read
+// from tensor memory and folded into fp32 registers as acc += (sx * sw) * d. x is the
+// M operand: a TMEM lane is a token, its scale one register of the thread that reads
+// the lane, and the weight's scale is uniform over the columns of a warp, so the fold
+// costs one FMA per value. Two TMEM accumulators alternate: the tensor cores work on
+// block b + 1 while the warps fold block b.
+//
+// Per CTA: warps 0-7 fold (warp w: lanes 32 (w % 4).., column half w / 4), lane 0 of
+// warp 8 loads tiles by TMA into a ring of stages, lane 0 of warp 9 issues the MMAs.
+// Few rows leave few tiles: then a cluster of up to 8 CTAs splits the blocks of k and
+// the partial tiles are summed in rank order through distributed shared memory, so
+// results do not depend on scheduling.
+#include <string.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "abi_util.h"
+#include "fp8.cuh"
+
+namespace aiosb {
+namespace {
+
+constexpr int kBM = 128;                      // tokens per tile (UMMA M, TMEM lanes)
+constexpr int kBK = kFp8Block;                // bytes of k per stage: one scale block, one swizzle row
+constexpr int kFoldWarps = 8;
+constexpr int kThreads = (kFoldWarps + 2) * 32;
+constexpr int kMaxStages = 16;
+constexpr int kMaxSplit = 8;
+
+struct Fp8LinearArgs {
+  const float* x_scale;  // [rows, kblocks]
+  const float* w_scale;  // [ceil(n / 128), kblocks]
+  __nv_bfloat16* y;
+  const __nv_bfloat16* residual;  // or NULL
+  int64_t y_stride, residual_stride;
+  int rows, n, kblocks;
+  int m_tiles, n_tiles;
+  int split;
+  int stages;
+  int a_rows;  // token rows a stage holds: rows, rounded up to the swizzle's 8, at most 128
+  int32_t* status;
+};
+
+__device__ __forceinline__ void tc_mma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Instruction descriptor: fp32 accumulator, e4m3 A and B (format 0), both K-major.
+__host__ __device__ constexpr uint32_t umma_idesc_e4m3(int M, int N) {
+  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// 32 lanes x 32 consecutive columns; the values are there after tmem_wait32.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// Waits for this thread's tensor-memory loads; naming the registers keeps their
+// uses behind the wait.
+__device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                 "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                 "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                 "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+
+// Eight finished sums of one row to bf16, the residual added in fp32 (one rounding).
+__device__ __forceinline__ void store8(const Fp8LinearArgs& a, int64_t row, int col, const float (&v)[8]) {
+  float o[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j] = v[j];
+  if (a.residual != nullptr) {
+    float r[8];
+    unpack8(*reinterpret_cast<const uint4*>(a.residual + row * a.residual_stride + col), r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] += r[j];
+  }
+  *reinterpret_cast<uint4*>(a.y + row * a.y_stride + col) =
+      make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
+}
+
+template <int BN>
+__global__ void __launch_bounds__(kThreads, BN == 64 ? 2 : 1)
+    linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                      const Fp8LinearArgs a) {
+  constexpr uint32_t kBBytes = BN * kBK;
+  constexpr int kHalf = BN / 2;        // columns of one fold warp
+  constexpr int kRedStride = BN + 4;   // floats per row of the partial tile: conflict-free 16-byte accesses
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t a_bytes = (uint32_t)a.a_rows * kBK;
+  uint8_t* const smem_a = smem;
+  uint8_t* const smem_b = smem + (uint32_t)a.stages * a_bytes;
+  // fold warps whose lanes hold tokens (a tile of fewer than 128 rows is the only m tile)
+  const int lane_groups = (a.a_rows + 31) / 32;
+  const bool folds = warp < kFoldWarps && (warp & 3) < lane_groups;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&acc_full[s], 1);
+      mbar_init(&acc_empty[s], (uint32_t)lane_groups * 2);
+    }
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == kFoldWarps + 1) {
+    tmem_alloc(&tmem_slot, 2 * BN);
+    tmem_relinquish();
+  }
+  if (threadIdx.x == kFoldWarps * 32) {
+    tma_prefetch_desc(&tm_x);
+    tma_prefetch_desc(&tm_w);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();  // after the wait: whoever follows may rely on this kernel's predecessors being done
+
+  const int split = a.split;
+  const int rank = blockIdx.x % split;
+  const int kb0 = (int)((int64_t)a.kblocks * rank / split), kb1 = (int)((int64_t)a.kblocks * (rank + 1) / split);
+  const int tiles = a.m_tiles * a.n_tiles;
+  const int step = gridDim.x / split;
+
+  if (threadIdx.x == kFoldWarps * 32) {
+    // ---- TMA producer
+    uint32_t it = 0;
+    for (int tile = blockIdx.x / split; tile < tiles; tile += step) {
+      const int m0 = tile % a.m_tiles * kBM, n0 = tile / a.m_tiles * BN;
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const int s = it % a.stages;
+        if (!mbar_wait(&empty[s], ((it / a.stages) & 1) ^ 1)) {
+          report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
+          abort_flag = 1;
+        }
+        if (abort_flag) break;
+        mbar_arrive_expect_tx(&full[s], a_bytes + kBBytes);
+        tma_load_2d(smem_b + s * kBBytes, &tm_w, &full[s], kb * kBK, n0);
+        tma_load_2d(smem_a + s * a_bytes, &tm_x, &full[s], kb * kBK, m0);
+      }
+      if (abort_flag) break;
+    }
+    if (abort_flag) {  // let the copies that are still in flight land before this CTA returns
+      for (uint32_t i = it > (uint32_t)a.stages ? it - a.stages : 0; i < it; ++i)
+        mbar_wait(&full[i % a.stages], (i / a.stages) & 1);
+    }
+  } else if (threadIdx.x == (kFoldWarps + 1) * 32) {
+    // ---- MMA issuer. With fewer than 128 rows staged the A operand's unused rows are
+    // whatever follows the slot in shared memory (inside the allocation): a row of A
+    // reaches its own TMEM lane only, and those lanes are not read.
+    constexpr uint32_t idesc = umma_idesc_e4m3(kBM, BN);
+    uint32_t it = 0;
+    for (int tile = blockIdx.x / split; tile < tiles; tile += step) {
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const int s = it % a.stages, t = it & 1;
+        if (!mbar_wait(&acc_empty[t], ((it >> 1) & 1) ^ 1) || !mbar_wait(&full[s], (it / a.stages) & 1)) {
+          report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
+          abort_flag = 1;
+        }
+        if (abort_flag) break;
+        tc_fence_after();
+        const uint32_t pa = smem_u32(smem_a + s * a_bytes), pb = smem_u32(smem_b + s * kBBytes);
+#pragma unroll
+        for (int kk = 0; kk < kBK / 32; ++kk)
+          tc_mma_e4m3(tmem + t * BN, umma_desc_sw128(pa + kk * 32), umma_desc_sw128(pb + kk * 32), idesc, kk != 0);
+        tc_commit(&empty[s]);
+        tc_commit(&acc_full[t]);
+      }
+      if (abort_flag) break;
+    }
+  } else if (folds) {
+    // ---- fold: acc += (sx * sw) * d per block of k
+    const int half = warp >> 2;
+    const int tile_row = (warp & 3) * 32 + lane;
+    const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(half * kHalf);
+    uint32_t it = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x / split; tile < tiles && ok; tile += step) {
+      const int64_t row = (int64_t)(tile % a.m_tiles) * kBM + tile_row;
+      const int c0 = tile / a.m_tiles * BN + half * kHalf;
+      const float* sx = a.x_scale + min(row, (int64_t)a.rows - 1) * a.kblocks;
+      const float* sw = a.w_scale + (int64_t)(min(c0, a.n - 1) / kFp8Block) * a.kblocks;
+      float acc[kHalf];
+#pragma unroll
+      for (int j = 0; j < kHalf; ++j) acc[j] = 0.f;
+      float next = sx[kb0] * sw[kb0];
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const int t = it & 1;
+        const float s = next;
+        const int kn = min(kb + 1, kb1 - 1);
+        next = sx[kn] * sw[kn];
+        ok = mbar_wait(&acc_full[t], (it >> 1) & 1);
+        __syncwarp();
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {
+          report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
+          abort_flag = 1;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < kHalf; c += 32) {
+          uint32_t d[32];
+          tmem_ld32(t_lane + t * BN + c, d);
+          tmem_wait32(d);
+          if (c + 32 == kHalf) {  // this block's values are in registers: the accumulator may be reused
+            tc_fence_before();
+            if (lane == 0) mbar_arrive(&acc_empty[t]);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[c + j] = fmaf(s, __uint_as_float(d[j]), acc[c + j]);
+        }
+      }
+      if (!ok) break;
+      if (split == 1) {
+        if (row < a.rows) {
+#pragma unroll
+          for (int j = 0; j < kHalf; j += 8) {
+            const float v[8] = {acc[j],     acc[j + 1], acc[j + 2], acc[j + 3],
+                                acc[j + 4], acc[j + 5], acc[j + 6], acc[j + 7]};
+            if (c0 + j < a.n) store8(a, row, c0 + j, v);
+          }
+        }
+      } else if (tile_row < a.a_rows) {
+        // every MMA of this CTA has read its operands: the partial tile takes their place
+        float* red = reinterpret_cast<float*>(smem) + tile_row * kRedStride + half * kHalf;
+#pragma unroll
+        for (int j = 0; j < kHalf; j += 4)
+          *reinterpret_cast<float4*>(red + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+      }
+    }
+  }
+
+  __syncwarp();
+  __syncthreads();
+  if (split > 1) {
+    cluster_sync();
+    // Rank r sums and stores every split-th group of 8 columns, in rank order.
+    if (!abort_flag) {
+      const int tile = blockIdx.x / split;
+      const int m0 = tile % a.m_tiles * kBM, n0 = tile / a.m_tiles * BN;
+      const uint32_t base = smem_u32(smem);
+      const int live = min(a.rows - m0, kBM);
+      for (int u = threadIdx.x * split + rank; u < live * (BN / 8); u += kThreads * split) {
+        const int r = u / (BN / 8), c = u % (BN / 8) * 8;
+        if (n0 + c >= a.n) continue;
+        const uint32_t off = base + (uint32_t)(r * kRedStride + c) * 4;
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int p = 0; p < split; ++p) {
+          const uint32_t at = map_shared_rank(off, (uint32_t)p);
+          const float4 lo = ld_dsmem_f4(at), hi = ld_dsmem_f4(at + 16);
+          v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w;
+          v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
+        }
+        store8(a, m0 + r, n0 + c, v);
+      }
+    }
+    cluster_sync();  // peers may still read this CTA's partial tile
+  }
+  if (warp == kFoldWarps + 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 2 * BN);
+  }
+}
+
+// ---- host side -------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  });
+  return fn;
+}
+
+// Tensor map of a row-major byte matrix [rows, cols] in boxes of box_rows x 128;
+// reads past an edge give zeros.
+int make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t row_stride, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return set_error(AIOSB_ERR_LAUNCH, "cuTensorMapEncodeTiled unavailable");
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)row_stride};
+  const cuuint32_t box[2] = {(cuuint32_t)kBK, box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(AIOSB_ERR_LAUNCH, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return AIOSB_OK;
+}
+
+template <int BN>
+int launch(const CUtensorMap& tx, const CUtensorMap& tw, Fp8LinearArgs a, cudaStream_t stream) {
+  constexpr int kOne = 224 * 1024;                         // shared memory of a CTA that has the SM to itself
+  constexpr int kBudget = BN == 64 ? kOne / 2 - 1024 : kOne;  // two CTAs per SM at BN = 64
+  auto kern = linear_fp8_kernel<BN>;
+  static bool configured[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBudget);
+    if (e != cudaSuccess) return set_error(AIOSB_ERR_LAUNCH, "linear_fp8: %s", cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  const int stage_bytes = a.a_rows * kBK + BN * kBK;
+  const int tiles = a.m_tiles * a.n_tiles;
+  const int per_cta = (a.kblocks + a.split - 1) / a.split * (a.split > 1 ? 1 : (tiles + sm_count() - 1) / sm_count());
+  a.stages = std::max(2, std::min({(kBudget - 1024) / stage_bytes, kMaxStages, per_cta}));
+  // at least the partial tile, and 16 KB past the last A slot (two B slots have that)
+  const int body = std::max(a.stages * stage_bytes, a.split > 1 ? a.a_rows * (BN + 4) * 4 : 0);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.split > 1 ? tiles * a.split : std::min(tiles, sm_count() * (BN == 64 ? 2 : 1))));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = (size_t)body + 1024;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)a.split;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tx, tw, a);
+  if (e != cudaSuccess) return set_error(AIOSB_ERR_LAUNCH, "linear_fp8: %s", cudaGetErrorString(e));
+  return AIOSB_OK;
+}
+
+}  // namespace
+}  // namespace aiosb
+
+using namespace aiosb;
+
+extern "C" int aiosb_linear_fp8(const void* x, int64_t x_row_stride, const float* x_scale, int64_t rows, int64_t k,
+                                const void* w, const float* w_scale, int64_t n, void* y, int64_t y_row_stride,
+                                int epilogue, const void* residual, int64_t residual_stride, int32_t* status,
+                                void* stream) {
+  AIOSB_REQUIRE(rows >= 0 && k > 0 && n > 0, AIOSB_ERR_INVALID_ARG, "linear_fp8: bad sizes");
+  AIOSB_REQUIRE(n % 8 == 0, AIOSB_ERR_UNSUPPORTED, "linear_fp8: n=%lld must be a multiple of 8", (long long)n);
+  AIOSB_REQUIRE(k % 16 == 0, AIOSB_ERR_UNSUPPORTED, "linear_fp8: k=%lld must be a multiple of 16", (long long)k);
+  constexpr int64_t kMost = (int64_t)1 << 30;
+  AIOSB_REQUIRE(rows <= kMost && n <= kMost && k <= kMost && (rows / kBM + 1) * (n / 64 + 1) < kMost,
+                AIOSB_ERR_UNSUPPORTED, "linear_fp8: too large");
+  AIOSB_REQUIRE(epilogue == AIOSB_EPI_STORE || epilogue == AIOSB_EPI_ADD, AIOSB_ERR_INVALID_ARG,
+                "linear_fp8: unknown epilogue %d (store or add)", epilogue);
+  AIOSB_REQUIRE(epilogue != AIOSB_EPI_ADD ||
+                    (residual != nullptr && aligned16(residual) && residual_stride >= n && residual_stride % 8 == 0),
+                AIOSB_ERR_INVALID_ARG, "linear_fp8: the add epilogue needs an aligned residual [rows, >= n]");
+  AIOSB_REQUIRE(x_row_stride >= k && x_row_stride % 16 == 0, AIOSB_ERR_INVALID_ARG,
+                "linear_fp8: x row stride must cover the row and be a multiple of 16");
+  AIOSB_REQUIRE(y_row_stride >= n && y_row_stride % 8 == 0, AIOSB_ERR_INVALID_ARG,
+                "linear_fp8: y row stride must cover the output and be a multiple of 8");
+  if (rows == 0) return AIOSB_OK;
+  AIOSB_REQUIRE(x && x_scale && w && w_scale && y, AIOSB_ERR_INVALID_ARG, "linear_fp8: null pointer");
+  AIOSB_REQUIRE(aligned16(x) && aligned16(w) && aligned16(y) && (reinterpret_cast<uintptr_t>(x_scale) & 3u) == 0 &&
+                    (reinterpret_cast<uintptr_t>(w_scale) & 3u) == 0,
+                AIOSB_ERR_MISALIGNED, "linear_fp8: x, w and y must be 16-byte aligned");
+  Fp8LinearArgs a;
+  memset(&a, 0, sizeof(a));
+  a.x_scale = x_scale;
+  a.w_scale = w_scale;
+  a.y = (__nv_bfloat16*)y;
+  a.y_stride = y_row_stride;
+  a.residual = epilogue == AIOSB_EPI_ADD ? (const __nv_bfloat16*)residual : nullptr;
+  a.residual_stride = residual_stride;
+  a.rows = (int)rows;
+  a.n = (int)n;
+  a.kblocks = (int)((k + kBK - 1) / kBK);
+  a.m_tiles = (int)((rows + kBM - 1) / kBM);
+  a.a_rows = (int)std::min<int64_t>(kBM, (rows + 7) / 8 * 8);
+  a.split = 1;
+  a.status = status;
+  // The widest tile that still gives every SM one: a wide tile reads x and the weight
+  // from L2 fewer times. Where none does, the narrowest, and k split until the grid
+  // covers the SMs.
+  const int sms = sm_count();
+  int bn = 64;
+  for (int b : {256, 128}) {
+    if ((int64_t)a.m_tiles * ((n + b - 1) / b) >= sms) {
+      bn = b;
+      break;
+    }
+  }
+  a.n_tiles = (int)((n + bn - 1) / bn);
+  while (a.split < kMaxSplit && a.split * 2 <= a.kblocks && (int64_t)a.m_tiles * a.n_tiles * a.split < sms)
+    a.split *= 2;
+  CUtensorMap tx, tw;
+  int rc = make_map(&tx, x, rows, k, x_row_stride, (uint32_t)a.a_rows);
+  if (rc == AIOSB_OK) rc = make_map(&tw, w, n, k, k, (uint32_t)bn);
+  if (rc != AIOSB_OK) return rc;
+  cudaStream_t s = as_stream(stream);
+  return bn == 256 ? launch<256>(tx, tw, a, s) : bn == 128 ? launch<128>(tx, tw, a, s) : launch<64>(tx, tw, a, s);
+}

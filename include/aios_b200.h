@@ -258,6 +258,54 @@ AIOSB_API int aiosb_linear_attnres_rmsnorm(const void* bank, int64_t sources, in
                                            int64_t n, int64_t k, void* y, int64_t y_row_stride, int epilogue,
                                            int32_t* status, void* stream);
 
+/* ---- 8-bit linears ------------------------------------------------------------
+ * e4m3 values with one fp32 scale for each block of 128 values: 128 columns of an
+ * activation row, 128 x 128 of a weight (blocks at the edge are smaller). With
+ * a = max(max |v|, 2^-100) over the block's fp32 values v:
+ *   scale = a / 448, q = e4m3(v * (448 / a)), v ~ q * scale.
+ * A NaN or an infinity makes its block's scale NaN or infinite. q is contiguous
+ * [rows, cols], scale contiguous [rows, ceil(cols / 128)] fp32. The 8-bit forms of
+ * aios/layers/norm.py:10-40, activation.py:9-12 and linear.py:11-54; the reference
+ * has none.
+ *
+ * Common rules: cols % 16 == 0; x rows x_row_stride elements apart (a multiple of
+ * 8, at least the row); x, q, weight and residual 16-byte aligned. rows may be 0. */
+
+/* bf16 rows to 8 bits. */
+AIOSB_API int aiosb_quantize_fp8(const void* x, int64_t rows, int64_t cols, int64_t x_row_stride, void* q,
+                                 float* scale, void* stream);
+
+/* A bf16 weight [n, k] to 8 bits, scale [ceil(n / 128), ceil(k / 128)]. n <= 8388480. */
+AIOSB_API int aiosb_quantize_weight_fp8(const void* w, int64_t n, int64_t k, int64_t w_row_stride, void* q,
+                                        float* scale, void* stream);
+
+/* RMSNorm with 8-bit output: v = s * (1 / sqrt(mean(s^2) + eps)) * weight in fp32,
+ * s = x, or s = x + residual with residual_out = bf16(s) (aiosb_add_rmsnorm's
+ * semantics; residual_out may be residual). residual and residual_out are contiguous
+ * [rows, hidden], both NULL for the plain norm. hidden <= 32768. */
+AIOSB_API int aiosb_rmsnorm_fp8(const void* x, int64_t rows, int64_t hidden, int64_t x_row_stride,
+                                const void* residual, void* residual_out, const void* weight, float eps, void* q,
+                                float* scale, void* stream);
+
+/* SwiGLU with 8-bit output: v[r, c] = silu(x[r, c]) * x[r, f + c] in fp32; x rows are
+ * [gate | up]. A gate below -87 gives 0. */
+AIOSB_API int aiosb_silu_mul_fp8(const void* x, int64_t rows, int64_t f, int64_t x_row_stride, void* q, float* scale,
+                                 void* stream);
+
+/* Linear on 8-bit operands (tcgen05): y = x W^T (AIOSB_EPI_STORE) or residual + x W^T
+ * (AIOSB_EPI_ADD, added in fp32, one rounding), bf16, with x and W the values that
+ * their bytes and scales stand for. x: [rows, k] e4m3, rows x_row_stride bytes apart
+ * (a multiple of 16); x_scale [rows, ceil(k / 128)]; w: contiguous [n, k] e4m3;
+ * w_scale [ceil(n / 128), ceil(k / 128)]. n % 8 == 0, k % 16 == 0. residual rows are
+ * residual_stride elements apart and may be y itself. Sums over a block of 128 are
+ * formed by the tensor cores, those across blocks in fp32, in an order that depends
+ * on the sizes alone. Every operand, the weight too, is read after the dependency
+ * wait: the kernel that quantised it may be the previous launch. */
+AIOSB_API int aiosb_linear_fp8(const void* x, int64_t x_row_stride, const float* x_scale, int64_t rows, int64_t k,
+                               const void* w, const float* w_scale, int64_t n, void* y, int64_t y_row_stride,
+                               int epilogue, const void* residual, int64_t residual_stride, int32_t* status,
+                               void* stream);
+
 /* ---- Attention ---------------------------------------------------------------
  * KV slots: token slot s of one layer lives at k_cache + s * num_kv_heads *
  * head_dim (the MHAKVCache layout [pages, page_size, Hkv, d] flattened); slot
