@@ -7,11 +7,12 @@
 // from tensor memory and folded into fp32 registers as acc += (sx * sw) * d. x is the
 // M operand: a TMEM lane is a token, its scale one register of the thread that reads
 // the lane, and the weight's scale is uniform over the columns of a warp, so the fold
-// costs one FMA per value. Two TMEM accumulators alternate: the tensor cores work on
-// block b + 1 while the warps fold block b.
+// costs one FMA per value. Two or four TMEM accumulators take turns: the tensor
+// cores work on the next blocks while the warps fold one.
 //
-// Per CTA: warps 0-7 fold (warp w: lanes 32 (w % 4).., column half w / 4), lane 0 of
-// warp 8 loads tiles by TMA into a ring of stages, lane 0 of warp 9 issues the MMAs.
+// Per CTA: the first 8 or 16 warps fold (warp w: lanes 32 (w % 4).., columns w / 4), one
+// lane of the next warp loads tiles by TMA into a ring of stages, one of the last issues
+// the MMAs.
 // Few rows leave few tiles: then a cluster of up to 8 CTAs splits the blocks of k and
 // the partial tiles are summed in rank order through distributed shared memory, so
 // results do not depend on scheduling.
@@ -28,8 +29,6 @@ namespace {
 
 constexpr int kBM = 128;                      // tokens per tile (UMMA M, TMEM lanes)
 constexpr int kBK = kFp8Block;                // bytes of k per stage: one scale block, one swizzle row
-constexpr int kFoldWarps = 8;
-constexpr int kThreads = (kFoldWarps + 2) * 32;
 constexpr int kMaxStages = 16;
 constexpr int kMaxSplit = 8;
 
@@ -61,8 +60,8 @@ __host__ __device__ constexpr uint32_t umma_idesc_e4m3(int M, int N) {
   return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-// 32 lanes x 32 consecutive columns; the values are there after tmem_wait32.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+// 32 lanes x 16 or 32 consecutive columns; the values are there after tmem_wait.
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
       "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -72,9 +71,22 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                 "+r"(r[15])::"memory");
+}
 // Waits for this thread's tensor-memory loads; naming the registers keeps their
 // uses behind the wait.
-__device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
                  "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
@@ -98,16 +110,28 @@ __device__ __forceinline__ void store8(const Fp8LinearArgs& a, int64_t row, int 
       make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
 }
 
+// Shape of the kernel for tiles of BN columns.
 template <int BN>
-__global__ void __launch_bounds__(kThreads, BN == 64 ? 2 : 1)
+struct Shape {
+  static constexpr int kCols = BN == 64 ? 32 : 64;      // columns of one fold warp
+  static constexpr int kFoldWarps = 4 * (BN / kCols);   // 4 groups of 32 TMEM lanes
+  static constexpr int kThreads = (kFoldWarps + 2) * 32;
+  static constexpr int kAccs = BN == 256 ? 2 : 4;       // TMEM accumulators in turn
+  static constexpr int kCtas = BN == 64 ? 2 : 1;        // CTAs per SM (TMEM: kAccs * BN of 512 columns each)
+};
+
+template <int BN>
+__global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
     linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                       const Fp8LinearArgs a) {
   constexpr uint32_t kBBytes = BN * kBK;
-  constexpr int kHalf = BN / 2;        // columns of one fold warp
+  constexpr int kCols = Shape<BN>::kCols, kFoldWarps = Shape<BN>::kFoldWarps, kThreads = Shape<BN>::kThreads;
+  constexpr int kAccs = Shape<BN>::kAccs;
+  constexpr int kLd = BN == 256 ? 16 : 32;  // columns per tensor-memory load (18 warps: 96 registers each)
   constexpr int kRedStride = BN + 4;   // floats per row of the partial tile: conflict-free 16-byte accesses
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[kAccs], acc_empty[kAccs];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
 
@@ -124,15 +148,15 @@ __global__ void __launch_bounds__(kThreads, BN == 64 ? 2 : 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < kAccs; ++s) {
       mbar_init(&acc_full[s], 1);
-      mbar_init(&acc_empty[s], (uint32_t)lane_groups * 2);
+      mbar_init(&acc_empty[s], (uint32_t)lane_groups * (BN / kCols));
     }
     abort_flag = 0;
     fence_mbar_init();
   }
   if (warp == kFoldWarps + 1) {
-    tmem_alloc(&tmem_slot, 2 * BN);
+    tmem_alloc(&tmem_slot, kAccs * BN);
     tmem_relinquish();
   }
   if (threadIdx.x == kFoldWarps * 32) {
@@ -182,8 +206,8 @@ __global__ void __launch_bounds__(kThreads, BN == 64 ? 2 : 1)
     uint32_t it = 0;
     for (int tile = blockIdx.x / split; tile < tiles; tile += step) {
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int s = it % a.stages, t = it & 1;
-        if (!mbar_wait(&acc_empty[t], ((it >> 1) & 1) ^ 1) || !mbar_wait(&full[s], (it / a.stages) & 1)) {
+        const int s = it % a.stages, t = it % kAccs;
+        if (!mbar_wait(&acc_empty[t], ((it / kAccs) & 1) ^ 1) || !mbar_wait(&full[s], (it / a.stages) & 1)) {
           report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
           abort_flag = 1;
         }
@@ -200,26 +224,32 @@ __global__ void __launch_bounds__(kThreads, BN == 64 ? 2 : 1)
     }
   } else if (folds) {
     // ---- fold: acc += (sx * sw) * d per block of k
-    const int half = warp >> 2;
+    const int part = warp >> 2;  // columns [part * kCols, +kCols) of the tile
     const int tile_row = (warp & 3) * 32 + lane;
-    const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(half * kHalf);
+    const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(part * kCols);
     uint32_t it = 0;
     bool ok = true;
     for (int tile = blockIdx.x / split; tile < tiles && ok; tile += step) {
       const int64_t row = (int64_t)(tile % a.m_tiles) * kBM + tile_row;
-      const int c0 = tile / a.m_tiles * BN + half * kHalf;
+      const int c0 = tile / a.m_tiles * BN + part * kCols;
       const float* sx = a.x_scale + min(row, (int64_t)a.rows - 1) * a.kblocks;
       const float* sw = a.w_scale + (int64_t)(min(c0, a.n - 1) / kFp8Block) * a.kblocks;
-      float acc[kHalf];
+      float2 acc[kCols / 2];  // pairs of neighbouring columns: one packed FMA each
 #pragma unroll
-      for (int j = 0; j < kHalf; ++j) acc[j] = 0.f;
-      float next = sx[kb0] * sw[kb0];
+      for (int j = 0; j < kCols / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+      // scales two blocks ahead, multiplied only where they are used: a product formed
+      // at the load would stall the warp for the load's latency in every block
+      const int last = kb1 - 1;
+      float x0 = sx[kb0], w0 = sw[kb0], x1 = sx[min(kb0 + 1, last)], w1 = sw[min(kb0 + 1, last)];
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int t = it & 1;
-        const float s = next;
-        const int kn = min(kb + 1, kb1 - 1);
-        next = sx[kn] * sw[kn];
-        ok = mbar_wait(&acc_full[t], (it >> 1) & 1);
+        const int t = it % kAccs;
+        const float s1 = x0 * w0;
+        const float2 s = make_float2(s1, s1);
+        x0 = x1;
+        w0 = w1;
+        x1 = sx[min(kb + 2, last)];
+        w1 = sw[min(kb + 2, last)];
+        ok = mbar_wait(&acc_full[t], (it / kAccs) & 1);
         __syncwarp();
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) {
@@ -229,34 +259,36 @@ __global__ void __launch_bounds__(kThreads, BN == 64 ? 2 : 1)
         }
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < kHalf; c += 32) {
-          uint32_t d[32];
-          tmem_ld32(t_lane + t * BN + c, d);
-          tmem_wait32(d);
-          if (c + 32 == kHalf) {  // this block's values are in registers: the accumulator may be reused
+        for (int c = 0; c < kCols; c += kLd) {
+          uint32_t d[kLd];
+          tmem_ld(t_lane + t * BN + c, d);
+          tmem_wait(d);
+          if (c + kLd == kCols) {  // this block's values are in registers: the accumulator may be reused
             tc_fence_before();
             if (lane == 0) mbar_arrive(&acc_empty[t]);
           }
 #pragma unroll
-          for (int j = 0; j < 32; ++j) acc[c + j] = fmaf(s, __uint_as_float(d[j]), acc[c + j]);
+          for (int j = 0; j < kLd / 2; ++j)
+            acc[c / 2 + j] = __ffma2_rn(s, make_float2(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1])),
+                                        acc[c / 2 + j]);
         }
       }
       if (!ok) break;
       if (split == 1) {
         if (row < a.rows) {
 #pragma unroll
-          for (int j = 0; j < kHalf; j += 8) {
-            const float v[8] = {acc[j],     acc[j + 1], acc[j + 2], acc[j + 3],
-                                acc[j + 4], acc[j + 5], acc[j + 6], acc[j + 7]};
-            if (c0 + j < a.n) store8(a, row, c0 + j, v);
+          for (int j = 0; j < kCols / 2; j += 4) {
+            const float v[8] = {acc[j].x,     acc[j].y,     acc[j + 1].x, acc[j + 1].y,
+                                acc[j + 2].x, acc[j + 2].y, acc[j + 3].x, acc[j + 3].y};
+            if (c0 + 2 * j < a.n) store8(a, row, c0 + 2 * j, v);
           }
         }
       } else if (tile_row < a.a_rows) {
         // every MMA of this CTA has read its operands: the partial tile takes their place
-        float* red = reinterpret_cast<float*>(smem) + tile_row * kRedStride + half * kHalf;
+        float* red = reinterpret_cast<float*>(smem) + tile_row * kRedStride + part * kCols;
 #pragma unroll
-        for (int j = 0; j < kHalf; j += 4)
-          *reinterpret_cast<float4*>(red + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+        for (int j = 0; j < kCols / 2; j += 2)
+          *reinterpret_cast<float4*>(red + 2 * j) = make_float4(acc[j].x, acc[j].y, acc[j + 1].x, acc[j + 1].y);
       }
     }
   }
@@ -289,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, BN == 64 ? 2 : 1)
   }
   if (warp == kFoldWarps + 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 2 * BN);
+    tmem_dealloc(tmem, kAccs * BN);
   }
 }
 
@@ -330,7 +362,7 @@ int make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64
 template <int BN>
 int launch(const CUtensorMap& tx, const CUtensorMap& tw, Fp8LinearArgs a, cudaStream_t stream) {
   constexpr int kOne = 224 * 1024;                         // shared memory of a CTA that has the SM to itself
-  constexpr int kBudget = BN == 64 ? kOne / 2 - 1024 : kOne;  // two CTAs per SM at BN = 64
+  constexpr int kCtas = Shape<BN>::kCtas, kBudget = kCtas == 2 ? kOne / 2 - 1024 : kOne;
   auto kern = linear_fp8_kernel<BN>;
   static bool configured[64] = {false};
   int dev = 0;
@@ -342,13 +374,13 @@ int launch(const CUtensorMap& tx, const CUtensorMap& tw, Fp8LinearArgs a, cudaSt
   }
   const int stage_bytes = a.a_rows * kBK + BN * kBK;
   const int tiles = a.m_tiles * a.n_tiles;
-  const int per_cta = (a.kblocks + a.split - 1) / a.split * (a.split > 1 ? 1 : (tiles + sm_count() - 1) / sm_count());
+  const int per_cta = (a.kblocks + a.split - 1) / a.split * (a.split > 1 ? 1 : (tiles + sm_count() * kCtas - 1) / (sm_count() * kCtas));
   a.stages = std::max(2, std::min({(kBudget - 1024) / stage_bytes, kMaxStages, per_cta}));
   // at least the partial tile, and 16 KB past the last A slot (two B slots have that)
   const int body = std::max(a.stages * stage_bytes, a.split > 1 ? a.a_rows * (BN + 4) * 4 : 0);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.split > 1 ? tiles * a.split : std::min(tiles, sm_count() * (BN == 64 ? 2 : 1))));
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3((unsigned)(a.split > 1 ? tiles * a.split : std::min(tiles, sm_count() * kCtas)));
+  cfg.blockDim = dim3(Shape<BN>::kThreads);
   cfg.dynamicSmemBytes = (size_t)body + 1024;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
