@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
   constexpr int kRedStride = BN + 4;   // floats per row of the partial tile: conflict-free 16-byte accesses
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[kAccs], acc_empty[kAccs];
+  __shared__ uint64_t full[kMaxStages], done[kMaxStages], acc_empty[kAccs];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
 
@@ -146,12 +146,9 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
   if (threadIdx.x == 0) {
     for (int s = 0; s < a.stages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&done[s], 1);
     }
-    for (int s = 0; s < kAccs; ++s) {
-      mbar_init(&acc_full[s], 1);
-      mbar_init(&acc_empty[s], (uint32_t)lane_groups * (BN / kCols));
-    }
+    for (int s = 0; s < kAccs; ++s) mbar_init(&acc_empty[s], (uint32_t)lane_groups * (BN / kCols));
     abort_flag = 0;
     fence_mbar_init();
   }
@@ -176,58 +173,83 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
   const int tiles = a.m_tiles * a.n_tiles;
   const int step = gridDim.x / split;
 
+  // The two single-thread loops below pace everything, once per block of k: ring
+  // positions and phases are counters (a division by the stage count costs more than
+  // the MMAs of a narrow tile), descriptors are one addition, and a wait that runs out
+  // ends its own role only (the other roles' waits then run out too).
   if (threadIdx.x == kFoldWarps * 32) {
     // ---- TMA producer
-    uint32_t it = 0;
-    for (int tile = blockIdx.x / split; tile < tiles; tile += step) {
+    int s = 0, issued = 0;
+    uint32_t phase = 1;
+    bool ok = true;
+    for (int tile = blockIdx.x / split; tile < tiles && ok; tile += step) {
       const int m0 = tile % a.m_tiles * kBM, n0 = tile / a.m_tiles * BN;
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int s = it % a.stages;
-        if (!mbar_wait(&empty[s], ((it / a.stages) & 1) ^ 1)) {
-          report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
-          abort_flag = 1;
-        }
-        if (abort_flag) break;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = mbar_wait(&done[s], phase);
+        if (!ok) break;
         mbar_arrive_expect_tx(&full[s], a_bytes + kBBytes);
         tma_load_2d(smem_b + s * kBBytes, &tm_w, &full[s], kb * kBK, n0);
         tma_load_2d(smem_a + s * a_bytes, &tm_x, &full[s], kb * kBK, m0);
+        issued = min(issued + 1, a.stages);
+        if (++s == a.stages) {
+          s = 0;
+          phase ^= 1;
+        }
       }
-      if (abort_flag) break;
     }
-    if (abort_flag) {  // let the copies that are still in flight land before this CTA returns
-      for (uint32_t i = it > (uint32_t)a.stages ? it - a.stages : 0; i < it; ++i)
-        mbar_wait(&full[i % a.stages], (i / a.stages) & 1);
+    if (!ok) {  // let the copies that are still in flight land before this CTA returns
+      report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
+      abort_flag = 1;
+      for (; issued > 0; --issued) {
+        if (--s < 0) {
+          s = a.stages - 1;
+          phase ^= 1;
+        }
+        mbar_wait(&full[s], phase ^ 1);
+      }
     }
   } else if (threadIdx.x == (kFoldWarps + 1) * 32) {
     // ---- MMA issuer. With fewer than 128 rows staged the A operand's unused rows are
     // whatever follows the slot in shared memory (inside the allocation): a row of A
     // reaches its own TMEM lane only, and those lanes are not read.
+    // One commit per block serves two readers of done[]: the producer (the stage's
+    // operands are read) and the fold (the product is in TMEM). The fold cannot fall a
+    // whole ring behind, because stages >= kAccs and an accumulator waits for its fold.
     constexpr uint32_t idesc = umma_idesc_e4m3(kBM, BN);
-    uint32_t it = 0;
-    for (int tile = blockIdx.x / split; tile < tiles; tile += step) {
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int s = it % a.stages, t = it % kAccs;
-        if (!mbar_wait(&acc_empty[t], ((it / kAccs) & 1) ^ 1) || !mbar_wait(&full[s], (it / a.stages) & 1)) {
-          report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
-          abort_flag = 1;
-        }
-        if (abort_flag) break;
+    const uint64_t a_desc = umma_desc_sw128(smem_u32(smem_a)), b_desc = umma_desc_sw128(smem_u32(smem_b));
+    int s = 0, t = 0;
+    uint32_t phase = 0, acc_phase = 1;
+    bool ok = true;
+    for (int tile = blockIdx.x / split; tile < tiles && ok; tile += step) {
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = mbar_wait(&acc_empty[t], acc_phase) && mbar_wait(&full[s], phase);
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t pa = smem_u32(smem_a + s * a_bytes), pb = smem_u32(smem_b + s * kBBytes);
+        const uint64_t da = a_desc + (uint32_t)s * (a_bytes >> 4), db = b_desc + (uint32_t)s * (kBBytes >> 4);
 #pragma unroll
-        for (int kk = 0; kk < kBK / 32; ++kk)
-          tc_mma_e4m3(tmem + t * BN, umma_desc_sw128(pa + kk * 32), umma_desc_sw128(pb + kk * 32), idesc, kk != 0);
-        tc_commit(&empty[s]);
-        tc_commit(&acc_full[t]);
+        for (int kk = 0; kk < kBK / 32; ++kk) tc_mma_e4m3(tmem + t * BN, da + 2 * kk, db + 2 * kk, idesc, kk != 0);
+        tc_commit(&done[s]);
+        if (++s == a.stages) {
+          s = 0;
+          phase ^= 1;
+        }
+        if (++t == kAccs) {
+          t = 0;
+          acc_phase ^= 1;
+        }
       }
-      if (abort_flag) break;
+    }
+    if (!ok) {
+      report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
+      abort_flag = 1;
     }
   } else if (folds) {
     // ---- fold: acc += (sx * sw) * d per block of k
     const int part = warp >> 2;  // columns [part * kCols, +kCols) of the tile
     const int tile_row = (warp & 3) * 32 + lane;
     const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(part * kCols);
-    uint32_t it = 0;
+    int ring = 0, t = 0;
+    uint32_t phase = 0;
     bool ok = true;
     for (int tile = blockIdx.x / split; tile < tiles && ok; tile += step) {
       const int64_t row = (int64_t)(tile % a.m_tiles) * kBM + tile_row;
@@ -241,15 +263,14 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
       // at the load would stall the warp for the load's latency in every block
       const int last = kb1 - 1;
       float x0 = sx[kb0], w0 = sw[kb0], x1 = sx[min(kb0 + 1, last)], w1 = sw[min(kb0 + 1, last)];
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int t = it % kAccs;
+      for (int kb = kb0; kb < kb1; ++kb) {
         const float s1 = x0 * w0;
         const float2 s = make_float2(s1, s1);
         x0 = x1;
         w0 = w1;
         x1 = sx[min(kb + 2, last)];
         w1 = sw[min(kb + 2, last)];
-        ok = mbar_wait(&acc_full[t], (it / kAccs) & 1);
+        ok = mbar_wait(&done[ring], phase);
         __syncwarp();
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) {
@@ -272,6 +293,11 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
             acc[c / 2 + j] = __ffma2_rn(s, make_float2(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1])),
                                         acc[c / 2 + j]);
         }
+        if (++ring == a.stages) {
+          ring = 0;
+          phase ^= 1;
+        }
+        if (++t == kAccs) t = 0;
       }
       if (!ok) break;
       if (split == 1) {
@@ -375,7 +401,7 @@ int launch(const CUtensorMap& tx, const CUtensorMap& tw, Fp8LinearArgs a, cudaSt
   const int stage_bytes = a.a_rows * kBK + BN * kBK;
   const int tiles = a.m_tiles * a.n_tiles;
   const int per_cta = (a.kblocks + a.split - 1) / a.split * (a.split > 1 ? 1 : (tiles + sm_count() * kCtas - 1) / (sm_count() * kCtas));
-  a.stages = std::max(2, std::min({(kBudget - 1024) / stage_bytes, kMaxStages, per_cta}));
+  a.stages = std::max(Shape<BN>::kAccs, std::min({(kBudget - 1024) / stage_bytes, kMaxStages, per_cta}));
   // at least the partial tile, and 16 KB past the last A slot (two B slots have that)
   const int body = std::max(a.stages * stage_bytes, a.split > 1 ? a.a_rows * (BN + 4) * 4 : 0);
   cudaLaunchConfig_t cfg = {};
