@@ -10,9 +10,12 @@
 // costs one FMA per value. Two or four TMEM accumulators take turns: the tensor
 // cores work on the next blocks while the warps fold one.
 //
-// Per CTA: the first 8 or 16 warps fold (warp w: lanes 32 (w % 4).., columns w / 4), one
-// lane of the next warp loads tiles by TMA into a ring of stages, one of the last issues
-// the MMAs.
+// Per CTA: the first 8 or 16 warps fold (warp w: lanes 32 (w % 4).., columns w / 4). Of
+// the four warps after them one lane loads tiles by TMA into a ring of stages, one issues
+// the MMAs, and a third warp forms the products sx * sw eight blocks of k at a time and
+// hands them over in shared memory: read by the folding threads themselves, each row's
+// scale is a cache line of its own, and 16 warps fetching 32 lines each per block took
+// as long as the MMAs.
 // Few rows leave few tiles: then a cluster of up to 8 CTAs splits the blocks of k and
 // the partial tiles are summed in rank order through distributed shared memory, so
 // results do not depend on scheduling.
@@ -31,6 +34,7 @@ constexpr int kBM = 128;                      // tokens per tile (UMMA M, TMEM l
 constexpr int kBK = kFp8Block;                // bytes of k per stage: one scale block, one swizzle row
 constexpr int kMaxStages = 16;
 constexpr int kMaxSplit = 8;
+constexpr int kScaleGroup = 8;
 
 struct Fp8LinearArgs {
   const float* x_scale;  // [rows, kblocks]
@@ -42,6 +46,7 @@ struct Fp8LinearArgs {
   int m_tiles, n_tiles;
   int split;
   int stages;
+  int scale_offset;  // of the scale products, bytes from the start of dynamic shared memory
   int a_rows;  // token rows a stage holds: rows, rounded up to the swizzle's 8, at most 128
   int32_t* status;
 };
@@ -115,8 +120,11 @@ template <int BN>
 struct Shape {
   static constexpr int kCols = BN == 64 ? 32 : 64;      // columns of one fold warp
   static constexpr int kFoldWarps = 4 * (BN / kCols);   // 4 groups of 32 TMEM lanes
-  static constexpr int kThreads = (kFoldWarps + 2) * 32;
+  static constexpr int kThreads = (kFoldWarps + 4) * 32;
   static constexpr int kAccs = BN == 256 ? 2 : 4;       // TMEM accumulators in turn
+  static constexpr int kWBlocks = BN == 256 ? 2 : 1;    // 128-wide weight blocks of the tile
+  // scale products: two groups of kScaleGroup blocks of k, [kWBlocks][128 rows] each
+  static constexpr int kScaleBytes = 2 * kScaleGroup * kWBlocks * kBM * 4;
   static constexpr int kCtas = BN == 64 ? 2 : 1;        // CTAs per SM (TMEM: kAccs * BN of 512 columns each)
 };
 
@@ -127,11 +135,12 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
   constexpr uint32_t kBBytes = BN * kBK;
   constexpr int kCols = Shape<BN>::kCols, kFoldWarps = Shape<BN>::kFoldWarps, kThreads = Shape<BN>::kThreads;
   constexpr int kAccs = Shape<BN>::kAccs;
-  constexpr int kLd = BN == 256 ? 16 : 32;  // columns per tensor-memory load (18 warps: 96 registers each)
+  constexpr int kWBlocks = Shape<BN>::kWBlocks;
+  constexpr int kLd = BN == 128 ? 32 : 16;  // columns per tensor-memory load, by the registers a thread has
   constexpr int kRedStride = BN + 4;   // floats per row of the partial tile: conflict-free 16-byte accesses
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[kMaxStages], done[kMaxStages], acc_empty[kAccs];
+  __shared__ uint64_t full[kMaxStages], done[kMaxStages], acc_empty[kAccs], scale_full[2], scale_empty[2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
 
@@ -139,6 +148,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
   const uint32_t a_bytes = (uint32_t)a.a_rows * kBK;
   uint8_t* const smem_a = smem;
   uint8_t* const smem_b = smem + (uint32_t)a.stages * a_bytes;
+  float* const scales = reinterpret_cast<float*>(smem_raw + a.scale_offset);
   // fold warps whose lanes hold tokens (a tile of fewer than 128 rows is the only m tile)
   const int lane_groups = (a.a_rows + 31) / 32;
   const bool folds = warp < kFoldWarps && (warp & 3) < lane_groups;
@@ -149,6 +159,10 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
       mbar_init(&done[s], 1);
     }
     for (int s = 0; s < kAccs; ++s) mbar_init(&acc_empty[s], (uint32_t)lane_groups * (BN / kCols));
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&scale_full[s], 1);
+      mbar_init(&scale_empty[s], (uint32_t)lane_groups * (BN / kCols));
+    }
     abort_flag = 0;
     fence_mbar_init();
   }
@@ -243,35 +257,71 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
       report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
       abort_flag = 1;
     }
+  } else if (warp == kFoldWarps + 2) {
+    // ---- scale products, a group of blocks of k at a time; lane l has rows l + 32 i
+    int g = 0;
+    uint32_t phase = 1;
+    bool ok = true;
+    for (int tile = blockIdx.x / split; tile < tiles && ok; tile += step) {
+      const int m0 = tile % a.m_tiles * kBM, n0 = tile / a.m_tiles * BN;
+      const float *sx[4], *sw[kWBlocks];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sx[i] = a.x_scale + (int64_t)min(m0 + i * 32 + lane, a.rows - 1) * a.kblocks;
+#pragma unroll
+      for (int b = 0; b < kWBlocks; ++b)
+        sw[b] = a.w_scale + (int64_t)(min(n0 + b * kFp8Block, a.n - 1) / kFp8Block) * a.kblocks;
+      for (int kb = kb0; kb < kb1; kb += kScaleGroup) {
+        ok = mbar_wait(&scale_empty[g], phase);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        // every load of the group in flight before the first product
+        float x[4][kScaleGroup], w[kWBlocks][kScaleGroup];
+#pragma unroll
+        for (int j = 0; j < kScaleGroup; ++j) {
+          const bool in = kb + j < kb1;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i][j] = in && i < lane_groups ? sx[i][kb + j] : 0.f;
+#pragma unroll
+          for (int b = 0; b < kWBlocks; ++b) w[b][j] = in ? sw[b][kb + j] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < kScaleGroup; ++j) {
+#pragma unroll
+          for (int b = 0; b < kWBlocks; ++b) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (i < lane_groups)
+                scales[((g * kScaleGroup + j) * kWBlocks + b) * kBM + i * 32 + lane] = x[i][j] * w[b][j];
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&scale_full[g]);
+        g ^= 1;
+        if (g == 0) phase ^= 1;
+      }
+    }
+    if (!ok) {
+      report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
+      abort_flag = 1;
+    }
   } else if (folds) {
     // ---- fold: acc += (sx * sw) * d per block of k
     const int part = warp >> 2;  // columns [part * kCols, +kCols) of the tile
     const int tile_row = (warp & 3) * 32 + lane;
     const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(part * kCols);
-    int ring = 0, t = 0;
-    uint32_t phase = 0;
+    const float* const my_scales = scales + part * kCols / kFp8Block * kBM + tile_row;
+    int ring = 0, t = 0, g = 0;
+    uint32_t phase = 0, g_phase = 0;
     bool ok = true;
     for (int tile = blockIdx.x / split; tile < tiles && ok; tile += step) {
       const int64_t row = (int64_t)(tile % a.m_tiles) * kBM + tile_row;
       const int c0 = tile / a.m_tiles * BN + part * kCols;
-      const float* sx = a.x_scale + min(row, (int64_t)a.rows - 1) * a.kblocks;
-      const float* sw = a.w_scale + (int64_t)(min(c0, a.n - 1) / kFp8Block) * a.kblocks;
       float2 acc[kCols / 2];  // pairs of neighbouring columns: one packed FMA each
 #pragma unroll
       for (int j = 0; j < kCols / 2; ++j) acc[j] = make_float2(0.f, 0.f);
-      // scales two blocks ahead, multiplied only where they are used: a product formed
-      // at the load would stall the warp for the load's latency in every block
-      const int last = kb1 - 1;
-      float x0 = sx[kb0], w0 = sw[kb0], x1 = sx[min(kb0 + 1, last)], w1 = sw[min(kb0 + 1, last)];
+      int in_group = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
-        const float s1 = x0 * w0;
-        const float2 s = make_float2(s1, s1);
-        x0 = x1;
-        w0 = w1;
-        x1 = sx[min(kb + 2, last)];
-        w1 = sw[min(kb + 2, last)];
-        ok = mbar_wait(&done[ring], phase);
-        __syncwarp();
+        ok = (in_group != 0 || mbar_wait(&scale_full[g], g_phase)) && mbar_wait(&done[ring], phase);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) {
           report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
@@ -279,6 +329,15 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
           break;
         }
         tc_fence_after();
+        const float s1 = my_scales[(g * kScaleGroup + in_group) * kWBlocks * kBM];
+        const float2 s = make_float2(s1, s1);
+        if (++in_group == kScaleGroup || kb + 1 == kb1) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&scale_empty[g]);
+          in_group = 0;
+          g ^= 1;
+          if (g == 0) g_phase ^= 1;
+        }
 #pragma unroll
         for (int c = 0; c < kCols; c += kLd) {
           uint32_t d[kLd];
@@ -387,7 +446,8 @@ int make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64
 
 template <int BN>
 int launch(const CUtensorMap& tx, const CUtensorMap& tw, Fp8LinearArgs a, cudaStream_t stream) {
-  constexpr int kOne = 224 * 1024;                         // shared memory of a CTA that has the SM to itself
+  constexpr int kOne = 224 * 1024;  // shared memory of a CTA that has the SM to itself
+  constexpr int kScaleBytes = Shape<BN>::kScaleBytes;
   constexpr int kCtas = Shape<BN>::kCtas, kBudget = kCtas == 2 ? kOne / 2 - 1024 : kOne;
   auto kern = linear_fp8_kernel<BN>;
   static bool configured[64] = {false};
@@ -401,13 +461,14 @@ int launch(const CUtensorMap& tx, const CUtensorMap& tw, Fp8LinearArgs a, cudaSt
   const int stage_bytes = a.a_rows * kBK + BN * kBK;
   const int tiles = a.m_tiles * a.n_tiles;
   const int per_cta = (a.kblocks + a.split - 1) / a.split * (a.split > 1 ? 1 : (tiles + sm_count() * kCtas - 1) / (sm_count() * kCtas));
-  a.stages = std::max(Shape<BN>::kAccs, std::min({(kBudget - 1024) / stage_bytes, kMaxStages, per_cta}));
+  a.stages = std::max(Shape<BN>::kAccs, std::min({(kBudget - 1024 - kScaleBytes) / stage_bytes, kMaxStages, per_cta}));
   // at least the partial tile, and 16 KB past the last A slot (two B slots have that)
   const int body = std::max(a.stages * stage_bytes, a.split > 1 ? a.a_rows * (BN + 4) * 4 : 0);
+  a.scale_offset = body + 1024;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.split > 1 ? tiles * a.split : std::min(tiles, sm_count() * kCtas)));
   cfg.blockDim = dim3(Shape<BN>::kThreads);
-  cfg.dynamicSmemBytes = (size_t)body + 1024;
+  cfg.dynamicSmemBytes = (size_t)body + 1024 + kScaleBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
