@@ -271,11 +271,19 @@ _NON_LAUNCHING = frozenset({"aiosb_version", "aiosb_last_error", "aiosb_host_dev
                             "aiosb_prefill_tile_tokens", "aiosb_decode_step_sync_words",
                             "aiosb_decode_step_work_bytes", "aiosb_linear_tile_stats_eligible"})
 launches = 0
+_functions: dict[str, object] = {}
+
+
+def _function(name: str):
+    fn = _functions[name] = getattr(load(), name)
+    return fn
 
 
 def call(name: str, *args) -> None:
     global launches
-    check(getattr(load(), name)(*args), name)
+    rc = (_functions.get(name) or _function(name))(*args)
+    if rc != OK:
+        check(rc, name)
     if name not in _NON_LAUNCHING:
         launches += 1
 

@@ -35,6 +35,11 @@ def status_word(device: torch.device) -> torch.Tensor:
     return st
 
 
+def _status_pointer(index: int) -> int:
+    st = _STATUS.get(index)
+    return (st if st is not None else status_word(torch.device("cuda", index))).data_ptr()
+
+
 def check_status(device: torch.device, reset: bool = True) -> None:
     """Raises if any kernel on `device` reported a device-side fault (syncs)."""
     st = status_word(device)
@@ -585,46 +590,51 @@ FP8_BLOCK = 128
 FP8_DTYPE = torch.float8_e4m3fn
 
 
-def _launch(device: torch.device, name: str, *args) -> None:
-    """Calls a launching entry point on `device`'s current stream (its last argument),
-    with that device current."""
-    index = device.index
-    if index == torch.cuda.current_device():
+def _launch(index: int, name: str, *args) -> None:
+    """Calls a launching entry point on the current stream of device `index` (its last
+    argument), with that device current."""
+    if index == torch._C._cuda_getDevice():
         _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
             _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _check_rows(what: str, x: torch.Tensor, dtype: torch.dtype) -> int:
-    """`x` as rows with contiguous columns on a CUDA device; returns the row stride."""
+# These wrappers run in about the time of one small launch, so their checks are spelled
+# out on plain attributes: a decode step is bound by the host's launch rate otherwise.
+def _check_rows(what: str, x: torch.Tensor, dtype: torch.dtype) -> tuple[int, int, int]:
+    """`x` as rows with contiguous columns on a CUDA device: (rows, cols, row stride)."""
     if not x.is_cuda:
         raise ValueError(f"{what} requires CUDA tensors")
-    if x.ndim != 2 or x.dtype != dtype:
+    if x.dtype is not dtype or x.ndim != 2:
         raise ValueError(f"{what} expects a 2-D {dtype} tensor")
     rows, cols = x.shape
-    if cols > 1 and x.stride(1) != 1:
+    if rows == 1 or x.is_contiguous():
+        if cols > 1 and x.stride(1) != 1:
+            raise ValueError(f"{what} rows must be contiguous")
+        return rows, cols, cols
+    stride, inner = x.stride()
+    if inner != 1 and cols > 1:
         raise ValueError(f"{what} rows must be contiguous")
-    return x.stride(0) if rows > 1 else cols
+    return rows, cols, stride
 
 
 def _check_dense(what: str, name: str, t: torch.Tensor, shape: tuple[int, ...], dtype: torch.dtype,
-                 device: torch.device) -> None:
-    if t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{what}: {name} must be a contiguous {dtype} tensor of shape {list(shape)} on {device}")
+                 index: int) -> None:
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be a contiguous {dtype} tensor of shape {list(shape)} on cuda:{index}")
 
 
-def _fp8_outputs(what: str, rows: int, cols: int, device: torch.device, out: torch.Tensor | None,
+def _fp8_outputs(what: str, x: torch.Tensor, rows: int, cols: int, out: torch.Tensor | None,
                  scale: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:
-    blocks = -(-cols // FP8_BLOCK)
     if out is None:
-        out = torch.empty((rows, cols), dtype=FP8_DTYPE, device=device)
+        out = x.new_empty(rows, cols, dtype=FP8_DTYPE)
     else:
-        _check_dense(what, "out", out, (rows, cols), FP8_DTYPE, device)
+        _check_dense(what, "out", out, (rows, cols), FP8_DTYPE, x.get_device())
     if scale is None:
-        scale = torch.empty((rows, blocks), dtype=torch.float32, device=device)
+        scale = x.new_empty(rows, -(-cols // FP8_BLOCK), dtype=torch.float32)
     else:
-        _check_dense(what, "scale", scale, (rows, blocks), torch.float32, device)
+        _check_dense(what, "scale", scale, (rows, -(-cols // FP8_BLOCK)), torch.float32, x.get_device())
     return out, scale
 
 
@@ -632,21 +642,19 @@ def quantize_fp8(x: torch.Tensor, *, out: torch.Tensor | None = None,
                  scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """bf16 rows [T, H] to (e4m3 [T, H], scale [T, ceil(H / 128)]): a scale for each 128
     columns of a row, ``x ~ q * scale``. H is a multiple of 16; rows may be strided."""
-    stride = _check_rows("quantize_fp8", x, torch.bfloat16)
-    rows, cols = x.shape
-    out, scale = _fp8_outputs("quantize_fp8", rows, cols, x.device, out, scale)
-    _launch(x.device, "aiosb_quantize_fp8", x.data_ptr(), rows, cols, stride, out.data_ptr(), scale.data_ptr())
+    rows, cols, stride = _check_rows("quantize_fp8", x, torch.bfloat16)
+    out, scale = _fp8_outputs("quantize_fp8", x, rows, cols, out, scale)
+    _launch(x.get_device(), "aiosb_quantize_fp8", x.data_ptr(), rows, cols, stride, out.data_ptr(), scale.data_ptr())
     return out, scale
 
 
 def quantize_weight_fp8(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """A bf16 weight [N, K] to (e4m3 [N, K], scale [ceil(N / 128), ceil(K / 128)]): a scale
     for each 128 x 128 block. K is a multiple of 16; rows may be strided."""
-    stride = _check_rows("quantize_weight_fp8", weight, torch.bfloat16)
-    n, k = weight.shape
-    out = torch.empty((n, k), dtype=FP8_DTYPE, device=weight.device)
-    scale = torch.empty((-(-n // FP8_BLOCK), -(-k // FP8_BLOCK)), dtype=torch.float32, device=weight.device)
-    _launch(weight.device, "aiosb_quantize_weight_fp8", weight.data_ptr(), n, k, stride, out.data_ptr(),
+    n, k, stride = _check_rows("quantize_weight_fp8", weight, torch.bfloat16)
+    out = weight.new_empty(n, k, dtype=FP8_DTYPE)
+    scale = weight.new_empty(-(-n // FP8_BLOCK), -(-k // FP8_BLOCK), dtype=torch.float32)
+    _launch(weight.get_device(), "aiosb_quantize_weight_fp8", weight.data_ptr(), n, k, stride, out.data_ptr(),
             scale.data_ptr())
     return out, scale
 
@@ -655,12 +663,12 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, out: torch
                 scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """``quantize_fp8(rmsnorm(x, weight, eps))`` in one kernel, without the bf16 rounding
     between the two. x is [T, H] with H a multiple of 16, at most 32768."""
-    stride = _check_rows("rmsnorm_fp8", x, torch.bfloat16)
-    rows, hidden = x.shape
-    _check_dense("rmsnorm_fp8", "weight", weight, (hidden,), torch.bfloat16, x.device)
-    out, scale = _fp8_outputs("rmsnorm_fp8", rows, hidden, x.device, out, scale)
-    _launch(x.device, "aiosb_rmsnorm_fp8", x.data_ptr(), rows, hidden, stride, None, None, weight.data_ptr(),
-            float(eps), out.data_ptr(), scale.data_ptr())
+    rows, hidden, stride = _check_rows("rmsnorm_fp8", x, torch.bfloat16)
+    index = x.get_device()
+    _check_dense("rmsnorm_fp8", "weight", weight, (hidden,), torch.bfloat16, index)
+    out, scale = _fp8_outputs("rmsnorm_fp8", x, rows, hidden, out, scale)
+    _launch(index, "aiosb_rmsnorm_fp8", x.data_ptr(), rows, hidden, stride, None, None, weight.data_ptr(), float(eps),
+            out.data_ptr(), scale.data_ptr())
     return out, scale
 
 
@@ -669,17 +677,17 @@ def fused_add_rmsnorm_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torch
                           scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """``fused_add_rmsnorm`` with 8-bit output: residual += x (in place, or into
     ``residual_out``), and the quantised rmsnorm of the fp32 sum is returned; x is kept."""
-    stride = _check_rows("fused_add_rmsnorm_fp8", x, torch.bfloat16)
-    rows, hidden = x.shape
-    _check_dense("fused_add_rmsnorm_fp8", "weight", weight, (hidden,), torch.bfloat16, x.device)
-    _check_dense("fused_add_rmsnorm_fp8", "residual", residual, (rows, hidden), torch.bfloat16, x.device)
+    rows, hidden, stride = _check_rows("fused_add_rmsnorm_fp8", x, torch.bfloat16)
+    index = x.get_device()
+    _check_dense("fused_add_rmsnorm_fp8", "weight", weight, (hidden,), torch.bfloat16, index)
+    _check_dense("fused_add_rmsnorm_fp8", "residual", residual, (rows, hidden), torch.bfloat16, index)
     if residual_out is None:
         residual_out = residual
     else:
-        _check_dense("fused_add_rmsnorm_fp8", "residual_out", residual_out, (rows, hidden), torch.bfloat16, x.device)
-    out, scale = _fp8_outputs("fused_add_rmsnorm_fp8", rows, hidden, x.device, out, scale)
+        _check_dense("fused_add_rmsnorm_fp8", "residual_out", residual_out, (rows, hidden), torch.bfloat16, index)
+    out, scale = _fp8_outputs("fused_add_rmsnorm_fp8", x, rows, hidden, out, scale)
     if rows:
-        _launch(x.device, "aiosb_rmsnorm_fp8", x.data_ptr(), rows, hidden, stride, residual.data_ptr(),
+        _launch(index, "aiosb_rmsnorm_fp8", x.data_ptr(), rows, hidden, stride, residual.data_ptr(),
                 residual_out.data_ptr(), weight.data_ptr(), float(eps), out.data_ptr(), scale.data_ptr())
     return out, scale
 
@@ -688,12 +696,12 @@ def silu_and_mul_fp8(x: torch.Tensor, *, out: torch.Tensor | None = None,
                      scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """``quantize_fp8(silu_and_mul(x))`` in one kernel, without the bf16 rounding between
     the two: x is [T, 2F] ([gate | up]) with F a multiple of 16."""
-    stride = _check_rows("silu_and_mul_fp8", x, torch.bfloat16)
-    rows, width = x.shape
+    rows, width, stride = _check_rows("silu_and_mul_fp8", x, torch.bfloat16)
     if width % 2:
         raise ValueError("silu_and_mul_fp8 expects a [T, 2F] tensor")
-    out, scale = _fp8_outputs("silu_and_mul_fp8", rows, width // 2, x.device, out, scale)
-    _launch(x.device, "aiosb_silu_mul_fp8", x.data_ptr(), rows, width // 2, stride, out.data_ptr(), scale.data_ptr())
+    f = width // 2
+    out, scale = _fp8_outputs("silu_and_mul_fp8", x, rows, f, out, scale)
+    _launch(x.get_device(), "aiosb_silu_mul_fp8", x.data_ptr(), rows, f, stride, out.data_ptr(), scale.data_ptr())
     return out, scale
 
 
@@ -712,31 +720,33 @@ def linear_fp8(
 
     ``epilogue=EPI_ADD`` returns ``residual + x @ weight.T`` with one rounding (residual
     may be ``out`` for an in-place add). N is a multiple of 8, K of 16."""
-    stride = _check_rows("linear_fp8", x, FP8_DTYPE)
-    rows, k = x.shape
+    rows, k, stride = _check_rows("linear_fp8", x, FP8_DTYPE)
     if weight.ndim != 2 or weight.shape[1] != k:
         raise ValueError("linear_fp8 expects x [T, K] and weight [N, K]")
     n = weight.shape[0]
-    device = x.device
+    index = x.get_device()
     blocks = -(-k // FP8_BLOCK)
-    _check_dense("linear_fp8", "weight", weight, (n, k), FP8_DTYPE, device)
-    _check_dense("linear_fp8", "x_scale", x_scale, (rows, blocks), torch.float32, device)
-    _check_dense("linear_fp8", "weight_scale", weight_scale, (-(-n // FP8_BLOCK), blocks), torch.float32, device)
+    _check_dense("linear_fp8", "weight", weight, (n, k), FP8_DTYPE, index)
+    _check_dense("linear_fp8", "x_scale", x_scale, (rows, blocks), torch.float32, index)
+    _check_dense("linear_fp8", "weight_scale", weight_scale, (-(-n // FP8_BLOCK), blocks), torch.float32, index)
+    res_ptr, res_stride = None, 0
     if epilogue == _lib.EPI_ADD:
-        if (residual is None or residual.shape != (rows, n) or residual.dtype != torch.bfloat16
-                or residual.device != device or residual.stride(1) != 1):
+        if (residual is None or residual.shape != (rows, n) or residual.dtype is not torch.bfloat16
+                or residual.get_device() != index or (residual.stride(1) != 1 and n > 1)):
             raise ValueError("the add epilogue needs a bf16 residual [rows, n] with contiguous rows")
-    else:
-        residual = None
+        res_ptr, res_stride = residual.data_ptr(), residual.stride(0) if rows > 1 else n
     if out is None:
-        out = torch.empty((rows, n), dtype=torch.bfloat16, device=device)
-    elif out.shape != (rows, n) or out.dtype != torch.bfloat16 or out.device != device or out.stride(1) != 1:
-        raise ValueError("linear_fp8 output must be bf16 [rows, n] with contiguous rows")
-    if rows == 0:
-        return out
-    _launch(device, "aiosb_linear_fp8", x.data_ptr(), stride, x_scale.data_ptr(), rows, k, weight.data_ptr(),
-            weight_scale.data_ptr(), n, out.data_ptr(), out.stride(0) if rows > 1 else n, epilogue, _ptr(residual),
-            (residual.stride(0) if rows > 1 else n) if residual is not None else 0, status_word(device).data_ptr())
+        out = x.new_empty(rows, n, dtype=torch.bfloat16)
+        out_stride = n
+    else:
+        if (out.shape != (rows, n) or out.dtype is not torch.bfloat16 or out.get_device() != index
+                or (out.stride(1) != 1 and n > 1)):
+            raise ValueError("linear_fp8 output must be bf16 [rows, n] with contiguous rows")
+        out_stride = out.stride(0) if rows > 1 else n
+    if rows:
+        _launch(index, "aiosb_linear_fp8", x.data_ptr(), stride, x_scale.data_ptr(), rows, k, weight.data_ptr(),
+                weight_scale.data_ptr(), n, out.data_ptr(), out_stride, epilogue, res_ptr, res_stride,
+                _status_pointer(index))
     return out
 
 
