@@ -24,96 +24,10 @@
 #include <algorithm>
 #include <mutex>
 
-#include "abi_util.h"
-#include "fp8.cuh"
+#include "fp8_linear.cuh"
 
 namespace aiosb {
 namespace {
-
-constexpr int kBM = 128;                      // tokens per tile (UMMA M, TMEM lanes)
-constexpr int kBK = kFp8Block;                // bytes of k per stage: one scale block, one swizzle row
-constexpr int kMaxStages = 16;
-constexpr int kMaxSplit = 8;
-constexpr int kScaleGroup = 8;
-
-struct Fp8LinearArgs {
-  const float* x_scale;  // [rows, kblocks]
-  const float* w_scale;  // [ceil(n / 128), kblocks]
-  __nv_bfloat16* y;
-  const __nv_bfloat16* residual;  // or NULL
-  int64_t y_stride, residual_stride;
-  int rows, n, kblocks;
-  int m_tiles, n_tiles;
-  int split;
-  int stages;
-  int scale_offset;  // of the scale products, bytes from the start of dynamic shared memory
-  int a_rows;  // token rows a stage holds: rows, rounded up to the swizzle's 8, at most 128
-  int32_t* status;
-};
-
-__device__ __forceinline__ void tc_mma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                            uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-// Instruction descriptor: fp32 accumulator, e4m3 A and B (format 0), both K-major.
-__host__ __device__ constexpr uint32_t umma_idesc_e4m3(int M, int N) {
-  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-}
-
-// 32 lanes x 16 or 32 consecutive columns; the values are there after tmem_wait.
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                 "+r"(r[15])::"memory");
-}
-// Waits for this thread's tensor-memory loads; naming the registers keeps their
-// uses behind the wait.
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                 "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
-                 "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
-                 "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
-}
-
-// Eight finished sums of one row to bf16, the residual added in fp32 (one rounding).
-__device__ __forceinline__ void store8(const Fp8LinearArgs& a, int64_t row, int col, const float (&v)[8]) {
-  float o[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) o[j] = v[j];
-  if (a.residual != nullptr) {
-    float r[8];
-    unpack8(*reinterpret_cast<const uint4*>(a.residual + row * a.residual_stride + col), r);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] += r[j];
-  }
-  *reinterpret_cast<uint4*>(a.y + row * a.y_stride + col) =
-      make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
-}
 
 // Shape of the kernel for tiles of BN columns.
 template <int BN>
@@ -144,7 +58,8 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the shuffle tells the compiler that the warp index, and every branch on it, is uniform
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t a_bytes = (uint32_t)a.a_rows * kBK;
   uint8_t* const smem_a = smem;
   uint8_t* const smem_b = smem + (uint32_t)a.stages * a_bytes;
@@ -191,7 +106,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
   // positions and phases are counters (a division by the stage count costs more than
   // the MMAs of a narrow tile), descriptors are one addition, and a wait that runs out
   // ends its own role only (the other roles' waits then run out too).
-  if (threadIdx.x == kFoldWarps * 32) {
+  if (warp == kFoldWarps) {
     // ---- TMA producer
     int s = 0, issued = 0;
     uint32_t phase = 1;
@@ -199,11 +114,13 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
     for (int tile = blockIdx.x / split; tile < tiles && ok; tile += step) {
       const int m0 = tile % a.m_tiles * kBM, n0 = tile / a.m_tiles * BN;
       for (int kb = kb0; kb < kb1; ++kb) {
-        ok = mbar_wait(&done[s], phase);
+        ok = __all_sync(0xffffffffu, mbar_wait(&done[s], phase));
         if (!ok) break;
-        mbar_arrive_expect_tx(&full[s], a_bytes + kBBytes);
-        tma_load_2d(smem_b + s * kBBytes, &tm_w, &full[s], kb * kBK, n0);
-        tma_load_2d(smem_a + s * a_bytes, &tm_x, &full[s], kb * kBK, m0);
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&full[s], a_bytes + kBBytes);
+          tma_load_2d(smem_b + s * kBBytes, &tm_w, &full[s], kb * kBK, n0);
+          tma_load_2d(smem_a + s * a_bytes, &tm_x, &full[s], kb * kBK, m0);
+        }
         issued = min(issued + 1, a.stages);
         if (++s == a.stages) {
           s = 0;
@@ -222,7 +139,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
         mbar_wait(&full[s], phase ^ 1);
       }
     }
-  } else if (threadIdx.x == (kFoldWarps + 1) * 32) {
+  } else if (warp == kFoldWarps + 1) {
     // ---- MMA issuer. With fewer than 128 rows staged the A operand's unused rows are
     // whatever follows the slot in shared memory (inside the allocation): a row of A
     // reaches its own TMEM lane only, and those lanes are not read.
@@ -236,13 +153,15 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
     bool ok = true;
     for (int tile = blockIdx.x / split; tile < tiles && ok; tile += step) {
       for (int kb = kb0; kb < kb1; ++kb) {
-        ok = mbar_wait(&acc_empty[t], acc_phase) && mbar_wait(&full[s], phase);
+        ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[t], acc_phase) && mbar_wait(&full[s], phase));
         if (!ok) break;
         tc_fence_after();
         const uint64_t da = a_desc + (uint32_t)s * (a_bytes >> 4), db = b_desc + (uint32_t)s * (kBBytes >> 4);
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < kBK / 32; ++kk) tc_mma_e4m3(tmem + t * BN, da + 2 * kk, db + 2 * kk, idesc, kk != 0);
-        tc_commit(&done[s]);
+          for (int kk = 0; kk < kBK / 32; ++kk) tc_mma_e4m3(tmem + t * BN, da + 2 * kk, db + 2 * kk, idesc, kk != 0);
+          tc_commit(&done[s]);
+        }
         if (++s == a.stages) {
           s = 0;
           phase ^= 1;
@@ -428,9 +347,9 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// Tensor map of a row-major byte matrix [rows, cols] in boxes of box_rows x 128;
-// reads past an edge give zeros.
-int make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t row_stride, uint32_t box_rows) {
+}  // namespace
+
+int fp8_tensor_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t row_stride, uint32_t box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return set_error(AIOSB_ERR_LAUNCH, "cuTensorMapEncodeTiled unavailable");
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
@@ -444,44 +363,27 @@ int make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64
   return AIOSB_OK;
 }
 
+namespace {
+
 template <int BN>
 int launch(const CUtensorMap& tx, const CUtensorMap& tw, Fp8LinearArgs a, cudaStream_t stream) {
   constexpr int kOne = 224 * 1024;  // shared memory of a CTA that has the SM to itself
-  constexpr int kScaleBytes = Shape<BN>::kScaleBytes;
   constexpr int kCtas = Shape<BN>::kCtas, kBudget = kCtas == 2 ? kOne / 2 - 1024 : kOne;
+  constexpr int kScaleBytes = Shape<BN>::kScaleBytes;
   auto kern = linear_fp8_kernel<BN>;
   static bool configured[64] = {false};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBudget);
-    if (e != cudaSuccess) return set_error(AIOSB_ERR_LAUNCH, "linear_fp8: %s", cudaGetErrorString(e));
-    if (dev >= 0 && dev < 64) configured[dev] = true;
-  }
+  const int rc = fp8_configure(kern, kBudget, configured);
+  if (rc != AIOSB_OK) return rc;
   const int stage_bytes = a.a_rows * kBK + BN * kBK;
-  const int tiles = a.m_tiles * a.n_tiles;
-  const int per_cta = (a.kblocks + a.split - 1) / a.split * (a.split > 1 ? 1 : (tiles + sm_count() * kCtas - 1) / (sm_count() * kCtas));
-  a.stages = std::max(Shape<BN>::kAccs, std::min({(kBudget - 1024 - kScaleBytes) / stage_bytes, kMaxStages, per_cta}));
-  // at least the partial tile, and 16 KB past the last A slot (two B slots have that)
+  const int tiles = a.m_tiles * a.n_tiles, slots = sm_count() * kCtas;
+  const int per_cta = (a.kblocks + a.split - 1) / a.split * (a.split > 1 ? 1 : (tiles + slots - 1) / slots);
+  a.stages = std::max(Shape<BN>::kAccs,
+                      std::min({(kBudget - 1024 - kScaleBytes) / stage_bytes, kMaxStages, per_cta}));
+  // at least the partial tile, and 16 KB past the last A slot (the B slots have that)
   const int body = std::max(a.stages * stage_bytes, a.split > 1 ? a.a_rows * (BN + 4) * 4 : 0);
   a.scale_offset = body + 1024;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.split > 1 ? tiles * a.split : std::min(tiles, sm_count() * kCtas)));
-  cfg.blockDim = dim3(Shape<BN>::kThreads);
-  cfg.dynamicSmemBytes = (size_t)body + 1024 + kScaleBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)a.split;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tx, tw, a);
-  if (e != cudaSuccess) return set_error(AIOSB_ERR_LAUNCH, "linear_fp8: %s", cudaGetErrorString(e));
-  return AIOSB_OK;
+  return fp8_launch(kern, a.split > 1 ? tiles * a.split : std::min(tiles, slots), Shape<BN>::kThreads,
+                    body + 1024 + kScaleBytes, a.split, stream, tx, tw, a);
 }
 
 }  // namespace
@@ -528,6 +430,7 @@ extern "C" int aiosb_linear_fp8(const void* x, int64_t x_row_stride, const float
   a.a_rows = (int)std::min<int64_t>(kBM, (rows + 7) / 8 * 8);
   a.split = 1;
   a.status = status;
+  if (rows <= 64) return fp8_linear_few(x, x_row_stride, k, w, a, as_stream(stream));
   // The widest tile that still gives every SM one: a wide tile reads x and the weight
   // from L2 fewer times. Where none does, the narrowest, and k split until the grid
   // covers the SMs.
@@ -543,8 +446,8 @@ extern "C" int aiosb_linear_fp8(const void* x, int64_t x_row_stride, const float
   while (a.split < kMaxSplit && a.split * 2 <= a.kblocks && (int64_t)a.m_tiles * a.n_tiles * a.split < sms)
     a.split *= 2;
   CUtensorMap tx, tw;
-  int rc = make_map(&tx, x, rows, k, x_row_stride, (uint32_t)a.a_rows);
-  if (rc == AIOSB_OK) rc = make_map(&tw, w, n, k, k, (uint32_t)bn);
+  int rc = fp8_tensor_map(&tx, x, rows, k, x_row_stride, (uint32_t)a.a_rows);
+  if (rc == AIOSB_OK) rc = fp8_tensor_map(&tw, w, n, k, k, (uint32_t)bn);
   if (rc != AIOSB_OK) return rc;
   cudaStream_t s = as_stream(stream);
   return bn == 256 ? launch<256>(tx, tw, a, s) : bn == 128 ? launch<128>(tx, tw, a, s) : launch<64>(tx, tw, a, s);

@@ -1,0 +1,148 @@
+// Shared by the 8-bit linear kernels: arguments, the tcgen05 / TMA / mbarrier pieces that
+// only they use, and the epilogue's store.
+#pragma once
+
+#include "abi_util.h"
+#include "fp8.cuh"
+
+namespace aiosb {
+
+constexpr int kBM = 128;                      // tokens per tile (UMMA M, TMEM lanes)
+constexpr int kBK = kFp8Block;                // bytes of k per stage: one scale block, one swizzle row
+constexpr int kMaxStages = 16;
+constexpr int kMaxSplit = 8;
+constexpr int kScaleGroup = 8;
+
+struct Fp8LinearArgs {
+  const float* x_scale;  // [rows, kblocks]
+  const float* w_scale;  // [ceil(n / 128), kblocks]
+  __nv_bfloat16* y;
+  const __nv_bfloat16* residual;  // or NULL
+  int64_t y_stride, residual_stride;
+  int rows, n, kblocks;
+  int m_tiles, n_tiles;
+  int split;
+  int stages;
+  int scale_offset;  // of the scale products, bytes from the start of dynamic shared memory
+  int a_rows;  // token rows a stage holds: rows, rounded up to the swizzle's 8, at most 128
+  int32_t* status;
+};
+
+__device__ __forceinline__ void tc_mma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Instruction descriptor: fp32 accumulator, e4m3 A and B (format 0), both K-major.
+__host__ __device__ constexpr uint32_t umma_idesc_e4m3(int M, int N) {
+  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// 32 lanes x 16 or 32 consecutive columns; the values are there after tmem_wait.
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                 "+r"(r[15])::"memory");
+}
+// Waits for this thread's tensor-memory loads; naming the registers keeps their
+// uses behind the wait.
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                 "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                 "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                 "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+
+// Eight finished sums of one row to bf16, the residual added in fp32 (one rounding).
+__device__ __forceinline__ void store8(const Fp8LinearArgs& a, int64_t row, int col, const float (&v)[8]) {
+  float o[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j] = v[j];
+  if (a.residual != nullptr) {
+    float r[8];
+    unpack8(*reinterpret_cast<const uint4*>(a.residual + row * a.residual_stride + col), r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] += r[j];
+  }
+  *reinterpret_cast<uint4*>(a.y + row * a.y_stride + col) =
+      make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// ---- host side -------------------------------------------------------------------
+// Tensor map of a row-major byte matrix [rows, cols] in boxes of box_rows x 128; reads
+// past an edge give zeros.
+int fp8_tensor_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t row_stride,
+                   uint32_t box_rows);
+
+// Opts `kern` into `bytes` of dynamic shared memory once per device.
+template <typename Kern>
+int fp8_configure(Kern kern, int bytes, bool (&configured)[64]) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return set_error(AIOSB_ERR_LAUNCH, "linear_fp8: %s", cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  return AIOSB_OK;
+}
+
+// Launches with programmatic dependent launch, in clusters of `cluster` CTAs along x.
+template <typename Kern>
+int fp8_launch(Kern kern, int grid, int threads, int smem, int cluster, cudaStream_t stream, const CUtensorMap& tx,
+               const CUtensorMap& tw, const Fp8LinearArgs& a) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tx, tw, a);
+  if (e != cudaSuccess) return set_error(AIOSB_ERR_LAUNCH, "linear_fp8: %s", cudaGetErrorString(e));
+  return AIOSB_OK;
+}
+
+// Few token rows: the weight is the M operand (fp8_linear_few.cu).
+int fp8_linear_few(const void* x, int64_t x_row_stride, int64_t k, const void* w, Fp8LinearArgs a,
+                   cudaStream_t stream);
+
+}  // namespace aiosb

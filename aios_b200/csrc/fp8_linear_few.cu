@@ -1,0 +1,303 @@
+// The 8-bit linear for few token rows (decode): bound by the weight's bytes.
+//
+// The weight is the UMMA M operand (128 features per tile) and the tokens the N operand
+// (16, 32 or 64 columns), so an MMA's time follows the token count: with the tokens as
+// M, a decode step's MMAs would run at the speed of 128 rows. A TMEM lane is a feature,
+// a column a token: the fold's scale is one product per column, the same for every lane,
+// read from shared memory four at a time. Otherwise as fp8_linear.cu: a ring of TMA
+// stages, four accumulators in turn, the products sx * sw formed eight blocks of k ahead
+// by a warp of their own, and k split over a cluster whose partial tiles are summed in
+// rank order.
+#include <algorithm>
+
+#include "fp8_linear.cuh"
+
+namespace aiosb {
+namespace {
+
+template <int TN>
+struct Few {
+  static constexpr int kCols = TN < 32 ? TN : 32;      // tokens of one fold warp
+  static constexpr int kFoldWarps = 4 * (TN / kCols);  // 4 groups of 32 TMEM lanes
+  static constexpr int kThreads = (kFoldWarps + 4) * 32;
+  static constexpr int kAccs = 4;
+  static constexpr int kTmemCols = kAccs * TN;         // 64, 128 or 256: two CTAs per SM
+  static constexpr int kScaleBytes = 2 * kScaleGroup * TN * 4;
+  static constexpr int kStageBytes = (kBM + TN) * kBK;
+};
+constexpr int kRedStride = kBM + 4;  // floats per token of the partial tile
+
+template <int TN>
+__global__ void __launch_bounds__(Few<TN>::kThreads, 2)
+    linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                          const Fp8LinearArgs a) {
+  using S = Few<TN>;
+  constexpr int kCols = S::kCols, kFoldWarps = S::kFoldWarps, kAccs = S::kAccs;
+  constexpr uint32_t kWBytes = kBM * kBK;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full[kMaxStages], done[kMaxStages], acc_empty[kAccs], scale_full[2], scale_empty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+  float* const scales = reinterpret_cast<float*>(smem_raw + a.scale_offset);  // [2][kScaleGroup][TN]
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&done[s], 1);
+    }
+    for (int s = 0; s < kAccs; ++s) mbar_init(&acc_empty[s], kFoldWarps);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&scale_full[s], 1);
+      mbar_init(&scale_empty[s], kFoldWarps);
+    }
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == kFoldWarps + 1) {
+    tmem_alloc(&tmem_slot, S::kTmemCols);
+    tmem_relinquish();
+  }
+  if (warp == kFoldWarps && elect_one()) {
+    tma_prefetch_desc(&tm_x);
+    tma_prefetch_desc(&tm_w);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();  // after the wait: whoever follows may rely on this kernel's predecessors being done
+
+  // m tiles are features, n tiles tokens; the token tiles of one feature tile are
+  // neighbours, so that the second reads the weight from L2
+  const int split = a.split, rank = blockIdx.x % split, tile = blockIdx.x / split;
+  const int kb0 = (int)((int64_t)a.kblocks * rank / split), kb1 = (int)((int64_t)a.kblocks * (rank + 1) / split);
+  const int f0 = tile / a.n_tiles * kBM, t0 = tile % a.n_tiles * TN;
+
+  if (warp == kFoldWarps) {
+    // ---- TMA producer
+    int s = 0, issued = 0;
+    uint32_t phase = 1;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&done[s], phase));
+      if (!ok) break;
+      if (elect_one()) {
+        uint8_t* const dst = smem + s * S::kStageBytes;
+        mbar_arrive_expect_tx(&full[s], S::kStageBytes);
+        tma_load_2d(dst, &tm_w, &full[s], kb * kBK, f0);
+        tma_load_2d(dst + kWBytes, &tm_x, &full[s], kb * kBK, t0);
+      }
+      issued = min(issued + 1, a.stages);
+      if (++s == a.stages) {
+        s = 0;
+        phase ^= 1;
+      }
+    }
+    if (!ok) {  // let the copies that are still in flight land before this CTA returns
+      report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
+      abort_flag = 1;
+      for (; issued > 0; --issued) {
+        if (--s < 0) {
+          s = a.stages - 1;
+          phase ^= 1;
+        }
+        mbar_wait(&full[s], phase ^ 1);
+      }
+    }
+  } else if (warp == kFoldWarps + 1) {
+    // ---- MMA issuer
+    constexpr uint32_t idesc = umma_idesc_e4m3(kBM, TN);
+    const uint64_t w_desc = umma_desc_sw128(smem_u32(smem)), x_desc = umma_desc_sw128(smem_u32(smem + kWBytes));
+    int s = 0, t = 0;
+    uint32_t phase = 0, acc_phase = 1;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[t], acc_phase) && mbar_wait(&full[s], phase));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t off = (uint32_t)s * (S::kStageBytes >> 4);
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < kBK / 32; ++kk)
+          tc_mma_e4m3(tmem + t * TN, w_desc + off + 2 * kk, x_desc + off + 2 * kk, idesc, kk != 0);
+        tc_commit(&done[s]);
+      }
+      if (++s == a.stages) {
+        s = 0;
+        phase ^= 1;
+      }
+      if (++t == kAccs) {
+        t = 0;
+        acc_phase ^= 1;
+      }
+    }
+    if (!ok) {
+      report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
+      abort_flag = 1;
+    }
+  } else if (warp == kFoldWarps + 2) {
+    // ---- scale products, a group of blocks of k at a time; lane l has tokens l + 32 i
+    constexpr int kPer = (TN + 31) / 32;
+    const float* sx[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) sx[i] = a.x_scale + (int64_t)min(t0 + i * 32 + lane, a.rows - 1) * a.kblocks;
+    const float* const sw = a.w_scale + (int64_t)(f0 / kFp8Block) * a.kblocks;
+    int g = 0;
+    uint32_t phase = 1;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; kb += kScaleGroup) {
+      float x[kPer][kScaleGroup], w[kScaleGroup];
+#pragma unroll
+      for (int j = 0; j < kScaleGroup; ++j) {
+        const bool in = kb + j < kb1;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) x[i][j] = in ? sx[i][kb + j] : 0.f;
+        w[j] = in ? sw[kb + j] : 0.f;
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait(&scale_empty[g], phase));
+      if (!ok) break;
+#pragma unroll
+      for (int j = 0; j < kScaleGroup; ++j) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (TN >= 32 || lane < TN) scales[(g * kScaleGroup + j) * TN + i * 32 + lane] = x[i][j] * w[j];
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&scale_full[g]);
+      g ^= 1;
+      if (g == 0) phase ^= 1;
+    }
+    if (!ok) {
+      report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
+      abort_flag = 1;
+    }
+  } else if (warp < kFoldWarps) {
+    // ---- fold: acc[token] += (sx * sw)[token] * d[token] per block of k
+    const int part = warp >> 2;
+    const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(part * kCols);
+    const float* const my_scales = scales + part * kCols;
+    float2 acc[kCols / 2];
+#pragma unroll
+    for (int j = 0; j < kCols / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+    int ring = 0, t = 0, g = 0, in_group = 0;
+    uint32_t phase = 0, g_phase = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      ok = (in_group != 0 || mbar_wait(&scale_full[g], g_phase)) && mbar_wait(&done[ring], phase);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t d[kCols];
+      tmem_ld(t_lane + t * TN, d);
+      float4 s[kCols / 4];
+#pragma unroll
+      for (int j = 0; j < kCols / 4; ++j)
+        s[j] = *reinterpret_cast<const float4*>(my_scales + (g * kScaleGroup + in_group) * TN + 4 * j);
+      tmem_wait(d);
+      tc_fence_before();
+      if (lane == 0) mbar_arrive(&acc_empty[t]);
+#pragma unroll
+      for (int j = 0; j < kCols / 4; ++j) {
+        acc[2 * j] = __ffma2_rn(make_float2(s[j].x, s[j].y),
+                                make_float2(__uint_as_float(d[4 * j]), __uint_as_float(d[4 * j + 1])), acc[2 * j]);
+        acc[2 * j + 1] =
+            __ffma2_rn(make_float2(s[j].z, s[j].w),
+                       make_float2(__uint_as_float(d[4 * j + 2]), __uint_as_float(d[4 * j + 3])), acc[2 * j + 1]);
+      }
+      if (++in_group == kScaleGroup) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&scale_empty[g]);
+        in_group = 0;
+        g ^= 1;
+        if (g == 0) g_phase ^= 1;
+      }
+      if (++ring == a.stages) {
+        ring = 0;
+        phase ^= 1;
+      }
+      if (++t == kAccs) t = 0;
+    }
+    if (ok) {
+      // every MMA of this CTA has read its operands: the partial tile takes their place
+      float* const red = reinterpret_cast<float*>(smem) + part * kCols * kRedStride + (warp & 3) * 32 + lane;
+#pragma unroll
+      for (int j = 0; j < kCols / 2; ++j) {
+        red[(2 * j) * kRedStride] = acc[j].x;
+        red[(2 * j + 1) * kRedStride] = acc[j].y;
+      }
+    } else {
+      report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
+      abort_flag = 1;
+    }
+  }
+
+  __syncwarp();
+  __syncthreads();
+  if (split > 1) cluster_sync();
+  // Rank r sums and stores every split-th group of 8 features of a token, in rank order.
+  if (!abort_flag) {
+    const uint32_t base = smem_u32(smem);
+    const int live = min(a.rows - t0, TN);
+    for (int u = threadIdx.x * split + rank; u < live * (kBM / 8); u += S::kThreads * split) {
+      const int r = u / (kBM / 8), c = u % (kBM / 8) * 8;
+      if (f0 + c >= a.n) continue;
+      const uint32_t off = base + (uint32_t)(r * kRedStride + c) * 4;
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      for (int p = 0; p < split; ++p) {
+        const uint32_t at = split > 1 ? map_shared_rank(off, (uint32_t)p) : off;
+        const float4 lo = ld_dsmem_f4(at), hi = ld_dsmem_f4(at + 16);
+        v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w;
+        v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
+      }
+      store8(a, t0 + r, f0 + c, v);
+    }
+  }
+  if (split > 1) cluster_sync();  // peers may still read this CTA's partial tile
+  if (warp == kFoldWarps + 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, S::kTmemCols);
+  }
+}
+
+template <int TN>
+int launch_few(const void* x, int64_t x_row_stride, int64_t k, const void* w, Fp8LinearArgs a, cudaStream_t stream) {
+  using S = Few<TN>;
+  constexpr int kBudget = 111 * 1024;  // two CTAs per SM
+  auto kern = linear_fp8_few_kernel<TN>;
+  static bool configured[64] = {false};
+  int rc = fp8_configure(kern, kBudget, configured);
+  if (rc != AIOSB_OK) return rc;
+  a.m_tiles = (a.n + kBM - 1) / kBM;
+  a.n_tiles = (a.rows + TN - 1) / TN;
+  const int tiles = a.m_tiles * a.n_tiles;
+  // Split k where the tiles leave SMs idle, but only a k long enough: a block of k costs a
+  // lone CTA about 0.18 us, the cluster's barriers and reduction 1.2 us together (8 x 768,
+  // 16 blocks: 5.97 us whole, 4.70 in 4, 4.52 in 8; 8 x 1280, 6 blocks: 3.76 whole, 4.44
+  // in 6). One CTA to an SM streams the weight as fast as two.
+  a.split = 1;
+  while (a.kblocks > 10 && a.split < kMaxSplit && a.kblocks >= 4 * a.split && tiles * a.split * 2 <= sm_count())
+    a.split *= 2;
+  const int per_cta = (a.kblocks + a.split - 1) / a.split;
+  a.stages = std::max(S::kAccs, std::min({(kBudget - 1024 - S::kScaleBytes) / S::kStageBytes, kMaxStages, per_cta}));
+  const int body = std::max(a.stages * S::kStageBytes, TN * kRedStride * 4);
+  a.scale_offset = body + 1024;
+  CUtensorMap tx, tw;
+  rc = fp8_tensor_map(&tx, x, a.rows, k, x_row_stride, TN);
+  if (rc == AIOSB_OK) rc = fp8_tensor_map(&tw, w, a.n, k, k, kBM);
+  if (rc != AIOSB_OK) return rc;
+  return fp8_launch(kern, tiles * a.split, S::kThreads, body + 1024 + S::kScaleBytes, a.split, stream, tx, tw, a);
+}
+
+}  // namespace
+
+int fp8_linear_few(const void* x, int64_t x_row_stride, int64_t k, const void* w, Fp8LinearArgs a,
+                   cudaStream_t stream) {
+  if (a.rows <= 16) return launch_few<16>(x, x_row_stride, k, w, a, stream);
+  if (a.rows <= 32) return launch_few<32>(x, x_row_stride, k, w, a, stream);
+  return launch_few<64>(x, x_row_stride, k, w, a, stream);
+}
+
+}  // namespace aiosb
