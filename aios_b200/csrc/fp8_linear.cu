@@ -431,6 +431,8 @@ extern "C" int aiosb_linear_fp8(const void* x, int64_t x_row_stride, const float
   a.split = 1;
   a.status = status;
   if (rows <= 64) return fp8_linear_few(x, x_row_stride, k, w, a, as_stream(stream));
+  if ((int64_t)((rows + 255) / 256) * ((n + 255) / 256) >= 60)
+    return fp8_linear_pair(x, x_row_stride, k, w, a, as_stream(stream));
   // The widest tile that still gives every SM one: a wide tile reads x and the weight
   // from L2 fewer times. Where none does, the narrowest, and k split until the grid
   // covers the SMs.

@@ -141,6 +141,9 @@ int fp8_launch(Kern kern, int grid, int threads, int smem, int cluster, cudaStre
   return AIOSB_OK;
 }
 
+// Many token rows: two CTAs share a 256 x 256 tile (fp8_linear_pair.cu).
+int fp8_linear_pair(const void* x, int64_t x_row_stride, int64_t k, const void* w, Fp8LinearArgs a,
+                    cudaStream_t stream);
 // Few token rows: the weight is the M operand (fp8_linear_few.cu).
 int fp8_linear_few(const void* x, int64_t x_row_stride, int64_t k, const void* w, Fp8LinearArgs a,
                    cudaStream_t stream);
