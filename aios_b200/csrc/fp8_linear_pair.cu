@@ -6,8 +6,13 @@
 // reads 48 KB, which is what bounded that form. The even CTA issues every MMA; each CTA
 // holds the accumulators of its own tokens (lane = token) and folds them as in
 // fp8_linear.cu, 16 warps of 64 columns each. The grid is one pair per two SMs and walks
-// the tiles; two accumulators let the MMAs of the next blocks, or of the next tile, run
-// while a block is folded or a tile stored.
+// the tiles.
+//
+// An accumulator is busy from its first MMA to the last read of its fold, commit and
+// barrier latencies included, and tensor memory holds two of 256 columns: taken whole,
+// they left the tensor cores waiting half of the time. So a block's product is formed as
+// two halves of 128 features, each with two accumulators and its own 8 fold warps: while
+// one half is read the other half's MMAs run.
 //
 // Finished rows go through shared memory (one 128-byte row piece per lane in, whole lines
 // out); a residual is fetched into the same place by asynchronous copies issued at the
@@ -23,7 +28,9 @@ constexpr int kBN = 256;           // features per pair tile
 constexpr int kCols = 64;          // columns of one fold warp
 constexpr int kFoldWarps = 16;     // 4 groups of 32 TMEM lanes x 4 column parts
 constexpr int kThreads = (kFoldWarps + 4) * 32;
-constexpr int kAccs = 2;           // x 256 columns: all of tensor memory
+constexpr int kAccs = 2;           // of each 128-feature half: all of tensor memory
+constexpr int kHalf = kBN / 2;     // features of a half; each CTA stages 64 weight rows of it
+constexpr uint32_t kHalfBytes = kHalf / 2 * kBK;
 constexpr int kPairStages = 4;
 constexpr int kWBlocks = kBN / kFp8Block;
 constexpr uint32_t kABytes = kBM * kBK, kBBytes = kBN / 2 * kBK, kStageBytes = kABytes + kBBytes;
@@ -72,8 +79,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                            const Fp8LinearArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  // full, acc_empty: the even CTA's are used; done, scale_*: each CTA's own
-  __shared__ uint64_t full[kPairStages], done[kPairStages], acc_empty[kAccs], scale_full[2], scale_empty[2];
+  // full, acc_empty: the even CTA's are used; the others each CTA's own. done[h][s]: half h
+  // of the block in stage s is in TMEM; with h = 1 the stage's operands are read, too
+  __shared__ uint64_t full[kPairStages], done[2][kPairStages], acc_empty[2 * kAccs], scale_full[2], scale_empty[2];
   __shared__ uint32_t tmem_slot;
   float* const scales = reinterpret_cast<float*>(smem + kScaleOffset);
 
@@ -82,9 +90,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < kPairStages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&done[s], 1);
+      mbar_init(&done[0][s], 1);
+      mbar_init(&done[1][s], 1);
     }
-    for (int s = 0; s < kAccs; ++s) mbar_init(&acc_empty[s], 2 * kFoldWarps);
+    for (int s = 0; s < 2 * kAccs; ++s) mbar_init(&acc_empty[s], kFoldWarps);  // half of the warps, of two CTAs
     for (int s = 0; s < 2; ++s) {
       mbar_init(&scale_full[s], 1);
       mbar_init(&scale_empty[s], kFoldWarps);
@@ -130,14 +139,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       int m0, n0;
       place(tile, &m0, &n0);
       for (int kb = 0; kb < kblocks; ++kb) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&done[s], phase));
+        ok = __all_sync(0xffffffffu, mbar_wait(&done[1][s], phase));
         if (!ok) break;
         if (elect_one()) {
           uint8_t* const dst = smem + s * kStageBytes;
           const uint32_t bar = map_shared_rank(smem_u32(&full[s]), 0);
           if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kStageBytes);
           tma_load_2d_pair(dst, &tm_x, bar, kb * kBK, m0);
-          tma_load_2d_pair(dst + kABytes, &tm_w, bar, kb * kBK, n0 + (int)rank * (kBN / 2));
+          tma_load_2d_pair(dst + kABytes, &tm_w, bar, kb * kBK, n0 + (int)rank * (kHalf / 2));
+          tma_load_2d_pair(dst + kABytes + kHalfBytes, &tm_w, bar, kb * kBK, n0 + kHalf + (int)rank * (kHalf / 2));
         }
         issued = min(issued + 1, kPairStages);
         if (++s == kPairStages) {
@@ -156,25 +166,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == kFoldWarps + 1) {
-    // ---- MMA issuer (even CTA). One commit per block tells both CTAs that the stage's
-    // operands are read and that the product is in TMEM; an accumulator waits for the
-    // folds of both CTAs, so neither falls a whole ring of stages behind.
+    // ---- MMA issuer (even CTA). A half's accumulator waits for the folds of both CTAs, so
+    // neither falls a whole ring of stages behind the done[] phases.
     if (rank == 0) {
-      constexpr uint32_t idesc = umma_idesc_e4m3(2 * kBM, kBN);
+      constexpr uint32_t idesc = umma_idesc_e4m3(2 * kBM, kHalf);
       const uint64_t a_desc = umma_desc_sw128(smem_u32(smem)), b_desc = umma_desc_sw128(smem_u32(smem + kABytes));
       int s = 0, t = 0;
       uint32_t phase = 0, acc_phase = 1;
       for (int tile = first; tile < tiles && ok; tile += step) {
-        for (int kb = 0; kb < kblocks; ++kb) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[t], acc_phase) && mbar_wait(&full[s], phase));
+        for (int kb = 0; kb < kblocks && ok; ++kb) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&full[s], phase));
           if (!ok) break;
-          tc_fence_after();
           const uint32_t off = (uint32_t)s * (kStageBytes >> 4);
-          if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < kBK / 32; ++kk)
-              tc_mma_e4m3_pair(tmem + t * kBN, a_desc + off + 2 * kk, b_desc + off + 2 * kk, idesc, kk != 0);
-            tc_commit_pair(&done[s]);
+          for (int h = 0; h < 2; ++h) {
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(&acc_empty[2 * t + h], acc_phase));
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < kBK / 32; ++kk)
+                tc_mma_e4m3_pair(tmem + (2 * t + h) * kHalf, a_desc + off + 2 * kk,
+                                 b_desc + off + h * (kHalfBytes >> 4) + 2 * kk, idesc, kk != 0);
+              tc_commit_pair(&done[h][s]);
+            }
           }
           if (++s == kPairStages) {
             s = 0;
@@ -230,10 +245,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp < kFoldWarps) {
     // ---- fold and store
     const int part = warp >> 2, lane_group = warp & 3;
+    const int half = part >> 1;
     const uint32_t t_lane = tmem + ((uint32_t)(lane_group * 32) << 16) + (uint32_t)(part * kCols);
     const float* const my_scales = scales + part * kCols / kFp8Block * kBM + lane_group * 32 + lane;
     uint8_t* const out = smem + kOutOffset + warp * kOutWarpBytes;
-    const uint32_t acc_bar = map_shared_rank(smem_u32(&acc_empty[0]), 0);
+    const uint32_t acc_bar = map_shared_rank(smem_u32(&acc_empty[half]), 0);
     int ring = 0, t = 0, g = 0;
     uint32_t phase = 0, g_phase = 0;
     for (int tile = first; tile < tiles && ok; tile += step) {
@@ -259,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = 0; j < kCols / 2; ++j) acc[j] = make_float2(0.f, 0.f);
       int in_group = 0;
       for (int kb = 0; kb < kblocks; ++kb) {
-        ok = (in_group != 0 || mbar_wait(&scale_full[g], g_phase)) && mbar_wait(&done[ring], phase);
+        ok = (in_group != 0 || mbar_wait(&scale_full[g], g_phase)) && mbar_wait(&done[half][ring], phase);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
@@ -280,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (c + 16 == kCols) {  // this block's values are in registers: the accumulator may be reused
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(acc_bar + t * 8);
+            if (lane == 0) mbar_arrive_cluster(acc_bar + t * 16);
           }
 #pragma unroll
           for (int j = 0; j < 8; ++j)
@@ -344,7 +360,7 @@ int fp8_linear_pair(const void* x, int64_t x_row_stride, int64_t k, const void* 
   a.n_tiles = (a.n + kBN - 1) / kBN;
   CUtensorMap tx, tw;
   rc = fp8_tensor_map(&tx, x, a.rows, k, x_row_stride, kBM);
-  if (rc == AIOSB_OK) rc = fp8_tensor_map(&tw, w, a.n, k, k, kBN / 2);
+  if (rc == AIOSB_OK) rc = fp8_tensor_map(&tw, w, a.n, k, k, kHalf / 2);
   if (rc != AIOSB_OK) return rc;
   const int pairs = std::min(a.m_tiles * a.n_tiles, std::max(1, sm_count() / 2));
   return fp8_launch(linear_fp8_pair_kernel, 2 * pairs, kThreads, (int)kSmemBytes, 2, stream, tx, tw, a);
