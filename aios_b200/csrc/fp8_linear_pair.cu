@@ -5,16 +5,16 @@
 // so a block of k costs 32 KB of L2 reads per SM where a CTA alone with a 128 x 256 tile
 // reads 48 KB, which is what bounded that form. The even CTA issues every MMA; each CTA
 // holds the accumulators of its own tokens (lane = token) and folds them as in
-// fp8_linear.cu, 16 warps of 64 columns each. The grid is one pair per two SMs and walks
+// fp8_linear.cu, 8 warps of 128 columns each. The grid is one pair per two SMs and walks
 // the tiles.
 //
 // An accumulator is busy from its first MMA to the last read of its fold, commit and
 // barrier latencies included, and tensor memory holds two of 256 columns: taken whole,
 // they left the tensor cores waiting half of the time. So a block's product is formed as
-// two halves of 128 features, each with two accumulators and its own 8 fold warps: while
+// two halves of 128 features, each with two accumulators and its own 4 fold warps: while
 // one half is read the other half's MMAs run.
 //
-// Finished rows go through shared memory (one 128-byte row piece per lane in, whole lines
+// Finished rows go through shared memory (one 256-byte row piece per lane in, whole lines
 // out); a residual is fetched into the same place by asynchronous copies issued at the
 // tile's start.
 #include <algorithm>
@@ -25,8 +25,8 @@ namespace aiosb {
 namespace {
 
 constexpr int kBN = 256;           // features per pair tile
-constexpr int kCols = 64;          // columns of one fold warp
-constexpr int kFoldWarps = 16;     // 4 groups of 32 TMEM lanes x 4 column parts
+constexpr int kCols = 128;         // columns of one fold warp
+constexpr int kFoldWarps = 8;      // 4 groups of 32 TMEM lanes x 2 halves of the features
 constexpr int kThreads = (kFoldWarps + 4) * 32;
 constexpr int kAccs = 2;           // of each 128-feature half: all of tensor memory
 constexpr int kHalf = kBN / 2;     // features of a half; each CTA stages 64 weight rows of it
@@ -244,10 +244,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp < kFoldWarps) {
     // ---- fold and store
-    const int part = warp >> 2, lane_group = warp & 3;
-    const int half = part >> 1;
-    const uint32_t t_lane = tmem + ((uint32_t)(lane_group * 32) << 16) + (uint32_t)(part * kCols);
-    const float* const my_scales = scales + part * kCols / kFp8Block * kBM + lane_group * 32 + lane;
+    const int half = warp >> 2, lane_group = warp & 3;
+    const uint32_t t_lane = tmem + ((uint32_t)(lane_group * 32) << 16) + (uint32_t)(half * kHalf);
+    const float* const my_scales = scales + half * kBM + lane_group * 32 + lane;
     uint8_t* const out = smem + kOutOffset + warp * kOutWarpBytes;
     const uint32_t acc_bar = map_shared_rank(smem_u32(&acc_empty[half]), 0);
     int ring = 0, t = 0, g = 0;
@@ -255,18 +254,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int tile = first; tile < tiles && ok; tile += step) {
       int m0, n0;
       place(tile, &m0, &n0);
-      const int r0 = m0 + lane_group * 32, c0 = n0 + part * kCols;
-      // 16-byte piece `chunk` of row `row` of this warp's 32 x 64 outputs, the pieces of a
+      const int r0 = m0 + lane_group * 32, c0 = n0 + half * kCols;
+      // 16-byte piece `chunk` of row `row` of this warp's 32 x 128 outputs, the pieces of a
       // row permuted by the row so that both directions are free of bank conflicts
-      const int chunk = lane & 7;
+      const int chunk = lane & 15;
       const bool col_in = c0 + chunk * 8 < a.n;
       if (a.residual != nullptr) {
         __syncwarp();  // the previous tile's rows have been read out
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int row = i * 4 + (lane >> 3);
+        for (int i = 0; i < 16; ++i) {
+          const int row = i * 2 + (lane >> 4);
           if (col_in && r0 + row < a.rows)
-            cp_async16(out + row * 128 + ((chunk ^ (row & 7)) << 4),
+            cp_async16(out + row * 256 + ((chunk ^ (row & 7)) << 4),
                        a.residual + (int64_t)(r0 + row) * a.residual_stride + c0 + chunk * 8);
         }
       }
@@ -288,20 +287,25 @@ __global__ void __launch_bounds__(kThreads, 1)
           g ^= 1;
           if (g == 0) g_phase ^= 1;
         }
+        // the next 32 columns are on their way while 32 are folded
+        uint32_t d[2][32];
+        tmem_ld(t_lane + t * kBN, d[0]);
+        tmem_wait(d[0]);
 #pragma unroll
-        for (int c = 0; c < kCols; c += 16) {
-          uint32_t d[16];
-          tmem_ld(t_lane + t * kBN + c, d);
-          tmem_wait(d);
-          if (c + 16 == kCols) {  // this block's values are in registers: the accumulator may be reused
+        for (int c = 0; c < kCols / 32; ++c) {
+          if (c + 1 < kCols / 32) {
+            tmem_ld(t_lane + t * kBN + (c + 1) * 32, d[(c + 1) & 1]);
+          } else {  // this block's values are in registers: the accumulator may be reused
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(acc_bar + t * 16);
           }
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            acc[c / 2 + j] = __ffma2_rn(s, make_float2(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1])),
-                                        acc[c / 2 + j]);
+          for (int j = 0; j < 16; ++j)
+            acc[c * 16 + j] = __ffma2_rn(
+                s, make_float2(__uint_as_float(d[c & 1][2 * j]), __uint_as_float(d[c & 1][2 * j + 1])),
+                acc[c * 16 + j]);
+          if (c + 1 < kCols / 32) tmem_wait(d[(c + 1) & 1]);
         }
         if (++ring == kPairStages) {
           ring = 0;
@@ -313,8 +317,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (a.residual != nullptr) cp_async_wait_all();
       __syncwarp();
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        uint4* const at = reinterpret_cast<uint4*>(out + lane * 128 + ((c ^ (lane & 7)) << 4));
+      for (int c = 0; c < 16; ++c) {
+        uint4* const at = reinterpret_cast<uint4*>(out + lane * 256 + ((c ^ (lane & 7)) << 4));
         float v[8] = {acc[4 * c].x,     acc[4 * c].y,     acc[4 * c + 1].x, acc[4 * c + 1].y,
                       acc[4 * c + 2].x, acc[4 * c + 2].y, acc[4 * c + 3].x, acc[4 * c + 3].y};
         if (a.residual != nullptr) {
@@ -328,11 +332,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int row = i * 4 + (lane >> 3);
+      for (int i = 0; i < 16; ++i) {
+        const int row = i * 2 + (lane >> 4);
         if (col_in && r0 + row < a.rows)
           *reinterpret_cast<uint4*>(a.y + (int64_t)(r0 + row) * a.y_stride + c0 + chunk * 8) =
-              *reinterpret_cast<const uint4*>(out + row * 128 + ((chunk ^ (row & 7)) << 4));
+              *reinterpret_cast<const uint4*>(out + row * 256 + ((chunk ^ (row & 7)) << 4));
       }
       __syncwarp();
     }
