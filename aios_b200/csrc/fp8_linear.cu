@@ -301,24 +301,16 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
   __syncthreads();
   if (split > 1) {
     cluster_sync();
-    // Rank r sums and stores every split-th group of 8 columns, in rank order.
+    // Rank r sums and stores every split-th row: a warp reads whole lines of its peers'
+    // partial tiles (16-byte pieces of many rows took four times as long).
     if (!abort_flag) {
       const int tile = blockIdx.x / split;
       const int m0 = tile % a.m_tiles * kBM, n0 = tile / a.m_tiles * BN;
       const uint32_t base = smem_u32(smem);
       const int live = min(a.rows - m0, kBM);
-      for (int u = threadIdx.x * split + rank; u < live * (BN / 8); u += kThreads * split) {
-        const int r = u / (BN / 8), c = u % (BN / 8) * 8;
-        if (n0 + c >= a.n) continue;
-        const uint32_t off = base + (uint32_t)(r * kRedStride + c) * 4;
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (int p = 0; p < split; ++p) {
-          const uint32_t at = map_shared_rank(off, (uint32_t)p);
-          const float4 lo = ld_dsmem_f4(at), hi = ld_dsmem_f4(at + 16);
-          v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w;
-          v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
-        }
-        store8(a, m0 + r, n0 + c, v);
+      for (int u = threadIdx.x; u < (live - rank + split - 1) / split * (BN / 4); u += kThreads) {
+        const int r = u / (BN / 4) * split + rank, c = u % (BN / 4) * 4;
+        if (n0 + c < a.n) store4(a, m0 + r, n0 + c, sum_ranks4(base + (uint32_t)(r * kRedStride + c) * 4, split));
       }
     }
     cluster_sync();  // peers may still read this CTA's partial tile

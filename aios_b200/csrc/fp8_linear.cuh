@@ -92,6 +92,39 @@ __device__ __forceinline__ void store8(const Fp8LinearArgs& a, int64_t row, int 
       make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
 }
 
+// Four finished sums of one row, as store8.
+__device__ __forceinline__ void store4(const Fp8LinearArgs& a, int64_t row, int col, float4 v) {
+  if (a.residual != nullptr) {
+    const uint2 r = *reinterpret_cast<const uint2*>(a.residual + row * a.residual_stride + col);
+    v.x += bf16_lo(r.x);
+    v.y += bf16_hi(r.x);
+    v.z += bf16_lo(r.y);
+    v.w += bf16_hi(r.y);
+  }
+  *reinterpret_cast<uint2*>(a.y + row * a.y_stride + col) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+}
+
+// Four neighbouring floats at shared-memory offset `off`, summed over the first `split`
+// CTAs of the cluster in rank order. Every rank's load is issued before the first sum: one
+// round trip to the peers, not one per rank.
+__device__ __forceinline__ float4 sum_ranks4(uint32_t off, int split) {
+  float4 part[kMaxSplit];
+#pragma unroll
+  for (int p = 0; p < kMaxSplit; ++p)
+    if (p < split) part[p] = ld_dsmem_f4(split > 1 ? map_shared_rank(off, (uint32_t)p) : off);
+  float4 v = part[0];
+#pragma unroll
+  for (int p = 1; p < kMaxSplit; ++p) {
+    if (p < split) {
+      v.x += part[p].x;
+      v.y += part[p].y;
+      v.z += part[p].z;
+      v.w += part[p].w;
+    }
+  }
+  return v;
+}
+
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;

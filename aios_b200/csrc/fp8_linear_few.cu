@@ -237,22 +237,14 @@ __global__ void __launch_bounds__(Few<TN>::kThreads, 2)
   __syncwarp();
   __syncthreads();
   if (split > 1) cluster_sync();
-  // Rank r sums and stores every split-th group of 8 features of a token, in rank order.
+  // Rank r sums and stores every split-th token: a warp reads whole lines of its peers'
+  // partial tiles (16-byte pieces of many tokens took four times as long).
   if (!abort_flag) {
     const uint32_t base = smem_u32(smem);
     const int live = min(a.rows - t0, TN);
-    for (int u = threadIdx.x * split + rank; u < live * (kBM / 8); u += S::kThreads * split) {
-      const int r = u / (kBM / 8), c = u % (kBM / 8) * 8;
-      if (f0 + c >= a.n) continue;
-      const uint32_t off = base + (uint32_t)(r * kRedStride + c) * 4;
-      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      for (int p = 0; p < split; ++p) {
-        const uint32_t at = split > 1 ? map_shared_rank(off, (uint32_t)p) : off;
-        const float4 lo = ld_dsmem_f4(at), hi = ld_dsmem_f4(at + 16);
-        v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w;
-        v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
-      }
-      store8(a, t0 + r, f0 + c, v);
+    for (int u = threadIdx.x; u < (live - rank + split - 1) / split * (kBM / 4); u += S::kThreads) {
+      const int r = u / (kBM / 4) * split + rank, c = u % (kBM / 4) * 4;
+      if (f0 + c < a.n) store4(a, t0 + r, f0 + c, sum_ranks4(base + (uint32_t)(r * kRedStride + c) * 4, split));
     }
   }
   if (split > 1) cluster_sync();  // peers may still read this CTA's partial tile
