@@ -35,10 +35,9 @@ struct Shape {
   static constexpr int kCols = BN == 64 ? 32 : 64;      // columns of one fold warp
   static constexpr int kFoldWarps = 4 * (BN / kCols);   // 4 groups of 32 TMEM lanes
   static constexpr int kThreads = (kFoldWarps + 4) * 32;
-  static constexpr int kAccs = BN == 256 ? 2 : 4;       // TMEM accumulators in turn
-  static constexpr int kWBlocks = BN == 256 ? 2 : 1;    // 128-wide weight blocks of the tile
-  // scale products: two groups of kScaleGroup blocks of k, [kWBlocks][128 rows] each
-  static constexpr int kScaleBytes = 2 * kScaleGroup * kWBlocks * kBM * 4;
+  static constexpr int kAccs = 4;                       // TMEM accumulators in turn
+  // scale products: two groups of kScaleGroup blocks of k, 128 rows each
+  static constexpr int kScaleBytes = 2 * kScaleGroup * kBM * 4;
   static constexpr int kCtas = BN == 64 ? 2 : 1;        // CTAs per SM (TMEM: kAccs * BN of 512 columns each)
 };
 
@@ -49,7 +48,6 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
   constexpr uint32_t kBBytes = BN * kBK;
   constexpr int kCols = Shape<BN>::kCols, kFoldWarps = Shape<BN>::kFoldWarps, kThreads = Shape<BN>::kThreads;
   constexpr int kAccs = Shape<BN>::kAccs;
-  constexpr int kWBlocks = Shape<BN>::kWBlocks;
   constexpr int kLd = BN == 128 ? 32 : 16;  // columns per tensor-memory load, by the registers a thread has
   constexpr int kRedStride = BN + 4;   // floats per row of the partial tile: conflict-free 16-byte accesses
   extern __shared__ uint8_t smem_raw[];
@@ -183,35 +181,27 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
     bool ok = true;
     for (int tile = blockIdx.x / split; tile < tiles && ok; tile += step) {
       const int m0 = tile % a.m_tiles * kBM, n0 = tile / a.m_tiles * BN;
-      const float *sx[4], *sw[kWBlocks];
+      const float *sx[4], *const sw = a.w_scale + (int64_t)(min(n0, a.n - 1) / kFp8Block) * a.kblocks;
 #pragma unroll
       for (int i = 0; i < 4; ++i) sx[i] = a.x_scale + (int64_t)min(m0 + i * 32 + lane, a.rows - 1) * a.kblocks;
-#pragma unroll
-      for (int b = 0; b < kWBlocks; ++b)
-        sw[b] = a.w_scale + (int64_t)(min(n0 + b * kFp8Block, a.n - 1) / kFp8Block) * a.kblocks;
       for (int kb = kb0; kb < kb1; kb += kScaleGroup) {
         ok = mbar_wait(&scale_empty[g], phase);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         // every load of the group in flight before the first product
-        float x[4][kScaleGroup], w[kWBlocks][kScaleGroup];
+        float x[4][kScaleGroup], w[kScaleGroup];
 #pragma unroll
         for (int j = 0; j < kScaleGroup; ++j) {
           const bool in = kb + j < kb1;
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[i][j] = in && i < lane_groups ? sx[i][kb + j] : 0.f;
-#pragma unroll
-          for (int b = 0; b < kWBlocks; ++b) w[b][j] = in ? sw[b][kb + j] : 0.f;
+          w[j] = in ? sw[kb + j] : 0.f;
         }
 #pragma unroll
         for (int j = 0; j < kScaleGroup; ++j) {
 #pragma unroll
-          for (int b = 0; b < kWBlocks; ++b) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (i < lane_groups)
-                scales[((g * kScaleGroup + j) * kWBlocks + b) * kBM + i * 32 + lane] = x[i][j] * w[b][j];
-          }
+          for (int i = 0; i < 4; ++i)
+            if (i < lane_groups) scales[(g * kScaleGroup + j) * kBM + i * 32 + lane] = x[i][j] * w[j];
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&scale_full[g]);
@@ -228,7 +218,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
     const int part = warp >> 2;  // columns [part * kCols, +kCols) of the tile
     const int tile_row = (warp & 3) * 32 + lane;
     const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(part * kCols);
-    const float* const my_scales = scales + part * kCols / kFp8Block * kBM + tile_row;
+    const float* const my_scales = scales + tile_row;
     int ring = 0, t = 0, g = 0;
     uint32_t phase = 0, g_phase = 0;
     bool ok = true;
@@ -248,7 +238,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
           break;
         }
         tc_fence_after();
-        const float s1 = my_scales[(g * kScaleGroup + in_group) * kWBlocks * kBM];
+        const float s1 = my_scales[(g * kScaleGroup + in_group) * kBM];
         const float2 s = make_float2(s1, s1);
         if (++in_group == kScaleGroup || kb + 1 == kb1) {
           __syncwarp();
@@ -378,6 +368,63 @@ int launch(const CUtensorMap& tx, const CUtensorMap& tw, Fp8LinearArgs a, cudaSt
                     body + 1024 + kScaleBytes, a.split, stream, tx, tw, a);
 }
 
+// ---- choice of the kernel ----------------------------------------------------------
+// Which tile, and how many ways k is split, by an estimate of the time of each: a start,
+// a time per 128-wide block of k (more where two CTAs share an SM, and where the grid
+// needs several rounds), and the cluster's cost where k is split. The figures were fitted
+// to sweeps on a B200 over 24 to 1536 rows and nine weights of 768 x 768 to 8192 x 8192
+// (k of 768 to 8192); the choice was within 12% of the best of its options there. Some of
+// both sides, in us:
+//   512 x 768 x 768:    128 x 64 tiles 5.0, 64-token tiles 4.9, the pair 6.4
+//   128 x 768 x 2048:   32-token tiles split in 4 5.2, 128 x 64 tiles whole 7.4
+//   256 x 4096 x 4096:  128 x 128 tiles in 2 11.9, whole 14.1; 128 x 64 whole 12.9
+//   512 x 4096 x 4096:  128 x 128 tiles 14.5, the pair 18.0
+//   1024 x 4096 x 4096: the pair 19, 128 x 128 tiles 26
+enum Kind { kFew, kTile, kPair };
+struct ShapeCost {
+  Kind kind;
+  int rows, cols;              // tokens and features of a tile
+  int per_sm;                  // CTAs an SM holds (the pair: half of one)
+  float start, start_per_row;  // us
+  float block, block_shared, block_rounds;
+};
+constexpr ShapeCost kShapes[] = {
+    {kFew, 16, 128, 2, 2.6f, 0.f, 0.20f, 0.33f, 0.36f},      {kFew, 32, 128, 2, 2.65f, 0.f, 0.244f, 0.41f, 0.45f},
+    {kFew, 64, 128, 2, 2.9f, 0.f, 0.33f, 0.54f, 0.60f},      {kTile, 128, 64, 2, 2.4f, 0.005f, 0.28f, 0.42f, 0.58f},
+    {kTile, 128, 128, 1, 2.6f, 0.0135f, 0.295f, 0.295f, 0.40f}, {kPair, 256, 256, 0, 3.3f, 0.f, 0.49f, 0.49f, 0.50f},
+};
+struct Choice {
+  const ShapeCost* shape;
+  int split;
+};
+
+Choice choose(int64_t rows, int64_t n, int kblocks, int sms) {
+  const float weight_us = (float)n * (float)kblocks * kBK / 5.9e6f + 3.0f;  // the weight's bytes from HBM
+  Choice best = {&kShapes[0], 1};
+  float best_us = 1e30f;
+  for (const ShapeCost& c : kShapes) {
+    if (c.kind == kFew && c.rows == 16 && rows > 16) continue;  // half of a 32-token tile at the same cost
+    const int64_t tiles = ((rows + c.rows - 1) / c.rows) * ((n + c.cols - 1) / c.cols);
+    const float live = (float)std::min<int64_t>(rows, c.rows);
+    for (int split = 1; split <= kMaxSplit && split <= kblocks; split *= 2) {
+      if (split > 1 && (c.kind == kPair || tiles * split > 2 * sms)) break;
+      const int64_t ctas = tiles * split, slots = c.per_sm > 0 ? (int64_t)sms * c.per_sm : sms / 2;
+      const float rounds = (float)((ctas + slots - 1) / slots);
+      const bool crowded = c.per_sm == 2 && ctas > sms;
+      const float block = rounds > 1.f ? c.block_rounds : crowded ? c.block_shared : c.block;
+      float us = c.start + c.start_per_row * live + (crowded ? 1.0f : 0.f) +
+                 rounds * ((float)((kblocks + split - 1) / split) * block + 0.6f) - 0.6f;
+      if (split > 1) us += 1.3f + 0.003f * live * (float)split;
+      us = std::max(us, weight_us) + 0.1f * us;
+      if (us < best_us) {
+        best_us = us;
+        best = {&c, split};
+      }
+    }
+  }
+  return best;
+}
+
 }  // namespace
 }  // namespace aiosb
 
@@ -422,27 +469,16 @@ extern "C" int aiosb_linear_fp8(const void* x, int64_t x_row_stride, const float
   a.a_rows = (int)std::min<int64_t>(kBM, (rows + 7) / 8 * 8);
   a.split = 1;
   a.status = status;
-  if (rows <= 64) return fp8_linear_few(x, x_row_stride, k, w, a, as_stream(stream));
-  if ((int64_t)((rows + 255) / 256) * ((n + 255) / 256) >= 60)
-    return fp8_linear_pair(x, x_row_stride, k, w, a, as_stream(stream));
-  // The widest tile that still gives every SM one: a wide tile reads x and the weight
-  // from L2 fewer times. Where none does, the narrowest, and k split until the grid
-  // covers the SMs.
-  const int sms = sm_count();
-  int bn = 64;
-  for (int b : {256, 128}) {
-    if ((int64_t)a.m_tiles * ((n + b - 1) / b) >= sms) {
-      bn = b;
-      break;
-    }
-  }
+  const Choice c = choose(rows, n, a.kblocks, sm_count());
+  cudaStream_t s = as_stream(stream);
+  a.split = c.split;
+  if (c.shape->kind == kFew) return fp8_linear_few(c.shape->rows, x, x_row_stride, k, w, a, s);
+  if (c.shape->kind == kPair) return fp8_linear_pair(x, x_row_stride, k, w, a, s);
+  const int bn = c.shape->cols;
   a.n_tiles = (int)((n + bn - 1) / bn);
-  while (a.split < kMaxSplit && a.split * 2 <= a.kblocks && (int64_t)a.m_tiles * a.n_tiles * a.split < sms)
-    a.split *= 2;
   CUtensorMap tx, tw;
   int rc = fp8_tensor_map(&tx, x, rows, k, x_row_stride, (uint32_t)a.a_rows);
   if (rc == AIOSB_OK) rc = fp8_tensor_map(&tw, w, n, k, k, (uint32_t)bn);
   if (rc != AIOSB_OK) return rc;
-  cudaStream_t s = as_stream(stream);
-  return bn == 256 ? launch<256>(tx, tw, a, s) : bn == 128 ? launch<128>(tx, tw, a, s) : launch<64>(tx, tw, a, s);
+  return bn == 128 ? launch<128>(tx, tw, a, s) : launch<64>(tx, tw, a, s);
 }

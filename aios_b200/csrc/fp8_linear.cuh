@@ -111,7 +111,7 @@ __device__ __forceinline__ float4 sum_ranks4(uint32_t off, int split) {
   float4 part[kMaxSplit];
 #pragma unroll
   for (int p = 0; p < kMaxSplit; ++p)
-    if (p < split) part[p] = ld_dsmem_f4(split > 1 ? map_shared_rank(off, (uint32_t)p) : off);
+    if (p < split) part[p] = ld_dsmem_f4(map_shared_rank(off, (uint32_t)p));
   float4 v = part[0];
 #pragma unroll
   for (int p = 1; p < kMaxSplit; ++p) {
@@ -177,8 +177,9 @@ int fp8_launch(Kern kern, int grid, int threads, int smem, int cluster, cudaStre
 // Many token rows: two CTAs share a 256 x 256 tile (fp8_linear_pair.cu).
 int fp8_linear_pair(const void* x, int64_t x_row_stride, int64_t k, const void* w, Fp8LinearArgs a,
                     cudaStream_t stream);
-// Few token rows: the weight is the M operand (fp8_linear_few.cu).
-int fp8_linear_few(const void* x, int64_t x_row_stride, int64_t k, const void* w, Fp8LinearArgs a,
+// Few token rows: the weight is the M operand, `tokens` (16, 32, 64) rows to a tile; a.split
+// is set (fp8_linear_few.cu).
+int fp8_linear_few(int tokens, const void* x, int64_t x_row_stride, int64_t k, const void* w, Fp8LinearArgs a,
                    cudaStream_t stream);
 
 }  // namespace aiosb

@@ -237,17 +237,31 @@ __global__ void __launch_bounds__(Few<TN>::kThreads, 2)
   __syncwarp();
   __syncthreads();
   if (split > 1) cluster_sync();
-  // Rank r sums and stores every split-th token: a warp reads whole lines of its peers'
-  // partial tiles (16-byte pieces of many tokens took four times as long).
-  if (!abort_flag) {
-    const uint32_t base = smem_u32(smem);
-    const int live = min(a.rows - t0, TN);
-    for (int u = threadIdx.x; u < (live - rank + split - 1) / split * (kBM / 4); u += S::kThreads) {
-      const int r = u / (kBM / 4) * split + rank, c = u % (kBM / 4) * 4;
-      if (f0 + c < a.n) store4(a, t0 + r, f0 + c, sum_ranks4(base + (uint32_t)(r * kRedStride + c) * 4, split));
+  const int live = min(a.rows - t0, TN);
+  if (split == 1) {
+    const float* const red = reinterpret_cast<const float*>(smem);
+    if (!abort_flag) {
+#pragma unroll 2
+      for (int u = threadIdx.x; u < live * (kBM / 8); u += S::kThreads) {
+        const int r = u / (kBM / 8), c = u % (kBM / 8) * 8;
+        const float4 lo = *reinterpret_cast<const float4*>(red + r * kRedStride + c);
+        const float4 hi = *reinterpret_cast<const float4*>(red + r * kRedStride + c + 4);
+        const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        if (f0 + c < a.n) store8(a, t0 + r, f0 + c, v);
+      }
     }
+  } else {
+    // Rank r sums and stores every split-th token: a warp reads whole lines of its peers'
+    // partial tiles (16-byte pieces of many tokens took four times as long).
+    if (!abort_flag) {
+      const uint32_t base = smem_u32(smem);
+      for (int u = threadIdx.x; u < (live - rank + split - 1) / split * (kBM / 4); u += S::kThreads) {
+        const int r = u / (kBM / 4) * split + rank, c = u % (kBM / 4) * 4;
+        if (f0 + c < a.n) store4(a, t0 + r, f0 + c, sum_ranks4(base + (uint32_t)(r * kRedStride + c) * 4, split));
+      }
+    }
+    cluster_sync();  // peers may still read this CTA's partial tile
   }
-  if (split > 1) cluster_sync();  // peers may still read this CTA's partial tile
   if (warp == kFoldWarps + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, S::kTmemCols);
@@ -265,13 +279,6 @@ int launch_few(const void* x, int64_t x_row_stride, int64_t k, const void* w, Fp
   a.m_tiles = (a.n + kBM - 1) / kBM;
   a.n_tiles = (a.rows + TN - 1) / TN;
   const int tiles = a.m_tiles * a.n_tiles;
-  // Split k where the tiles leave SMs idle, but only a k long enough: a block of k costs a
-  // lone CTA about 0.18 us, the cluster's barriers and reduction 1.2 us together (8 x 768,
-  // 16 blocks: 5.97 us whole, 4.70 in 4, 4.52 in 8; 8 x 1280, 6 blocks: 3.76 whole, 4.44
-  // in 6). One CTA to an SM streams the weight as fast as two.
-  a.split = 1;
-  while (a.kblocks > 10 && a.split < kMaxSplit && a.kblocks >= 4 * a.split && tiles * a.split * 2 <= sm_count())
-    a.split *= 2;
   const int per_cta = (a.kblocks + a.split - 1) / a.split;
   a.stages = std::max(S::kAccs, std::min({(kBudget - 1024 - S::kScaleBytes) / S::kStageBytes, kMaxStages, per_cta}));
   const int body = std::max(a.stages * S::kStageBytes, TN * kRedStride * 4);
@@ -285,10 +292,10 @@ int launch_few(const void* x, int64_t x_row_stride, int64_t k, const void* w, Fp
 
 }  // namespace
 
-int fp8_linear_few(const void* x, int64_t x_row_stride, int64_t k, const void* w, Fp8LinearArgs a,
+int fp8_linear_few(int tokens, const void* x, int64_t x_row_stride, int64_t k, const void* w, Fp8LinearArgs a,
                    cudaStream_t stream) {
-  if (a.rows <= 16) return launch_few<16>(x, x_row_stride, k, w, a, stream);
-  if (a.rows <= 32) return launch_few<32>(x, x_row_stride, k, w, a, stream);
+  if (tokens == 16) return launch_few<16>(x, x_row_stride, k, w, a, stream);
+  if (tokens == 32) return launch_few<32>(x, x_row_stride, k, w, a, stream);
   return launch_few<64>(x, x_row_stride, k, w, a, stream);
 }
 
