@@ -601,22 +601,31 @@ def _launch(index: int, name: str, *args) -> None:
 
 
 # These wrappers run in about the time of one small launch, so their checks are spelled
-# out on plain attributes: a decode step is bound by the host's launch rate otherwise.
+# out on plain attributes and outputs come from the allocator's shortest entry: a decode
+# step is bound by the host's launch rate otherwise.
+_new_cuda = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+
+
+def _empty_rows(x: torch.Tensor, rows: int, cols: int, dtype: torch.dtype) -> torch.Tensor:
+    """An uninitialised contiguous [rows, cols] tensor on x's device."""
+    if _new_cuda is not None and x.get_device() == torch._C._cuda_getDevice():
+        return _new_cuda((rows, cols), (cols, 1), dtype)
+    return x.new_empty(rows, cols, dtype=dtype)
+
+
 def _check_rows(what: str, x: torch.Tensor, dtype: torch.dtype) -> tuple[int, int, int]:
     """`x` as rows with contiguous columns on a CUDA device: (rows, cols, row stride)."""
+    if x.dtype is dtype and x.ndim == 2 and x.is_cuda:
+        rows, cols = x.shape
+        if x.is_contiguous():
+            return rows, cols, cols
+        stride, inner = x.stride()
+        if inner == 1 or cols == 1:
+            return rows, cols, stride if rows > 1 else cols
+        raise ValueError(f"{what} rows must be contiguous")
     if not x.is_cuda:
         raise ValueError(f"{what} requires CUDA tensors")
-    if x.dtype is not dtype or x.ndim != 2:
-        raise ValueError(f"{what} expects a 2-D {dtype} tensor")
-    rows, cols = x.shape
-    if rows == 1 or x.is_contiguous():
-        if cols > 1 and x.stride(1) != 1:
-            raise ValueError(f"{what} rows must be contiguous")
-        return rows, cols, cols
-    stride, inner = x.stride()
-    if inner != 1 and cols > 1:
-        raise ValueError(f"{what} rows must be contiguous")
-    return rows, cols, stride
+    raise ValueError(f"{what} expects a 2-D {dtype} tensor")
 
 
 def _check_dense(what: str, name: str, t: torch.Tensor, shape: tuple[int, ...], dtype: torch.dtype,
@@ -628,11 +637,11 @@ def _check_dense(what: str, name: str, t: torch.Tensor, shape: tuple[int, ...], 
 def _fp8_outputs(what: str, x: torch.Tensor, rows: int, cols: int, out: torch.Tensor | None,
                  scale: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:
     if out is None:
-        out = x.new_empty(rows, cols, dtype=FP8_DTYPE)
+        out = _empty_rows(x, rows, cols, FP8_DTYPE)
     else:
         _check_dense(what, "out", out, (rows, cols), FP8_DTYPE, x.get_device())
     if scale is None:
-        scale = x.new_empty(rows, -(-cols // FP8_BLOCK), dtype=torch.float32)
+        scale = _empty_rows(x, rows, -(-cols // FP8_BLOCK), torch.float32)
     else:
         _check_dense(what, "scale", scale, (rows, -(-cols // FP8_BLOCK)), torch.float32, x.get_device())
     return out, scale
@@ -652,8 +661,8 @@ def quantize_weight_fp8(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tenso
     """A bf16 weight [N, K] to (e4m3 [N, K], scale [ceil(N / 128), ceil(K / 128)]): a scale
     for each 128 x 128 block. K is a multiple of 16; rows may be strided."""
     n, k, stride = _check_rows("quantize_weight_fp8", weight, torch.bfloat16)
-    out = weight.new_empty(n, k, dtype=FP8_DTYPE)
-    scale = weight.new_empty(-(-n // FP8_BLOCK), -(-k // FP8_BLOCK), dtype=torch.float32)
+    out = _empty_rows(weight, n, k, FP8_DTYPE)
+    scale = _empty_rows(weight, -(-n // FP8_BLOCK), -(-k // FP8_BLOCK), torch.float32)
     _launch(weight.get_device(), "aiosb_quantize_weight_fp8", weight.data_ptr(), n, k, stride, out.data_ptr(),
             scale.data_ptr())
     return out, scale
@@ -726,9 +735,14 @@ def linear_fp8(
     n = weight.shape[0]
     index = x.get_device()
     blocks = -(-k // FP8_BLOCK)
-    _check_dense("linear_fp8", "weight", weight, (n, k), FP8_DTYPE, index)
-    _check_dense("linear_fp8", "x_scale", x_scale, (rows, blocks), torch.float32, index)
-    _check_dense("linear_fp8", "weight_scale", weight_scale, (-(-n // FP8_BLOCK), blocks), torch.float32, index)
+    tall = -(-n // FP8_BLOCK)
+    if not (weight.dtype is FP8_DTYPE and x_scale.dtype is weight_scale.dtype is torch.float32
+            and x_scale.shape == (rows, blocks) and weight_scale.shape == (tall, blocks)
+            and weight.get_device() == x_scale.get_device() == weight_scale.get_device() == index
+            and weight.is_contiguous() and x_scale.is_contiguous() and weight_scale.is_contiguous()):
+        _check_dense("linear_fp8", "weight", weight, (n, k), FP8_DTYPE, index)
+        _check_dense("linear_fp8", "x_scale", x_scale, (rows, blocks), torch.float32, index)
+        _check_dense("linear_fp8", "weight_scale", weight_scale, (tall, blocks), torch.float32, index)
     res_ptr, res_stride = None, 0
     if epilogue == _lib.EPI_ADD:
         if (residual is None or residual.shape != (rows, n) or residual.dtype is not torch.bfloat16
@@ -736,7 +750,7 @@ def linear_fp8(
             raise ValueError("the add epilogue needs a bf16 residual [rows, n] with contiguous rows")
         res_ptr, res_stride = residual.data_ptr(), residual.stride(0) if rows > 1 else n
     if out is None:
-        out = x.new_empty(rows, n, dtype=torch.bfloat16)
+        out = _empty_rows(x, rows, n, torch.bfloat16)
         out_stride = n
     else:
         if (out.shape != (rows, n) or out.dtype is not torch.bfloat16 or out.get_device() != index
