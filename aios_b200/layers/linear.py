@@ -17,9 +17,28 @@ class Linear(BaseOP):
             raise ValueError("the B200 linear kernels have no bias epilogue (the reference models use none)")
         self.weight = torch.empty(output_size, input_size)
         self.bias = None
+        self._fp8: tuple[torch.Tensor, torch.Tensor] | None = None  # e4m3 weight and block scales
+
+    def on_weights_loaded(self) -> None:
+        self._fp8 = None
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return ops.linear(x, self.weight)
+
+    def quantize_fp8(self) -> None:
+        """Builds the 8-bit copy of the weight that ``forward_fp8`` runs on."""
+        n, k = self.weight.shape
+        if n % 8 or k % 16:
+            raise ValueError(f"an 8-bit linear needs n % 8 == 0 and k % 16 == 0, got a [{n}, {k}] weight")
+        self._fp8 = ops.quantize_weight_fp8(self.weight)
+
+    def forward_fp8(self, x: torch.Tensor, x_scale: torch.Tensor, *, out: torch.Tensor | None = None,
+                    residual: torch.Tensor | None = None) -> torch.Tensor:
+        """The linear on quantised rows (``ops.linear_fp8``), ``residual`` added when given."""
+        if self._fp8 is None:
+            raise RuntimeError("forward_fp8 needs quantize_fp8() after the weights are loaded")
+        epilogue = _lib.EPI_STORE if residual is None else _lib.EPI_ADD
+        return ops.linear_fp8(x, x_scale, *self._fp8, out=out, epilogue=epilogue, residual=residual)
 
 
 class LinearQKVMerged(Linear):
@@ -42,6 +61,7 @@ class LinearColParallelMerged(Linear):
         self._packed: torch.Tensor | None = None
 
     def on_weights_loaded(self) -> None:
+        super().on_weights_loaded()
         self._packed = None
 
     def packed_weight(self) -> torch.Tensor:

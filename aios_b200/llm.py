@@ -10,6 +10,9 @@ KV pool: ``page_size`` 1 (the reference's layout; slot ids then equal the
 reference's bit for bit) or 16 (16-token pages). ``num_pages`` may be given
 directly; otherwise ``kv_cache_max_tokens`` / free memory decide, as in
 aios/llm/llm.py:77-96. The newest LLM owns the process-global context.
+
+``linear_dtype="fp8"`` runs the decoder layers' linears on e4m3 weights and rows
+with a scale for each block of 128 (``ops.linear_fp8``); the default is "bf16".
 """
 
 from __future__ import annotations
@@ -68,6 +71,7 @@ class LLM:
             from transformers import AutoTokenizer
 
             self.tokenizer = kwargs.get("tokenizer") or AutoTokenizer.from_pretrained(model_path)
+        self.model.set_linear_dtype(str(kwargs.get("linear_dtype", "bf16")))
         self.model.model._rotary_emb.set_device(self.device)
         self.page_size = int(kwargs.get("page_size", 1))
         self.num_pages = self._determine_num_pages(

@@ -119,11 +119,22 @@ class MiniMindAttnResDecoderLayer(BaseOP):
         batch: Batch,
         mixed: torch.Tensor,
         out: torch.Tensor | None = None,
+        fp8: bool = False,
     ) -> torch.Tensor:
         # without a partial this is a block's first layer, whose newest bank
         # source was written by the kernel just before
         stable = bank.shape[0] if partial is not None else bank.shape[0] - 1
         mixer, norm = self.attn_res_mixer, self.input_layernorm
+        if fp8:
+            # 8-bit linears: the mixers stay bf16, their rows are quantised for the linear
+            # that follows; the deltas are added in the linears' epilogues as below. Each
+            # kernel lets its successor launch only after its own wait, as `stable` needs.
+            rows = ops.quantize_fp8(mix_and_norm(mixer, norm, bank, partial, mixed, stable))
+            attn = self.self_attn.attend_qkv(self.self_attn.qkv_proj.forward_fp8(*rows), rotary, paged_kv_cache, batch)
+            partial = self.self_attn.o_proj.forward_fp8(*ops.quantize_fp8(attn), out=partial, residual=partial)
+            mixer, norm = self.mlp_res_mixer, self.post_attention_layernorm
+            rows = ops.quantize_fp8(mix_and_norm(mixer, norm, bank, partial, mixed, bank.shape[0]))
+            return self.mlp.forward_fp8(*rows, out=partial if out is None else out, residual=partial)
         if _FUSED_MIXER and ops.linear_attnres_rmsnorm_eligible(bank, partial, stable):
             # decode: the mixer and its norm inside the qkv projection
             qkv = ops.linear_attnres_rmsnorm(bank, partial, stable, mixer._routing_query(), mixer.key_norm.eps,
@@ -170,6 +181,7 @@ class MiniMindBlockAttnResModel(BaseOP):
         self._rotary_emb = RotaryEmbedding(config.head_dim, config.max_position_embeddings, config.rope_theta)
         self._num_blocks = config.attnres_num_blocks
         self._layers_per_block = config.layers_per_attnres_block
+        self._fp8_linears = False
 
     def forward_hidden(self) -> torch.Tensor:
         """Trunk up to the final mixer (before the final norm)."""
@@ -197,7 +209,7 @@ class MiniMindBlockAttnResModel(BaseOP):
             for index in range(first, last + 1):
                 partial = self.layers.op_list[index].forward(
                     bank, partial, self._rotary_emb, ctx.kv_cache, batch, mixed,
-                    out=bank_storage[source_count] if index == last else None,
+                    out=bank_storage[source_count] if index == last else None, fp8=self._fp8_linears,
                 )
             source_count += 1
         return bank_storage[:source_count], mixed

@@ -9,6 +9,8 @@ RMSNormFused (aios/layers/norm.py:34-40) is thereby split across the GEMM before
 and the GEMM after it, and no normalised tensor is written. ``forward`` keeps the
 reference's call structure for any other attention backend. The parameter
 names and their order equal the reference's, so checkpoints load unchanged.
+``set_linear_dtype("fp8")`` runs the layers' linears on 8-bit weights and rows
+instead (``forward_fp8``).
 """
 
 from __future__ import annotations
@@ -116,6 +118,12 @@ class Qwen3MLP(BaseOP):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return self.down_proj.forward(self.gate_up_proj.forward_silu_mul(x))
 
+    def forward_fp8(self, x: torch.Tensor, x_scale: torch.Tensor, *, out: torch.Tensor | None = None,
+                    residual: torch.Tensor | None = None) -> torch.Tensor:
+        """The MLP on quantised rows, with 8-bit linears; ``residual`` added when given."""
+        act = ops.silu_and_mul_fp8(self.gate_up_proj.forward_fp8(x, x_scale))
+        return self.down_proj.forward_fp8(*act, out=out, residual=residual)
+
 
 class Qwen3DecoderLayer(BaseOP):
     def __init__(self, config: ModelConfig, layer_idx: int, attn_backend: BaseAttentionBackend):
@@ -129,6 +137,16 @@ class Qwen3DecoderLayer(BaseOP):
         hidden_states = self.self_attn.forward(hidden_states, rotary, paged_kv_cache, batch)
         hidden_states, residual = self.post_attention_layernorm.forward(hidden_states, residual)
         return self.mlp.forward(hidden_states), residual
+
+    def forward_fp8(self, hidden_states, rotary, paged_kv_cache, batch, residual):
+        """``forward`` with 8-bit linears: each norm, the attention output and the SwiGLU
+        are quantised (a scale per 128 columns of a row) for the linear that follows."""
+        attn = self.self_attn
+        rows, residual = self.input_layernorm.forward_fp8(hidden_states, residual)
+        a = attn.attend_qkv(attn.qkv_proj.forward_fp8(*rows), rotary, paged_kv_cache, batch)
+        hidden_states = attn.o_proj.forward_fp8(*ops.quantize_fp8(a))
+        rows, residual = self.post_attention_layernorm.forward_fp8(hidden_states, residual)
+        return self.mlp.forward_fp8(*rows), residual
 
     def forward_stat(self, stats: ops.RowStats, residual: torch.Tensor, rotary, paged_kv_cache,
                      batch) -> ops.RowStats:
@@ -162,6 +180,7 @@ class Qwen3Model(BaseOP):
         self.layers = OPList([Qwen3DecoderLayer(config, i, self.attn_backend) for i in range(config.num_layers)])
         self.norm = RMSNormFused(config.hidden_size, config.rms_norm_eps)
         self._rotary_emb = RotaryEmbedding(config.head_dim, config.max_position_embeddings, config.rope_theta)
+        self._fp8_linears = False
 
     def forward_hidden(self) -> tuple[torch.Tensor, torch.Tensor | None]:
         """Decoder trunk without the final norm: (hidden, residual)."""
@@ -170,7 +189,8 @@ class Qwen3Model(BaseOP):
         hidden_states = self.embed_tokens.forward(batch.input_ids)
         residual: torch.Tensor | None = None
         for layer in self.layers.op_list:
-            hidden_states, residual = layer.forward(hidden_states, self._rotary_emb, ctx.kv_cache, batch, residual)
+            step = layer.forward_fp8 if self._fp8_linears else layer.forward
+            hidden_states, residual = step(hidden_states, self._rotary_emb, ctx.kv_cache, batch, residual)
         return hidden_states, residual
 
     def forward_stats(self) -> ops.RowStats:
@@ -202,9 +222,27 @@ class Qwen3ForCausalLM(BaseLLMModel):
             tied_embedding=self.model.embed_tokens if config.tie_word_embeddings else None,
         )
 
+    @property
+    def linear_dtype(self) -> str:
+        """What the decoder layers' linears run on: "bf16" or "fp8"."""
+        return "fp8" if self.model._fp8_linears else "bf16"
+
+    def set_linear_dtype(self, name: str) -> None:
+        """Runs the decoder layers' linears on bf16 weights or on 8-bit copies of them, which
+        are built here (the bf16 weights stay). Embedding, attention and LM head are bf16
+        either way. Call it after the weights are loaded and before graphs are captured."""
+        if name not in ("bf16", "fp8"):
+            raise ValueError(f"linear_dtype must be 'bf16' or 'fp8', got {name!r}")
+        if name == "fp8":
+            for layer in self.model.layers.op_list:
+                for linear in (layer.self_attn.qkv_proj, layer.self_attn.o_proj, layer.mlp.gate_up_proj,
+                               layer.mlp.down_proj):
+                    linear.quantize_fp8()
+        self.model._fp8_linears = name == "fp8"
+
     def forward(self) -> torch.Tensor:
         norm = self.model.norm
-        if isinstance(self.attn_backend, B200AttentionBackend):
+        if isinstance(self.attn_backend, B200AttentionBackend) and not self.model._fp8_linears:
             return self.lm_head.forward_stat(self.model.forward_stats(), norm.weight, norm.eps)
         hidden_states, residual = self.model.forward_hidden()
         return self.lm_head.forward_normed(hidden_states, residual, norm.weight, norm.eps)

@@ -88,7 +88,7 @@ def _stat_trunk(model) -> bool:
     from ..models.qwen3 import Qwen3ForCausalLM, Qwen3Model
 
     return (isinstance(model, Qwen3ForCausalLM) and type(model.model) is Qwen3Model
-            and isinstance(model.attn_backend, B200AttentionBackend))
+            and isinstance(model.attn_backend, B200AttentionBackend) and model.linear_dtype == "bf16")
 
 
 def stage_class(prefix_len: int) -> int:
@@ -270,8 +270,8 @@ class CandidateGroupRuntime:
         llm, cfg = self.llm, self.llm.config
         model = llm.model
         if (not isinstance(model, Qwen3ForCausalLM) or cfg.residual_type != "standard"
-                or type(model.attn_backend).__name__ != "B200AttentionBackend"):
-            return None  # the Block AttnRes trunk keeps the per-kernel forward
+                or type(model.attn_backend).__name__ != "B200AttentionBackend" or model.linear_dtype != "bf16"):
+            return None  # the Block AttnRes trunk and 8-bit linears keep the per-kernel forward
         if (cfg.hidden_size != 768 or cfg.intermediate_size != 2048 or cfg.head_dim not in (64, 96)
                 or cfg.num_qo_heads % cfg.num_kv_heads or cfg.num_qo_heads // cfg.num_kv_heads > 7
                 or cfg.num_qo_heads * cfg.head_dim != 768 or cfg.vocab_size % 16 or self.max_rows > 16):
