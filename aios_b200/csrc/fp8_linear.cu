@@ -440,6 +440,8 @@ extern "C" int aiosb_linear_fp8(const void* x, int64_t x_row_stride, const float
   constexpr int64_t kMost = (int64_t)1 << 30;
   AIOSB_REQUIRE(rows <= kMost && n <= kMost && k <= kMost && (rows / kBM + 1) * (n / 64 + 1) < kMost,
                 AIOSB_ERR_UNSUPPORTED, "linear_fp8: too large");
+  const int stable_weight = (epilogue & AIOSB_LINEAR_STABLE_WEIGHT) != 0;
+  epilogue &= ~AIOSB_LINEAR_STABLE_WEIGHT;
   AIOSB_REQUIRE(epilogue == AIOSB_EPI_STORE || epilogue == AIOSB_EPI_ADD, AIOSB_ERR_INVALID_ARG,
                 "linear_fp8: unknown epilogue %d (store or add)", epilogue);
   AIOSB_REQUIRE(epilogue != AIOSB_EPI_ADD ||
@@ -468,6 +470,7 @@ extern "C" int aiosb_linear_fp8(const void* x, int64_t x_row_stride, const float
   a.m_tiles = (int)((rows + kBM - 1) / kBM);
   a.a_rows = (int)std::min<int64_t>(kBM, (rows + 7) / 8 * 8);
   a.split = 1;
+  a.stable_weight = stable_weight;
   a.status = status;
   const Choice c = choose(rows, n, a.kblocks, sm_count());
   cudaStream_t s = as_stream(stream);

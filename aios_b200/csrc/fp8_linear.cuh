@@ -25,6 +25,7 @@ struct Fp8LinearArgs {
   int stages;
   int scale_offset;  // of the scale products, bytes from the start of dynamic shared memory
   int a_rows;  // token rows a stage holds: rows, rounded up to the swizzle's 8, at most 128
+  int stable_weight;  // AIOSB_LINEAR_STABLE_WEIGHT
   int32_t* status;
 };
 

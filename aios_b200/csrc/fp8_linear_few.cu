@@ -67,8 +67,6 @@ __global__ void __launch_bounds__(Few<TN>::kThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  pdl_wait();
-  pdl_launch_dependents();  // after the wait: whoever follows may rely on this kernel's predecessors being done
 
   // m tiles are features, n tiles tokens; the token tiles of one feature tile are
   // neighbours, so that the second reads the weight from L2
@@ -76,8 +74,22 @@ __global__ void __launch_bounds__(Few<TN>::kThreads, 2)
   const int kb0 = (int)((int64_t)a.kblocks * rank / split), kb1 = (int)((int64_t)a.kblocks * (rank + 1) / split);
   const int f0 = tile / a.n_tiles * kBM, t0 = tile % a.n_tiles * TN;
 
+  // The weight's first stages and scales are asked for before the dependency wait when the
+  // caller vouches for them; everything else comes after it.
+  if (warp != kFoldWarps && warp != kFoldWarps + 2) pdl_wait();
+
   if (warp == kFoldWarps) {
     // ---- TMA producer
+    const int early = a.stable_weight ? min(kb1 - kb0, a.stages) : 0;
+    if (early > 0 && elect_one()) {
+      for (int i = 0; i < early; ++i) {
+        mbar_arrive_expect_tx(&full[i], S::kStageBytes);
+        tma_load_2d(smem + i * S::kStageBytes, &tm_w, &full[i], (kb0 + i) * kBK, f0);
+      }
+    }
+    __syncwarp();
+    pdl_wait();
+    pdl_launch_dependents();  // after the wait: whoever follows may rely on this kernel's predecessors being done
     int s = 0, issued = 0;
     uint32_t phase = 1;
     bool ok = true;
@@ -86,8 +98,10 @@ __global__ void __launch_bounds__(Few<TN>::kThreads, 2)
       if (!ok) break;
       if (elect_one()) {
         uint8_t* const dst = smem + s * S::kStageBytes;
-        mbar_arrive_expect_tx(&full[s], S::kStageBytes);
-        tma_load_2d(dst, &tm_w, &full[s], kb * kBK, f0);
+        if (kb - kb0 >= early) {
+          mbar_arrive_expect_tx(&full[s], S::kStageBytes);
+          tma_load_2d(dst, &tm_w, &full[s], kb * kBK, f0);
+        }
         tma_load_2d(dst + kWBytes, &tm_x, &full[s], kb * kBK, t0);
       }
       issued = min(issued + 1, a.stages);
@@ -148,14 +162,16 @@ __global__ void __launch_bounds__(Few<TN>::kThreads, 2)
     int g = 0;
     uint32_t phase = 1;
     bool ok = true;
+    if (!a.stable_weight) pdl_wait();
     for (int kb = kb0; kb < kb1; kb += kScaleGroup) {
       float x[kPer][kScaleGroup], w[kScaleGroup];
 #pragma unroll
-      for (int j = 0; j < kScaleGroup; ++j) {
-        const bool in = kb + j < kb1;
+      for (int j = 0; j < kScaleGroup; ++j) w[j] = kb + j < kb1 ? sw[kb + j] : 0.f;
+      if (a.stable_weight && kb == kb0) pdl_wait();
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) x[i][j] = in ? sx[i][kb + j] : 0.f;
-        w[j] = in ? sw[kb + j] : 0.f;
+      for (int j = 0; j < kScaleGroup; ++j) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) x[i][j] = kb + j < kb1 ? sx[i][kb + j] : 0.f;
       }
       ok = __all_sync(0xffffffffu, mbar_wait(&scale_empty[g], phase));
       if (!ok) break;

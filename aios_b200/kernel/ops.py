@@ -723,12 +723,15 @@ def linear_fp8(
     out: torch.Tensor | None = None,
     epilogue: int = _lib.EPI_STORE,
     residual: torch.Tensor | None = None,
+    stable_weight: bool = False,
 ) -> torch.Tensor:
     """y = x @ weight.T of quantised rows [T, K] and weight [N, K] (``quantize_fp8``,
     ``quantize_weight_fp8``) on the 8-bit tensor cores, fp32 sums, bf16 out.
 
     ``epilogue=EPI_ADD`` returns ``residual + x @ weight.T`` with one rounding (residual
-    may be ``out`` for an in-place add). N is a multiple of 8, K of 16."""
+    may be ``out`` for an in-place add). N is a multiple of 8, K of 16.
+    ``stable_weight``: the weight and its scales were written before the previous kernel on
+    the stream began (``LINEAR_STABLE_WEIGHT``), so they may be fetched ahead of its end."""
     rows, k, stride = _check_rows("linear_fp8", x, FP8_DTYPE)
     if weight.ndim != 2 or weight.shape[1] != k:
         raise ValueError("linear_fp8 expects x [T, K] and weight [N, K]")
@@ -759,7 +762,8 @@ def linear_fp8(
         out_stride = out.stride(0) if rows > 1 else n
     if rows:
         _launch(index, "aiosb_linear_fp8", x.data_ptr(), stride, x_scale.data_ptr(), rows, k, weight.data_ptr(),
-                weight_scale.data_ptr(), n, out.data_ptr(), out_stride, epilogue, res_ptr, res_stride,
+                weight_scale.data_ptr(), n, out.data_ptr(), out_stride,
+                epilogue | _lib.LINEAR_STABLE_WEIGHT if stable_weight else epilogue, res_ptr, res_stride,
                 _status_pointer(index))
     return out
 

@@ -31,6 +31,7 @@ class Linear(BaseOP):
         if n % 8 or k % 16:
             raise ValueError(f"an 8-bit linear needs n % 8 == 0 and k % 16 == 0, got a [{n}, {k}] weight")
         self._fp8 = ops.quantize_weight_fp8(self.weight)
+        torch.cuda.synchronize(self.weight.device)  # forward_fp8 reads it ahead of its stream order
 
     def forward_fp8(self, x: torch.Tensor, x_scale: torch.Tensor, *, out: torch.Tensor | None = None,
                     residual: torch.Tensor | None = None) -> torch.Tensor:
@@ -38,7 +39,8 @@ class Linear(BaseOP):
         if self._fp8 is None:
             raise RuntimeError("forward_fp8 needs quantize_fp8() after the weights are loaded")
         epilogue = _lib.EPI_STORE if residual is None else _lib.EPI_ADD
-        return ops.linear_fp8(x, x_scale, *self._fp8, out=out, epilogue=epilogue, residual=residual)
+        return ops.linear_fp8(x, x_scale, *self._fp8, out=out, epilogue=epilogue, residual=residual,
+                              stable_weight=True)
 
 
 class LinearQKVMerged(Linear):

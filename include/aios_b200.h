@@ -66,6 +66,11 @@ extern "C" {
  * and row metadata come from kernels that have completed whenever it can start. */
 #define AIOSB_LINEAR_EARLY_DEPENDENTS 0x100
 
+/* OR-ed into the epilogue of aiosb_linear_fp8: the weight and its scales were written
+ * before the previous kernel on the stream began (a loaded model's), so the kernels for
+ * few rows ask for them before the dependency wait. */
+#define AIOSB_LINEAR_STABLE_WEIGHT 0x200
+
 /* Library version (major*10000 + minor*100 + patch). */
 AIOSB_API int aiosb_version(void);
 
@@ -300,7 +305,8 @@ AIOSB_API int aiosb_silu_mul_fp8(const void* x, int64_t rows, int64_t f, int64_t
  * residual_stride elements apart and may be y itself. Sums over a block of 128 are
  * formed by the tensor cores, those across blocks in fp32, in an order that depends
  * on the sizes alone. Every operand, the weight too, is read after the dependency
- * wait: the kernel that quantised it may be the previous launch. */
+ * wait, so the kernel that quantised it may be the previous launch, unless the epilogue
+ * carries AIOSB_LINEAR_STABLE_WEIGHT. */
 AIOSB_API int aiosb_linear_fp8(const void* x, int64_t x_row_stride, const float* x_scale, int64_t rows, int64_t k,
                                const void* w, const float* w_scale, int64_t n, void* y, int64_t y_row_stride,
                                int epilogue, const void* residual, int64_t residual_stride, int32_t* status,

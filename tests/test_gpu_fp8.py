@@ -158,7 +158,9 @@ def test_linear_fp8(cuda_device, rows: int, n: int, k: int) -> None:
     torch.cuda.synchronize()
     ops.check_status(cuda_device)
     _linear_check(y, q, s, wq, ws)
-    assert torch.equal(y, ops.linear_fp8(q, s, wq, ws))  # the order of the sums depends on the sizes alone
+    # the order of the sums depends on the sizes alone, and an early fetched weight is the same weight
+    assert torch.equal(y, ops.linear_fp8(q, s, wq, ws))
+    assert torch.equal(y, ops.linear_fp8(q, s, wq, ws, stable_weight=True))
 
 
 @pytest.mark.parametrize("rows,n,k", [(1, 768, 2048), (8, 768, 768), (130, 1000, 272), (2048, 2560, 528)])
