@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   pdl_wait();
-  pdl_launch_dependents();  // after the wait: whoever follows may rely on this kernel's predecessors being done
+  if (warp == kFoldWarps) pdl_launch_dependents();  // after the wait: whoever follows may rely on this kernel's predecessors being done
 
   const int split = a.split;
   const int rank = blockIdx.x % split;

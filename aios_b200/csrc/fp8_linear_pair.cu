@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   pdl_wait();
-  pdl_launch_dependents();  // after the wait: whoever follows may rely on this kernel's predecessors being done
+  if (warp == kFoldWarps) pdl_launch_dependents();  // after the wait: whoever follows may rely on this kernel's predecessors being done
 
   const int tiles = a.m_tiles * a.n_tiles;  // pair tiles
   const int first = blockIdx.x / 2, step = gridDim.x / 2;

@@ -38,7 +38,7 @@ struct NormArgs {
 template <int TPR, int U, bool RES>
 __global__ void __launch_bounds__(TPR == 32 ? kThreads : TPR) norm_fp8_kernel(const NormArgs a) {
   pdl_wait();
-  pdl_launch_dependents();
+  if (threadIdx.x < 32) pdl_launch_dependents();
   __shared__ float scratch[32];
   const int64_t r = TPR == 32 ? (int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32 : (int64_t)blockIdx.x;
   const int t = TPR == 32 ? threadIdx.x & 31 : threadIdx.x;
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(kThreads)
     rows_fp8_kernel(const __nv_bfloat16* __restrict__ x, int64_t x_stride, uint32_t groups, uint32_t blocks, int cols,
                     uint8_t* __restrict__ q, float* __restrict__ scale) {
   pdl_wait();
-  pdl_launch_dependents();
+  if (threadIdx.x < 32) pdl_launch_dependents();
   const int lane16 = threadIdx.x & 15;
   const uint32_t g0 = blockIdx.x * (uint32_t)(kThreads / 16 * UPT) + threadIdx.x / 16;
   uint4 gv[UPT], uv[UPT];
