@@ -46,12 +46,17 @@ __global__ void __launch_bounds__(TPR == 32 ? kThreads : TPR) norm_fp8_kernel(co
   const int units = a.hidden / 8;
   const __nv_bfloat16* xr = a.x + r * a.x_stride;
   const int64_t base = r * a.hidden;
-  uint4 xv[U], rv[U];
+  // The weight comes with the row, so that its latency hides behind the row's (8 x 768: 2.2
+  // -> 1.8 us), except where four units without a residual would lose occupancy to it (4096 x
+  // 1024: 4.6 us without, 5.1 with).
+  constexpr bool kEarlyWeight = U < 4 || RES;
+  uint4 xv[U], rv[U], wv[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int i = t + u * TPR;
     xv[u] = i < units ? ld16(xr + 8 * i) : make_uint4(0, 0, 0, 0);
     if (RES) rv[u] = i < units ? ld16(a.res + base + 8 * i) : make_uint4(0, 0, 0, 0);
+    if (kEarlyWeight) wv[u] = i < units ? ld16(a.w + 8 * i) : make_uint4(0, 0, 0, 0);
   }
   float s[U][8];
   float2 ss2 = make_float2(0.f, 0.f);
@@ -84,7 +89,8 @@ __global__ void __launch_bounds__(TPR == 32 ? kThreads : TPR) norm_fp8_kernel(co
   for (int u = 0; u < U; ++u) {
     const int i = t + u * TPR;
     float g[8];
-    unpack8(i < units ? ld16(a.w + 8 * i) : make_uint4(0, 0, 0, 0), g);
+    if (!kEarlyWeight) wv[u] = i < units ? ld16(a.w + 8 * i) : make_uint4(0, 0, 0, 0);
+    unpack8(wv[u], g);
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
       const float2 v = __fmul2_rn(__fmul2_rn(make_float2(s[u][j], s[u][j + 1]), rcp2), make_float2(g[j], g[j + 1]));
