@@ -163,7 +163,8 @@ def test_linear_fp8(cuda_device, rows: int, n: int, k: int) -> None:
     assert torch.equal(y, ops.linear_fp8(q, s, wq, ws, stable_weight=True))
 
 
-@pytest.mark.parametrize("rows,n,k", [(1, 768, 2048), (8, 768, 768), (130, 1000, 272), (2048, 2560, 528)])
+@pytest.mark.parametrize("rows,n,k", [(1, 768, 2048), (8, 768, 768), (130, 1000, 272), (2048, 2560, 528),
+                                         (2040, 2568, 272), (1100, 2440, 528), (4100, 4104, 144), (77, 8200, 144)])
 def test_linear_fp8_add_and_strides(cuda_device, rows: int, n: int, k: int) -> None:
     q, s, wq, ws = _linear_inputs(rows, n, k)
     wide = torch.zeros(rows, k + 48, dtype=torch.uint8, device=cuda_device)
