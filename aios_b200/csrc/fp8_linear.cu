@@ -7,18 +7,23 @@
 // from tensor memory and folded into fp32 registers as acc += (sx * sw) * d. x is the
 // M operand: a TMEM lane is a token, its scale one register of the thread that reads
 // the lane, and the weight's scale is uniform over the columns of a warp, so the fold
-// costs one FMA per value. Two or four TMEM accumulators take turns: the tensor
-// cores work on the next blocks while the warps fold one.
+// costs one FMA per value. Four TMEM accumulators take turns: the tensor cores work
+// on the next blocks while the warps fold one.
 //
-// Per CTA: the first 8 or 16 warps fold (warp w: lanes 32 (w % 4).., columns w / 4). Of
-// the four warps after them one lane loads tiles by TMA into a ring of stages, one issues
-// the MMAs, and a third warp forms the products sx * sw eight blocks of k at a time and
-// hands them over in shared memory: read by the folding threads themselves, each row's
-// scale is a cache line of its own, and 16 warps fetching 32 lines each per block took
-// as long as the MMAs.
+// Per CTA: the first 8 warps fold (warp w: lanes 32 (w % 4).., columns w / 4). Of the
+// four warps after them one lane loads tiles by TMA into a ring of stages, one issues the
+// MMAs, and a third warp forms the products sx * sw (in fp32) eight blocks of k at a time
+// and hands them over in shared memory: read by the folding threads themselves, each
+// row's scale is a cache line of its own, and fetching 32 lines per warp and block took as
+// long as the MMAs.
 // Few rows leave few tiles: then a cluster of up to 8 CTAs splits the blocks of k and
 // the partial tiles are summed in rank order through distributed shared memory, so
 // results do not depend on scheduling.
+//
+// These tiles (128 x 64, two CTAs per SM, and 128 x 128) serve tens to hundreds of rows;
+// fp8_linear_few.cu has the shape for fewer, fp8_linear_pair.cu for more, and choose() below
+// picks. Measured: 77 x 10000 x 5008 17.0 us (its bytes take 8.0), 500 x 4096 x 768 6.9 us,
+// 512 x 8192 x 8192 35 us (1960 TFLOP/s).
 #include <string.h>
 
 #include <algorithm>
@@ -92,7 +97,8 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   pdl_wait();
-  if (warp == kFoldWarps) pdl_launch_dependents();  // after the wait: whoever follows may rely on this kernel's predecessors being done
+  // after the wait: whoever follows may rely on this kernel's predecessors being done
+  if (warp == kFoldWarps) pdl_launch_dependents();
 
   const int split = a.split;
   const int rank = blockIdx.x % split;
@@ -331,7 +337,8 @@ EncodeTiledFn encode_fn() {
 
 }  // namespace
 
-int fp8_tensor_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t row_stride, uint32_t box_rows) {
+int fp8_tensor_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t row_stride,
+                   uint32_t box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return set_error(AIOSB_ERR_LAUNCH, "cuTensorMapEncodeTiled unavailable");
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
@@ -372,10 +379,10 @@ int launch(const CUtensorMap& tx, const CUtensorMap& tw, Fp8LinearArgs a, cudaSt
 // Which tile, and how many ways k is split, by an estimate of the time of each: a start,
 // a time per 128-wide block of k (more where two CTAs share an SM, and where the grid
 // needs several rounds), and the cluster's cost where k is split. The figures were fitted
-// to sweeps on a B200 over 24 to 1536 rows and nine weights of 768 x 768 to 8192 x 8192
-// (k of 768 to 8192); the choice was within 12% of the best of its options there. Some of
-// both sides, in us:
-//   512 x 768 x 768:    128 x 64 tiles 5.0, 64-token tiles 4.9, the pair 6.4
+// to sweeps on a B200 over 1 to 1536 rows and nine weights of 768 x 768 to 8192 x 8192;
+// there the choice was within 6% of the best of its options in 122 of 126 sizes, and within
+// 18% in all. Some of both sides, in us:
+//   512 x 768 x 768:    32-token tiles 4.1, 64-token 4.75, 128 x 64 tiles 5.0, the pair 6.4
 //   128 x 768 x 2048:   32-token tiles split in 4 5.2, 128 x 64 tiles whole 7.4
 //   256 x 4096 x 4096:  128 x 128 tiles in 2 11.9, whole 14.1; 128 x 64 whole 12.9
 //   512 x 4096 x 4096:  128 x 128 tiles 14.5, the pair 18.0
@@ -389,9 +396,12 @@ struct ShapeCost {
   float block, block_shared, block_rounds;
 };
 constexpr ShapeCost kShapes[] = {
-    {kFew, 16, 128, 2, 2.6f, 0.f, 0.20f, 0.33f, 0.36f},      {kFew, 32, 128, 2, 2.65f, 0.f, 0.244f, 0.41f, 0.45f},
-    {kFew, 64, 128, 2, 2.9f, 0.f, 0.33f, 0.54f, 0.60f},      {kTile, 128, 64, 2, 2.4f, 0.005f, 0.28f, 0.42f, 0.58f},
-    {kTile, 128, 128, 1, 2.6f, 0.0135f, 0.295f, 0.295f, 0.40f}, {kPair, 256, 256, 0, 3.3f, 0.f, 0.49f, 0.49f, 0.50f},
+    {kFew, 16, 128, 2, 2.6f, 0.f, 0.20f, 0.33f, 0.36f},
+    {kFew, 32, 128, 2, 2.65f, 0.f, 0.244f, 0.41f, 0.45f},
+    {kFew, 64, 128, 2, 2.9f, 0.f, 0.33f, 0.54f, 0.60f},
+    {kTile, 128, 64, 2, 2.4f, 0.005f, 0.28f, 0.42f, 0.58f},
+    {kTile, 128, 128, 1, 2.6f, 0.0135f, 0.295f, 0.295f, 0.40f},
+    {kPair, 256, 256, 0, 3.3f, 0.f, 0.49f, 0.49f, 0.50f},
 };
 struct Choice {
   const ShapeCost* shape;

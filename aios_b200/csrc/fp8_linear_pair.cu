@@ -17,6 +17,13 @@
 // Finished rows go through shared memory (one 256-byte row piece per lane in, whole lines
 // out); a residual is fetched into the same place by asynchronous copies issued at the
 // tile's start.
+//
+// Measured: 2048 x 4096 x 4096 35 us (1960 TFLOP/s; its 128 tiles fill 1.7 of 2 rounds of
+// 74 pairs), 8192^3 470 us (2340 TFLOP/s) in a short burst and 515 us under sustained load,
+// where the board's power limit sets the pace: the SM clock drops to 1.4-1.7 GHz. The
+// tensor pipe is active 52% of the SM cycles at 2048 x 4096 x 4096 and L2 at 28% of its
+// throughput: what is left there are the half-empty second round and the prologue. Tried
+// without gain: two issuing warps, six stages, an undivided 256-column product, TMA stores.
 #include <algorithm>
 
 #include "fp8_linear.cuh"
@@ -116,7 +123,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   pdl_wait();
-  if (warp == kFoldWarps) pdl_launch_dependents();  // after the wait: whoever follows may rely on this kernel's predecessors being done
+  // after the wait: whoever follows may rely on this kernel's predecessors being done
+  if (warp == kFoldWarps) pdl_launch_dependents();
 
   const int tiles = a.m_tiles * a.n_tiles;  // pair tiles
   const int first = blockIdx.x / 2, step = gridDim.x / 2;

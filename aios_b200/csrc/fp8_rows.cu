@@ -4,7 +4,13 @@
 // block (fp8.cuh). All of them read each input once and write each output once, so
 // HBM bounds them at size; the layouts below serve that: a lane holds 8 consecutive
 // values (a 16-byte load), 16 lanes hold one block of 128, so the block's maximum is
-// four shuffles and a warp's loads and stores are whole lines.
+// a few shuffles and a warp's loads and stores are whole lines.
+//
+// Measured (GB/s of the bytes that have to move; a copy reaches 6520): norm with residual of
+// 16384 x 8192 137 us, 6850 GB/s; plain norm 79 us, 5130 GB/s (3 bytes a value where the
+// residual's form moves 7, so the arithmetic shows); SwiGLU of 12001 x 10240 100.5 us, 6110 GB/s (three
+// quarters of the issue slots taken); rows of 16384 x 8192 66 us, 6110 GB/s; weight of 16384
+// x 8192 60.5 us, 6650 GB/s.
 #include <algorithm>
 
 #include "abi_util.h"
@@ -196,7 +202,9 @@ void launch_rows(const void* x, int64_t x_stride, int64_t rows, int64_t cols, vo
   const uint32_t blocks = (uint32_t)((cols + kFp8Block - 1) / kFp8Block);
   const uint32_t groups = (uint32_t)rows * blocks;
   const uint32_t per_sm = groups / (kThreads / 16) / (uint32_t)sm_count();  // blocks of one group per thread
-  const auto launch = per_sm < 3 ? launch_rows_as<SILU, 1> : per_sm < 8 ? launch_rows_as<SILU, 2> : launch_rows_as<SILU, 4>;
+  const auto launch = per_sm < 3   ? launch_rows_as<SILU, 1>
+                      : per_sm < 8 ? launch_rows_as<SILU, 2>
+                                   : launch_rows_as<SILU, 4>;
   launch((const __nv_bfloat16*)x, x_stride, groups, blocks, (int)cols, (uint8_t*)q, scale, s);
 }
 

@@ -145,7 +145,8 @@ def _linear_inputs(rows: int, n: int, k: int):
 # 128 x 128 tiles, the pair of SMs; k whole and split in 2, 4 and 8; tiles cut by rows, n and k.
 LINEARS = [(r, n, k) for r in (1, 8, 33, 128, 129, 300) for n, k in ((8, 16), (136, 144), (1280, 768), (776, 2064))]
 LINEARS += [(1, 4104, 1024), (77, 1000, 5008), (64, 128, 8192), (500, 4096, 768), (1024, 2440, 144), (1100, 2432, 768),
-            (2048, 2568, 144), (2040, 2560, 1040), (4096, 4096, 272), (513, 16384, 768), (16, 104, 128), (17, 10000, 1040), (40, 776, 8192)]
+            (2048, 2568, 144), (2040, 2560, 1040), (4096, 4096, 272), (513, 16384, 768), (16, 104, 128),
+            (17, 10000, 1040), (40, 776, 8192)]
 LINEARS += [(1, 8192, 1680), (5, 4096, 2064), (40, 4096, 1680), (40, 2056, 2064), (50, 16384, 400), (64, 8192, 4096),
             (40, 4096, 2064), (50, 2056, 8192), (77, 8192, 400), (77, 2056, 4096), (3, 776, 1040), (40, 16384, 1040),
             (100, 8192, 4096), (50, 4096, 8192), (77, 2056, 8192), (128, 16384, 400), (200, 8192, 400)]

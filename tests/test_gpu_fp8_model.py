@@ -140,7 +140,8 @@ def test_engine_on_8_bit_linears(cuda_device, config) -> None:
         result = engine.complete(text, ImeGenerationConfig(seed=4, max_new_tokens=8))
         runs.append([(c.text, c.average_logprob) for c in result.raw_candidates])
     assert len(runs[0]) >= 8 and runs[0] == runs[1]
-    cands = [llm.tokenizer.text_for(torch.randint(10, config.vocab_size, (n,), generator=g).tolist()) for n in (1, 4, 9)]
+    cands = [llm.tokenizer.text_for(torch.randint(10, config.vocab_size, (n,), generator=g).tolist())
+             for n in (1, 4, 9)]
     stable = engine.score_candidates(text, cands, mode="stable")
     shared = engine.score_candidates(text, cands, mode="shared_decode")
     a = {c.text: c.average_logprob for c in stable.candidates}
