@@ -43,6 +43,10 @@ struct Shape {
   static constexpr int kAccs = 4;                       // TMEM accumulators in turn
   // scale products: two groups of kScaleGroup blocks of k, 128 rows each
   static constexpr int kScaleBytes = 2 * kScaleGroup * kBM * 4;
+  // MMA warps: a wait that is over and the issue behind it take about 500 clocks of a warp per
+  // block, the MMAs of 128 columns 256. Two warps in turn: 77 x 10000 x 10240 27.3 -> 23.9 us.
+  // With 64 columns two CTAs share the SM and one each is enough (two: 3% slower).
+  static constexpr int kIssuers = BN == 64 ? 1 : 2;
   static constexpr int kCtas = BN == 64 ? 2 : 1;        // CTAs per SM (TMEM: kAccs * BN of 512 columns each)
 };
 
@@ -52,8 +56,9 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
                       const Fp8LinearArgs a) {
   constexpr uint32_t kBBytes = BN * kBK;
   constexpr int kCols = Shape<BN>::kCols, kFoldWarps = Shape<BN>::kFoldWarps, kThreads = Shape<BN>::kThreads;
-  constexpr int kAccs = Shape<BN>::kAccs;
-  constexpr int kLd = BN == 128 ? 32 : 16;  // columns per tensor-memory load, by the registers a thread has
+  constexpr int kAccs = Shape<BN>::kAccs, kIssuers = Shape<BN>::kIssuers;
+  // columns per tensor-memory load and loads in flight, by the registers a thread has
+  constexpr int kLd = BN == 128 ? 32 : 16, kLoads = BN == 128 ? 2 : 1;
   constexpr int kRedStride = BN + 4;   // floats per row of the partial tile: conflict-free 16-byte accesses
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -143,28 +148,32 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
         mbar_wait(&full[s], phase ^ 1);
       }
     }
-  } else if (warp == kFoldWarps + 1) {
-    // ---- MMA issuer. With fewer than 128 rows staged the A operand's unused rows are
+  } else if (warp == kFoldWarps + 1 || (kIssuers == 2 && warp == kFoldWarps + 3)) {
+    // ---- MMA issuers, taking blocks in turn. With fewer than 128 rows staged the A operand's unused rows are
     // whatever follows the slot in shared memory (inside the allocation): a row of A
     // reaches its own TMEM lane only, and those lanes are not read.
     // One commit per block serves two readers of done[]: the producer (the stage's
     // operands are read) and the fold (the product is in TMEM). The fold cannot fall a
-    // whole ring behind, because stages >= kAccs and an accumulator waits for its fold.
+    // whole ring behind, because stages >= kAccs and an accumulator waits for its fold;
+    // for the same reason one issuer is never more than kAccs blocks ahead of the other.
     constexpr uint32_t idesc = umma_idesc_e4m3(kBM, BN);
     const uint64_t a_desc = umma_desc_sw128(smem_u32(smem_a)), b_desc = umma_desc_sw128(smem_u32(smem_b));
     int s = 0, t = 0;
     uint32_t phase = 0, acc_phase = 1;
-    bool ok = true;
+    bool ok = true, mine = warp == kFoldWarps + 1;
     for (int tile = blockIdx.x / split; tile < tiles && ok; tile += step) {
-      for (int kb = kb0; kb < kb1; ++kb) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[t], acc_phase) && mbar_wait(&full[s], phase));
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t da = a_desc + (uint32_t)s * (a_bytes >> 4), db = b_desc + (uint32_t)s * (kBBytes >> 4);
-        if (elect_one()) {
+      for (int kb = kb0; kb < kb1; ++kb, mine = kIssuers == 1 || !mine) {
+        if (mine) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[t], acc_phase) && mbar_wait(&full[s], phase));
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t da = a_desc + (uint32_t)s * (a_bytes >> 4), db = b_desc + (uint32_t)s * (kBBytes >> 4);
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kBK / 32; ++kk) tc_mma_e4m3(tmem + t * BN, da + 2 * kk, db + 2 * kk, idesc, kk != 0);
-          tc_commit(&done[s]);
+            for (int kk = 0; kk < kBK / 32; ++kk)
+              tc_mma_e4m3(tmem + t * BN, da + 2 * kk, db + 2 * kk, idesc, kk != 0);
+            tc_commit(&done[s]);
+          }
         }
         if (++s == a.stages) {
           s = 0;
@@ -254,17 +263,21 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
           if (g == 0) g_phase ^= 1;
         }
 #pragma unroll
-        for (int c = 0; c < kCols; c += kLd) {
-          uint32_t d[kLd];
-          tmem_ld(t_lane + t * BN + c, d);
-          tmem_wait(d);
-          if (c + kLd == kCols) {  // this block's values are in registers: the accumulator may be reused
+        for (int c = 0; c < kCols; c += kLoads * kLd) {
+          uint32_t d[kLoads][kLd];
+#pragma unroll
+          for (int l = 0; l < kLoads; ++l) tmem_ld(t_lane + t * BN + c + l * kLd, d[l]);
+#pragma unroll
+          for (int l = 0; l < kLoads; ++l) tmem_wait(d[l]);
+          if (c + kLoads * kLd == kCols) {  // this block's values are in registers: the accumulator may be reused
             tc_fence_before();
             if (lane == 0) mbar_arrive(&acc_empty[t]);
           }
 #pragma unroll
-          for (int j = 0; j < kLd / 2; ++j)
-            acc[c / 2 + j] = __ffma2_rn(s, make_float2(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1])),
+          for (int j = 0; j < kLoads * kLd / 2; ++j)
+            acc[c / 2 + j] = __ffma2_rn(s,
+                                        make_float2(__uint_as_float(d[2 * j / kLd][2 * j % kLd]),
+                                                    __uint_as_float(d[2 * j / kLd][2 * j % kLd + 1])),
                                         acc[c / 2 + j]);
         }
         if (++ring == a.stages) {

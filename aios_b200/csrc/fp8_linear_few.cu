@@ -25,6 +25,9 @@ struct Few {
   static constexpr int kFoldWarps = 4 * (TN / kCols);  // 4 groups of 32 TMEM lanes
   static constexpr int kThreads = (kFoldWarps + 4) * 32;
   static constexpr int kAccs = 4;
+  // MMA warps, as in fp8_linear.cu: a second one gives 3% with 16 tokens (8 x 8192 x 8192 17.9 ->
+  // 17.3 us) and costs 2 to 4% with 64
+  static constexpr int kIssuers = TN == 16 ? 2 : 1;
   static constexpr int kTmemCols = kAccs * TN;         // 64, 128 or 256: two CTAs per SM
   static constexpr int kScaleBytes = 2 * kScaleGroup * TN * 4;
   static constexpr int kStageBytes = (kBM + TN) * kBK;
@@ -125,23 +128,25 @@ __global__ void __launch_bounds__(Few<TN>::kThreads, 2)
         mbar_wait(&full[s], phase ^ 1);
       }
     }
-  } else if (warp == kFoldWarps + 1) {
-    // ---- MMA issuer
+  } else if (warp == kFoldWarps + 1 || (S::kIssuers == 2 && warp == kFoldWarps + 3)) {
+    // ---- MMA issuers, taking blocks in turn
     constexpr uint32_t idesc = umma_idesc_e4m3(kBM, TN);
     const uint64_t w_desc = umma_desc_sw128(smem_u32(smem)), x_desc = umma_desc_sw128(smem_u32(smem + kWBytes));
     int s = 0, t = 0;
     uint32_t phase = 0, acc_phase = 1;
-    bool ok = true;
-    for (int kb = kb0; kb < kb1; ++kb) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[t], acc_phase) && mbar_wait(&full[s], phase));
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t off = (uint32_t)s * (S::kStageBytes >> 4);
-      if (elect_one()) {
+    bool ok = true, mine = warp == kFoldWarps + 1;
+    for (int kb = kb0; kb < kb1; ++kb, mine = S::kIssuers == 1 || !mine) {
+      if (mine) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[t], acc_phase) && mbar_wait(&full[s], phase));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t off = (uint32_t)s * (S::kStageBytes >> 4);
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < kBK / 32; ++kk)
-          tc_mma_e4m3(tmem + t * TN, w_desc + off + 2 * kk, x_desc + off + 2 * kk, idesc, kk != 0);
-        tc_commit(&done[s]);
+          for (int kk = 0; kk < kBK / 32; ++kk)
+            tc_mma_e4m3(tmem + t * TN, w_desc + off + 2 * kk, x_desc + off + 2 * kk, idesc, kk != 0);
+          tc_commit(&done[s]);
+        }
       }
       if (++s == a.stages) {
         s = 0;
