@@ -409,12 +409,12 @@ struct ShapeCost {
   float block, block_shared, block_rounds;
 };
 constexpr ShapeCost kShapes[] = {
-    {kFew, 16, 128, 2, 2.6f, 0.f, 0.20f, 0.33f, 0.36f},
-    {kFew, 32, 128, 2, 2.65f, 0.f, 0.244f, 0.41f, 0.45f},
-    {kFew, 64, 128, 2, 2.9f, 0.f, 0.33f, 0.54f, 0.60f},
-    {kTile, 128, 64, 2, 2.4f, 0.005f, 0.28f, 0.42f, 0.58f},
-    {kTile, 128, 128, 1, 2.6f, 0.0135f, 0.295f, 0.295f, 0.40f},
-    {kPair, 256, 256, 0, 3.3f, 0.f, 0.49f, 0.49f, 0.50f},
+    {kFew, 16, 128, 2, 2.61f, 0.f, 0.194f, 0.32f, 0.36f},
+    {kFew, 32, 128, 2, 2.72f, 0.f, 0.231f, 0.337f, 0.454f},
+    {kFew, 64, 128, 2, 3.03f, 0.f, 0.325f, 0.511f, 0.60f},
+    {kTile, 128, 64, 2, 2.63f, 0.0053f, 0.343f, 0.388f, 0.527f},
+    {kTile, 128, 128, 1, 2.89f, 0.0126f, 0.295f, 0.295f, 0.328f},
+    {kPair, 256, 256, 0, 3.3f, 0.f, 0.569f, 0.569f, 0.507f},
 };
 struct Choice {
   const ShapeCost* shape;
@@ -422,7 +422,7 @@ struct Choice {
 };
 
 Choice choose(int64_t rows, int64_t n, int kblocks, int sms) {
-  const float weight_us = (float)n * (float)kblocks * kBK / 5.9e6f + 3.0f;  // the weight's bytes from HBM
+  const float weight_us = (float)n * (float)kblocks * kBK / 6.38e6f + 2.95f;  // the weight's bytes from HBM
   Choice best = {&kShapes[0], 1};
   float best_us = 1e30f;
   for (const ShapeCost& c : kShapes) {
@@ -431,13 +431,15 @@ Choice choose(int64_t rows, int64_t n, int kblocks, int sms) {
     const float live = (float)std::min<int64_t>(rows, c.rows);
     for (int split = 1; split <= kMaxSplit && split <= kblocks; split *= 2) {
       if (split > 1 && (c.kind == kPair || tiles * split > 2 * sms)) break;
-      const int64_t ctas = tiles * split, slots = c.per_sm > 0 ? (int64_t)sms * c.per_sm : sms / 2;
+      // a cluster stays inside one group of SMs: those of 4 reach 132 of 148 SMs, of 8 120
+      const int reach = split == 8 ? sms * 120 / 148 : split == 4 ? sms * 132 / 148 : sms;
+      const int64_t ctas = tiles * split, slots = c.per_sm > 0 ? (int64_t)reach * c.per_sm : sms / 2;
       const float rounds = (float)((ctas + slots - 1) / slots);
-      const bool crowded = c.per_sm == 2 && ctas > sms;
+      const bool crowded = c.per_sm == 2 && ctas > reach;
       const float block = rounds > 1.f ? c.block_rounds : crowded ? c.block_shared : c.block;
-      float us = c.start + c.start_per_row * live + (crowded ? 1.0f : 0.f) +
-                 rounds * ((float)((kblocks + split - 1) / split) * block + 0.6f) - 0.6f;
-      if (split > 1) us += 1.3f + 0.003f * live * (float)split;
+      float us = c.start + c.start_per_row * live + (crowded ? 1.1f : 0.f) +
+                 rounds * ((float)((kblocks + split - 1) / split) * block + 0.5f) - 0.5f;
+      if (split > 1) us += 1.4f + 0.0036f * live * (float)split;
       us = std::max(us, weight_us) + 0.1f * us;
       if (us < best_us) {
         best_us = us;
