@@ -50,7 +50,7 @@ struct Shape {
   static constexpr int kCtas = BN == 64 ? 2 : 1;        // CTAs per SM (TMEM: kAccs * BN of 512 columns each)
 };
 
-template <int BN>
+template <int BN, bool RES>
 __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
     linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                       const Fp8LinearArgs a) {
@@ -290,10 +290,14 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
       if (split == 1) {
         if (row < a.rows) {
 #pragma unroll
-          for (int j = 0; j < kCols / 2; j += 4) {
-            const float v[8] = {acc[j].x,     acc[j].y,     acc[j + 1].x, acc[j + 1].y,
-                                acc[j + 2].x, acc[j + 2].y, acc[j + 3].x, acc[j + 3].y};
-            if (c0 + 2 * j < a.n) store8(a, row, c0 + 2 * j, v);
+          for (int h = 0; h < kCols / 8; h += 4) {
+            uint4 res[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (RES && c0 + 8 * (h + j) < a.n) res[j] = residual8(a, row, c0 + 8 * (h + j));
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (c0 + 8 * (h + j) < a.n) store8<RES>(a, row, c0 + 8 * (h + j), acc + 4 * (h + j), res[j]);
           }
         }
       } else if (tile_row < a.a_rows) {
@@ -309,17 +313,28 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
   __syncwarp();
   __syncthreads();
   if (split > 1) {
-    cluster_sync();
     // Rank r sums and stores every split-th row: a warp reads whole lines of its peers'
     // partial tiles (16-byte pieces of many rows took four times as long).
+    constexpr int kUnits = (kBM / 2 * (BN / 4) + kThreads - 1) / kThreads;  // of a thread, at most
+    const int tile = blockIdx.x / split;
+    const int m0 = tile % a.m_tiles * kBM, n0 = tile / a.m_tiles * BN;
+    const int units = (min(a.rows - m0, kBM) - rank + split - 1) / split * (BN / 4);
+    uint2 res[kUnits];
+    if (RES) {
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        const int u = threadIdx.x + i * kThreads, r = u / (BN / 4) * split + rank, c = u % (BN / 4) * 4;
+        if (u < units && n0 + c < a.n) res[i] = residual4(a, m0 + r, n0 + c);
+      }
+    }
+    cluster_sync();
     if (!abort_flag) {
-      const int tile = blockIdx.x / split;
-      const int m0 = tile % a.m_tiles * kBM, n0 = tile / a.m_tiles * BN;
       const uint32_t base = smem_u32(smem);
-      const int live = min(a.rows - m0, kBM);
-      for (int u = threadIdx.x; u < (live - rank + split - 1) / split * (BN / 4); u += kThreads) {
-        const int r = u / (BN / 4) * split + rank, c = u % (BN / 4) * 4;
-        if (n0 + c < a.n) store4(a, m0 + r, n0 + c, sum_ranks4(base + (uint32_t)(r * kRedStride + c) * 4, split));
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        const int u = threadIdx.x + i * kThreads, r = u / (BN / 4) * split + rank, c = u % (BN / 4) * 4;
+        if (u < units && n0 + c < a.n)
+          store4<RES>(a, m0 + r, n0 + c, sum_ranks4(base + (uint32_t)(r * kRedStride + c) * 4, split), res[i]);
       }
     }
     cluster_sync();  // peers may still read this CTA's partial tile
@@ -367,12 +382,12 @@ int fp8_tensor_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols,
 
 namespace {
 
-template <int BN>
+template <int BN, bool RES>
 int launch(const CUtensorMap& tx, const CUtensorMap& tw, Fp8LinearArgs a, cudaStream_t stream) {
   constexpr int kOne = 224 * 1024;  // shared memory of a CTA that has the SM to itself
   constexpr int kCtas = Shape<BN>::kCtas, kBudget = kCtas == 2 ? kOne / 2 - 1024 : kOne;
   constexpr int kScaleBytes = Shape<BN>::kScaleBytes;
-  auto kern = linear_fp8_kernel<BN>;
+  auto kern = linear_fp8_kernel<BN, RES>;
   static bool configured[64] = {false};
   const int rc = fp8_configure(kern, kBudget, configured);
   if (rc != AIOSB_OK) return rc;
@@ -508,5 +523,6 @@ extern "C" int aiosb_linear_fp8(const void* x, int64_t x_row_stride, const float
   int rc = fp8_tensor_map(&tx, x, rows, k, x_row_stride, (uint32_t)a.a_rows);
   if (rc == AIOSB_OK) rc = fp8_tensor_map(&tw, w, n, k, k, (uint32_t)bn);
   if (rc != AIOSB_OK) return rc;
-  return bn == 128 ? launch<128>(tx, tw, a, s) : launch<64>(tx, tw, a, s);
+  if (a.residual != nullptr) return bn == 128 ? launch<128, true>(tx, tw, a, s) : launch<64, true>(tx, tw, a, s);
+  return bn == 128 ? launch<128, false>(tx, tw, a, s) : launch<64, false>(tx, tw, a, s);
 }

@@ -78,25 +78,29 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
                  "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
 }
 
-// Eight finished sums of one row to bf16, the residual added in fp32 (one rounding).
-__device__ __forceinline__ void store8(const Fp8LinearArgs& a, int64_t row, int col, const float (&v)[8]) {
-  float o[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) o[j] = v[j];
-  if (a.residual != nullptr) {
-    float r[8];
-    unpack8(*reinterpret_cast<const uint4*>(a.residual + row * a.residual_stride + col), r);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] += r[j];
-  }
-  *reinterpret_cast<uint4*>(a.y + row * a.y_stride + col) =
-      make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
+// ---- results: sums of one row to bf16; the residual is added in fp32 (one rounding).
+// A thread loads all of its pieces of the residual before its first store: the output may be
+// the residual's own memory, so the compiler keeps a load behind every store before it, and
+// 500 x 4096 x 768 spent 3.2 us on those round trips one after another. The kernels with a
+// residual are instances of their own: what they hold in registers cost the others 2%.
+__device__ __forceinline__ uint4 residual8(const Fp8LinearArgs& a, int64_t row, int col) {
+  return *reinterpret_cast<const uint4*>(a.residual + row * a.residual_stride + col);
 }
-
-// Four finished sums of one row, as store8.
-__device__ __forceinline__ void store4(const Fp8LinearArgs& a, int64_t row, int col, float4 v) {
-  if (a.residual != nullptr) {
-    const uint2 r = *reinterpret_cast<const uint2*>(a.residual + row * a.residual_stride + col);
+__device__ __forceinline__ uint2 residual4(const Fp8LinearArgs& a, int64_t row, int col) {
+  return *reinterpret_cast<const uint2*>(a.residual + row * a.residual_stride + col);
+}
+template <bool RES>
+__device__ __forceinline__ void store8(const Fp8LinearArgs& a, int64_t row, int col, const float2* v,
+                                       const uint4& residual) {
+  float r[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (RES) unpack8(residual, r);
+  *reinterpret_cast<uint4*>(a.y + row * a.y_stride + col) =
+      make_uint4(pack_bf16x2(v[0].x + r[0], v[0].y + r[1]), pack_bf16x2(v[1].x + r[2], v[1].y + r[3]),
+                 pack_bf16x2(v[2].x + r[4], v[2].y + r[5]), pack_bf16x2(v[3].x + r[6], v[3].y + r[7]));
+}
+template <bool RES>
+__device__ __forceinline__ void store4(const Fp8LinearArgs& a, int64_t row, int col, float4 v, const uint2& r) {
+  if (RES) {
     v.x += bf16_lo(r.x);
     v.y += bf16_hi(r.x);
     v.z += bf16_lo(r.y);

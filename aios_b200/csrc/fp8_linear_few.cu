@@ -34,7 +34,7 @@ struct Few {
 };
 constexpr int kRedStride = kBM + 4;  // floats per token of the partial tile
 
-template <int TN>
+template <int TN, bool RES>
 __global__ void __launch_bounds__(Few<TN>::kThreads, 2)
     linear_fp8_few_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                           const Fp8LinearArgs a) {
@@ -261,28 +261,50 @@ __global__ void __launch_bounds__(Few<TN>::kThreads, 2)
 
   __syncwarp();
   __syncthreads();
-  if (split > 1) cluster_sync();
   const int live = min(a.rows - t0, TN);
   if (split == 1) {
     const float* const red = reinterpret_cast<const float*>(smem);
+    constexpr int kUnits = (TN * (kBM / 8) + S::kThreads - 1) / S::kThreads;  // of a thread, at most
+    uint4 res[kUnits];
+    if (RES) {
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        const int u = threadIdx.x + i * S::kThreads, r = u / (kBM / 8), c = u % (kBM / 8) * 8;
+        if (r < live && f0 + c < a.n) res[i] = residual8(a, t0 + r, f0 + c);
+      }
+    }
     if (!abort_flag) {
-#pragma unroll 2
-      for (int u = threadIdx.x; u < live * (kBM / 8); u += S::kThreads) {
-        const int r = u / (kBM / 8), c = u % (kBM / 8) * 8;
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        const int u = threadIdx.x + i * S::kThreads, r = u / (kBM / 8), c = u % (kBM / 8) * 8;
+        if (r >= live || f0 + c >= a.n) continue;
         const float4 lo = *reinterpret_cast<const float4*>(red + r * kRedStride + c);
         const float4 hi = *reinterpret_cast<const float4*>(red + r * kRedStride + c + 4);
-        const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-        if (f0 + c < a.n) store8(a, t0 + r, f0 + c, v);
+        const float2 v[4] = {{lo.x, lo.y}, {lo.z, lo.w}, {hi.x, hi.y}, {hi.z, hi.w}};
+        store8<RES>(a, t0 + r, f0 + c, v, res[i]);
       }
     }
   } else {
     // Rank r sums and stores every split-th token: a warp reads whole lines of its peers'
     // partial tiles (16-byte pieces of many tokens took four times as long).
+    constexpr int kUnits = (TN / 2 * (kBM / 4) + S::kThreads - 1) / S::kThreads;
+    const int units = (live - rank + split - 1) / split * (kBM / 4);
+    uint2 res[kUnits];
+    if (RES) {
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        const int u = threadIdx.x + i * S::kThreads, r = u / (kBM / 4) * split + rank, c = u % (kBM / 4) * 4;
+        if (u < units && f0 + c < a.n) res[i] = residual4(a, t0 + r, f0 + c);
+      }
+    }
+    cluster_sync();
     if (!abort_flag) {
       const uint32_t base = smem_u32(smem);
-      for (int u = threadIdx.x; u < (live - rank + split - 1) / split * (kBM / 4); u += S::kThreads) {
-        const int r = u / (kBM / 4) * split + rank, c = u % (kBM / 4) * 4;
-        if (f0 + c < a.n) store4(a, t0 + r, f0 + c, sum_ranks4(base + (uint32_t)(r * kRedStride + c) * 4, split));
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        const int u = threadIdx.x + i * S::kThreads, r = u / (kBM / 4) * split + rank, c = u % (kBM / 4) * 4;
+        if (u < units && f0 + c < a.n)
+          store4<RES>(a, t0 + r, f0 + c, sum_ranks4(base + (uint32_t)(r * kRedStride + c) * 4, split), res[i]);
       }
     }
     cluster_sync();  // peers may still read this CTA's partial tile
@@ -293,11 +315,11 @@ __global__ void __launch_bounds__(Few<TN>::kThreads, 2)
   }
 }
 
-template <int TN>
+template <int TN, bool RES>
 int launch_few(const void* x, int64_t x_row_stride, int64_t k, const void* w, Fp8LinearArgs a, cudaStream_t stream) {
   using S = Few<TN>;
   constexpr int kBudget = 111 * 1024;  // two CTAs per SM
-  auto kern = linear_fp8_few_kernel<TN>;
+  auto kern = linear_fp8_few_kernel<TN, RES>;
   static bool configured[64] = {false};
   int rc = fp8_configure(kern, kBudget, configured);
   if (rc != AIOSB_OK) return rc;
@@ -315,13 +337,20 @@ int launch_few(const void* x, int64_t x_row_stride, int64_t k, const void* w, Fp
   return fp8_launch(kern, tiles * a.split, S::kThreads, body + 1024 + S::kScaleBytes, a.split, stream, tx, tw, a);
 }
 
+template <bool RES>
+int launch_tokens(int tokens, const void* x, int64_t x_row_stride, int64_t k, const void* w, const Fp8LinearArgs& a,
+                  cudaStream_t stream) {
+  if (tokens == 16) return launch_few<16, RES>(x, x_row_stride, k, w, a, stream);
+  if (tokens == 32) return launch_few<32, RES>(x, x_row_stride, k, w, a, stream);
+  return launch_few<64, RES>(x, x_row_stride, k, w, a, stream);
+}
+
 }  // namespace
 
 int fp8_linear_few(int tokens, const void* x, int64_t x_row_stride, int64_t k, const void* w, Fp8LinearArgs a,
                    cudaStream_t stream) {
-  if (tokens == 16) return launch_few<16>(x, x_row_stride, k, w, a, stream);
-  if (tokens == 32) return launch_few<32>(x, x_row_stride, k, w, a, stream);
-  return launch_few<64>(x, x_row_stride, k, w, a, stream);
+  return a.residual != nullptr ? launch_tokens<true>(tokens, x, x_row_stride, k, w, a, stream)
+                               : launch_tokens<false>(tokens, x, x_row_stride, k, w, a, stream);
 }
 
 }  // namespace aiosb
