@@ -22,8 +22,12 @@
 //
 // These tiles (128 x 64, two CTAs per SM, and 128 x 128) serve tens to hundreds of rows;
 // fp8_linear_few.cu has the shape for fewer, fp8_linear_pair.cu for more, and choose() below
-// picks. Measured: 77 x 10000 x 5008 17.0 us (its bytes take 8.0), 500 x 4096 x 768 6.9 us,
-// 512 x 8192 x 8192 35 us (1960 TFLOP/s).
+// picks. Measured: 77 x 10000 x 5008 16.8-17.9 us (its bytes take 8.0: 79 tiles leave half of the
+// SMs idle, and a fold warp's wait, TMEM loads and FMAs take 460 clocks per block of k in
+// the others; with k = 5120, rows on 128-byte lines, 14.2), 500 x 4096 x 768 6.6 us,
+// 256 x 4096 x 4096 11.2 us, 512 x 8192 x 8192 35 us (1930-1970 TFLOP/s). Loading the next
+// block's columns behind the last FMAs brought 2% at 77 x 10000 x 10240 and cost the 64-wide
+// tile 8%.
 #include <string.h>
 
 #include <algorithm>
@@ -407,14 +411,17 @@ int launch(const CUtensorMap& tx, const CUtensorMap& tw, Fp8LinearArgs a, cudaSt
 // Which tile, and how many ways k is split, by an estimate of the time of each: a start,
 // a time per 128-wide block of k (more where two CTAs share an SM, and where the grid
 // needs several rounds), and the cluster's cost where k is split. The figures were fitted
-// to sweeps on a B200 over 1 to 1536 rows and nine weights of 768 x 768 to 8192 x 8192;
-// there the choice was within 6% of the best of its options in 122 of 126 sizes, and within
-// 18% in all. Some of both sides, in us:
-//   512 x 768 x 768:    32-token tiles 4.1, 64-token 4.75, 128 x 64 tiles 5.0, the pair 6.4
-//   128 x 768 x 2048:   32-token tiles split in 4 5.2, 128 x 64 tiles whole 7.4
-//   256 x 4096 x 4096:  128 x 128 tiles in 2 11.9, whole 14.1; 128 x 64 whole 12.9
-//   512 x 4096 x 4096:  128 x 128 tiles 14.5, the pair 18.0
-//   1024 x 4096 x 4096: the pair 19, 128 x 128 tiles 26
+// to sweeps on a B200 of 286 sizes (1 to 1536 rows; weights of 768 x 768 to 14336 x 4096).
+// On 99 sizes of other rows and weights the choice was within 5% of the best of its options
+// in 93 and within 8% in all. Some of both sides, in us:
+//   1 x 768 x 2048:     16-token tiles split in 8 3.1, in 4 3.5, whole 4.8
+//   512 x 768 x 768:    32-token tiles 3.5, 64-token 4.1, 128 x 64 tiles 5.0, the pair 6.4
+//   128 x 768 x 2048:   32-token tiles split in 4 4.5, whole 5.8; 64-token in 4 5.3
+//   77 x 10000 x 5008:  128 x 128 tiles 16.9, 128 x 64 21.8, 64-token 26.2
+//   300 x 1536 x 8960:  64-token tiles split in 4 14.3; 128 x 128 in 2 14.9, in 4 20.6
+//   256 x 4096 x 4096:  128 x 128 tiles in 2 11.5, whole 12.6; 128 x 64 whole 12.7
+//   512 x 4096 x 4096:  128 x 128 tiles 13.1, the pair 17.9
+//   1024 x 4096 x 4096: the pair 19.1, 128 x 128 tiles 23.9
 enum Kind { kFew, kTile, kPair };
 struct ShapeCost {
   Kind kind;

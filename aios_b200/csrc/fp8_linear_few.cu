@@ -10,7 +10,7 @@
 // rank order.
 //
 // Measured: 1 x 8192 x 14336 21.9 us (5376 GB/s, 82% of measured HBM; 117.5 MB read, each
-// weight byte once). A short k is latency: 8 x 1280 x 768 3.1 us and 8 x 768 x 2048 3.2 us in
+// weight byte once). A short k is latency: 8 x 1280 x 768 2.9 us and 8 x 768 x 2048 3.1 us in
 // a chain of launches, for 0.15 and 0.24 us of bytes.
 #include <algorithm>
 
