@@ -411,12 +411,13 @@ int launch(const CUtensorMap& tx, const CUtensorMap& tw, Fp8LinearArgs a, cudaSt
 // Which tile, and how many ways k is split, by an estimate of the time of each: a start,
 // a time per 128-wide block of k (more where two CTAs share an SM, and where the grid
 // needs several rounds), and the cluster's cost where k is split. The figures were fitted
-// to sweeps on a B200 of 286 sizes (1 to 1536 rows; weights of 768 x 768 to 14336 x 4096).
-// On 99 sizes of other rows and weights the choice was within 5% of the best of its options
-// in 93 and within 8% in all. Some of both sides, in us:
+// to sweeps on a B200 of 495 sizes (1 to 4096 rows, k of 128 to 14336). On 144 sizes of
+// other rows and weights the choice was within 5% of the best of its options in 136 and
+// within 12% in all. Some of both sides, in us:
 //   1 x 768 x 2048:     16-token tiles split in 8 3.1, in 4 3.5, whole 4.8
 //   512 x 768 x 768:    32-token tiles 3.5, 64-token 4.1, 128 x 64 tiles 5.0, the pair 6.4
 //   128 x 768 x 2048:   32-token tiles split in 4 4.5, whole 5.8; 64-token in 4 5.3
+//   100 x 11008 x 256:  64-token tiles 4.4, 128 x 128 tiles 5.0, the pair 5.8
 //   77 x 10000 x 5008:  128 x 128 tiles 16.9, 128 x 64 21.8, 64-token 26.2
 //   300 x 1536 x 8960:  64-token tiles split in 4 14.3; 128 x 128 in 2 14.9, in 4 20.6
 //   256 x 4096 x 4096:  128 x 128 tiles in 2 11.5, whole 12.6; 128 x 64 whole 12.7
@@ -431,12 +432,12 @@ struct ShapeCost {
   float block, block_shared, block_rounds;
 };
 constexpr ShapeCost kShapes[] = {
-    {kFew, 16, 128, 2, 2.61f, 0.f, 0.194f, 0.32f, 0.36f},
-    {kFew, 32, 128, 2, 2.72f, 0.f, 0.231f, 0.337f, 0.454f},
-    {kFew, 64, 128, 2, 3.03f, 0.f, 0.325f, 0.511f, 0.60f},
-    {kTile, 128, 64, 2, 2.63f, 0.0053f, 0.343f, 0.388f, 0.527f},
-    {kTile, 128, 128, 1, 2.89f, 0.0126f, 0.295f, 0.295f, 0.328f},
-    {kPair, 256, 256, 0, 3.3f, 0.f, 0.569f, 0.569f, 0.507f},
+    {kFew, 16, 128, 2, 2.61f, 0.f, 0.194f, 0.317f, 0.303f},
+    {kFew, 32, 128, 2, 2.58f, 0.f, 0.231f, 0.337f, 0.454f},
+    {kFew, 64, 128, 2, 2.82f, 0.f, 0.325f, 0.529f, 0.60f},
+    {kTile, 128, 64, 2, 2.63f, 0.0053f, 0.309f, 0.388f, 0.55f},
+    {kTile, 128, 128, 1, 3.19f, 0.0126f, 0.286f, 0.286f, 0.329f},
+    {kPair, 256, 256, 0, 4.64f, 0.f, 0.569f, 0.569f, 0.50f},
 };
 struct Choice {
   const ShapeCost* shape;
@@ -454,14 +455,14 @@ Choice choose(int64_t rows, int64_t n, int kblocks, int sms) {
     for (int split = 1; split <= kMaxSplit && split <= kblocks; split *= 2) {
       if (split > 1 && (c.kind == kPair || tiles * split > 2 * sms)) break;
       // a cluster stays inside one group of SMs: those of 4 reach 132 of 148 SMs, of 8 120
-      const int reach = split == 8 ? sms * 120 / 148 : split == 4 ? sms * 132 / 148 : sms;
-      const int64_t ctas = tiles * split, slots = c.per_sm > 0 ? (int64_t)reach * c.per_sm : sms / 2;
+      const int reach = std::max(1, split == 8 ? sms * 120 / 148 : split == 4 ? sms * 132 / 148 : sms);
+      const int64_t ctas = tiles * split, slots = c.per_sm > 0 ? (int64_t)reach * c.per_sm : std::max(1, sms / 2);
       const float rounds = (float)((ctas + slots - 1) / slots);
       const bool crowded = c.per_sm == 2 && ctas > reach;
       const float block = rounds > 1.f ? c.block_rounds : crowded ? c.block_shared : c.block;
       float us = c.start + c.start_per_row * live + (crowded ? 1.1f : 0.f) +
-                 rounds * ((float)((kblocks + split - 1) / split) * block + 0.5f) - 0.5f;
-      if (split > 1) us += 1.4f + 0.0036f * live * (float)split;
+                 rounds * ((float)((kblocks + split - 1) / split) * block + 0.52f) - 0.52f;
+      if (split > 1) us += 1.32f + 0.0036f * live * (float)split;
       us = std::max(us, weight_us) + 0.1f * us;
       if (us < best_us) {
         best_us = us;

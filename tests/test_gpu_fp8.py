@@ -181,6 +181,32 @@ def test_linear_fp8_add_and_strides(cuda_device, rows: int, n: int, k: int) -> N
     assert torch.equal(buf[:, n:], before[:, n:]) and torch.equal(buf[rows:], before[rows:])  # nothing beside it
 
 
+# One size or more for each tile and each split of k, with and without a residual (instances
+# of their own): 16-, 32- and 64-token tiles, 128 x 64, 128 x 128, the pair.
+EACH = [(3, 1064, 560), (1, 4280, 1696), (8, 2288, 4432), (13, 552, 2112), (16, 264, 4512)]
+EACH += [(18, 72, 144), (355, 272, 1760), (45, 1040, 2720), (18, 488, 2528), (21, 64, 1568)]
+EACH += [(957, 520, 160), (482, 608, 3760), (80, 1584, 4704), (35, 1056, 5936)]
+EACH += [(1370, 824, 144), (359, 3096, 1472), (947, 576, 2160), (34, 2112, 1872), (355, 264, 10032), (43, 912, 7888)]
+EACH += [(795, 1424, 416), (216, 6664, 1808), (693, 792, 3472), (633, 424, 5216), (66, 1440, 7312)]
+EACH += [(711, 3152, 144)]
+
+
+@pytest.mark.parametrize("rows,n,k", EACH)
+def test_each_tile_and_split_with_and_without_residual(cuda_device, rows: int, n: int, k: int) -> None:
+    q, s, wq, ws = _linear_inputs(rows, n, k)
+    y = ops.linear_fp8(q, s, wq, ws)
+    _linear_check(y, q, s, wq, ws)
+    r = torch.randn(rows, n + 8, device=cuda_device).to(torch.bfloat16)[:, :n]
+    z = ops.linear_fp8(q, s, wq, ws, epilogue=_lib.EPI_ADD, residual=r)
+    _linear_check(z, q, s, wq, ws, r)
+    buf = torch.full((rows + 1, n + 16), float("nan"), dtype=torch.bfloat16, device=cuda_device)
+    buf[:rows, :n] = r
+    ops.linear_fp8(q, s, wq, ws, epilogue=_lib.EPI_ADD, residual=buf[:rows, :n], out=buf[:rows, :n])
+    assert torch.equal(buf[:rows, :n], z)
+    assert bool(buf[:, n:].isnan().all()) and bool(buf[rows:].isnan().all())  # nothing beside it
+    ops.check_status(cuda_device)
+
+
 def test_nonfinite_values_show_in_their_rows_only(cuda_device) -> None:
     x = _rows(9, 768, 1).clone()
     x[2, 5], x[4, 300], x[6, 700] = float("nan"), float("inf"), -float("inf")
