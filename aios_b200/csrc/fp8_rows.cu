@@ -8,9 +8,8 @@
 //
 // Measured (GB/s of the bytes that have to move; a copy reaches 6520): norm with residual of
 // 16384 x 8192 137 us, 6850 GB/s; plain norm 79 us, 5130 GB/s (3 bytes a value where the
-// residual's form moves 7, so the arithmetic shows); SwiGLU of 12001 x 10240 100.5 us, 6110 GB/s (three
-// quarters of the issue slots taken); rows of 16384 x 8192 66 us, 6110 GB/s; weight of 16384
-// x 8192 60.5 us, 6650 GB/s.
+// residual's form moves 7, so the arithmetic shows); SwiGLU of 12001 x 10240 91 us, 6740 GB/s;
+// rows of 16384 x 8192 66 us, 6110 GB/s; weight of 16384 x 8192 60.5 us, 6650 GB/s.
 #include <algorithm>
 
 #include "abi_util.h"
@@ -129,9 +128,26 @@ void launch_norm(const NormArgs& a, cudaStream_t s) {
 }
 
 // ---- SwiGLU and the plain quantiser ---------------------------------------------
-// silu(g) * u with the hardware exponential and reciprocal (each within a few units
-// of 2^-23), far below the e4m3 rounding that follows; g < -88 gives g / inf = 0.
-__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+// silu(g) * u of two columns, with the hardware exponential and reciprocal (each within a few
+// units of 2^-23, the exponential's argument within 2^-24 of itself), far below the e4m3
+// rounding that follows. In their flushing forms: a subnormal e^-g vanishes beside 1, and a
+// subnormal reciprocal belongs to g < -87, which gives g * 0 (with their range checks, one column at
+// a time, the SwiGLU of 12001 x 10240 took 102 us).
+__device__ __forceinline__ float ex2_ftz(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_ftz(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float2 silu_mul2(float2 g, float2 u) {
+  const float2 t = __fmul2_rn(g, make_float2(-1.4426950408889634f, -1.4426950408889634f));  // log2(e)
+  const float2 d = __fadd2_rn(make_float2(1.f, 1.f), make_float2(ex2_ftz(t.x), ex2_ftz(t.y)));
+  return __fmul2_rn(__fmul2_rn(g, make_float2(rcp_ftz(d.x), rcp_ftz(d.y))), u);
+}
 
 // One 16-lane group per block of 128 columns: group index = row * blocks + block.
 // (rows * blocks stays below 2^31: that many blocks would be 275 G values.)
@@ -158,31 +174,28 @@ __global__ void __launch_bounds__(kThreads)
     gv[k] = in[k] ? ld16(p) : make_uint4(0, 0, 0, 0);
     if (SILU) uv[k] = in[k] ? ld16(p + cols) : make_uint4(0, 0, 0, 0);
   }
-  // All loads are in flight; the groups are then finished kStep at a time, as many as the
-  // registers of the arithmetic leave room for (SwiGLU of 12001 x 10240: four at once 118 us,
-  // two 100.5, one 101.5).
-  constexpr int kStep = SILU && UPT > 2 ? 2 : UPT;
+  float v[UPT][8], m[UPT];
 #pragma unroll
-  for (int k0 = 0; k0 < UPT; k0 += kStep) {
-    float v[kStep][8], m[kStep];
+  for (int k = 0; k < UPT; ++k) {
+    unpack8(gv[k], v[k]);
+    if (SILU) {
+      float u[8];
+      unpack8(uv[k], u);
 #pragma unroll
-    for (int k = 0; k < kStep; ++k) {
-      unpack8(gv[k0 + k], v[k]);
-      if (SILU) {
-        float u[8];
-        unpack8(uv[k0 + k], u);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[k][j] = silu_mul(v[k][j], u[j]);
+      for (int j = 0; j < 8; j += 2) {
+        const float2 y = silu_mul2(make_float2(v[k][j], v[k][j + 1]), make_float2(u[j], u[j + 1]));
+        v[k][j] = y.x;
+        v[k][j + 1] = y.y;
       }
-      m[k] = amax8_nan(v[k]);
     }
-    const HalfWarpScales<kStep> f(m);
-#pragma unroll
-    for (int k = 0; k < kStep; ++k)
-      if (in[k0 + k]) *reinterpret_cast<uint2*>(q + row[k0 + k] * cols + c[k0 + k]) = fp8_pack8(v[k], f.inv[k]);
-    const uint32_t g = g0 + (k0 + f.unit) * (kThreads / 16);
-    if (f.first && f.unit < kStep && g < groups) scale[g] = f.scale;
+    m[k] = amax8_nan(v[k]);
   }
+  const HalfWarpScales<UPT> f(m);
+#pragma unroll
+  for (int k = 0; k < UPT; ++k)
+    if (in[k]) *reinterpret_cast<uint2*>(q + row[k] * cols + c[k]) = fp8_pack8(v[k], f.inv[k]);
+  const uint32_t g = g0 + f.unit * (kThreads / 16);
+  if (f.first && f.unit < UPT && g < groups) scale[g] = f.scale;
 }
 
 template <bool SILU, int UPT>
@@ -193,18 +206,19 @@ void launch_rows_as(const __nv_bfloat16* x, int64_t x_stride, uint32_t groups, u
              blocks, cols, q, scale);
 }
 
-// Groups per thread: one while that spreads the work over the SMs, up to four once every SM
-// has several blocks, for the loads in flight (SwiGLU of 12001 x 10240 with 1, 2, 4, 8: 120,
-// 107, 100, 145 us; of 512 x 2048: 2.7, 2.3, 2.7 us; rows of 512 x 768: 1.3, 1.4, 1.8 us,
-// of 16384 x 8192: 84, 72, 66, 78 us).
+// Groups per thread, by the blocks of one group per thread that each SM gets: one while the SMs
+// hold them all at once, then more for the loads in flight. With 1 / 2 / 4, in us:
+//   SwiGLU of 1024 x 2048 (7 per SM) 3.5 / 4.0 / 4.0, 2048 x 2048 (14) 5.5 / 5.3 / 5.7,
+//   2048 x 4096 (28) 9.6 / 8.7 / 8.9, 4096 x 4096 (55) 17.5 / 15.7 / 15.4, 12001 x 10240 112 / 97 / 91;
+//   rows of 1024 x 2048 2.6 / 2.7 / 2.8, 2048 x 2048 4.1 / 4.1 / 3.9, 8192 x 8192 43 / 37 / 34.
 template <bool SILU>
 void launch_rows(const void* x, int64_t x_stride, int64_t rows, int64_t cols, void* q, float* scale, cudaStream_t s) {
   const uint32_t blocks = (uint32_t)((cols + kFp8Block - 1) / kFp8Block);
   const uint32_t groups = (uint32_t)rows * blocks;
   const uint32_t per_sm = groups / (kThreads / 16) / (uint32_t)sm_count();  // blocks of one group per thread
-  const auto launch = per_sm < 3   ? launch_rows_as<SILU, 1>
-                      : per_sm < 8 ? launch_rows_as<SILU, 2>
-                                   : launch_rows_as<SILU, 4>;
+  auto launch = per_sm < 10 ? launch_rows_as<SILU, 1> : launch_rows_as<SILU, 4>;
+  if constexpr (SILU)
+    if (per_sm >= 10 && per_sm < 40) launch = launch_rows_as<SILU, 2>;
   launch((const __nv_bfloat16*)x, x_stride, groups, blocks, (int)cols, (uint8_t*)q, scale, s);
 }
 
