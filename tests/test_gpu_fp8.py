@@ -115,7 +115,9 @@ def test_rmsnorm_fp8(cuda_device, rows: int, cols: int, residual: bool) -> None:
     _check_quantised(q, scale, v, 2.0**-18)
 
 
-@pytest.mark.parametrize("rows,f", [(1, 16), (8, 2048), (13, 144), (257, 1008), (3, 10240), (1000, 128)])
+# the last two: two and four groups of 128 columns to 16 lanes
+@pytest.mark.parametrize("rows,f", [(1, 16), (8, 2048), (13, 144), (257, 1008), (3, 10240), (1000, 128), (3001, 1040),
+                                    (5001, 2576)])
 def test_silu_and_mul_fp8(cuda_device, rows: int, f: int) -> None:
     x = _rows(rows, 2 * f, rows + f, 2 * f + 8)
     q, s = ops.silu_and_mul_fp8(x)
@@ -123,6 +125,24 @@ def test_silu_and_mul_fp8(cuda_device, rows: int, f: int) -> None:
     v = g * torch.sigmoid(g) * u
     v[g < -87] = 0  # documented: a gate below -87 gives 0
     _check_quantised(q, s, v, 2.0**-16)
+
+
+def test_silu_and_mul_fp8_of_extreme_gates(cuda_device) -> None:
+    """One gate to a block of 128, times a factor that brings small results back into range."""
+    gates = [0.0, -0.0, 1e-30, 20.0, 88.5, 3e38, -1.0, -20.0, -60.0, -86.5, -88.0, -100.0, -3e38]
+    x = torch.zeros(1, 2 * BLOCK * len(gates), dtype=torch.bfloat16, device=cuda_device)
+    f = BLOCK * len(gates)
+    for i, g in enumerate(gates):
+        x[0, i * BLOCK + 5] = g
+        x[0, f + i * BLOCK + 5] = 0.5 if g > 1 else 1e30 if g > -30 else 1e38
+    q, s = ops.silu_and_mul_fp8(x)
+    g, u = x[:, :f].double(), x[:, f:].double()
+    v = g / (1 + torch.exp(-g)) * u
+    v[g < -87] = 0  # documented: a gate below -87 gives 0
+    _check_quantised(q, s, v, 2.0**-16)
+    x[0, 5], x[0, BLOCK + 5], x[0, 2 * BLOCK + 5] = float("inf"), float("-inf"), float("nan")
+    q, s = ops.silu_and_mul_fp8(x)
+    assert float(s[0, 0]) == float("inf") and bool(s[0, 1:3].isnan().all()) and bool(s[0, 3:].isfinite().all())
 
 
 def _linear_check(y, q, s, wq, ws, residual=None) -> None:
@@ -139,6 +159,13 @@ def _linear_inputs(rows: int, n: int, k: int):
     q, s = ops.quantize_fp8(_rows(rows, k, rows + k))
     w = (torch.randn(n, k, generator=torch.Generator().manual_seed(n + k)) * 0.02).to(torch.bfloat16).cuda()
     return q, s, *ops.quantize_weight_fp8(w)
+
+
+def _wide(n: int, k: int):
+    """A quantised weight made in place on the device, for sizes that the host would be slow to make."""
+    w = torch.empty(n, k, dtype=torch.bfloat16, device="cuda")
+    w.normal_(std=0.02, generator=torch.Generator("cuda").manual_seed(n))
+    return ops.quantize_weight_fp8(w)
 
 
 # Sizes that the estimate gives to each kernel: 16, 32 and 64 tokens to a tile, 128 x 64 and
@@ -205,6 +232,48 @@ def test_each_tile_and_split_with_and_without_residual(cuda_device, rows: int, n
     assert torch.equal(buf[:rows, :n], z)
     assert bool(buf[:, n:].isnan().all()) and bool(buf[rows:].isnan().all())  # nothing beside it
     ops.check_status(cuda_device)
+
+
+def test_row_operators_past_32_bit_offsets(cuda_device) -> None:
+    """More than 2^31 values: the last rows equal those rows alone, bit for bit."""
+    rows, cols, tail = 65600, 32768, 5
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device=cuda_device)
+    last = _rows(tail, cols, 3).contiguous()
+    x[-tail:] = last
+    g = _rows(1, cols, 4)[0].contiguous()
+    cases = ((ops.quantize_fp8, ()), (ops.silu_and_mul_fp8, ()), (ops.rmsnorm_fp8, (g, 1e-6)),
+             (ops.quantize_weight_fp8, ()))
+    for op, more in cases:
+        own = tail if op is not ops.quantize_weight_fp8 else rows % BLOCK or BLOCK  # the last block of a weight
+        q, s = op(x, *more)
+        want, scale = op(x[-own:].contiguous(), *more)
+        assert torch.equal(q[-own:].view(torch.uint8), want.view(torch.uint8)), op.__name__
+        assert torch.equal(s[-scale.shape[0]:], scale), op.__name__
+        del q, s
+    r = torch.zeros_like(x)
+    r[-tail:] = last.flip(0)
+    q, s = ops.fused_add_rmsnorm_fp8(x, r, g, 1e-6)
+    alone = last.flip(0).contiguous()
+    want, scale = ops.fused_add_rmsnorm_fp8(last, alone, g, 1e-6)
+    assert torch.equal(q[-tail:].view(torch.uint8), want.view(torch.uint8)) and torch.equal(s[-tail:], scale)
+    assert torch.equal(r[-tail:], alone) and not bool(r[:-tail].any())
+
+
+@pytest.mark.parametrize("rows,n", [(65600, 32768), (16, 100000)])
+def test_linear_past_32_bit_offsets(cuda_device, rows: int, n: int) -> None:
+    """Outputs (65600 rows) or weight (100000 x 21504) of more than 2^31 values."""
+    k = 272 if rows > 16 else 21504
+    q, s, wq, ws = _linear_inputs(rows, n, k) if rows > 16 else (*ops.quantize_fp8(_rows(rows, k, 1)), *_wide(n, k))
+    y = ops.linear_fp8(q, s, wq, ws)
+    ops.check_status(cuda_device)
+    t = slice(max(0, rows - 40), rows)
+    w, v = wq[-512:], ws[-4:] if n % BLOCK == 0 else None
+    if v is None:  # whole blocks of the weight's end
+        first = n // BLOCK * BLOCK - 384
+        w, v, y = wq[first:], ws[first // BLOCK:], y[:, first:]
+    else:
+        y = y[:, -512:]
+    _linear_check(y[t], q[t], s[t], w, v)
 
 
 def test_nonfinite_values_show_in_their_rows_only(cuda_device) -> None:
