@@ -89,14 +89,20 @@ __device__ __forceinline__ uint4 residual8(const Fp8LinearArgs& a, int64_t row, 
 __device__ __forceinline__ uint2 residual4(const Fp8LinearArgs& a, int64_t row, int col) {
   return *reinterpret_cast<const uint2*>(a.residual + row * a.residual_stride + col);
 }
+__device__ __forceinline__ uint4 pack8(const float2* v) {
+  return make_uint4(pack_bf16x2(v[0].x, v[0].y), pack_bf16x2(v[1].x, v[1].y), pack_bf16x2(v[2].x, v[2].y),
+                    pack_bf16x2(v[3].x, v[3].y));
+}
+__device__ __forceinline__ uint4 add8(const float2* v, const uint4& residual) {
+  float r[8];
+  unpack8(residual, r);
+  return make_uint4(pack_bf16x2(v[0].x + r[0], v[0].y + r[1]), pack_bf16x2(v[1].x + r[2], v[1].y + r[3]),
+                    pack_bf16x2(v[2].x + r[4], v[2].y + r[5]), pack_bf16x2(v[3].x + r[6], v[3].y + r[7]));
+}
 template <bool RES>
 __device__ __forceinline__ void store8(const Fp8LinearArgs& a, int64_t row, int col, const float2* v,
                                        const uint4& residual) {
-  float r[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (RES) unpack8(residual, r);
-  *reinterpret_cast<uint4*>(a.y + row * a.y_stride + col) =
-      make_uint4(pack_bf16x2(v[0].x + r[0], v[0].y + r[1]), pack_bf16x2(v[1].x + r[2], v[1].y + r[3]),
-                 pack_bf16x2(v[2].x + r[4], v[2].y + r[5]), pack_bf16x2(v[3].x + r[6], v[3].y + r[7]));
+  *reinterpret_cast<uint4*>(a.y + row * a.y_stride + col) = RES ? add8(v, residual) : pack8(v);
 }
 template <bool RES>
 __device__ __forceinline__ void store4(const Fp8LinearArgs& a, int64_t row, int col, float4 v, const uint2& r) {

@@ -321,8 +321,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         t ^= 1;
       }
+      if (a.residual != nullptr) cp_async_wait_all();  // also where a wait ran out: nothing stays in flight
       if (!ok) break;
-      if (a.residual != nullptr) cp_async_wait_all();
       __syncwarp();
 #pragma unroll
       for (int c = 0; c < 16; ++c) {
