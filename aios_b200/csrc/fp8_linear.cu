@@ -20,14 +20,13 @@
 // the partial tiles are summed in rank order through distributed shared memory, so
 // results do not depend on scheduling.
 //
-// These tiles (128 x 64, two CTAs per SM, and 128 x 128) serve tens to hundreds of rows;
-// fp8_linear_few.cu has the shape for fewer, fp8_linear_pair.cu for more, and choose() below
-// picks. Measured: 77 x 10000 x 5008 16.8-17.9 us (its bytes take 8.0: 79 tiles leave half of the
-// SMs idle, and a fold warp's wait, TMEM loads and FMAs take 460 clocks per block of k in
-// the others; with k = 5120, rows on 128-byte lines, 14.2), 500 x 4096 x 768 6.6 us,
-// 256 x 4096 x 4096 11.2 us, 512 x 8192 x 8192 35 us (1930-1970 TFLOP/s). Loading the next
-// block's columns behind the last FMAs brought 2% at 77 x 10000 x 10240 and cost the 64-wide
-// tile 8%.
+// These 128 x 128 tiles serve tens to hundreds of rows; fp8_linear_few.cu has the shape for fewer,
+// fp8_linear_pair.cu for more, and choose() below picks. Measured: 77 x 10000 x 5008 16.8-17.9 us
+// (its bytes take 8.0: 79 tiles leave half of the SMs idle, and a fold warp's wait, TMEM loads
+// and FMAs take 460 clocks per block of k in the others; with k = 5120, rows on 128-byte lines,
+// 14.2), 500 x 4096 x 768 6.0 us, 256 x 4096 x 4096 11.2 us, 512 x 8192 x 8192 35-40 us (1700-1970
+// TFLOP/s, two rounds). Loading the next block's columns behind the last FMAs brought 2% at
+// 77 x 10000 x 10240 and nothing elsewhere.
 #include <string.h>
 
 #include <algorithm>
@@ -38,40 +37,26 @@
 namespace aiosb {
 namespace {
 
-// Shape of the kernel for tiles of BN columns.
-template <int BN>
-struct Shape {
-  static constexpr int kCols = BN == 64 ? 32 : 64;      // columns of one fold warp
-  static constexpr int kFoldWarps = 4 * (BN / kCols);   // 4 groups of 32 TMEM lanes
-  static constexpr int kThreads = (kFoldWarps + 4) * 32;
-  static constexpr int kAccs = 4;                       // TMEM accumulators in turn
-  // scale products: two groups of kScaleGroup blocks of k, 128 rows each
-  static constexpr int kScaleBytes = 2 * kScaleGroup * kBM * 4;
-  // MMA warps: a wait that is over and the issue behind it take about 500 clocks of a warp per
-  // block, the MMAs of 128 columns 256. Two warps in turn: 77 x 10000 x 10240 27.3 -> 23.9 us.
-  // With 64 columns two CTAs share the SM and one each is enough (two: 3% slower).
-  static constexpr int kIssuers = BN == 64 ? 1 : 2;
-  static constexpr int kCtas = BN == 64 ? 2 : 1;        // CTAs per SM (TMEM: kAccs * BN of 512 columns each)
-  // Where an SM has room for it (one stage less), a bf16 tile of staging: the residual comes
-  // into it while the products are formed, and rows leave it in whole lines. With a row to a
-  // lane, 16 bytes at a time: 500 x 4096 x 768 6.6 -> 6.0 us, with a residual 8.6 -> 6.8; 128 x 10240
-  // x 768 7.6 -> 6.1, with a residual 9.8 -> 6.8.
-  static constexpr bool kStaged = BN == 128;
-  static constexpr int kOutWarpBytes = 32 * kCols * 2;
-};
+constexpr int kBN = 128;                         // features per tile
+constexpr int kCols = 64;                        // columns of one fold warp
+constexpr int kFoldWarps = 4 * (kBN / kCols);    // 4 groups of 32 TMEM lanes
+constexpr int kThreads = (kFoldWarps + 4) * 32;
+constexpr int kAccs = 4;                         // TMEM accumulators in turn: all of tensor memory
+// scale products: two groups of kScaleGroup blocks of k, 128 rows each
+constexpr int kScaleBytes = 2 * kScaleGroup * kBM * 4;
+// A bf16 tile of staging, at the price of a stage: the residual comes into it while the products
+// are formed, and rows leave it in whole lines. With a row to a lane, 16 bytes at a time: 500 x
+// 4096 x 768 6.6 -> 6.0 us, with a residual 8.6 -> 6.8; 128 x 10240 x 768 7.6 -> 6.1, with a residual
+// 9.8 -> 6.8. (Tiles of 64 features, two CTAs to an SM, have no room for it and lost to these.)
+constexpr int kPieces = kCols / 8;               // 16-byte pieces of a fold warp's row
+constexpr int kOutWarpBytes = 32 * kCols * 2;
+constexpr int kRedStride = kBN + 4;              // floats per row of the partial tile: free of bank conflicts
 
-template <int BN, bool RES>
-__global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
+template <bool RES>
+__global__ void __launch_bounds__(kThreads, 1)
     linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                       const Fp8LinearArgs a) {
-  constexpr uint32_t kBBytes = BN * kBK;
-  constexpr int kCols = Shape<BN>::kCols, kFoldWarps = Shape<BN>::kFoldWarps, kThreads = Shape<BN>::kThreads;
-  constexpr int kAccs = Shape<BN>::kAccs, kIssuers = Shape<BN>::kIssuers;
-  // columns per tensor-memory load and loads in flight, by the registers a thread has
-  constexpr int kLd = BN == 128 ? 32 : 16, kLoads = BN == 128 ? 2 : 1;
-  constexpr bool kStaged = Shape<BN>::kStaged;
-  constexpr int kPieces = kCols / 8;   // 16-byte pieces of a fold warp's row
-  constexpr int kRedStride = BN + 4;   // floats per row of the partial tile: conflict-free 16-byte accesses
+  constexpr uint32_t kBBytes = kBN * kBK;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[kMaxStages], done[kMaxStages], acc_empty[kAccs], scale_full[2], scale_empty[2];
@@ -93,16 +78,16 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
       mbar_init(&full[s], 1);
       mbar_init(&done[s], 1);
     }
-    for (int s = 0; s < kAccs; ++s) mbar_init(&acc_empty[s], (uint32_t)lane_groups * (BN / kCols));
+    for (int s = 0; s < kAccs; ++s) mbar_init(&acc_empty[s], (uint32_t)lane_groups * (kBN / kCols));
     for (int s = 0; s < 2; ++s) {
       mbar_init(&scale_full[s], 1);
-      mbar_init(&scale_empty[s], (uint32_t)lane_groups * (BN / kCols));
+      mbar_init(&scale_empty[s], (uint32_t)lane_groups * (kBN / kCols));
     }
     abort_flag = 0;
     fence_mbar_init();
   }
   if (warp == kFoldWarps + 1) {
-    tmem_alloc(&tmem_slot, kAccs * BN);
+    tmem_alloc(&tmem_slot, kAccs * kBN);
     tmem_relinquish();
   }
   if (threadIdx.x == kFoldWarps * 32) {
@@ -133,7 +118,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
     uint32_t phase = 1;
     bool ok = true;
     for (int tile = blockIdx.x / split; tile < tiles && ok; tile += step) {
-      const int m0 = tile % a.m_tiles * kBM, n0 = tile / a.m_tiles * BN;
+      const int m0 = tile % a.m_tiles * kBM, n0 = tile / a.m_tiles * kBN;
       for (int kb = kb0; kb < kb1; ++kb) {
         ok = __all_sync(0xffffffffu, mbar_wait(&done[s], phase));
         if (!ok) break;
@@ -160,21 +145,23 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
         mbar_wait(&full[s], phase ^ 1);
       }
     }
-  } else if (warp == kFoldWarps + 1 || (kIssuers == 2 && warp == kFoldWarps + 3)) {
-    // ---- MMA issuers, taking blocks in turn. With fewer than 128 rows staged the A operand's unused rows are
+  } else if (warp == kFoldWarps + 1 || warp == kFoldWarps + 3) {
+    // ---- MMA issuers, two warps that take blocks in turn: a wait that is over and the issue
+    // behind it take about 500 clocks of a warp, the MMAs of a block 256 (77 x 10000 x 10240 with
+    // one warp 27.3 us, with two 23.9). With fewer than 128 rows staged the A operand's unused rows are
     // whatever follows the slot in shared memory (inside the allocation): a row of A
     // reaches its own TMEM lane only, and those lanes are not read.
     // One commit per block serves two readers of done[]: the producer (the stage's
     // operands are read) and the fold (the product is in TMEM). The fold cannot fall a
     // whole ring behind, because stages >= kAccs and an accumulator waits for its fold;
     // for the same reason one issuer is never more than kAccs blocks ahead of the other.
-    constexpr uint32_t idesc = umma_idesc_e4m3(kBM, BN);
+    constexpr uint32_t idesc = umma_idesc_e4m3(kBM, kBN);
     const uint64_t a_desc = umma_desc_sw128(smem_u32(smem_a)), b_desc = umma_desc_sw128(smem_u32(smem_b));
     int s = 0, t = 0;
     uint32_t phase = 0, acc_phase = 1;
     bool ok = true, mine = warp == kFoldWarps + 1;
     for (int tile = blockIdx.x / split; tile < tiles && ok; tile += step) {
-      for (int kb = kb0; kb < kb1; ++kb, mine = kIssuers == 1 || !mine) {
+      for (int kb = kb0; kb < kb1; ++kb, mine = !mine) {
         if (mine) {
           ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[t], acc_phase) && mbar_wait(&full[s], phase));
           if (!ok) break;
@@ -183,7 +170,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
           if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < kBK / 32; ++kk)
-              tc_mma_e4m3(tmem + t * BN, da + 2 * kk, db + 2 * kk, idesc, kk != 0);
+              tc_mma_e4m3(tmem + t * kBN, da + 2 * kk, db + 2 * kk, idesc, kk != 0);
             tc_commit(&done[s]);
           }
         }
@@ -207,7 +194,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
     uint32_t phase = 1;
     bool ok = true;
     for (int tile = blockIdx.x / split; tile < tiles && ok; tile += step) {
-      const int m0 = tile % a.m_tiles * kBM, n0 = tile / a.m_tiles * BN;
+      const int m0 = tile % a.m_tiles * kBM, n0 = tile / a.m_tiles * kBN;
       const float *sx[4], *const sw = a.w_scale + (int64_t)(min(n0, a.n - 1) / kFp8Block) * a.kblocks;
 #pragma unroll
       for (int i = 0; i < 4; ++i) sx[i] = a.x_scale + (int64_t)min(m0 + i * 32 + lane, a.rows - 1) * a.kblocks;
@@ -251,13 +238,13 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
     bool ok = true;
     for (int tile = blockIdx.x / split; tile < tiles && ok; tile += step) {
       const int64_t row = (int64_t)(tile % a.m_tiles) * kBM + tile_row;
-      const int c0 = tile / a.m_tiles * BN + part * kCols;
+      const int c0 = tile / a.m_tiles * kBN + part * kCols;
       // 16-byte piece `piece` of a row of this warp's 32 x kCols outputs; in the staging the
       // pieces of a row are permuted by the row, so that both directions are free of conflicts
       const int piece = lane & (kPieces - 1);
       const int64_t row0 = row - lane;
-      uint8_t* const out = smem_raw + a.scale_offset + Shape<BN>::kScaleBytes + warp * Shape<BN>::kOutWarpBytes;
-      if (kStaged && RES && split == 1) {  // the residual comes while the products are formed
+      uint8_t* const out = smem_raw + a.scale_offset + kScaleBytes + warp * kOutWarpBytes;
+      if (RES && split == 1) {  // the residual comes while the products are formed
         __syncwarp();  // the previous tile's rows have been read out
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
@@ -289,33 +276,29 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
           g ^= 1;
           if (g == 0) g_phase ^= 1;
         }
+        uint32_t d[kCols / 32][32];
 #pragma unroll
-        for (int c = 0; c < kCols; c += kLoads * kLd) {
-          uint32_t d[kLoads][kLd];
+        for (int l = 0; l < kCols / 32; ++l) tmem_ld(t_lane + t * kBN + l * 32, d[l]);
 #pragma unroll
-          for (int l = 0; l < kLoads; ++l) tmem_ld(t_lane + t * BN + c + l * kLd, d[l]);
+        for (int l = 0; l < kCols / 32; ++l) tmem_wait(d[l]);
+        // this block's values are in registers: the accumulator may be reused
+        tc_fence_before();
+        if (lane == 0) mbar_arrive(&acc_empty[t]);
 #pragma unroll
-          for (int l = 0; l < kLoads; ++l) tmem_wait(d[l]);
-          if (c + kLoads * kLd == kCols) {  // this block's values are in registers: the accumulator may be reused
-            tc_fence_before();
-            if (lane == 0) mbar_arrive(&acc_empty[t]);
-          }
-#pragma unroll
-          for (int j = 0; j < kLoads * kLd / 2; ++j)
-            acc[c / 2 + j] = __ffma2_rn(s,
-                                        make_float2(__uint_as_float(d[2 * j / kLd][2 * j % kLd]),
-                                                    __uint_as_float(d[2 * j / kLd][2 * j % kLd + 1])),
-                                        acc[c / 2 + j]);
-        }
+        for (int j = 0; j < kCols / 2; ++j)
+          acc[j] = __ffma2_rn(s,
+                              make_float2(__uint_as_float(d[j / 16][2 * j % 32]),
+                                          __uint_as_float(d[j / 16][2 * j % 32 + 1])),
+                              acc[j]);
         if (++ring == a.stages) {
           ring = 0;
           phase ^= 1;
         }
         if (++t == kAccs) t = 0;
       }
-      if (kStaged && RES) cp_async_wait_all();  // also where a wait ran out: nothing stays in flight
+      if (RES) cp_async_wait_all();  // also where a wait ran out: nothing stays in flight
       if (!ok) break;
-      if (kStaged && split == 1) {
+      if (split == 1) {
         __syncwarp();  // copies of every lane have landed, and the previous tile's rows are out
 #pragma unroll
         for (int j = 0; j < kPieces; ++j) {
@@ -329,19 +312,6 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
           if (row0 + r < a.rows && c0 + 8 * piece < a.n)
             *reinterpret_cast<uint4*>(a.y + (row0 + r) * a.y_stride + c0 + 8 * piece) =
                 *reinterpret_cast<const uint4*>(out + r * (kCols * 2) + ((piece ^ (r & 7)) << 4));
-        }
-      } else if (split == 1) {
-        if (row < a.rows) {
-#pragma unroll
-          for (int h = 0; h < kCols / 8; h += 4) {
-            uint4 res[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (RES && c0 + 8 * (h + j) < a.n) res[j] = residual8(a, row, c0 + 8 * (h + j));
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (c0 + 8 * (h + j) < a.n) store8<RES>(a, row, c0 + 8 * (h + j), acc + 4 * (h + j), res[j]);
-          }
         }
       } else if (tile_row < a.a_rows) {
         // every MMA of this CTA has read its operands: the partial tile takes their place
@@ -358,15 +328,15 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
   if (split > 1) {
     // Rank r sums and stores every split-th row: a warp reads whole lines of its peers'
     // partial tiles (16-byte pieces of many rows took four times as long).
-    constexpr int kUnits = (kBM / 2 * (BN / 4) + kThreads - 1) / kThreads;  // of a thread, at most
+    constexpr int kUnits = (kBM / 2 * (kBN / 4) + kThreads - 1) / kThreads;  // of a thread, at most
     const int tile = blockIdx.x / split;
-    const int m0 = tile % a.m_tiles * kBM, n0 = tile / a.m_tiles * BN;
-    const int units = (min(a.rows - m0, kBM) - rank + split - 1) / split * (BN / 4);
+    const int m0 = tile % a.m_tiles * kBM, n0 = tile / a.m_tiles * kBN;
+    const int units = (min(a.rows - m0, kBM) - rank + split - 1) / split * (kBN / 4);
     uint2 res[kUnits];
     if (RES) {
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) {
-        const int u = threadIdx.x + i * kThreads, r = u / (BN / 4) * split + rank, c = u % (BN / 4) * 4;
+        const int u = threadIdx.x + i * kThreads, r = u / (kBN / 4) * split + rank, c = u % (kBN / 4) * 4;
         if (u < units && n0 + c < a.n) res[i] = residual4(a, m0 + r, n0 + c);
       }
     }
@@ -375,7 +345,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
       const uint32_t base = smem_u32(smem);
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) {
-        const int u = threadIdx.x + i * kThreads, r = u / (BN / 4) * split + rank, c = u % (BN / 4) * 4;
+        const int u = threadIdx.x + i * kThreads, r = u / (kBN / 4) * split + rank, c = u % (kBN / 4) * 4;
         if (u < units && n0 + c < a.n)
           store4<RES>(a, m0 + r, n0 + c, sum_ranks4(base + (uint32_t)(r * kRedStride + c) * 4, split), res[i]);
       }
@@ -384,7 +354,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, Shape<BN>::kCtas)
   }
   if (warp == kFoldWarps + 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, kAccs * BN);
+    tmem_dealloc(tmem, kAccs * kBN);
   }
 }
 
@@ -425,26 +395,23 @@ int fp8_tensor_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols,
 
 namespace {
 
-template <int BN, bool RES>
+template <bool RES>
 int launch(const CUtensorMap& tx, const CUtensorMap& tw, Fp8LinearArgs a, cudaStream_t stream) {
-  constexpr int kOne = 224 * 1024;  // shared memory of a CTA that has the SM to itself
-  constexpr int kCtas = Shape<BN>::kCtas, kBudget = kCtas == 2 ? kOne / 2 - 1024 : kOne;
-  constexpr int kScaleBytes = Shape<BN>::kScaleBytes;
-  auto kern = linear_fp8_kernel<BN, RES>;
+  constexpr int kBudget = 224 * 1024;  // one CTA per SM
+  auto kern = linear_fp8_kernel<RES>;
   static bool configured[64] = {false};
   const int rc = fp8_configure(kern, kBudget, configured);
   if (rc != AIOSB_OK) return rc;
-  const int stage_bytes = a.a_rows * kBK + BN * kBK;
-  const int out_bytes =
-      Shape<BN>::kStaged && a.split == 1 ? Shape<BN>::kFoldWarps * Shape<BN>::kOutWarpBytes : 0;
-  const int tiles = a.m_tiles * a.n_tiles, slots = sm_count() * kCtas;
+  const int stage_bytes = a.a_rows * kBK + kBN * kBK;
+  const int out_bytes = a.split == 1 ? kFoldWarps * kOutWarpBytes : 0;
+  const int tiles = a.m_tiles * a.n_tiles, slots = sm_count();
   const int per_cta = (a.kblocks + a.split - 1) / a.split * (a.split > 1 ? 1 : (tiles + slots - 1) / slots);
-  a.stages = std::max(Shape<BN>::kAccs,
-                      std::min({(kBudget - 1024 - kScaleBytes - out_bytes) / stage_bytes, kMaxStages, per_cta}));
+  a.stages =
+      std::max(kAccs, std::min({(kBudget - 1024 - kScaleBytes - out_bytes) / stage_bytes, kMaxStages, per_cta}));
   // at least the partial tile, and 16 KB past the last A slot (the B slots have that)
-  const int body = std::max(a.stages * stage_bytes, a.split > 1 ? a.a_rows * (BN + 4) * 4 : 0);
+  const int body = std::max(a.stages * stage_bytes, a.split > 1 ? a.a_rows * kRedStride * 4 : 0);
   a.scale_offset = body + 1024;
-  return fp8_launch(kern, a.split > 1 ? tiles * a.split : std::min(tiles, slots), Shape<BN>::kThreads,
+  return fp8_launch(kern, a.split > 1 ? tiles * a.split : std::min(tiles, slots), kThreads,
                     body + 1024 + kScaleBytes + out_bytes, a.split, stream, tx, tw, a);
 }
 
@@ -452,17 +419,15 @@ int launch(const CUtensorMap& tx, const CUtensorMap& tw, Fp8LinearArgs a, cudaSt
 // Which tile, and how many ways k is split, by an estimate of the time of each: a start,
 // a time per 128-wide block of k (more where two CTAs share an SM, and where the grid
 // needs several rounds), and the cluster's cost where k is split. The figures were fitted
-// to sweeps on a B200 of 495 sizes (1 to 4096 rows, k of 128 to 14336). On 144 sizes of
-// other rows and weights the choice was within 5% of the best of its options in 136 and
-// within 12% in all. Some of both sides, in us:
+// to a sweep on a B200 of 272 sizes (8 to 2500 rows, 16 weights). Some of both sides, in us:
 //   1 x 768 x 2048:     16-token tiles split in 8 3.1, in 4 3.5, whole 4.8
-//   512 x 768 x 768:    32-token tiles 3.5, 64-token 4.1, 128 x 64 tiles 5.0, the pair 6.4
+//   512 x 768 x 768:    32-token tiles 3.5, 64-token 4.1
 //   128 x 768 x 2048:   32-token tiles split in 4 4.5, whole 5.8; 64-token in 4 5.3
-//   100 x 11008 x 256:  64-token tiles 4.4, 128 x 128 tiles 5.0, the pair 5.8
-//   77 x 10000 x 5008:  128 x 128 tiles 16.9, 128 x 64 21.8, 64-token 26.2
+//   128 x 10240 x 768:  128 x 128 tiles 6.1, 64-token tiles 6.6, the pair 8.0
+//   77 x 10000 x 5008:  128 x 128 tiles 16.9, 64-token 26.2
 //   300 x 1536 x 8960:  64-token tiles split in 4 14.3; 128 x 128 in 2 14.9, in 4 20.6
-//   256 x 4096 x 4096:  128 x 128 tiles in 2 11.5, whole 12.6; 128 x 64 whole 12.7
-//   512 x 4096 x 4096:  128 x 128 tiles 13.1, the pair 17.9
+//   256 x 4096 x 4096:  128 x 128 tiles in 2 11.2, whole 12.6
+//   512 x 4096 x 4096:  128 x 128 tiles 12.4, the pair 17.9
 //   1024 x 4096 x 4096: the pair 19.1, 128 x 128 tiles 23.9
 enum Kind { kFew, kTile, kPair };
 struct ShapeCost {
@@ -473,12 +438,11 @@ struct ShapeCost {
   float block, block_shared, block_rounds;
 };
 constexpr ShapeCost kShapes[] = {
-    {kFew, 16, 128, 2, 2.61f, 0.f, 0.194f, 0.317f, 0.303f},
-    {kFew, 32, 128, 2, 2.58f, 0.f, 0.231f, 0.337f, 0.454f},
-    {kFew, 64, 128, 2, 2.82f, 0.f, 0.325f, 0.529f, 0.60f},
-    {kTile, 128, 64, 2, 2.63f, 0.0053f, 0.309f, 0.388f, 0.55f},
-    {kTile, 128, 128, 1, 3.19f, 0.0126f, 0.286f, 0.286f, 0.329f},
-    {kPair, 256, 256, 0, 4.64f, 0.f, 0.569f, 0.569f, 0.50f},
+    {kFew, 16, 128, 2, 2.38f, 0.f, 0.201f, 0.308f, 0.303f},
+    {kFew, 32, 128, 2, 2.81f, 0.f, 0.238f, 0.344f, 0.396f},
+    {kFew, 64, 128, 2, 2.82f, 0.f, 0.292f, 0.477f, 0.60f},
+    {kTile, 128, 128, 1, 2.68f, 0.0059f, 0.286f, 0.286f, 0.355f},
+    {kPair, 256, 256, 0, 5.19f, 0.f, 0.407f, 0.407f, 0.517f},
 };
 struct Choice {
   const ShapeCost* shape;
@@ -502,7 +466,7 @@ Choice choose(int64_t rows, int64_t n, int kblocks, int sms) {
       const bool crowded = c.per_sm == 2 && ctas > reach;
       const float block = rounds > 1.f ? c.block_rounds : crowded ? c.block_shared : c.block;
       float us = c.start + c.start_per_row * live + (crowded ? 1.1f : 0.f) +
-                 rounds * ((float)((kblocks + split - 1) / split) * block + 0.52f) - 0.52f;
+                 rounds * ((float)((kblocks + split - 1) / split) * block + 0.54f) - 0.54f;
       if (split > 1) us += 1.32f + 0.0036f * live * (float)split;
       us = std::max(us, weight_us) + 0.1f * us;
       if (us < best_us) {
@@ -566,12 +530,10 @@ extern "C" int aiosb_linear_fp8(const void* x, int64_t x_row_stride, const float
   a.split = c.split;
   if (c.shape->kind == kFew) return fp8_linear_few(c.shape->rows, x, x_row_stride, k, w, a, s);
   if (c.shape->kind == kPair) return fp8_linear_pair(x, x_row_stride, k, w, a, s);
-  const int bn = c.shape->cols;
-  a.n_tiles = (int)((n + bn - 1) / bn);
+  a.n_tiles = (int)((n + kBN - 1) / kBN);
   CUtensorMap tx, tw;
   int rc = fp8_tensor_map(&tx, x, rows, k, x_row_stride, (uint32_t)a.a_rows);
-  if (rc == AIOSB_OK) rc = fp8_tensor_map(&tw, w, n, k, k, (uint32_t)bn);
+  if (rc == AIOSB_OK) rc = fp8_tensor_map(&tw, w, n, k, k, kBN);
   if (rc != AIOSB_OK) return rc;
-  if (a.residual != nullptr) return bn == 128 ? launch<128, true>(tx, tw, a, s) : launch<64, true>(tx, tw, a, s);
-  return bn == 128 ? launch<128, false>(tx, tw, a, s) : launch<64, false>(tx, tw, a, s);
+  return a.residual != nullptr ? launch<true>(tx, tw, a, s) : launch<false>(tx, tw, a, s);
 }

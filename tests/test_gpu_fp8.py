@@ -168,8 +168,8 @@ def _wide(n: int, k: int):
     return ops.quantize_weight_fp8(w)
 
 
-# Sizes that the estimate gives to each kernel: 16, 32 and 64 tokens to a tile, 128 x 64 and
-# 128 x 128 tiles, the pair of SMs; k whole and split in 2, 4 and 8; tiles cut by rows, n and k.
+# Sizes that the estimate gives to each kernel: 16, 32 and 64 tokens to a tile, 128 x 128 tiles,
+# the pair of SMs; k whole and split in 2, 4 and 8; tiles cut by rows, n and k.
 LINEARS = [(r, n, k) for r in (1, 8, 33, 128, 129, 300) for n, k in ((8, 16), (136, 144), (1280, 768), (776, 2064))]
 LINEARS += [(1, 4104, 1024), (77, 1000, 5008), (64, 128, 8192), (500, 4096, 768), (1024, 2440, 144), (1100, 2432, 768),
             (2048, 2568, 144), (2040, 2560, 1040), (4096, 4096, 272), (513, 16384, 768), (16, 104, 128),
@@ -209,13 +209,14 @@ def test_linear_fp8_add_and_strides(cuda_device, rows: int, n: int, k: int) -> N
 
 
 # One size or more for each tile and each split of k, with and without a residual (instances
-# of their own): 16-, 32- and 64-token tiles, 128 x 64, 128 x 128, the pair.
+# of their own): 16-, 32- and 64-token tiles, 128 x 128 (also several to a CTA), the pair.
 EACH = [(3, 1064, 560), (1, 4280, 1696), (8, 2288, 4432), (13, 552, 2112), (16, 264, 4512)]
 EACH += [(18, 72, 144), (355, 272, 1760), (45, 1040, 2720), (18, 488, 2528), (21, 64, 1568)]
 EACH += [(957, 520, 160), (482, 608, 3760), (80, 1584, 4704), (35, 1056, 5936)]
 EACH += [(1370, 824, 144), (359, 3096, 1472), (947, 576, 2160), (34, 2112, 1872), (355, 264, 10032), (43, 912, 7888)]
 EACH += [(795, 1424, 416), (216, 6664, 1808), (693, 792, 3472), (633, 424, 5216), (66, 1440, 7312)]
-EACH += [(711, 3152, 144)]
+EACH += [(711, 3152, 144), (459, 616, 2448), (150, 2456, 4560), (2242, 1056, 528), (284, 8432, 2736)]
+EACH += [(2500, 1400, 272), (300, 16392, 144)]
 
 
 @pytest.mark.parametrize("rows,n,k", EACH)
