@@ -10,12 +10,11 @@
 // costs one FMA per value. Four TMEM accumulators take turns: the tensor cores work
 // on the next blocks while the warps fold one.
 //
-// Per CTA: the first 8 warps fold (warp w: lanes 32 (w % 4).., columns w / 4). Of the
-// four warps after them one lane loads tiles by TMA into a ring of stages, one issues the
-// MMAs, and a third warp forms the products sx * sw (in fp32) eight blocks of k at a time
-// and hands them over in shared memory: read by the folding threads themselves, each
-// row's scale is a cache line of its own, and fetching 32 lines per warp and block took as
-// long as the MMAs.
+// Per CTA: the first 8 warps fold (warp w: lanes 32 (w % 4).., columns w / 4). Of the four
+// warps after them one loads tiles by TMA into a ring of stages, two issue the MMAs in turn,
+// and one forms the products sx * sw (in fp32) eight blocks of k at a time and hands them
+// over in shared memory: read by the folding threads themselves, each row's scale is a cache
+// line of its own, and fetching 32 lines per warp and block took as long as the MMAs.
 // Few rows leave few tiles: then a cluster of up to 8 CTAs splits the blocks of k and
 // the partial tiles are summed in rank order through distributed shared memory, so
 // results do not depend on scheduling.
