@@ -152,10 +152,13 @@ __device__ __forceinline__ float2 silu_mul2(float2 g, float2 u) {
 // One 16-lane group per block of 128 columns: group index = row * blocks + block.
 // (rows * blocks stays below 2^31: that many blocks would be 275 G values.)
 // UPT groups per thread, kThreads / 16 apart, to keep more loads in flight.
+// x is not `const __restrict__`, here and in the weight's quantiser: the grid may start while
+// its predecessor still writes x, and a load that is declared read-only for the grid's whole
+// life need not stay behind pdl_wait().
 template <bool SILU, int UPT>
 __global__ void __launch_bounds__(kThreads)
-    rows_fp8_kernel(const __nv_bfloat16* __restrict__ x, int64_t x_stride, uint32_t groups, uint32_t blocks, int cols,
-                    uint8_t* __restrict__ q, float* __restrict__ scale) {
+    rows_fp8_kernel(const __nv_bfloat16* x, int64_t x_stride, uint32_t groups, uint32_t blocks, int cols, uint8_t* q,
+                    float* scale) {
   pdl_wait();
   if (threadIdx.x < 32) pdl_launch_dependents();
   const int lane16 = threadIdx.x & 15;
@@ -227,8 +230,7 @@ void launch_rows(const void* x, int64_t x_stride, int64_t rows, int64_t cols, vo
 // loads in flight before the block's maximum. It lets no kernel launch early: the
 // linears that read the weight may be the next launch.
 __global__ void __launch_bounds__(kThreads)
-    weight_fp8_kernel(const __nv_bfloat16* __restrict__ w, int64_t w_stride, int64_t n, int64_t k,
-                      uint8_t* __restrict__ q, float* __restrict__ scale) {
+    weight_fp8_kernel(const __nv_bfloat16* w, int64_t w_stride, int64_t n, int64_t k, uint8_t* q, float* scale) {
   pdl_wait();
   __shared__ float part[kThreads / 32];
   constexpr int kPasses = kFp8Block / (kThreads / 16);

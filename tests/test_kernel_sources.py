@@ -1,0 +1,44 @@
+"""Rules that the kernels' sources keep and that no run on a GPU would show reliably.
+
+Kernels launched with programmatic dependent launch may be running while their predecessor
+still writes what they read. Their loads stay behind ``griddepcontrol.wait`` because its
+``memory`` clobber orders them; a ``const T* __restrict__`` parameter tells the compiler that
+the data is read-only for the grid's whole life, and such a load may move ahead of the wait.
+"""
+
+from __future__ import annotations
+
+import re
+from pathlib import Path
+
+import pytest
+
+CSRC = Path(__file__).resolve().parents[1] / "aios_b200" / "csrc"
+FILES = ["fp8_rows.cu", "fp8_linear.cu", "fp8_linear_few.cu", "fp8_linear_pair.cu"]
+
+
+def _kernels(text: str) -> list[tuple[str, str, str]]:
+    """(name, parameters, body) of every __global__ function."""
+    out = []
+    for m in re.finditer(r"__global__\s+void\s+(?:__launch_bounds__\s*\((?:[^()]|\([^()]*\))*\)\s*)?(\w+)\s*\(", text):
+        depth, at = 1, m.end()
+        while depth:
+            depth += {"(": 1, ")": -1}.get(text[at], 0)
+            at += 1
+        start = text.index("{", at)
+        depth, end = 1, start + 1
+        while depth:
+            depth += {"{": 1, "}": -1}.get(text[end], 0)
+            end += 1
+        out.append((m.group(1), text[m.end() : at - 1], text[start:end]))
+    return out
+
+
+@pytest.mark.parametrize("name", FILES)
+def test_inputs_of_dependent_launches_are_not_declared_read_only(name: str) -> None:
+    kernels = _kernels((CSRC / name).read_text())
+    assert kernels and any("pdl_wait()" in body or "pdl_enter()" in body for _, _, body in kernels)
+    for kernel, parameters, body in kernels:
+        if "pdl_wait()" in body or "pdl_enter()" in body:
+            bad = re.findall(r"const\s+[\w:]+\s*\*\s*__restrict__\s+(\w+)", parameters)
+            assert not bad, f"{kernel}: {bad}"
