@@ -282,6 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int l = 0; l < kCols / 32; ++l) tmem_wait(d[l]);
         // this block's values are in registers: the accumulator may be reused
         tc_fence_before();
+        __syncwarp();
         if (lane == 0) mbar_arrive(&acc_empty[t]);
 #pragma unroll
         for (int j = 0; j < kCols / 2; ++j)

@@ -223,6 +223,7 @@ __global__ void __launch_bounds__(Few<TN>::kThreads, 2)
         s[j] = *reinterpret_cast<const float4*>(my_scales + (g * kScaleGroup + in_group) * TN + 4 * j);
       tmem_wait(d);
       tc_fence_before();
+      __syncwarp();
       if (lane == 0) mbar_arrive(&acc_empty[t]);
 #pragma unroll
       for (int j = 0; j < kCols / 4; ++j) {

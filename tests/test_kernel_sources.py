@@ -4,6 +4,9 @@ Kernels launched with programmatic dependent launch may be running while their p
 still writes what they read. Their loads stay behind ``griddepcontrol.wait`` because its
 ``memory`` clobber orders them; a ``const T* __restrict__`` parameter tells the compiler that
 the data is read-only for the grid's whole life, and such a load may move ahead of the wait.
+
+Where one lane arrives on a barrier for its warp, the other lanes' reads are ordered before
+the arrival by a ``__syncwarp()`` only.
 """
 
 from __future__ import annotations
@@ -42,3 +45,11 @@ def test_inputs_of_dependent_launches_are_not_declared_read_only(name: str) -> N
         if "pdl_wait()" in body or "pdl_enter()" in body:
             bad = re.findall(r"const\s+[\w:]+\s*\*\s*__restrict__\s+(\w+)", parameters)
             assert not bad, f"{kernel}: {bad}"
+
+
+@pytest.mark.parametrize("name", sorted(p.name for p in CSRC.glob("*.cu")))
+def test_a_lane_that_arrives_for_its_warp_follows_the_others(name: str) -> None:
+    lines = [line.strip() for line in (CSRC / name).read_text().splitlines()]
+    for i, line in enumerate(lines):
+        if re.match(r"if \(lane == 0\) mbar_arrive\w*\(", line):
+            assert lines[i - 1] == "__syncwarp();", f"line {i + 1}: {line}"
