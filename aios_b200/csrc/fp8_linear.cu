@@ -12,9 +12,10 @@
 //
 // Per CTA: the first 8 warps fold (warp w: lanes 32 (w % 4).., columns w / 4). Of the four
 // warps after them one loads tiles by TMA into a ring of stages, two issue the MMAs in turn,
-// and one forms the products sx * sw (in fp32) eight blocks of k at a time and hands them
-// over in shared memory: read by the folding threads themselves, each row's scale is a cache
-// line of its own, and fetching 32 lines per warp and block took as long as the MMAs.
+// and one forms the products sx * sw eight blocks of k at a time (in fp32; split_scales has
+// those that fp32 does not hold) and hands them over in shared memory: read by the folding
+// threads themselves, each row's scale is a cache line of its own, and fetching 32 lines per
+// warp and block took as long as the MMAs.
 // Few rows leave few tiles: then a cluster of up to 8 CTAs splits the blocks of k and
 // the partial tiles are summed in rank order through distributed shared memory, so
 // results do not depend on scheduling.
@@ -30,6 +31,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "fp8_linear.cuh"
 
@@ -59,7 +61,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[kMaxStages], done[kMaxStages], acc_empty[kAccs], scale_full[2], scale_empty[2];
-  __shared__ uint32_t tmem_slot;
+  __shared__ uint32_t tmem_slot, far_blocks[2];
   __shared__ volatile int abort_flag;
 
   // the shuffle tells the compiler that the warp index, and every branch on it, is uniform
@@ -207,15 +209,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < kScaleGroup; ++j) {
           const bool in = kb + j < kb1;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i][j] = in && i < lane_groups ? sx[i][kb + j] : 0.f;
-          w[j] = in ? sw[kb + j] : 0.f;
+          for (int i = 0; i < 4; ++i) x[i][j] = in && i < lane_groups ? sx[i][kb + j] : 1.f;
+          w[j] = in ? sw[kb + j] : 1.f;
         }
+        auto store = [&](int i, int j, float product, float) {
+          if (i < lane_groups) scales[(g * kScaleGroup + j) * kBM + i * 32 + lane] = product;
+        };
+        ScaleRange range;
 #pragma unroll
         for (int j = 0; j < kScaleGroup; ++j) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (i < lane_groups) scales[(g * kScaleGroup + j) * kBM + i * 32 + lane] = x[i][j] * w[j];
+          for (int i = 0; i < 4; ++i) {
+            const float p = x[i][j] * w[j];
+            range.add(p);
+            store(i, j, p, 1.f);
+          }
         }
+        uint32_t blocks = 0;
+        if (__any_sync(0xffffffffu, range.far())) blocks = split_group(sx, sw, kb, min(kScaleGroup, kb1 - kb), store);
+        if (lane == 0) far_blocks[g] = blocks;
         __syncwarp();
         if (lane == 0) mbar_arrive(&scale_full[g]);
         g ^= 1;
@@ -256,25 +268,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       float2 acc[kCols / 2];  // pairs of neighbouring columns: one packed FMA each
 #pragma unroll
       for (int j = 0; j < kCols / 2; ++j) acc[j] = make_float2(0.f, 0.f);
-      int in_group = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        ok = (in_group != 0 || mbar_wait(&scale_full[g], g_phase)) && mbar_wait(&done[ring], phase);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) {
-          report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
-          abort_flag = 1;
-          break;
-        }
+      // One block of k; `far`: the group has products of scales that split_scales divides.
+      auto fold_block = [&](int kb, int in_group, auto far) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&done[ring], phase));
+        if (!ok) return;
         tc_fence_after();
         const float s1 = my_scales[(g * kScaleGroup + in_group) * kBM];
         const float2 s = make_float2(s1, s1);
-        if (++in_group == kScaleGroup || kb + 1 == kb1) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&scale_empty[g]);
-          in_group = 0;
-          g ^= 1;
-          if (g == 0) g_phase ^= 1;
-        }
         uint32_t d[kCols / 32][32];
 #pragma unroll
         for (int l = 0; l < kCols / 32; ++l) tmem_ld(t_lane + t * kBN + l * 32, d[l]);
@@ -284,6 +284,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&acc_empty[t]);
+        if (far && ((far_blocks[g] >> in_group) & 1)) {
+          float first, second;
+          split_scales(a.x_scale[min(row, (int64_t)a.rows - 1) * a.kblocks + kb],
+                       a.w_scale[(int64_t)(min(c0, a.n - 1) / kFp8Block) * a.kblocks + kb], &first, &second);
+#pragma unroll
+          for (int l = 0; l < kCols / 32; ++l) scale_all(d[l], first);
+        }
 #pragma unroll
         for (int j = 0; j < kCols / 2; ++j)
           acc[j] = __ffma2_rn(s,
@@ -295,6 +302,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           phase ^= 1;
         }
         if (++t == kAccs) t = 0;
+      };
+      for (int kb = kb0; kb < kb1 && ok; kb += kScaleGroup) {
+        const int count = min(kScaleGroup, kb1 - kb);
+        ok = __all_sync(0xffffffffu, mbar_wait(&scale_full[g], g_phase));
+        if (ok && far_blocks[g] == 0) {
+#pragma unroll 1
+          for (int j = 0; j < count && ok; ++j) fold_block(kb + j, j, std::false_type());
+        } else {
+#pragma unroll 1
+          for (int j = 0; j < count && ok; ++j) fold_block(kb + j, j, std::true_type());
+        }
+        if (!ok) {
+          report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
+          abort_flag = 1;
+          break;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&scale_empty[g]);
+        g ^= 1;
+        if (g == 0) g_phase ^= 1;
       }
       if (RES) cp_async_wait_all();  // also where a wait ran out: nothing stays in flight
       if (!ok) break;

@@ -2,6 +2,8 @@
 // only they use, and the epilogue's store.
 #pragma once
 
+#include <float.h>
+
 #include "abi_util.h"
 #include "fp8.cuh"
 
@@ -134,6 +136,58 @@ __device__ __forceinline__ float4 sum_ranks4(uint32_t off, int split) {
     }
   }
   return v;
+}
+
+// ---- scales ------------------------------------------------------------------------
+// A block's product d (0, or 2^-18 to 448 * 448 * 128) counts x * w * d, with x * w formed once
+// for all of its values. Where x * w overflows, or falls so low that its rounding to a subnormal
+// would show (below 2^-134 it is off by more than 2^-16 of itself), the scales are applied one
+// after the other instead: d * first keeps in range with the smaller one first where x * w is
+// too large, with the larger one first where it is too small. (Below 2^-176 no d brings the
+// product back into fp32.) A value's bits do not depend on its neighbours' scales: d * 1 is d.
+// The range of the products that a lane forms, in two instructions each (a comparison of each
+// product with both limits kept the scale warp behind the fold: 256 x 4096 x 4096 11.3 -> 13.1 us).
+struct ScaleRange {
+  float lo = 1.f, hi = 1.f;
+  __device__ __forceinline__ void add(float p) {
+    lo = fminf(lo, fabsf(p));
+    hi = fmaxf(hi, fabsf(p));
+  }
+  __device__ __forceinline__ bool far() const { return lo < 0x1p-134f || hi > FLT_MAX; }
+};
+__device__ __forceinline__ void split_scales(float x, float w, float* first, float* second) {
+  const float p = x * w, lo = fminf(fabsf(x), fabsf(w)), hi = fmaxf(fabsf(x), fabsf(w));
+  const bool over = fabsf(p) > FLT_MAX && hi <= FLT_MAX;  // not where a scale itself is infinite or NaN
+  const bool under = fabsf(p) < 0x1p-134f && lo * 0x1p26f * hi != 0.f;
+  const bool x_first = over == (fabsf(x) == lo);
+  *first = !(over || under) ? 1.f : x_first ? x : w;
+  *second = !(over || under) ? p : x_first ? w : x;
+}
+template <int N>
+__device__ __forceinline__ void scale_all(uint32_t (&d)[N], float first) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) d[j] = __float_as_uint(__uint_as_float(d[j]) * first);
+}
+// The blocks (bits) among `count` from `kb` on whose products need split_scales in any of the
+// warp's rows (kRows a lane); their factors go to store(row, block, second, first). Reads the
+// scales again: the caller keeps none of them in registers for a case that hardly occurs.
+template <int kRows, typename Store>
+__device__ __forceinline__ uint32_t split_group(const float* const (&sx)[kRows], const float* sw, int kb, int count,
+                                                Store store) {
+  uint32_t blocks = 0;
+#pragma unroll 1
+  for (int j = 0; j < count; ++j) {
+    bool split = false;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      float first, second;
+      split_scales(sx[i][kb + j], sw[kb + j], &first, &second);
+      split |= first != 1.f;
+      store(i, j, second, first);
+    }
+    blocks |= (uint32_t)__any_sync(0xffffffffu, split) << j;
+  }
+  return blocks;
 }
 
 // One lane of a converged warp.

@@ -13,6 +13,7 @@
 // weight byte once). A short k is latency: 8 x 1280 x 768 2.9 us and 8 x 768 x 2048 3.1 us in
 // a chain of launches, for 0.15 and 0.24 us of bytes.
 #include <algorithm>
+#include <type_traits>
 
 #include "fp8_linear.cuh"
 
@@ -29,7 +30,7 @@ struct Few {
   // 17.3 us) and costs 2 to 4% with 64
   static constexpr int kIssuers = TN == 16 ? 2 : 1;
   static constexpr int kTmemCols = kAccs * TN;         // 64, 128 or 256: two CTAs per SM
-  static constexpr int kScaleBytes = 2 * kScaleGroup * TN * 4;
+  static constexpr int kScaleBytes = 2 * 2 * kScaleGroup * TN * 4;
   static constexpr int kStageBytes = (kBM + TN) * kBK;
 };
 constexpr int kRedStride = kBM + 4;  // floats per token of the partial tile
@@ -44,9 +45,11 @@ __global__ void __launch_bounds__(Few<TN>::kThreads, 2)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[kMaxStages], done[kMaxStages], acc_empty[kAccs], scale_full[2], scale_empty[2];
-  __shared__ uint32_t tmem_slot;
+  __shared__ uint32_t tmem_slot, far_blocks[2];
   __shared__ volatile int abort_flag;
-  float* const scales = reinterpret_cast<float*>(smem_raw + a.scale_offset);  // [2][kScaleGroup][TN]
+  // [2][kScaleGroup][TN], and as many first factors, written and read for far blocks only
+  float* const scales = reinterpret_cast<float*>(smem_raw + a.scale_offset);
+  constexpr int kFirsts = 2 * kScaleGroup * TN;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -175,21 +178,34 @@ __global__ void __launch_bounds__(Few<TN>::kThreads, 2)
     for (int kb = kb0; kb < kb1; kb += kScaleGroup) {
       float x[kPer][kScaleGroup], w[kScaleGroup];
 #pragma unroll
-      for (int j = 0; j < kScaleGroup; ++j) w[j] = kb + j < kb1 ? sw[kb + j] : 0.f;
+      for (int j = 0; j < kScaleGroup; ++j) w[j] = kb + j < kb1 ? sw[kb + j] : 1.f;
       if (a.stable_weight && kb == kb0) pdl_wait();
 #pragma unroll
       for (int j = 0; j < kScaleGroup; ++j) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) x[i][j] = kb + j < kb1 ? sx[i][kb + j] : 0.f;
+        for (int i = 0; i < kPer; ++i) x[i][j] = kb + j < kb1 ? sx[i][kb + j] : 1.f;
       }
       ok = __all_sync(0xffffffffu, mbar_wait(&scale_empty[g], phase));
       if (!ok) break;
+      auto store = [&](int i, int j, float product, float first) {
+        float* const at = scales + (g * kScaleGroup + j) * TN + i * 32 + lane;
+        if (TN < 32 && lane >= TN) return;
+        at[0] = product;
+        at[kFirsts] = first;
+      };
+      ScaleRange range;
 #pragma unroll
       for (int j = 0; j < kScaleGroup; ++j) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i)
-          if (TN >= 32 || lane < TN) scales[(g * kScaleGroup + j) * TN + i * 32 + lane] = x[i][j] * w[j];
+        for (int i = 0; i < kPer; ++i) {
+          const float p = x[i][j] * w[j];
+          range.add(p);
+          if (TN >= 32 || lane < TN) scales[(g * kScaleGroup + j) * TN + i * 32 + lane] = p;
+        }
       }
+      uint32_t blocks = 0;
+      if (__any_sync(0xffffffffu, range.far())) blocks = split_group(sx, sw, kb, min(kScaleGroup, kb1 - kb), store);
+      if (lane == 0) far_blocks[g] = blocks;
       __syncwarp();
       if (lane == 0) mbar_arrive(&scale_full[g]);
       g ^= 1;
@@ -207,44 +223,65 @@ __global__ void __launch_bounds__(Few<TN>::kThreads, 2)
     float2 acc[kCols / 2];
 #pragma unroll
     for (int j = 0; j < kCols / 2; ++j) acc[j] = make_float2(0.f, 0.f);
-    int ring = 0, t = 0, g = 0, in_group = 0;
+    int ring = 0, t = 0, g = 0;
     uint32_t phase = 0, g_phase = 0;
     bool ok = true;
-    for (int kb = kb0; kb < kb1; ++kb) {
-      ok = (in_group != 0 || mbar_wait(&scale_full[g], g_phase)) && mbar_wait(&done[ring], phase);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
+    // One block of k; `far`: the group has products of scales that split_scales divides.
+    auto fold_block = [&](int in_group, auto far) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&done[ring], phase));
+      if (!ok) return;
       tc_fence_after();
+      const float* const block_scales = my_scales + (g * kScaleGroup + in_group) * TN;
       uint32_t d[kCols];
       tmem_ld(t_lane + t * TN, d);
-      float4 s[kCols / 4];
-#pragma unroll
-      for (int j = 0; j < kCols / 4; ++j)
-        s[j] = *reinterpret_cast<const float4*>(my_scales + (g * kScaleGroup + in_group) * TN + 4 * j);
-      tmem_wait(d);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[t]);
-#pragma unroll
-      for (int j = 0; j < kCols / 4; ++j) {
-        acc[2 * j] = __ffma2_rn(make_float2(s[j].x, s[j].y),
-                                make_float2(__uint_as_float(d[4 * j]), __uint_as_float(d[4 * j + 1])), acc[2 * j]);
-        acc[2 * j + 1] =
-            __ffma2_rn(make_float2(s[j].z, s[j].w),
-                       make_float2(__uint_as_float(d[4 * j + 2]), __uint_as_float(d[4 * j + 3])), acc[2 * j + 1]);
-      }
-      if (++in_group == kScaleGroup) {
+      auto release = [&] {  // the block's values are in registers: the accumulator may be reused
+        tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&scale_empty[g]);
-        in_group = 0;
-        g ^= 1;
-        if (g == 0) g_phase ^= 1;
+        if (lane == 0) mbar_arrive(&acc_empty[t]);
+      };
+      if (far && ((far_blocks[g] >> in_group) & 1)) {  // a value at a time: few registers
+        tmem_wait(d);
+        release();
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) {
+          float& sum = j & 1 ? acc[j / 2].y : acc[j / 2].x;
+          sum = fmaf(block_scales[j], __uint_as_float(d[j]) * block_scales[kFirsts + j], sum);
+        }
+      } else {
+        float4 s[kCols / 4];
+#pragma unroll
+        for (int j = 0; j < kCols / 4; ++j) s[j] = *reinterpret_cast<const float4*>(block_scales + 4 * j);
+        tmem_wait(d);
+        release();
+#pragma unroll
+        for (int j = 0; j < kCols / 4; ++j) {
+          acc[2 * j] = __ffma2_rn(make_float2(s[j].x, s[j].y),
+                                  make_float2(__uint_as_float(d[4 * j]), __uint_as_float(d[4 * j + 1])), acc[2 * j]);
+          acc[2 * j + 1] =
+              __ffma2_rn(make_float2(s[j].z, s[j].w),
+                         make_float2(__uint_as_float(d[4 * j + 2]), __uint_as_float(d[4 * j + 3])), acc[2 * j + 1]);
+        }
       }
       if (++ring == a.stages) {
         ring = 0;
         phase ^= 1;
       }
       if (++t == kAccs) t = 0;
+    };
+    for (int kb = kb0; kb < kb1 && ok; kb += kScaleGroup) {
+      const int count = min(kScaleGroup, kb1 - kb);
+      ok = __all_sync(0xffffffffu, mbar_wait(&scale_full[g], g_phase));
+      if (ok && far_blocks[g] == 0) {
+#pragma unroll 1
+        for (int j = 0; j < count && ok; ++j) fold_block(j, std::false_type());
+      } else {
+#pragma unroll 1
+        for (int j = 0; j < count && ok; ++j) fold_block(j, std::true_type());
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&scale_empty[g]);
+      g ^= 1;
+      if (g == 0) g_phase ^= 1;
     }
     if (ok) {
       // every MMA of this CTA has read its operands: the partial tile takes their place

@@ -25,6 +25,7 @@
 // throughput: what is left there are the half-empty second round and the prologue. Tried
 // without gain: two issuing warps, six stages, an undivided 256-column product, TMA stores.
 #include <algorithm>
+#include <type_traits>
 
 #include "fp8_linear.cuh"
 
@@ -89,7 +90,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // full, acc_empty: the even CTA's are used; the others each CTA's own. done[h][s]: half h
   // of the block in stage s is in TMEM; with h = 1 the stage's operands are read, too
   __shared__ uint64_t full[kPairStages], done[2][kPairStages], acc_empty[2 * kAccs], scale_full[2], scale_empty[2];
-  __shared__ uint32_t tmem_slot;
+  __shared__ uint32_t tmem_slot, far_blocks[2][kWBlocks];
   float* const scales = reinterpret_cast<float*>(smem + kScaleOffset);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -229,20 +230,35 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < kScaleGroup; ++j) {
           const bool in = kb + j < kblocks;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i][j] = in ? sx[i][kb + j] : 0.f;
+          for (int i = 0; i < 4; ++i) x[i][j] = in ? sx[i][kb + j] : 1.f;
 #pragma unroll
-          for (int b = 0; b < kWBlocks; ++b) w[b][j] = in ? sw[b][kb + j] : 0.f;
+          for (int b = 0; b < kWBlocks; ++b) w[b][j] = in ? sw[b][kb + j] : 1.f;
         }
         ok = __all_sync(0xffffffffu, mbar_wait(&scale_empty[g], phase));
         if (!ok) break;
+        ScaleRange range;
 #pragma unroll
         for (int j = 0; j < kScaleGroup; ++j) {
 #pragma unroll
           for (int b = 0; b < kWBlocks; ++b) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              scales[((g * kScaleGroup + j) * kWBlocks + b) * kBM + i * 32 + lane] = x[i][j] * w[b][j];
+            for (int i = 0; i < 4; ++i) {
+              const float p = x[i][j] * w[b][j];
+              range.add(p);
+              scales[((g * kScaleGroup + j) * kWBlocks + b) * kBM + i * 32 + lane] = p;
+            }
           }
+        }
+        const bool any_far = __any_sync(0xffffffffu, range.far());
+#pragma unroll
+        for (int b = 0; b < kWBlocks; ++b) {
+          uint32_t blocks = 0;
+          if (any_far)
+            blocks = split_group(sx, sw[b], kb, min(kScaleGroup, kblocks - kb),
+                                 [&](int i, int j, float product, float) {
+                                   scales[((g * kScaleGroup + j) * kWBlocks + b) * kBM + i * 32 + lane] = product;
+                                 });
+          if (lane == 0) far_blocks[g][b] = blocks;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&scale_full[g]);
@@ -280,46 +296,62 @@ __global__ void __launch_bounds__(kThreads, 1)
       float2 acc[kCols / 2];
 #pragma unroll
       for (int j = 0; j < kCols / 2; ++j) acc[j] = make_float2(0.f, 0.f);
-      int in_group = 0;
-      for (int kb = 0; kb < kblocks; ++kb) {
-        ok = (in_group != 0 || mbar_wait(&scale_full[g], g_phase)) && mbar_wait(&done[half][ring], phase);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+      // One block of k; `far`: the group has products of scales that split_scales divides.
+      auto fold_block = [&](int kb, int in_group, auto far) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&done[half][ring], phase));
+        if (!ok) return;
         tc_fence_after();
         const float s1 = my_scales[(g * kScaleGroup + in_group) * kWBlocks * kBM];
         const float2 s = make_float2(s1, s1);
-        if (++in_group == kScaleGroup || kb + 1 == kblocks) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&scale_empty[g]);
-          in_group = 0;
-          g ^= 1;
-          if (g == 0) g_phase ^= 1;
+        float first = 1.f;
+        if (far && ((far_blocks[g][half] >> in_group) & 1)) {
+          float second;
+          split_scales(a.x_scale[(int64_t)min(r0 + lane, a.rows - 1) * kblocks + kb],
+                       a.w_scale[(int64_t)(min(c0, a.n - 1) / kFp8Block) * kblocks + kb], &first, &second);
         }
-        // the next 32 columns are on their way while 32 are folded
-        uint32_t d[2][32];
+        // the next columns are on their way while kWide are folded; the rare form takes fewer at a
+        // time, for its registers
+        constexpr int kWide = decltype(far)::value ? 16 : 32;
+        uint32_t d[2][kWide];
         tmem_ld(t_lane + t * kBN, d[0]);
         tmem_wait(d[0]);
 #pragma unroll
-        for (int c = 0; c < kCols / 32; ++c) {
-          if (c + 1 < kCols / 32) {
-            tmem_ld(t_lane + t * kBN + (c + 1) * 32, d[(c + 1) & 1]);
+        for (int c = 0; c < kCols / kWide; ++c) {
+          if (c + 1 < kCols / kWide) {
+            tmem_ld(t_lane + t * kBN + (c + 1) * kWide, d[(c + 1) & 1]);
           } else {  // this block's values are in registers: the accumulator may be reused
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(acc_bar + t * 16);
           }
+          if (far) scale_all(d[c & 1], first);
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            acc[c * 16 + j] = __ffma2_rn(
+          for (int j = 0; j < kWide / 2; ++j)
+            acc[c * (kWide / 2) + j] = __ffma2_rn(
                 s, make_float2(__uint_as_float(d[c & 1][2 * j]), __uint_as_float(d[c & 1][2 * j + 1])),
-                acc[c * 16 + j]);
-          if (c + 1 < kCols / 32) tmem_wait(d[(c + 1) & 1]);
+                acc[c * (kWide / 2) + j]);
+          if (c + 1 < kCols / kWide) tmem_wait(d[(c + 1) & 1]);
         }
         if (++ring == kPairStages) {
           ring = 0;
           phase ^= 1;
         }
         t ^= 1;
+      };
+      for (int kb = 0; kb < kblocks && ok; kb += kScaleGroup) {
+        const int count = min(kScaleGroup, kblocks - kb);
+        ok = __all_sync(0xffffffffu, mbar_wait(&scale_full[g], g_phase));
+        if (ok && far_blocks[g][half] == 0) {
+#pragma unroll 1
+          for (int j = 0; j < count && ok; ++j) fold_block(kb + j, j, std::false_type());
+        } else {
+#pragma unroll 1
+          for (int j = 0; j < count && ok; ++j) fold_block(kb + j, j, std::true_type());
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&scale_empty[g]);
+        g ^= 1;
+        if (g == 0) g_phase ^= 1;
       }
       if (a.residual != nullptr) cp_async_wait_all();  // also where a wait ran out: nothing stays in flight
       if (!ok) break;

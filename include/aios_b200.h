@@ -302,10 +302,11 @@ AIOSB_API int aiosb_silu_mul_fp8(const void* x, int64_t rows, int64_t f, int64_t
  * their bytes and scales stand for. x: [rows, k] e4m3, rows x_row_stride bytes apart
  * (a multiple of 16); x_scale [rows, ceil(k / 128)]; w: contiguous [n, k] e4m3;
  * w_scale [ceil(n / 128), ceil(k / 128)]. n % 8 == 0, k % 16 == 0. residual rows are
- * residual_stride elements apart and may be y itself (same stride). x_scale * w_scale is
- * formed in fp32. Sums over a block of 128 are formed by the tensor cores, those across
- * blocks in fp32, in an order that depends on the sizes alone. Every operand, the weight
- * too, is read after the dependency wait, so the kernel that quantised it may be the
+ * residual_stride elements apart and may be y itself (same stride). Scales count as their
+ * exact product, also where fp32 holds only the result and not x_scale * w_scale. Sums
+ * over a block of 128 are formed by the tensor cores, those across blocks in fp32, in an
+ * order that depends on the sizes alone. Every operand, the weight too, is read after the
+ * dependency wait, so the kernel that quantised it may be the
  * previous launch, unless the epilogue carries AIOSB_LINEAR_STABLE_WEIGHT. */
 AIOSB_API int aiosb_linear_fp8(const void* x, int64_t x_row_stride, const float* x_scale, int64_t rows, int64_t k,
                                const void* w, const float* w_scale, int64_t n, void* y, int64_t y_row_stride,

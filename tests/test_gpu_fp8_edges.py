@@ -1,0 +1,92 @@
+"""The 8-bit operators on operands at the ends of their ranges, against 64 bits.
+
+Bounds as in test_gpu_fp8.py; an output below 2^-126 is bf16's subnormal, half a step 2^-134.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from aios_b200.kernel import ops
+from test_gpu_fp8 import BLOCK, EACH, _values
+
+pytestmark = pytest.mark.gpu
+
+
+def _operands(rows: int, n: int, k: int):
+    """Ordinary e4m3 rows and weight with scales as a model has them."""
+    g = torch.Generator("cuda").manual_seed(rows + n + k)
+    blocks = -(-k // BLOCK)
+
+    def values(m):
+        v = torch.empty(m, k, device="cuda").normal_(std=60.0, generator=g).clamp(-448, 448)
+        return v.to(torch.float8_e4m3fn)
+
+    def scales(m):
+        return torch.empty(m, blocks, device="cuda").uniform_(0.002, 0.01, generator=g)
+
+    return values(rows), scales(rows), values(n), scales(-(-n // BLOCK))
+
+
+def _check(y, q, s, wq, ws) -> None:
+    x, w = _values(q, s), _values(wq, ws, BLOCK)
+    want, size = x @ w.t(), x.abs() @ w.abs().t()
+    terms = BLOCK + -(-q.shape[1] // BLOCK)
+    bad = ~((y.double() - want).abs() <= 2.0**-8 * want.abs() + 2.0**-134 + 2.0**-23 * terms * size)
+    assert not bool(bad.any()), f"{int(bad.sum())} values off, first at {bad.nonzero()[0].tolist()}"
+
+
+@pytest.mark.parametrize("rows,n,k", EACH)
+def test_scales_whose_product_fp32_does_not_hold(cuda_device, rows: int, n: int, k: int) -> None:
+    """2^70 x 2^60 overflows and 1.3 x 2^-78 x 1.2 x 2^-70 is left with two bits, 2^-82 x 2^-70 with none;
+    the sums are ordinary numbers."""
+    q, s, wq, ws = _operands(rows, n, k)
+    last = -(-k // BLOCK) - 1
+    q8, w8 = q.view(torch.uint8), wq.view(torch.uint8)
+    edge = ws.shape[0] // 2  # the features whose weight scales are extreme in the first and the last block
+    large = torch.arange(rows, device="cuda") % 5 == 1
+    small = torch.arange(rows, device="cuda") % 5 == 2
+    empty = torch.arange(rows, device="cuda") % 5 == 3
+    plain = ~(large | small | empty)
+    ws[edge, 0], ws[edge, last] = 2.0**60, 1.2 * 2.0**-70
+    w8[:, 0] = torch.where(w8[:, 0] > 0x7F, 0x89, 0x09)  # +-2^-6 x 1.125
+    before = ops.linear_fp8(q, s, wq, ws)
+    # overflow: one value of 2^-9 in the first block, times 2^70; nothing at all in some of the rows
+    q8[large, :BLOCK] = 0
+    q8[large & (torch.arange(rows, device="cuda") % 2 == 0), 0] = 0x01
+    s[large, 0] = 2.0**70
+    # underflow: rows that are 448 in the last block and empty elsewhere
+    q8[small, : last * BLOCK] = 0
+    q8[small, last * BLOCK :] = 0x7E
+    s[small, last] = torch.where(torch.arange(int(small.sum()), device="cuda") % 2 == 0, 1.3 * 2.0**-78, 2.0**-82)
+    # empty rows, whose scales some quantisers leave at 0
+    q8[empty] = 0
+    s[empty] = 0
+    y = ops.linear_fp8(q, s, wq, ws)
+    _check(y, q, s, wq, ws)
+    assert torch.equal(y[plain], before[plain])  # a row's bits do not depend on its neighbours' scales
+    assert torch.equal(y, ops.linear_fp8(q, s, wq, ws, stable_weight=True))
+    ops.check_status(cuda_device)
+
+
+@pytest.mark.parametrize("rows", [8, 24, 60, 200, 1500])
+def test_every_pair_of_extreme_scales(cuda_device, rows: int) -> None:
+    """One value of 1 to a row, in the second of three blocks: an output is the product of its two scales."""
+    ends = [0.0, 2.0**-149, 2.0**-120, 2.0**-60, 1.0, -(2.0**60), 2.0**110, 3e38, float("inf"), float("nan")]
+    n, k = BLOCK * len(ends), 3 * BLOCK
+    q = torch.zeros(rows, k, device="cuda")
+    q[:, BLOCK + 7] = 1
+    wq = torch.zeros(n, k, device="cuda")
+    wq[:, BLOCK + 7] = 1
+    s, ws = torch.ones(rows, 3, device="cuda"), torch.ones(len(ends), 3, device="cuda")
+    s[:, 1] = torch.tensor(ends, device="cuda").repeat(-(-rows // len(ends)))[:rows]
+    ws[:, 1] = torch.tensor(ends, device="cuda")
+    y = ops.linear_fp8(q.to(torch.float8_e4m3fn), s, wq.to(torch.float8_e4m3fn), ws).double()
+    want = s[:, 1, None].double() * ws[:, 1].double().repeat_interleave(BLOCK)
+    over = want.abs() >= 2.0**128
+    assert torch.equal(y.isnan(), want.isnan())
+    assert torch.equal(y[over], torch.where(want[over] > 0, float("inf"), -float("inf")))
+    rest = ~over & ~want.isnan()
+    bad = (y - want).abs()[rest] > 2.0**-8 * want[rest].abs() + 2.0**-134 + 2.0**-149
+    assert not bool(bad.any())
