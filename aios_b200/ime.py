@@ -98,6 +98,7 @@ class ImeCompletionEngine:
         self._prefix_pages: list[int] | None = None
         self._prefix_slots: list[int] | None = None
         self._prefix_logits: torch.Tensor | None = None
+        self._prefix_key = llm.model.graph_key  # of the model that wrote the prefix
         self.page_size = llm.cache_manager.page_size
         self._page_table = torch.zeros(
             (self.MAX_TABLE_ROWS, llm.config.max_position_embeddings), dtype=torch.int32, device=llm.device
@@ -348,6 +349,9 @@ class ImeCompletionEngine:
         Slot ids are known on the host (the FIFO has an exact host mirror), so the
         prefill inputs travel in one copy and the forward replays as a CUDA graph."""
         cm = self.llm.cache_manager
+        if self._prefix_key != self.llm.model.graph_key:  # K/V of other weights or another linear type
+            self._reset_prefix_cache_unlocked()
+            self._prefix_key = self.llm.model.graph_key
         old_ids = self._prefix_token_ids
         old_pages = self._prefix_pages
         reused = token_longest_common_prefix(old_ids, token_ids)

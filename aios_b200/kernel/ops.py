@@ -657,12 +657,20 @@ def quantize_fp8(x: torch.Tensor, *, out: torch.Tensor | None = None,
     return out, scale
 
 
-def quantize_weight_fp8(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+def quantize_weight_fp8(weight: torch.Tensor, *, out: torch.Tensor | None = None,
+                        scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """A bf16 weight [N, K] to (e4m3 [N, K], scale [ceil(N / 128), ceil(K / 128)]): a scale
     for each 128 x 128 block. K is a multiple of 16; rows may be strided."""
     n, k, stride = _check_rows("quantize_weight_fp8", weight, torch.bfloat16)
-    out = _empty_rows(weight, n, k, FP8_DTYPE)
-    scale = _empty_rows(weight, -(-n // FP8_BLOCK), -(-k // FP8_BLOCK), torch.float32)
+    tall, wide = -(-n // FP8_BLOCK), -(-k // FP8_BLOCK)
+    if out is None:
+        out = _empty_rows(weight, n, k, FP8_DTYPE)
+    else:
+        _check_dense("quantize_weight_fp8", "out", out, (n, k), FP8_DTYPE, weight.get_device())
+    if scale is None:
+        scale = _empty_rows(weight, tall, wide, torch.float32)
+    else:
+        _check_dense("quantize_weight_fp8", "scale", scale, (tall, wide), torch.float32, weight.get_device())
     _launch(weight.get_device(), "aiosb_quantize_weight_fp8", weight.data_ptr(), n, k, stride, out.data_ptr(),
             scale.data_ptr())
     return out, scale

@@ -18,25 +18,33 @@ class Linear(BaseOP):
         self.weight = torch.empty(output_size, input_size)
         self.bias = None
         self._fp8: tuple[torch.Tensor, torch.Tensor] | None = None  # e4m3 weight and block scales
+        self._fp8_stale = False  # made from weights that have been replaced since
 
     def on_weights_loaded(self) -> None:
-        self._fp8 = None
+        self._fp8_stale = True
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return ops.linear(x, self.weight)
 
     def quantize_fp8(self) -> None:
-        """Builds the 8-bit copy of the weight that ``forward_fp8`` runs on."""
+        """Builds the 8-bit copy of the weight that ``forward_fp8`` runs on. A copy that is
+        there is written again in its place: captured graphs go on reading valid memory."""
         n, k = self.weight.shape
         if n % 8 or k % 16:
             raise ValueError(f"an 8-bit linear needs n % 8 == 0 and k % 16 == 0, got a [{n}, {k}] weight")
-        self._fp8 = ops.quantize_weight_fp8(self.weight)
+        out, scale = self._fp8 or (None, None)
+        if out is not None and out.device == self.weight.device:
+            torch.cuda.synchronize(out.device)  # kernels of any stream may still read it
+        else:
+            out = scale = None
+        self._fp8 = ops.quantize_weight_fp8(self.weight, out=out, scale=scale)
+        self._fp8_stale = False
         torch.cuda.synchronize(self.weight.device)  # forward_fp8 reads it ahead of its stream order
 
     def forward_fp8(self, x: torch.Tensor, x_scale: torch.Tensor, *, out: torch.Tensor | None = None,
                     residual: torch.Tensor | None = None) -> torch.Tensor:
         """The linear on quantised rows (``ops.linear_fp8``), ``residual`` added when given."""
-        if self._fp8 is None:
+        if self._fp8 is None or self._fp8_stale:
             raise RuntimeError("forward_fp8 needs quantize_fp8() after the weights are loaded")
         epilogue = _lib.EPI_STORE if residual is None else _lib.EPI_ADD
         return ops.linear_fp8(x, x_scale, *self._fp8, out=out, epilogue=epilogue, residual=residual,

@@ -227,10 +227,21 @@ class Qwen3ForCausalLM(BaseLLMModel):
         """What the decoder layers' linears run on: "bf16" or "fp8"."""
         return "fp8" if self.model._fp8_linears else "bf16"
 
+    @property
+    def graph_key(self) -> tuple:
+        return (*super().graph_key, self.linear_dtype)
+
+    def on_weights_loaded(self) -> None:
+        super().on_weights_loaded()
+        if self.model._fp8_linears and self.model.embed_tokens.weight.is_cuda:
+            self.set_linear_dtype("fp8")  # the 8-bit copies are of the weights before
+
     def set_linear_dtype(self, name: str) -> None:
         """Runs the decoder layers' linears on bf16 weights or on 8-bit copies of them, which
-        are built here (the bf16 weights stay). Embedding, attention and LM head are bf16
-        either way. Call it after the weights are loaded and before graphs are captured."""
+        are built here (the bf16 weights stay, and so do 8-bit copies when "bf16" is chosen
+        again). Embedding, attention and LM head are bf16 either way. Call it after the
+        weights are loaded. The engine's graphs and prefix cache follow a later change; a
+        graph that the caller captured keeps the type that it was captured with."""
         if name not in ("bf16", "fp8"):
             raise ValueError(f"linear_dtype must be 'bf16' or 'fp8', got {name!r}")
         if name == "fp8":

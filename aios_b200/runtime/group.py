@@ -198,35 +198,12 @@ class CandidateGroupRuntime:
             ring=llm.cache_manager.ring.data_ptr(),
             status=ops.status_word(dev).data_ptr(),
         )
-        # The step also embeds the tokens it samples for the next forward when that
-        # forward is the standard-residual trunk (it starts at its first linear)
-        self.pre_embedded = None
-        if _EMBED_IN_STEP and _stat_trunk(llm.model):
-            hidden = llm.config.hidden_size
-            emb_w = llm.model.model.embed_tokens.weight
-            self._emb_out = torch.zeros((max_rows, hidden), dtype=emb_w.dtype, device=dev)
-            self._emb_x = torch.zeros((max_rows, hidden), dtype=torch.float32, device=dev)
-            self._emb_ss = torch.zeros((1, max_rows), dtype=torch.float32, device=dev)
-            self.ptrs.embed_w = emb_w.data_ptr()
-            self.ptrs.embed_out = self._emb_out.data_ptr()
-            self.ptrs.embed_stat_x = self._emb_x.data_ptr()
-            self.ptrs.embed_stat_ss = self._emb_ss.data_ptr()
-            self.ptrs.hidden = hidden
-            self.pre_embedded = (self._emb_out, self._emb_x, self._emb_ss)
         # [vocab / 16, rows, 4] tile statistics of the decode logits, and per row
         # count whether the LM head of that count's step graph writes them (known
         # after the graph's eager warm-up forward)
         self.tile_stats = (torch.zeros(self.vocab // 16 * max_rows * 4, dtype=torch.float32, device=dev)
                            if _TILE_SAMPLING and self.vocab % 16 == 0 else None)
         self._tile_rows: dict[int, bool] = {}
-        # the steps inside a step graph follow that graph's forward
-        # (GROUP_AFTER_FORWARD: the step reads its state while the LM head runs)
-        self._ptrs_graph = _lib.GroupPtrs.from_buffer_copy(self.ptrs)
-        self._ptrs_graph.flags = _lib.GROUP_AFTER_FORWARD
-        self._ptrs_tiles = None
-        if self.tile_stats is not None:
-            self._ptrs_tiles = _lib.GroupPtrs.from_buffer_copy(self._ptrs_graph)
-            self._ptrs_tiles.tile_stats = self.tile_stats.data_ptr()
         self._graphs: dict[int, torch.cuda.CUDAGraph] = {}
         self._graph_launches: dict[int, int] = {}
         self.h2d_bytes = 0  # host->device bytes copied by rounds (bench accounting)
@@ -240,25 +217,67 @@ class CandidateGroupRuntime:
         # from ([attempts, vocab] fp32 per step; synchronises after every step).
         self.record_logits = False
         self.step_logits: list[torch.Tensor] = []
-        self._step_plan = self._persistent_plan() if _PERSISTENT else None
+        self._persistent = _PERSISTENT
+        self._bind_model()
         self.history_mode = _HISTORY
+
+    def _bind_model(self) -> None:
+        """What depends on the model's weights and the type of its linears."""
+        self._model_key = self.llm.model.graph_key
+        llm, dev, max_rows = self.llm, self.device, self.max_rows
+        # The step also embeds the tokens it samples for the next forward when that
+        # forward is the standard-residual trunk (it starts at its first linear)
+        self.pre_embedded = None
+        self.ptrs.embed_w = self.ptrs.embed_out = self.ptrs.embed_stat_x = self.ptrs.embed_stat_ss = None
+        if _EMBED_IN_STEP and _stat_trunk(llm.model):
+            hidden = llm.config.hidden_size
+            emb_w = llm.model.model.embed_tokens.weight
+            self._emb_out = torch.zeros((max_rows, hidden), dtype=emb_w.dtype, device=dev)
+            self._emb_x = torch.zeros((max_rows, hidden), dtype=torch.float32, device=dev)
+            self._emb_ss = torch.zeros((1, max_rows), dtype=torch.float32, device=dev)
+            self.ptrs.embed_w = emb_w.data_ptr()
+            self.ptrs.embed_out = self._emb_out.data_ptr()
+            self.ptrs.embed_stat_x = self._emb_x.data_ptr()
+            self.ptrs.embed_stat_ss = self._emb_ss.data_ptr()
+            self.ptrs.hidden = hidden
+            self.pre_embedded = (self._emb_out, self._emb_x, self._emb_ss)
+        # the steps inside a step graph follow that graph's forward
+        # (GROUP_AFTER_FORWARD: the step reads its state while the LM head runs)
+        self._ptrs_graph = _lib.GroupPtrs.from_buffer_copy(self.ptrs)
+        self._ptrs_graph.flags = _lib.GROUP_AFTER_FORWARD
+        self._ptrs_tiles = None
+        if self.tile_stats is not None:
+            self._ptrs_tiles = _lib.GroupPtrs.from_buffer_copy(self._ptrs_graph)
+            self._ptrs_tiles.tile_stats = self.tile_stats.data_ptr()
+        self._step_plan = self._persistent_plan() if self._persistent else None
+
+    def _drop_graphs(self) -> None:
+        self._tile_rows.clear()
+        self._graphs.clear()
+        self._graph_launches.clear()
+
+    def _follow_model(self) -> None:
+        """Captured graphs and pointers of other weights, or of another linear type, go."""
+        if self._model_key != self.llm.model.graph_key:
+            torch.cuda.synchronize(self.device)
+            self._drop_graphs()
+            self._pool = None
+            self._bind_model()
 
     def use_history_mode(self, mode: str) -> None:
         """Selects the decode attention's history mode (a HISTORY_MODES name) for
         this runtime's step graphs; captured graphs are dropped."""
         self.history_mode = HISTORY_MODES[mode]
-        self._tile_rows.clear()
-        self._graphs.clear()
-        self._graph_launches.clear()
+        self._drop_graphs()
 
     def use_persistent_step(self, enabled: bool = True) -> bool:
         """Switches this runtime's decode forward to (or away from) the persistent
         decode-step kernel; returns whether it is now in use (False when the model
         is not one the kernel serves). Captured step graphs are dropped."""
+        self._follow_model()
+        self._persistent = enabled
         self._step_plan = self._persistent_plan() if enabled else None
-        self._tile_rows.clear()
-        self._graphs.clear()
-        self._graph_launches.clear()
+        self._drop_graphs()
         return self._step_plan is not None
 
     # ------------------------------------------------------- persistent step
@@ -437,6 +456,7 @@ class CandidateGroupRuntime:
         large = not greedy and sort_k > SORT_K
         if large and self.vocab > LARGE_SORT_VOCAB:
             raise ValueError(f"a sorted candidate set of {sort_k} needs a vocabulary of at most {LARGE_SORT_VOCAB}")
+        self._follow_model()
         cm = self.llm.cache_manager
         stage = stage_class(prefix_len)
         graph = self._graph(attempts, large, stage)

@@ -43,6 +43,7 @@ class PrefixRunner:
         self.logits = torch.zeros((1, llm.config.vocab_size), dtype=torch.bfloat16, device=dev)
         self._graphs: dict[int, tuple[torch.cuda.CUDAGraph, int]] = {}
         self._pool = None
+        self._model_key = llm.model.graph_key  # of the captured graphs
         self.h2d_bytes = 0
 
     @property
@@ -94,6 +95,11 @@ class PrefixRunner:
         self._pending = True
         self.h2d_bytes += 4 * end
         self.fill_table(table, rows, width, T)
+        if self._model_key != self.llm.model.graph_key:
+            torch.cuda.synchronize(self.device)
+            self._graphs.clear()
+            self._pool = None
+            self._model_key = self.llm.model.graph_key
         entry = self._graphs.get(n)
         if entry is not None:
             entry[0].replay()
