@@ -185,6 +185,7 @@ _SIGNATURES = {
     "aiosb_rmsnorm_fp8": ([_p, _i64, _i64, _i64, _p, _p, _p, _f32, _p, _p, _p], _i32),
     "aiosb_silu_mul_fp8": ([_p, _i64, _i64, _i64, _p, _p, _p], _i32),
     "aiosb_linear_fp8": ([_p, _i64, _p, _i64, _i64, _p, _p, _i64, _p, _i64, _i32, _p, _i64, _p, _p], _i32),
+    "aiosb_linear_fp8_plan": ([_i64, _i64, _i64, _i64, _p], _i32),
     "aiosb_attention_decode": (
         [_p, _i64, _p, _i64, _p, _p, _f32, _p, _p, _i64, _p, _p, _p, _p, _i64, _p, _i64, _p, _p, _p, _p, _i32,
          _i64, _i64, _i64, _i64, _i64, _f32, _p, _i64, _p, _p],
@@ -270,7 +271,8 @@ def check(rc: int, what: str) -> None:
 # (the bench reports it as the number of this library's kernel launches).
 _NON_LAUNCHING = frozenset({"aiosb_version", "aiosb_last_error", "aiosb_host_device_pointer",
                             "aiosb_prefill_tile_tokens", "aiosb_decode_step_sync_words",
-                            "aiosb_decode_step_work_bytes", "aiosb_linear_tile_stats_eligible"})
+                            "aiosb_decode_step_work_bytes", "aiosb_linear_tile_stats_eligible",
+                            "aiosb_linear_fp8_plan"})
 launches = 0
 _functions: dict[str, object] = {}
 

@@ -505,6 +505,16 @@ Choice choose(int64_t rows, int64_t n, int kblocks, int sms) {
   return best;
 }
 
+int check_sizes(int64_t rows, int64_t n, int64_t k) {
+  AIOSB_REQUIRE(rows >= 0 && k > 0 && n > 0, AIOSB_ERR_INVALID_ARG, "linear_fp8: bad sizes");
+  AIOSB_REQUIRE(n % 8 == 0, AIOSB_ERR_UNSUPPORTED, "linear_fp8: n=%lld must be a multiple of 8", (long long)n);
+  AIOSB_REQUIRE(k % 16 == 0, AIOSB_ERR_UNSUPPORTED, "linear_fp8: k=%lld must be a multiple of 16", (long long)k);
+  constexpr int64_t kMost = (int64_t)1 << 30;
+  AIOSB_REQUIRE(rows <= kMost && n <= kMost && k <= kMost && (rows / kBM + 1) * (n / 64 + 1) < kMost,
+                AIOSB_ERR_UNSUPPORTED, "linear_fp8: too large");
+  return AIOSB_OK;
+}
+
 }  // namespace
 }  // namespace aiosb
 
@@ -514,12 +524,8 @@ extern "C" int aiosb_linear_fp8(const void* x, int64_t x_row_stride, const float
                                 const void* w, const float* w_scale, int64_t n, void* y, int64_t y_row_stride,
                                 int epilogue, const void* residual, int64_t residual_stride, int32_t* status,
                                 void* stream) {
-  AIOSB_REQUIRE(rows >= 0 && k > 0 && n > 0, AIOSB_ERR_INVALID_ARG, "linear_fp8: bad sizes");
-  AIOSB_REQUIRE(n % 8 == 0, AIOSB_ERR_UNSUPPORTED, "linear_fp8: n=%lld must be a multiple of 8", (long long)n);
-  AIOSB_REQUIRE(k % 16 == 0, AIOSB_ERR_UNSUPPORTED, "linear_fp8: k=%lld must be a multiple of 16", (long long)k);
-  constexpr int64_t kMost = (int64_t)1 << 30;
-  AIOSB_REQUIRE(rows <= kMost && n <= kMost && k <= kMost && (rows / kBM + 1) * (n / 64 + 1) < kMost,
-                AIOSB_ERR_UNSUPPORTED, "linear_fp8: too large");
+  const int sizes = check_sizes(rows, n, k);
+  if (sizes != AIOSB_OK) return sizes;
   const int stable_weight = (epilogue & AIOSB_LINEAR_STABLE_WEIGHT) != 0;
   epilogue &= ~AIOSB_LINEAR_STABLE_WEIGHT;
   AIOSB_REQUIRE(epilogue == AIOSB_EPI_STORE || epilogue == AIOSB_EPI_ADD, AIOSB_ERR_INVALID_ARG,
@@ -563,4 +569,16 @@ extern "C" int aiosb_linear_fp8(const void* x, int64_t x_row_stride, const float
   if (rc == AIOSB_OK) rc = fp8_tensor_map(&tw, w, n, k, k, kBN);
   if (rc != AIOSB_OK) return rc;
   return a.residual != nullptr ? launch<true>(tx, tw, a, s) : launch<false>(tx, tw, a, s);
+}
+
+extern "C" int aiosb_linear_fp8_plan(int64_t rows, int64_t n, int64_t k, int64_t sms, int32_t* plan) {
+  const int sizes = check_sizes(rows, n, k);
+  if (sizes != AIOSB_OK) return sizes;
+  AIOSB_REQUIRE(rows > 0 && sms >= 0 && sms <= 65536 && plan != nullptr, AIOSB_ERR_INVALID_ARG,
+                "linear_fp8_plan: no rows, bad SM count or null pointer");
+  const Choice c = choose(rows, n, (int)((k + kBK - 1) / kBK), sms > 0 ? (int)sms : sm_count());
+  plan[0] = c.shape->rows;
+  plan[1] = c.shape->cols;
+  plan[2] = c.split;
+  return AIOSB_OK;
 }

@@ -776,6 +776,14 @@ def linear_fp8(
     return out
 
 
+def linear_fp8_plan(rows: int, n: int, k: int, sms: int = 0) -> tuple[int, int, int]:
+    """How ``linear_fp8`` runs a size on a device of `sms` SMs (0: the current one): token
+    rows and features of a tile, and the parts that k is split into."""
+    plan = (ctypes.c_int32 * 3)()
+    _lib.call("aiosb_linear_fp8_plan", rows, n, k, sms, ctypes.addressof(plan))
+    return tuple(plan)
+
+
 # ---------------------------------------------------------------------------
 # Attention
 # ---------------------------------------------------------------------------

@@ -313,6 +313,11 @@ AIOSB_API int aiosb_linear_fp8(const void* x, int64_t x_row_stride, const float*
                                int epilogue, const void* residual, int64_t residual_stride, int32_t* status,
                                void* stream);
 
+/* How aiosb_linear_fp8 runs a size: plan[0] token rows and plan[1] features of a tile, plan[2]
+ * the parts that k is split into (one CTA of a cluster each). sms: the device's SMs, 0 for the
+ * current device's. Launches nothing. */
+AIOSB_API int aiosb_linear_fp8_plan(int64_t rows, int64_t n, int64_t k, int64_t sms, int32_t* plan);
+
 /* ---- Attention ---------------------------------------------------------------
  * KV slots: token slot s of one layer lives at k_cache + s * num_kv_heads *
  * head_dim (the MHAKVCache layout [pages, page_size, Hkv, d] flattened); slot

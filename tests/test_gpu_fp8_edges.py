@@ -8,8 +8,10 @@ from __future__ import annotations
 import pytest
 import torch
 
+from aios_b200 import _lib
 from aios_b200.kernel import ops
-from test_gpu_fp8 import BLOCK, EACH, _values
+from test_fp8_plan import PLANS
+from test_gpu_fp8 import BLOCK, EACH, _linear_check, _linear_inputs, _values
 
 pytestmark = pytest.mark.gpu
 
@@ -37,7 +39,27 @@ def _check(y, q, s, wq, ws) -> None:
     assert not bool(bad.any()), f"{int(bad.sum())} values off, first at {bad.nonzero()[0].tolist()}"
 
 
-@pytest.mark.parametrize("rows,n,k", EACH)
+def test_this_device_runs_every_tile_and_split(cuda_device) -> None:
+    assert {ops.linear_fp8_plan(*size) for size in EACH} == PLANS
+
+
+# more tiles than pairs of SMs, k in an odd number of groups of eight blocks: the order of the scale
+# buffers goes on from tile to tile
+@pytest.mark.parametrize("rows,n,k", [(3000, 2600, 2352), (2500, 3000, 2640), (4100, 4104, 400)])
+def test_pairs_that_walk_several_tiles(cuda_device, rows: int, n: int, k: int) -> None:
+    assert ops.linear_fp8_plan(rows, n, k) == (256, 256, 1)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert -(-rows // 256) * -(-n // 256) > sms // 2
+    q, s, wq, ws = _linear_inputs(rows, n, k)
+    y = ops.linear_fp8(q, s, wq, ws)
+    _linear_check(y, q, s, wq, ws)
+    r = torch.randn(rows, n, device=cuda_device).to(torch.bfloat16)
+    z = ops.linear_fp8(q, s, wq, ws, epilogue=_lib.EPI_ADD, residual=r)
+    _linear_check(z, q, s, wq, ws, r)
+    ops.check_status(cuda_device)
+
+
+@pytest.mark.parametrize("rows,n,k", [*EACH, (3000, 2600, 2352)])
 def test_scales_whose_product_fp32_does_not_hold(cuda_device, rows: int, n: int, k: int) -> None:
     """2^70 x 2^60 overflows and 1.3 x 2^-78 x 1.2 x 2^-70 is left with two bits, 2^-82 x 2^-70 with none;
     the sums are ordinary numbers."""
