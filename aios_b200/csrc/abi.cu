@@ -37,6 +37,12 @@ int check_launch(const char* what) {
   if (e != cudaSuccess) return set_error(AIOSB_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
   return AIOSB_OK;
 }
+
+int check_launch(const char* what, cudaError_t result) {
+  if (result == cudaSuccess) return AIOSB_OK;
+  cudaGetLastError();
+  return set_error(AIOSB_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(result));
+}
 }  // namespace aiosb
 
 extern "C" int aiosb_version(void) { return 100; }

@@ -12,6 +12,9 @@ namespace aiosb {
 int set_error(int code, const char* fmt, ...);
 // Turns a failed kernel launch into AIOSB_ERR_LAUNCH.
 int check_launch(const char* what);
+// The same for a launch whose own result is at hand: an earlier call's error is not taken for
+// its, and its error is not left for a later one.
+int check_launch(const char* what, cudaError_t result);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }

@@ -209,8 +209,9 @@ int fp8_configure(Kern kern, int bytes, bool (&configured)[64]) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return set_error(AIOSB_ERR_LAUNCH, "linear_fp8: %s", cudaGetErrorString(e));
+    const int rc =
+        check_launch("linear_fp8", cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (rc != AIOSB_OK) return rc;
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   return AIOSB_OK;
@@ -234,9 +235,7 @@ int fp8_launch(Kern kern, int grid, int threads, int smem, int cluster, cudaStre
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tx, tw, a);
-  if (e != cudaSuccess) return set_error(AIOSB_ERR_LAUNCH, "linear_fp8: %s", cudaGetErrorString(e));
-  return AIOSB_OK;
+  return check_launch("linear_fp8", cudaLaunchKernelEx(&cfg, kern, tx, tw, a));
 }
 
 // Many token rows: two CTAs share a 256 x 256 tile (fp8_linear_pair.cu).

@@ -118,13 +118,11 @@ __global__ void __launch_bounds__(TPR == 32 ? kThreads : TPR) norm_fp8_kernel(co
 }
 
 template <int TPR, int U>
-void launch_norm(const NormArgs& a, cudaStream_t s) {
+cudaError_t launch_norm(const NormArgs& a, cudaStream_t s) {
   const unsigned grid = TPR == 32 ? (unsigned)((a.rows + kThreads / 32 - 1) / (kThreads / 32)) : (unsigned)a.rows;
   const dim3 block(TPR == 32 ? kThreads : TPR);
-  if (a.res != nullptr)
-    launch_pdl(norm_fp8_kernel<TPR, U, true>, dim3(grid), block, 0, s, a);
-  else
-    launch_pdl(norm_fp8_kernel<TPR, U, false>, dim3(grid), block, 0, s, a);
+  return launch_pdl(a.res != nullptr ? norm_fp8_kernel<TPR, U, true> : norm_fp8_kernel<TPR, U, false>, dim3(grid),
+                    block, 0, s, a);
 }
 
 // ---- SwiGLU and the plain quantiser ---------------------------------------------
@@ -202,11 +200,11 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 template <bool SILU, int UPT>
-void launch_rows_as(const __nv_bfloat16* x, int64_t x_stride, uint32_t groups, uint32_t blocks, int cols, uint8_t* q,
-                    float* scale, cudaStream_t s) {
+cudaError_t launch_rows_as(const __nv_bfloat16* x, int64_t x_stride, uint32_t groups, uint32_t blocks, int cols,
+                           uint8_t* q, float* scale, cudaStream_t s) {
   constexpr uint32_t kPer = kThreads / 16 * UPT;
-  launch_pdl(rows_fp8_kernel<SILU, UPT>, dim3((groups + kPer - 1) / kPer), dim3(kThreads), 0, s, x, x_stride, groups,
-             blocks, cols, q, scale);
+  return launch_pdl(rows_fp8_kernel<SILU, UPT>, dim3((groups + kPer - 1) / kPer), dim3(kThreads), 0, s, x, x_stride,
+                    groups, blocks, cols, q, scale);
 }
 
 // Groups per thread, by the blocks of one group per thread that each SM gets: one while the SMs
@@ -215,14 +213,15 @@ void launch_rows_as(const __nv_bfloat16* x, int64_t x_stride, uint32_t groups, u
 //   2048 x 4096 (28) 9.6 / 8.7 / 8.9, 4096 x 4096 (55) 17.5 / 15.7 / 15.4, 12001 x 10240 112 / 97 / 91;
 //   rows of 1024 x 2048 2.6 / 2.7 / 2.8, 2048 x 2048 4.1 / 4.1 / 3.9, 8192 x 8192 43 / 37 / 34.
 template <bool SILU>
-void launch_rows(const void* x, int64_t x_stride, int64_t rows, int64_t cols, void* q, float* scale, cudaStream_t s) {
+cudaError_t launch_rows(const void* x, int64_t x_stride, int64_t rows, int64_t cols, void* q, float* scale,
+                        cudaStream_t s) {
   const uint32_t blocks = (uint32_t)((cols + kFp8Block - 1) / kFp8Block);
   const uint32_t groups = (uint32_t)rows * blocks;
   const uint32_t per_sm = groups / (kThreads / 16) / (uint32_t)sm_count();  // blocks of one group per thread
   auto launch = per_sm < 10 ? launch_rows_as<SILU, 1> : launch_rows_as<SILU, 4>;
   if constexpr (SILU)
     if (per_sm >= 10 && per_sm < 40) launch = launch_rows_as<SILU, 2>;
-  launch((const __nv_bfloat16*)x, x_stride, groups, blocks, (int)cols, (uint8_t*)q, scale, s);
+  return launch((const __nv_bfloat16*)x, x_stride, groups, blocks, (int)cols, (uint8_t*)q, scale, s);
 }
 
 // ---- weights ----------------------------------------------------------------------
@@ -312,38 +311,37 @@ extern "C" int aiosb_rmsnorm_fp8(const void* x, int64_t rows, int64_t hidden, in
   const int units = (int)(hidden / 8);
   const int tpr = units <= 128 ? 32 : units <= 512 ? 128 : units <= 1024 ? 256 : units <= 2048 ? 512 : 1024;
   const int u = (units + tpr - 1) / tpr;
+  cudaError_t e;
   switch (tpr * 8 + u) {
-    case 32 * 8 + 1: launch_norm<32, 1>(a, s); break;
-    case 32 * 8 + 2: launch_norm<32, 2>(a, s); break;
-    case 32 * 8 + 3: launch_norm<32, 3>(a, s); break;
-    case 32 * 8 + 4: launch_norm<32, 4>(a, s); break;
-    case 128 * 8 + 2: launch_norm<128, 2>(a, s); break;
-    case 128 * 8 + 3: launch_norm<128, 3>(a, s); break;
-    case 128 * 8 + 4: launch_norm<128, 4>(a, s); break;
-    case 256 * 8 + 3: launch_norm<256, 3>(a, s); break;
-    case 256 * 8 + 4: launch_norm<256, 4>(a, s); break;
-    case 512 * 8 + 3: launch_norm<512, 3>(a, s); break;
-    case 512 * 8 + 4: launch_norm<512, 4>(a, s); break;
-    case 1024 * 8 + 3: launch_norm<1024, 3>(a, s); break;
-    default: launch_norm<1024, 4>(a, s); break;
+    case 32 * 8 + 1: e = launch_norm<32, 1>(a, s); break;
+    case 32 * 8 + 2: e = launch_norm<32, 2>(a, s); break;
+    case 32 * 8 + 3: e = launch_norm<32, 3>(a, s); break;
+    case 32 * 8 + 4: e = launch_norm<32, 4>(a, s); break;
+    case 128 * 8 + 2: e = launch_norm<128, 2>(a, s); break;
+    case 128 * 8 + 3: e = launch_norm<128, 3>(a, s); break;
+    case 128 * 8 + 4: e = launch_norm<128, 4>(a, s); break;
+    case 256 * 8 + 3: e = launch_norm<256, 3>(a, s); break;
+    case 256 * 8 + 4: e = launch_norm<256, 4>(a, s); break;
+    case 512 * 8 + 3: e = launch_norm<512, 3>(a, s); break;
+    case 512 * 8 + 4: e = launch_norm<512, 4>(a, s); break;
+    case 1024 * 8 + 3: e = launch_norm<1024, 3>(a, s); break;
+    default: e = launch_norm<1024, 4>(a, s); break;
   }
-  return check_launch("rmsnorm_fp8");
+  return check_launch("rmsnorm_fp8", e);
 }
 
 extern "C" int aiosb_silu_mul_fp8(const void* x, int64_t rows, int64_t f, int64_t x_row_stride, void* q, float* scale,
                                   void* stream) {
   const int rc = check_rows("silu_mul_fp8", x, rows, f, 2 * f, x_row_stride, q, scale);
   if (rc != AIOSB_OK) return rc == 1 ? AIOSB_OK : rc;
-  launch_rows<true>(x, x_row_stride, rows, f, q, scale, as_stream(stream));
-  return check_launch("silu_mul_fp8");
+  return check_launch("silu_mul_fp8", launch_rows<true>(x, x_row_stride, rows, f, q, scale, as_stream(stream)));
 }
 
 extern "C" int aiosb_quantize_fp8(const void* x, int64_t rows, int64_t cols, int64_t x_row_stride, void* q,
                                   float* scale, void* stream) {
   const int rc = check_rows("quantize_fp8", x, rows, cols, cols, x_row_stride, q, scale);
   if (rc != AIOSB_OK) return rc == 1 ? AIOSB_OK : rc;
-  launch_rows<false>(x, x_row_stride, rows, cols, q, scale, as_stream(stream));
-  return check_launch("quantize_fp8");
+  return check_launch("quantize_fp8", launch_rows<false>(x, x_row_stride, rows, cols, q, scale, as_stream(stream)));
 }
 
 extern "C" int aiosb_quantize_weight_fp8(const void* w, int64_t n, int64_t k, int64_t w_row_stride, void* q,
@@ -353,7 +351,7 @@ extern "C" int aiosb_quantize_weight_fp8(const void* w, int64_t n, int64_t k, in
   const int64_t tall = (n + kFp8Block - 1) / kFp8Block, wide = (k + kFp8Block - 1) / kFp8Block;
   AIOSB_REQUIRE(tall <= 65535, AIOSB_ERR_UNSUPPORTED, "quantize_weight_fp8: more than %lld rows",
                 (long long)65535 * kFp8Block);
-  launch_pdl(weight_fp8_kernel, dim3((unsigned)wide, (unsigned)tall), dim3(kThreads), 0, as_stream(stream),
-             (const __nv_bfloat16*)w, w_row_stride, n, k, (uint8_t*)q, scale);
-  return check_launch("quantize_weight_fp8");
+  return check_launch("quantize_weight_fp8",
+                      launch_pdl(weight_fp8_kernel, dim3((unsigned)wide, (unsigned)tall), dim3(kThreads), 0,
+                                 as_stream(stream), (const __nv_bfloat16*)w, w_row_stride, n, k, (uint8_t*)q, scale));
 }
