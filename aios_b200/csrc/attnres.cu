@@ -155,8 +155,8 @@ struct RegRows {
 // partial are read after the wait.
 template <int VPL, int NSRC, bool NORM = false>
 __global__ void __launch_bounds__(kMixWarps * 32, 3)
-    attnres_reg_kernel(const uint4* __restrict__ bank, int nsrc_bank, int64_t tokens, int hidden,
-                       const uint4* __restrict__ partial, const float* __restrict__ wq, float eps,
+    attnres_reg_kernel(const uint4* bank, int nsrc_bank, int64_t tokens, int hidden,
+                       const uint4* partial, const float* __restrict__ wq, float eps,
                        uint4* __restrict__ out, const uint4* __restrict__ norm_w = nullptr, float norm_eps = 0.f,
                        int stable = 0) {
   pdl_launch_dependents();
@@ -238,8 +238,8 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 
 template <int VPL, int NSRC, int G>
 __global__ void __launch_bounds__((1 + kStreamTok * G) * 32, 1)
-    attnres_stream_kernel(const uint4* __restrict__ bank, int nsrc_bank, int64_t tokens, int hidden,
-                          const uint4* __restrict__ partial, const float* __restrict__ wq, float eps,
+    attnres_stream_kernel(const uint4* bank, int nsrc_bank, int64_t tokens, int hidden,
+                          const uint4* partial, const float* __restrict__ wq, float eps,
                           uint4* __restrict__ out, int spg, int32_t* status, int64_t stall_tile,
                           uint64_t wait_ns) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
@@ -342,8 +342,8 @@ __global__ void __launch_bounds__((1 + kStreamTok * G) * 32, 1)
 // Any hidden size / up to 16 sources: two passes over the sources (scores, then
 // the weighted sum), still one warp per token.
 __global__ void __launch_bounds__(kMixWarps * 32)
-    attnres_generic_kernel(const uint4* __restrict__ bank, int nsrc_bank, int64_t tokens, int hidden,
-                           const uint4* __restrict__ partial, const float* __restrict__ wq, float eps,
+    attnres_generic_kernel(const uint4* bank, int nsrc_bank, int64_t tokens, int hidden,
+                           const uint4* partial, const float* __restrict__ wq, float eps,
                            uint4* __restrict__ out) {
   pdl_enter();
   const int64_t t = (int64_t)blockIdx.x * kMixWarps + threadIdx.x / 32;

@@ -1,6 +1,9 @@
 // Memory-bound row kernels: KV scatter, RMSNorm, fused add+RMSNorm, SwiGLU and
 // the embedding gather. One warp per row, 128-bit vector accesses when the row
-// base and length allow it, fp32 math, bf16 storage.
+// base and length allow it, fp32 math, bf16 storage. Only model constants are
+// `const __restrict__`: what a predecessor may still write when the grid starts
+// must not be declared read-only for the grid's whole life, or its loads need
+// not stay behind the dependency wait.
 #include <algorithm>
 
 #include "abi_util.h"
@@ -13,10 +16,9 @@ constexpr int kRowThreads = 256;  // 8 warps, one row per warp
 
 // ---- KV scatter (aios/kernel/store.py:8-29) ------------------------------
 // One warp per token; k and v rows are `width` bf16 values.
-__global__ void kv_store_kernel(__nv_bfloat16* __restrict__ k_cache, __nv_bfloat16* __restrict__ v_cache,
-                                int64_t cache_stride, int64_t num_slots, const int32_t* __restrict__ indices,
-                                int64_t num_tokens, const __nv_bfloat16* __restrict__ k, int64_t k_stride,
-                                const __nv_bfloat16* __restrict__ v, int64_t v_stride, int64_t width, bool vec,
+__global__ void kv_store_kernel(__nv_bfloat16* k_cache, __nv_bfloat16* v_cache, int64_t cache_stride,
+                                int64_t num_slots, const int32_t* indices, int64_t num_tokens, const __nv_bfloat16* k,
+                                int64_t k_stride, const __nv_bfloat16* v, int64_t v_stride, int64_t width, bool vec,
                                 int32_t* status) {
   pdl_enter();
   const int64_t t = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
@@ -151,8 +153,7 @@ __global__ void add_rmsnorm_kernel(__nv_bfloat16* __restrict__ x, __nv_bfloat16*
 // ---- SwiGLU (FlashInfer silu_and_mul semantics) ---------------------------
 __device__ __forceinline__ float silu_f(float g) { return g / (1.0f + expf(-g)); }
 
-__global__ void silu_mul_kernel(const __nv_bfloat16* __restrict__ x, int64_t rows, int64_t f,
-                                __nv_bfloat16* __restrict__ out) {
+__global__ void silu_mul_kernel(const __nv_bfloat16* x, int64_t rows, int64_t f, __nv_bfloat16* out) {
   pdl_enter();
   const int64_t nvec = f / 8;
   const int64_t total = rows * nvec;
@@ -174,7 +175,7 @@ __global__ void silu_mul_kernel(const __nv_bfloat16* __restrict__ x, int64_t row
 // One warp per token. With stat_x, also writes the row in fp32 and its sum of
 // squares (stat_ss[t], a single part): the statistics a following
 // aiosb_linear_stat_norm normalises from.
-__global__ void embedding_kernel(const void* __restrict__ ids, bool ids64, int64_t n, const uint4* __restrict__ w,
+__global__ void embedding_kernel(const void* ids, bool ids64, int64_t n, const uint4* __restrict__ w,
                                  int64_t vocab, int64_t hidden, uint4* __restrict__ out, float* __restrict__ stat_x,
                                  float* __restrict__ stat_ss, int32_t* status) {
   pdl_enter();

@@ -798,10 +798,9 @@ __device__ __forceinline__ void apply_forbidden(RowSmem& s, int V, const int32_t
 
 // ---- generic sampler: Sampler.sample_with_logprobs ------------------------
 __global__ void __launch_bounds__(kSampThreads, 1)
-    sample_kernel(const __nv_bfloat16* __restrict__ logits, int64_t row_stride, int V, SampleParams p,
-                  const float* __restrict__ uniforms, const int32_t* __restrict__ forbidden, int n_forbidden,
-                  const int64_t* __restrict__ forbidden_rows, int n_forbidden_rows, int64_t* __restrict__ tok_out,
-                  float* __restrict__ lp_out, int32_t* status, int large) {
+    sample_kernel(const __nv_bfloat16* logits, int64_t row_stride, int V, SampleParams p, const float* uniforms,
+                  const int32_t* forbidden, int n_forbidden, const int64_t* forbidden_rows, int n_forbidden_rows,
+                  int64_t* tok_out, float* lp_out, int32_t* status, int large) {
   extern __shared__ uint8_t smem_raw[];
   RowSmem& s = *reinterpret_cast<RowSmem*>(smem_raw);
   uint32_t* keys = reinterpret_cast<uint32_t*>(smem_raw + sizeof(RowSmem));
@@ -1406,7 +1405,7 @@ __device__ __forceinline__ float splitmix_uniform(uint64_t seed, uint64_t step) 
   return __double2float_rn(d);
 }
 
-__global__ void group_begin_kernel(aiosb_group_ptrs g, const __nv_bfloat16* __restrict__ prefix_logits,
+__global__ void group_begin_kernel(aiosb_group_ptrs g, const __nv_bfloat16* prefix_logits,
                                    uint64_t seed_base, int attempts) {
   pdl_enter();
   aiosb_group_state* st = g.state;
@@ -1487,8 +1486,8 @@ size_t sample_smem_max() { return std::max(sample_smem(kMaxVocab), sample_smem_l
 // Page-table reset for a keystroke: rows [0, rows) get the prefix slots in
 // columns [0, n) and zeros in [n, width) (the reference builds a fresh zero table
 // per keystroke and writes the prefix slots into every row, aios/ime.py:482-485,1155).
-__global__ void page_table_fill_kernel(int32_t* __restrict__ table, int64_t stride, int rows, int width,
-                                       const int32_t* __restrict__ prefix, int n) {
+__global__ void page_table_fill_kernel(int32_t* table, int64_t stride, int rows, int width, const int32_t* prefix,
+                                       int n) {
   pdl_enter();
   const int64_t total = (int64_t)rows * width;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
@@ -1499,8 +1498,8 @@ __global__ void page_table_fill_kernel(int32_t* __restrict__ table, int64_t stri
 
 // Raw log-probability of a given target per row (teacher-forced scoring).
 __global__ void __launch_bounds__(kSampThreads)
-    token_logprob_kernel(const __nv_bfloat16* __restrict__ logits, int64_t row_stride, int V,
-                         const int64_t* __restrict__ targets, float* __restrict__ out, int32_t* status) {
+    token_logprob_kernel(const __nv_bfloat16* logits, int64_t row_stride, int V, const int64_t* targets, float* out,
+                         int32_t* status) {
   extern __shared__ uint8_t smem_raw[];
   RowSmem& s = *reinterpret_cast<RowSmem*>(smem_raw);
   pdl_enter();
