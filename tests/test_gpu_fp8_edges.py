@@ -112,3 +112,72 @@ def test_every_pair_of_extreme_scales(cuda_device, rows: int) -> None:
     rest = ~over & ~want.isnan()
     bad = (y - want).abs()[rest] > 2.0**-8 * want[rest].abs() + 2.0**-134 + 2.0**-149
     assert not bool(bad.any())
+
+
+def _every_operator(rows: int = 13, width: int = 784):
+    x = torch.randn(rows, width, device="cuda", generator=torch.Generator("cuda").manual_seed(3)).to(torch.bfloat16)
+    r, g = x.flip(0).contiguous(), x[0].contiguous()
+    wq, ws = ops.quantize_weight_fp8(x[:8].contiguous())
+    q, s = ops.quantize_fp8(x)
+    out = [q, s, wq, ws, *ops.rmsnorm_fp8(x, g, 1e-6), *ops.fused_add_rmsnorm_fp8(x, r, g, 1e-6), r]
+    out += [*ops.silu_and_mul_fp8(x[:, : width - 16]), ops.linear_fp8(q, s, wq, ws)]
+    return [t.view(torch.uint8) if t.dtype is ops.FP8_DTYPE else t for t in out]
+
+
+def test_outputs_do_not_depend_on_how_they_are_allocated(cuda_device, monkeypatch) -> None:
+    """The allocator's short entry, its fallback, and the fill of fresh memory that deterministic mode asks for."""
+    want = _every_operator()
+    monkeypatch.setattr(ops, "_new_cuda", None)
+    got = _every_operator()
+    torch.use_deterministic_algorithms(True)
+    try:
+        filled = _every_operator()
+    finally:
+        torch.use_deterministic_algorithms(False)
+    for a, b, c in zip(want, got, filled):
+        assert a.shape == b.shape and a.stride() == b.stride() and a.dtype == b.dtype
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_single_rows_of_wide_buffers(cuda_device) -> None:
+    """One row has no stride; its buffers' rows may be any distance apart."""
+    q, s, wq, ws = _linear_inputs(1, 264, 784)
+    wide = torch.zeros(3, 1008, dtype=torch.uint8, device=cuda_device)
+    wide[1:2, 16:800] = q.view(torch.uint8)
+    x = wide.view(ops.FP8_DTYPE)[1:2, 16:800]
+    want = ops.linear_fp8(q, s, wq, ws)
+    buf = torch.full((3, 500), float("nan"), dtype=torch.bfloat16, device=cuda_device)
+    out = buf[1:2, 4:268]  # row 1 begins 1000 bytes in: 16-byte aligned from its fifth value on
+    r = torch.randn(1, 264, device=cuda_device).to(torch.bfloat16)
+    ops.linear_fp8(q, s, wq, ws, out=out, epilogue=_lib.EPI_ADD, residual=r)
+    _linear_check(out, q, s, wq, ws, r)
+    assert int(buf.isnan().sum()) == buf.numel() - 264
+    assert torch.equal(ops.linear_fp8(x, s, wq, ws), want)
+
+
+@pytest.mark.parametrize("rows,n,k", [(100001, 8, 16), (70000, 72, 144), (1, 100008, 16)])
+def test_thin_linears(cuda_device, rows: int, n: int, k: int) -> None:
+    q, s, wq, ws = _linear_inputs(rows, n, k)
+    y = ops.linear_fp8(q, s, wq, ws)
+    _linear_check(y, q, s, wq, ws)
+    assert torch.equal(y, ops.linear_fp8(q, s, wq, ws, stable_weight=True))
+    ops.check_status(cuda_device)
+
+
+def test_operands_that_are_the_same_tensor(cuda_device) -> None:
+    """x + x in place, the sum written over x, and a weight that is its own input."""
+    x = torch.randn(40, 784, device=cuda_device).to(torch.bfloat16)
+    g = torch.ones(784, dtype=torch.bfloat16, device=cuda_device)
+    want = ops.rmsnorm_fp8((2 * x.float()).to(torch.bfloat16), g, 4e-6)
+    a = x.clone()
+    q, s = ops.fused_add_rmsnorm_fp8(a, a, g, 4e-6)
+    assert torch.equal(q.view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(s, want[1])
+    assert torch.equal(a, (2 * x.float()).to(torch.bfloat16))
+    b, r = x.clone(), x.flip(0).contiguous()
+    q, s = ops.fused_add_rmsnorm_fp8(b, r, g, 1e-6, residual_out=b)
+    q2, s2 = ops.fused_add_rmsnorm_fp8(x, r, g, 1e-6, residual_out=torch.empty_like(x))
+    assert torch.equal(q.view(torch.uint8), q2.view(torch.uint8)) and torch.equal(s, s2)
+    assert torch.equal(b, (x.float() + r.float()).to(torch.bfloat16)) and torch.equal(r, x.flip(0))
+    wq, ws = ops.quantize_weight_fp8(x)
+    xq, xs = ops.quantize_fp8(x)
+    _linear_check(ops.linear_fp8(wq, xs, wq, ws), wq, xs, wq, ws)
