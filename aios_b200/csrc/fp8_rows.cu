@@ -52,8 +52,10 @@ __global__ void __launch_bounds__(TPR == 32 ? kThreads : TPR) norm_fp8_kernel(co
   const __nv_bfloat16* xr = a.x + r * a.x_stride;
   const int64_t base = r * a.hidden;
   // The weight comes with the row, so that its latency hides behind the row's (8 x 768: 2.2
-  // -> 1.8 us), except where four units without a residual would lose occupancy to it (4096 x
-  // 1024: 4.6 us without, 5.1 with).
+  // -> 1.8 us), except with four units and no residual, where its registers cost occupancy. Late /
+  // early there, us: 4096 x 1024 4.6 / 5.0, 8192 x 4096 20.6 / 21.3, 8192 x 16384 84.1 / 88.4; a
+  // block to a row and few rows would gain: 2048 x 4096 7.4 / 7.3, 2048 x 8192 13.5 / 12.6, 1024 x
+  // 16384 15.0 / 14.1; 16384 x 8192 78.7 / 77.9.
   constexpr bool kEarlyWeight = U < 4 || RES;
   uint4 xv[U], rv[U], wv[U];
 #pragma unroll

@@ -127,8 +127,11 @@ class MiniMindAttnResDecoderLayer(BaseOP):
         mixer, norm = self.attn_res_mixer, self.input_layernorm
         if fp8:
             # 8-bit linears: the mixers stay bf16, their rows are quantised for the linear
-            # that follows; the deltas are added in the linears' epilogues as below. Each
-            # kernel lets its successor launch only after its own wait, as `stable` needs.
+            # that follows; the deltas are added in the linears' epilogues as below. `stable`
+            # rests on the kernels right before each mixer, which let it launch only after
+            # their own wait: the SwiGLU and down projection of the layer before, the
+            # attention's quantiser and the o projection here. (Attention and q/k norm do not
+            # wait first, so a mixer must not follow them directly.)
             rows = ops.quantize_fp8(mix_and_norm(mixer, norm, bank, partial, mixed, stable))
             attn = self.self_attn.attend_qkv(self.self_attn.qkv_proj.forward_fp8(*rows), rotary, paged_kv_cache, batch)
             partial = self.self_attn.o_proj.forward_fp8(*ops.quantize_fp8(attn), out=partial, residual=partial)
