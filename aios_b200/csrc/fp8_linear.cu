@@ -226,7 +226,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         uint32_t blocks = 0;
-        if (__any_sync(0xffffffffu, range.far())) blocks = split_group(sx, sw, kb, min(kScaleGroup, kb1 - kb), store);
+        if (__any_sync(0xffffffffu, range.far()))
+          blocks = split_group(x, w, sx, sw, kb, min(kScaleGroup, kb1 - kb), store);
         if (lane == 0) far_blocks[g] = blocks;
         __syncwarp();
         if (lane == 0) mbar_arrive(&scale_full[g]);

@@ -155,26 +155,42 @@ struct ScaleRange {
   }
   __device__ __forceinline__ bool far() const { return lo < 0x1p-134f || hi > FLT_MAX; }
 };
+__device__ __forceinline__ bool splits(float x, float w) {
+  const float p = fabsf(x * w), lo = fminf(fabsf(x), fabsf(w)), hi = fmaxf(fabsf(x), fabsf(w));
+  // not where a scale itself is zero, infinite or NaN
+  return (p > FLT_MAX && hi <= FLT_MAX) || (p < 0x1p-134f && lo * 0x1p26f * hi != 0.f);
+}
 __device__ __forceinline__ void split_scales(float x, float w, float* first, float* second) {
-  const float p = x * w, lo = fminf(fabsf(x), fabsf(w)), hi = fmaxf(fabsf(x), fabsf(w));
-  const bool over = fabsf(p) > FLT_MAX && hi <= FLT_MAX;  // not where a scale itself is infinite or NaN
-  const bool under = fabsf(p) < 0x1p-134f && lo * 0x1p26f * hi != 0.f;
-  const bool x_first = over == (fabsf(x) == lo);
-  *first = !(over || under) ? 1.f : x_first ? x : w;
-  *second = !(over || under) ? p : x_first ? w : x;
+  const float p = x * w;
+  const bool x_first = (fabsf(p) > FLT_MAX) == (fabsf(x) <= fabsf(w));
+  const bool split = splits(x, w);
+  *first = !split ? 1.f : x_first ? x : w;
+  *second = !split ? p : x_first ? w : x;
 }
 template <int N>
 __device__ __forceinline__ void scale_all(uint32_t (&d)[N], float first) {
 #pragma unroll
   for (int j = 0; j < N; ++j) d[j] = __float_as_uint(__uint_as_float(d[j]) * first);
 }
-// The blocks (bits) among `count` from `kb` on whose products need split_scales in any of the
-// warp's rows (kRows a lane); their factors go to store(row, block, second, first). Reads the
-// scales again: the caller keeps none of them in registers for a case that hardly occurs.
+// Behind ScaleRange: the blocks (bits) among `count` from `kb` on whose products need split_scales
+// in any of the warp's rows (kRows a lane); their factors go to store(row, block, second, first).
+// Most of what leaves the range are scales of 0, which some quantisers give empty rows: those are
+// told apart in registers. Factors are written from scales that are read again.
 template <int kRows, typename Store>
-__device__ __forceinline__ uint32_t split_group(const float* const (&sx)[kRows], const float* sw, int kb, int count,
+__device__ __forceinline__ uint32_t split_group(const float (&x)[kRows][kScaleGroup], const float (&w)[kScaleGroup],
+                                                const float* const (&sx)[kRows], const float* sw, int kb, int count,
                                                 Store store) {
+  bool any = false;
+#pragma unroll
+  for (int j = 0; j < kScaleGroup; ++j) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const float p = fabsf(x[i][j] * w[j]);
+      any |= (p < 0x1p-134f || p > FLT_MAX) && fminf(fabsf(x[i][j]), fabsf(w[j])) > 0.f;
+    }
+  }
   uint32_t blocks = 0;
+  if (!__any_sync(0xffffffffu, any)) return blocks;
 #pragma unroll 1
   for (int j = 0; j < count; ++j) {
     bool split = false;
@@ -182,7 +198,7 @@ __device__ __forceinline__ uint32_t split_group(const float* const (&sx)[kRows],
     for (int i = 0; i < kRows; ++i) {
       float first, second;
       split_scales(sx[i][kb + j], sw[kb + j], &first, &second);
-      split |= first != 1.f;
+      split |= splits(sx[i][kb + j], sw[kb + j]);
       store(i, j, second, first);
     }
     blocks |= (uint32_t)__any_sync(0xffffffffu, split) << j;

@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int b = 0; b < kWBlocks; ++b) {
           uint32_t blocks = 0;
           if (any_far)
-            blocks = split_group(sx, sw[b], kb, min(kScaleGroup, kblocks - kb),
+            blocks = split_group(x, w[b], sx, sw[b], kb, min(kScaleGroup, kblocks - kb),
                                  [&](int i, int j, float product, float) {
                                    scales[((g * kScaleGroup + j) * kWBlocks + b) * kBM + i * 32 + lane] = product;
                                  });
