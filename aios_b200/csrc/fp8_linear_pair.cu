@@ -18,8 +18,8 @@
 // out); a residual is fetched into the same place by asynchronous copies issued at the
 // tile's start.
 //
-// Measured: 2048 x 4096 x 4096 36 us (1910 TFLOP/s; its 128 tiles fill 1.7 of 2 rounds of
-// 74 pairs), 8192^3 480 us (2290 TFLOP/s) in a short burst and 515 us under sustained load,
+// Measured: 2048 x 4096 x 4096 35-36 us (1910-1960 TFLOP/s; its 128 tiles fill 1.7 of 2 rounds of
+// 74 pairs), 8192^3 469-485 us (2270-2345 TFLOP/s) in a short burst and 515 us under sustained load,
 // where the board's power limit sets the pace: the SM clock drops to 1.4-1.7 GHz. The
 // tensor pipe is active 51% of the SM cycles at 2048 x 4096 x 4096 and L2 at 26% of its
 // throughput: what is left there are the half-empty second round and the prologue. Tried
