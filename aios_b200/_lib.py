@@ -26,6 +26,8 @@ DEV_SLOT_RANGE = 2
 DEV_TOKEN_RANGE = 3
 DEV_POOL_EMPTY = 4
 DEV_POSITION_RANGE = 5
+DEV_TREE_RANGE = 6
+DEV_NO_DISTRIBUTION = 7
 
 DEVICE_STATUS_NAMES = {
     DEV_WAIT_TIMEOUT: "a bounded device wait ran out",
@@ -33,6 +35,8 @@ DEVICE_STATUS_NAMES = {
     DEV_TOKEN_RANGE: "token id outside the vocabulary",
     DEV_POOL_EMPTY: "free-slot FIFO exhausted",
     DEV_POSITION_RANGE: "position outside the RoPE table",
+    DEV_TREE_RANGE: "drafted tree or its history outside its arrays",
+    DEV_NO_DISTRIBUTION: "logits row that no token can be drawn from",
 }
 
 EPI_STORE = 0
@@ -48,6 +52,7 @@ _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _u64 = ctypes.c_uint64
 
 
@@ -206,6 +211,16 @@ _SIGNATURES = {
          _i64, _i64, _i64, _i64, _f32, _p, _i64, _p, _p],
         _i32,
     ),
+    "aiosb_draft_tree": ([_p, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p], _i32),
+    "aiosb_attention_tree_work_bytes": ([_i64] * 7, _i64),
+    "aiosb_attention_tree": (
+        [_p, _i64, _i64, _p, _p, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64,
+         _f32, _p, _i64, _p, _i64, _p, _p],
+        _i32,
+    ),
+    "aiosb_verify_draft": (
+        [_p, _i32, _i64, _i64, _i64, _p, _p, _p, _i64, _p, _p, _f64, _i32, _p, _i64, _p, _p, _p, _p, _p], _i32
+    ),
     "aiosb_sample": (
         [_p, _i64, _i64, _i64, _f32, _i64, _f32, _i32, _p, _p, _i64, _p, _i64, _p, _p, _p, _p],
         _i32,
@@ -272,7 +287,7 @@ def check(rc: int, what: str) -> None:
 _NON_LAUNCHING = frozenset({"aiosb_version", "aiosb_last_error", "aiosb_host_device_pointer",
                             "aiosb_prefill_tile_tokens", "aiosb_decode_step_sync_words",
                             "aiosb_decode_step_work_bytes", "aiosb_linear_tile_stats_eligible",
-                            "aiosb_linear_fp8_plan"})
+                            "aiosb_linear_fp8_plan", "aiosb_attention_tree_work_bytes"})
 launches = 0
 _functions: dict[str, object] = {}
 

@@ -1,0 +1,80 @@
+// Shared by the kernels of drafted token trees: the requests' trees and the attention's arguments.
+//
+// Tree of request r: rows tree_start[r] .. tree_start[r + 1] of the flat token arrays. Its keys are
+// the `cached` tokens of its page-table row, which every node sees, and one key per node behind
+// them (page-table entry cached + j is node j's slot), which node i sees if bit j of its mask is set.
+#pragma once
+
+#include "abi_util.h"
+#include "common.cuh"
+
+namespace aiosb {
+
+struct TreeAttnArgs {
+  const __nv_bfloat16* q;  // [tokens, q_stride], heads of a token side by side
+  int64_t q_stride;
+  const __nv_bfloat16* k_cache;  // [num_slots, hkv, d]
+  const __nv_bfloat16* v_cache;
+  int64_t num_slots;
+  const int32_t* page_table;  // [table_rows, table_stride], table_width entries each
+  int64_t table_stride;
+  int table_rows, table_width;
+  const int32_t* row_table;    // [requests]
+  const int32_t* cached_lens;  // [requests]
+  const int32_t* tree_start;   // [requests + 1]
+  const int32_t* mask;         // [tokens, words]
+  int words;
+  int requests, tokens;
+  int hq, hkv, group;
+  float scale_log2;  // scale * log2(e): exponents are taken to base 2
+  __nv_bfloat16* out;
+  int64_t out_stride;
+  void* work;
+  int32_t* status;
+};
+
+struct TreeRequest {
+  int start, nodes;  // rows of the flat token arrays
+  int cached, keys;  // keys [0, cached) are history, [cached, keys) the tree's
+  const int32_t* slots;
+};
+
+// Request r with its numbers held inside the arrays; `tell`: report what had to be cut.
+__device__ __forceinline__ TreeRequest tree_request(const TreeAttnArgs& a, int r, bool tell) {
+  TreeRequest t;
+  const int s = a.tree_start[r], e = a.tree_start[r + 1], c = a.cached_lens[r], row = a.row_table[r];
+  t.start = min(max(s, 0), a.tokens);
+  t.nodes = min(max(e, t.start), a.tokens) - t.start;
+  const bool row_ok = row >= 0 && row < a.table_rows;
+  t.cached = row_ok ? min(max(c, 0), a.table_width) : 0;
+  t.keys = row_ok ? t.cached + min(min(t.nodes, 32 * a.words), a.table_width - t.cached) : 0;
+  t.slots = a.page_table + (row_ok ? row : 0) * a.table_stride;
+  if (tell && (t.start != s || t.start + t.nodes != e || t.cached != c || t.keys - t.cached != t.nodes) && t.nodes > 0)
+    report(a.status, AIOSB_DEV_TREE_RANGE);
+  if (tell && (s < 0 || e < s || e > a.tokens)) report(a.status, AIOSB_DEV_TREE_RANGE);
+  return t;
+}
+
+__device__ __forceinline__ int64_t tree_slot(const TreeAttnArgs& a, int32_t slot) {
+  if (slot >= 0 && slot < a.num_slots) return slot;
+  report(a.status, AIOSB_DEV_SLOT_RANGE);
+  return 0;
+}
+
+// 2^x to fp32, x <= 0 or so: one special-function instruction, off by 2^-22.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ bool finite_bf16x2(uint32_t v) {
+  return (v & 0x7F800000u) != 0x7F800000u && (v & 0x7F80u) != 0x7F80u;
+}
+__device__ __forceinline__ uint32_t drop_nonfinite_bf16x2(uint32_t v) {
+  if ((v & 0x7F800000u) == 0x7F800000u) v &= 0x0000FFFFu;
+  if ((v & 0x7F80u) == 0x7F80u) v &= 0xFFFF0000u;
+  return v;
+}
+
+}  // namespace aiosb

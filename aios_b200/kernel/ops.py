@@ -1028,6 +1028,198 @@ def prefill_meta(
 
 
 # ---------------------------------------------------------------------------
+# Drafted token trees (speculative decoding)
+# ---------------------------------------------------------------------------
+TREE_MAX_NODES = 1024  # nodes of a tree
+
+
+def _check_ints(what: str, name: str, t: torch.Tensor, size: int, index: int, dtype: torch.dtype = torch.int32) -> None:
+    if t.dtype is not dtype or t.ndim != 1 or t.shape[0] != size or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be a contiguous {dtype} tensor of {size} on cuda:{index}")
+
+
+def _check_trees(what: str, tokens: int, tree_start: torch.Tensor, index: int) -> int:
+    """The number of trees."""
+    if tree_start.ndim != 1 or tree_start.shape[0] < 1:
+        raise ValueError(f"{what}: tree_start must have shape [requests + 1]")
+    requests = tree_start.shape[0] - 1
+    _check_ints(what, "tree_start", tree_start, requests + 1, index)
+    return requests
+
+
+def draft_tree(
+    parents: torch.Tensor,
+    tree_start: torch.Tensor,
+    *,
+    max_nodes: int,
+    cached_lens: torch.Tensor | None = None,
+    mask: torch.Tensor | None = None,
+    positions: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The ancestors' bits and the positions of drafted trees' nodes.
+
+    Tree r is rows ``tree_start[r]`` to ``tree_start[r + 1]`` (int32, ascending); node 0 is the
+    last token that is known, ``parents`` (int32) the number of each node's parent in its tree,
+    less than its own, or -1. Returns ``mask`` (int32 [tokens, ceil(max_nodes / 32)]: bit j is set
+    if node j is the node or an ancestor of it) and ``positions`` (int32: ``cached_lens[r]`` + the
+    number of ancestors). ``max_nodes``: a bound on the nodes of a tree, at most 1024. Rows behind
+    the last tree are left as they were."""
+    if not parents.is_cuda:
+        raise ValueError("draft_tree requires CUDA tensors")
+    if parents.ndim != 1:
+        raise ValueError("draft_tree: parents must have shape [tokens]")
+    if not 1 <= max_nodes <= TREE_MAX_NODES:
+        raise ValueError(f"draft_tree: max_nodes must be in [1, {TREE_MAX_NODES}]")
+    tokens, index, words = parents.shape[0], parents.get_device(), (max_nodes + 31) // 32
+    _check_ints("draft_tree", "parents", parents, tokens, index)
+    requests = _check_trees("draft_tree", tokens, tree_start, index)
+    if cached_lens is not None:
+        _check_ints("draft_tree", "cached_lens", cached_lens, requests, index)
+    if mask is None:
+        mask = _empty_rows(parents, tokens, words, torch.int32)
+    else:
+        _check_dense("draft_tree", "mask", mask, (tokens, words), torch.int32, index)
+    if positions is None:
+        positions = parents.new_empty(tokens)
+    else:
+        _check_ints("draft_tree", "positions", positions, tokens, index)
+    if tokens and requests:
+        _launch(index, "aiosb_draft_tree", parents.data_ptr(), tokens, tree_start.data_ptr(), requests, words,
+                _ptr(cached_lens), mask.data_ptr(), positions.data_ptr(), _status_pointer(index))
+    return mask, positions
+
+
+def attention_tree(
+    *,
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    page_table: torch.Tensor,
+    row_table: torch.Tensor,
+    cached_lens: torch.Tensor,
+    tree_start: torch.Tensor,
+    tree_mask: torch.Tensor,
+    num_qo_heads: int,
+    num_kv_heads: int,
+    head_dim: int,
+    scale: float,
+    max_cached: int = 0,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of drafted trees over the paged cache (``draft_tree`` for the arguments of the
+    trees). q and out are bf16 [tokens, Hq * d], rows may be strided; the nodes' own K/V are in
+    the cache (``qk_norm_rope_store``). Node i of request r sees the first ``cached_lens[r]``
+    entries of page-table row ``row_table[r]``, and entry ``cached_lens[r] + j`` for every set bit
+    j of ``tree_mask[i]`` (int32 [tokens, words]; any bits). A node that sees nothing gets 0.
+    ``max_cached``: a bound on ``cached_lens`` from which the split over the GPU is chosen (0: the
+    page table's width)."""
+    width = num_qo_heads * head_dim
+    tokens, cols, q_stride = _check_rows("attention_tree", q, torch.bfloat16)
+    index = q.get_device()
+    if cols != width:
+        raise ValueError("attention_tree: q must have shape [tokens, num_qo_heads * head_dim]")
+    if out is None:
+        out, out_stride = _empty_rows(q, tokens, width, torch.bfloat16), width
+    else:
+        rows, cols, out_stride = _check_rows("attention_tree", out, torch.bfloat16)
+        if rows != tokens or cols != width or out.get_device() != index:
+            raise ValueError("attention_tree: out must match q")
+    slots = k_cache.shape[0]
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if (t.dtype is not torch.bfloat16 or t.shape != (slots, num_kv_heads, head_dim) or t.get_device() != index
+                or not t.is_contiguous()):
+            raise ValueError(f"attention_tree: {name} must be a contiguous bf16 [slots, num_kv_heads, head_dim] tensor "
+                             f"on cuda:{index}")
+    requests = _check_trees("attention_tree", tokens, tree_start, index)
+    _check_ints("attention_tree", "row_table", row_table, requests, index)
+    _check_ints("attention_tree", "cached_lens", cached_lens, requests, index)
+    if (page_table.dtype is not torch.int32 or page_table.ndim != 2 or page_table.get_device() != index
+            or (page_table.shape[1] > 1 and page_table.stride(1) != 1)):
+        raise ValueError("attention_tree: page_table must be an int32 tensor of contiguous rows")
+    table_rows, table_width = page_table.shape
+    if tree_mask.ndim != 2:
+        raise ValueError("attention_tree: tree_mask must have shape [tokens, words]")
+    words = tree_mask.shape[1]
+    _check_dense("attention_tree", "tree_mask", tree_mask, (tokens, words), torch.int32, index)
+    if tokens and requests:
+        size = _lib.load().aiosb_attention_tree_work_bytes(tokens, requests, words, max_cached or table_width,
+                                                           num_qo_heads, num_kv_heads, head_dim)
+        work = _empty_rows(q, 1, size, torch.uint8) if size else None
+        _launch(index, "aiosb_attention_tree", q.data_ptr(), q_stride, tokens, k_cache.data_ptr(), v_cache.data_ptr(),
+                slots, page_table.data_ptr(), page_table.stride(0) if table_rows > 1 else table_width, table_rows,
+                table_width, row_table.data_ptr(), cached_lens.data_ptr(), tree_start.data_ptr(), requests,
+                tree_mask.data_ptr(), words, max_cached, num_qo_heads, num_kv_heads, head_dim, float(scale),
+                out.data_ptr(), out_stride, _ptr(work), size, _status_pointer(index))
+    return out
+
+
+def verify_draft(
+    logits: torch.Tensor,
+    draft_tokens: torch.Tensor,
+    parents: torch.Tensor,
+    tree_start: torch.Tensor,
+    accept_uniforms: torch.Tensor | None = None,
+    sample_uniforms: torch.Tensor | None = None,
+    *,
+    temperature: float = 1.0,
+    greedy: bool = False,
+    draft_probs: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Which drafted nodes stay, judged against the target model, and the token after them.
+
+    ``logits`` (bf16 or fp32 [tokens, vocab]): row i is the target's distribution after node i;
+    ``draft_tokens`` (int64): the nodes' tokens; the trees as for ``draft_tree``. From the root
+    on, a node's children are tried in order: child c stays if ``accept_uniforms[c] * q(x) *
+    sum(r) < r(x)``, where r is softmax(logits / temperature) less what the rejected ones took,
+    and q is ``draft_probs`` (fp32 [tokens, vocab]; row i: the distribution that i's children were
+    drawn from, independently) or 1 without it (distinct proposals). With no child left the next
+    token is drawn from r by inverse CDF with ``sample_uniforms``. What is kept has the target's
+    distribution. ``greedy``: children and next token by argmax (the lowest id of equal ones).
+    A sampler's filters (top-k, forbidden ids) go in as logits of -inf.
+
+    Returns ``accepted`` (int32 [requests]: nodes behind the root that stay), ``next_token``
+    (int64 [requests]; -1 where there is no tree or no distribution) and ``order`` (int32
+    [tokens]: each tree's node numbers, the path from the root first, then the others)."""
+    if not logits.is_cuda:
+        raise ValueError("verify_draft requires CUDA tensors")
+    if logits.ndim != 2 or logits.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("verify_draft: logits must be a bf16 or fp32 tensor of shape [tokens, vocab]")
+    tokens, vocab = logits.shape
+    index = logits.get_device()
+    if vocab > 1 and logits.stride(1) != 1:
+        raise ValueError("verify_draft: logits rows must be contiguous")
+    _check_ints("verify_draft", "draft_tokens", draft_tokens, tokens, index, torch.int64)
+    _check_ints("verify_draft", "parents", parents, tokens, index)
+    requests = _check_trees("verify_draft", tokens, tree_start, index)
+    if greedy:
+        if draft_probs is not None:
+            raise ValueError("verify_draft: greedy verification takes no draft_probs")
+        accept_uniforms = sample_uniforms = None
+    else:
+        if accept_uniforms is None or sample_uniforms is None:
+            raise ValueError("verify_draft: sampling needs accept_uniforms and sample_uniforms")
+        _check_ints("verify_draft", "accept_uniforms", accept_uniforms, tokens, index, torch.float32)
+        _check_ints("verify_draft", "sample_uniforms", sample_uniforms, requests, index, torch.float32)
+    probs_stride = 0
+    if draft_probs is not None:
+        if (draft_probs.dtype is not torch.float32 or draft_probs.shape != (tokens, vocab)
+                or draft_probs.get_device() != index or (vocab > 1 and draft_probs.stride(1) != 1)):
+            raise ValueError("verify_draft: draft_probs must be an fp32 [tokens, vocab] tensor with contiguous rows "
+                             f"on cuda:{index}")
+        probs_stride = draft_probs.stride(0) if tokens > 1 else vocab
+    accepted = parents.new_empty(requests)
+    next_token = draft_tokens.new_empty(requests)
+    order = parents.new_empty(tokens)
+    if requests:
+        _launch(index, "aiosb_verify_draft", logits.data_ptr(), int(logits.dtype is torch.float32),
+                logits.stride(0) if tokens > 1 else vocab, tokens, vocab, draft_tokens.data_ptr(), parents.data_ptr(),
+                tree_start.data_ptr(), requests, _ptr(accept_uniforms), _ptr(sample_uniforms), float(temperature),
+                int(bool(greedy)), _ptr(draft_probs), probs_stride, accepted.data_ptr(), next_token.data_ptr(),
+                order.data_ptr(), _status_pointer(index))
+    return accepted, next_token, order
+
+
+# ---------------------------------------------------------------------------
 # Sampler / uniforms / slot FIFO
 # ---------------------------------------------------------------------------
 def sample(

@@ -52,6 +52,8 @@ extern "C" {
 #define AIOSB_DEV_TOKEN_RANGE 3   /* token id outside [0, vocab)                    */
 #define AIOSB_DEV_POOL_EMPTY 4    /* free-slot FIFO had fewer entries than asked    */
 #define AIOSB_DEV_POSITION_RANGE 5 /* RoPE position outside the cos/sin table      */
+#define AIOSB_DEV_TREE_RANGE 6    /* a drafted tree or its history outside its arrays */
+#define AIOSB_DEV_NO_DISTRIBUTION 7 /* a logits row that no token can be drawn from  */
 
 /* GEMM epilogues for aiosb_linear. */
 #define AIOSB_EPI_STORE 0    /* y = x W^T, bf16                                         */
@@ -70,6 +72,10 @@ extern "C" {
  * before the previous kernel on the stream began (a loaded model's), so the kernels for
  * few rows ask for them before the dependency wait. */
 #define AIOSB_LINEAR_STABLE_WEIGHT 0x200
+
+/* Drafted token trees: nodes of a tree, query heads of a KV head. */
+#define AIOSB_TREE_MAX_NODES 1024
+#define AIOSB_TREE_MAX_GROUP 64
 
 /* Library version (major*10000 + minor*100 + patch). */
 AIOSB_API int aiosb_version(void);
@@ -442,6 +448,79 @@ AIOSB_API int aiosb_token_logprobs(const void* logits, int64_t rows, int64_t voc
 /* Replaces stateless_uniforms (aios/engine/sample.py:12-45): out[r, t] is the
  * splitmix64 uniform of (seeds[r], t), computed in fp64 and rounded to fp32. */
 AIOSB_API int aiosb_stateless_uniforms(const int64_t* seeds, int64_t rows, int64_t steps, float* out, void* stream);
+
+/* ---- Drafted token trees (speculative decoding) ------------------------------
+ * No counterpart in the reference. A drafting model proposes a tree of tokens after
+ * each request's last token; the target model runs over all nodes in one forward
+ * (aiosb_draft_tree, then per layer aiosb_qk_norm_rope_store and
+ * aiosb_attention_tree) and aiosb_verify_draft keeps one path.
+ *
+ * Tree of request r: rows tree_start[r] .. tree_start[r + 1] of the flat token
+ * arrays (tree_start: [requests + 1] int32, ascending, at most `tokens`); rows
+ * behind the last tree are neither read nor written. Node 0 is the root, the last
+ * token that is known; parents[i] is the number of node i's parent in its tree, less
+ * than i, or -1 for a root. At most AIOSB_TREE_MAX_NODES nodes. Numbers outside
+ * their arrays are cut to them and reported as AIOSB_DEV_TREE_RANGE. */
+
+/* mask[i] ([tokens, words] int32): bit j % 32 of word j / 32 is set if node j of the
+ * same tree is node i or an ancestor of it; positions[i] = cached_lens[r] (or 0, if
+ * NULL) + the number of its ancestors. A node that does not fit the words
+ * (32 * words nodes a tree) gets its earlier ancestors only. */
+AIOSB_API int aiosb_draft_tree(const int32_t* parents, int64_t tokens, const int32_t* tree_start, int64_t requests,
+                               int64_t words, const int32_t* cached_lens, int32_t* mask, int32_t* positions,
+                               int32_t* status, void* stream);
+
+/* Attention of the trees' nodes over a paged cache. q, out: [tokens, stride] bf16, the
+ * heads of a token side by side; k_cache, v_cache: [num_slots, num_kv_heads, head_dim]
+ * bf16, the nodes' own keys among them. Node i of request r sees the slots
+ * page_table[row_table[r], 0 .. cached_lens[r]) and page_table[row_table[r],
+ * cached_lens[r] + j] for each set bit j of its mask, any set of them; a node that sees
+ * nothing gets 0, and what a node does not see does not reach it, infinities and NaN
+ * included. head_dim 64, 96 or 128; at most AIOSB_TREE_MAX_GROUP query heads to a KV
+ * head; mask_words up to AIOSB_TREE_MAX_NODES / 32. max_cached: a bound on cached_lens
+ * from which the split over the GPU is chosen (0: the page table's width); longer
+ * histories are read all the same.
+ * work: aiosb_attention_tree_work_bytes() bytes, 16-byte aligned, of any content;
+ * launches that may overlap need one each. */
+AIOSB_API int64_t aiosb_attention_tree_work_bytes(int64_t tokens, int64_t requests, int64_t mask_words,
+                                                  int64_t max_cached, int64_t num_qo_heads, int64_t num_kv_heads,
+                                                  int64_t head_dim);
+AIOSB_API int aiosb_attention_tree(const void* q, int64_t q_stride, int64_t tokens, const void* k_cache,
+                                   const void* v_cache, int64_t num_slots, const int32_t* page_table,
+                                   int64_t table_stride, int64_t table_rows, int64_t table_width,
+                                   const int32_t* row_table, const int32_t* cached_lens, const int32_t* tree_start,
+                                   int64_t requests, const int32_t* mask, int64_t mask_words, int64_t max_cached,
+                                   int64_t num_qo_heads, int64_t num_kv_heads, int64_t head_dim, float scale,
+                                   void* out, int64_t out_stride, void* work, int64_t work_bytes, int32_t* status,
+                                   void* stream);
+
+/* Verifies drafted trees against the target model's logits ([tokens, vocab], bf16 or,
+ * with logits_fp32, fp32; row i is the distribution after node i). Per request, from
+ * the root:
+ *   p = softmax(logits[node] / temperature), r = p;
+ *   the node's children c in ascending order: c is accepted if
+ *     accept_uniforms[c] * q(x_c) * sum(r) < r(x_c),   x_c = draft_tokens[c];
+ *   rejected, r becomes max(r / sum(r) - q, 0) with draft_probs (kept as it is where
+ *   that is 0 for every token), and r with r(x_c) = 0 without;
+ *   an accepted child is the next node; with none, the next token is the first v with
+ *     r(0) + ... + r(v) > sample_uniforms[r] * sum(r).
+ * draft_probs ([tokens, vocab] fp32 or NULL): row `node` is the distribution q that the
+ * node's children were drawn from, independently; without it q = 1 (distinct proposals).
+ * greedy: a child is accepted if it is the logits' argmax (the lowest id of equal ones),
+ * which is the next token; the uniforms may be NULL and the temperature is not read.
+ * Logits of -inf take a token out. Everything is computed in fp64 from the inputs.
+ * Outputs: accepted[r], the accepted nodes behind the root; next_token[r] (int64); order
+ * ([tokens]): the tree's node numbers, the path from the root first, the others after it
+ * in ascending order (the order in which a caller keeps the page-table entries). An empty
+ * tree gets 0 and -1. A row with a NaN, with +inf (unless greedy) or with -inf only ends
+ * the path with next_token -1 and AIOSB_DEV_NO_DISTRIBUTION; a draft token outside the
+ * vocabulary is rejected (AIOSB_DEV_TOKEN_RANGE). */
+AIOSB_API int aiosb_verify_draft(const void* logits, int logits_fp32, int64_t logits_stride, int64_t tokens,
+                                 int64_t vocab, const int64_t* draft_tokens, const int32_t* parents,
+                                 const int32_t* tree_start, int64_t requests, const float* accept_uniforms,
+                                 const float* sample_uniforms, double temperature, int greedy,
+                                 const float* draft_probs, int64_t probs_stride, int32_t* accepted,
+                                 int64_t* next_token, int32_t* order, int32_t* status, void* stream);
 
 /* ---- Free-slot FIFO ----------------------------------------------------------
  * Replaces CacheManager.allocate / _free (aios/scheduler/cache.py:16-18,46-51):
