@@ -241,6 +241,9 @@ cudaError_t launch_small(const TreeAttnArgs& a, int64_t max_nodes, cudaStream_t 
   return launch_pdl(kernel, grid, dim3(kThreads), kSmallSmem<D>, stream, a);
 }
 
+// Whether the keys are dealt over the SMs (attn_tree_split.cu).
+bool splits(int64_t max_cached) { return max_cached > 256; }
+
 }  // namespace
 }  // namespace aiosb
 
@@ -249,9 +252,9 @@ using namespace aiosb;
 extern "C" int64_t aiosb_attention_tree_work_bytes(int64_t tokens, int64_t requests, int64_t mask_words,
                                                    int64_t max_cached, int64_t num_qo_heads, int64_t num_kv_heads,
                                                    int64_t head_dim) {
-  (void)tokens, (void)requests, (void)mask_words, (void)max_cached;
-  (void)num_qo_heads, (void)num_kv_heads, (void)head_dim;
-  return 0;
+  if (tokens <= 0 || requests <= 0 || num_kv_heads <= 0 || !splits(max_cached)) return 0;
+  const int64_t rows = std::min(mask_words * 32, tokens) * (num_qo_heads / num_kv_heads);
+  return tree_split_work_bytes(tree_split_grid(), tree_split_unit_rows(rows), (int)head_dim);
 }
 
 extern "C" int aiosb_attention_tree(const void* q, int64_t q_stride, int64_t tokens, const void* k_cache,
@@ -287,7 +290,12 @@ extern "C" int aiosb_attention_tree(const void* q, int64_t q_stride, int64_t tok
                 AIOSB_ERR_INVALID_ARG, "attention_tree: null pointer");
   AIOSB_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out), AIOSB_ERR_MISALIGNED,
                 "attention_tree: q, out and the KV cache must be 16-byte aligned");
-  (void)work, (void)max_cached;
+  const bool split = splits(max_cached > 0 ? max_cached : table_width);
+  const int64_t max_nodes = std::min<int64_t>(mask_words * 32, tokens);
+  const int unit_rows = tree_split_unit_rows(max_nodes * group), grid = tree_split_grid();
+  AIOSB_REQUIRE(!split || (work != nullptr && aligned16(work) &&
+                           work_bytes >= tree_split_work_bytes(grid, unit_rows, (int)head_dim)),
+                AIOSB_ERR_INVALID_ARG, "attention_tree: work area missing, misaligned or too small");
   TreeAttnArgs a;
   a.q = (const __nv_bfloat16*)q;
   a.q_stride = q_stride;
@@ -314,9 +322,9 @@ extern "C" int aiosb_attention_tree(const void* q, int64_t q_stride, int64_t tok
   a.work = work;
   a.status = status;
   cudaStream_t s = as_stream(stream);
-  const int64_t max_nodes = std::min<int64_t>(mask_words * 32, tokens);
   cudaError_t e;
-  if (head_dim == 64) e = launch_small<64>(a, max_nodes, s);
+  if (split) e = launch_tree_split(a, (int)head_dim, grid, unit_rows, s);
+  else if (head_dim == 64) e = launch_small<64>(a, max_nodes, s);
   else if (head_dim == 96) e = launch_small<96>(a, max_nodes, s);
   else e = launch_small<128>(a, max_nodes, s);
   return check_launch("attention_tree", e);

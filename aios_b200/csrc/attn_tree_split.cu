@@ -1,0 +1,783 @@
+// Attention of drafted trees on tcgen05, the keys of all requests dealt evenly over the SMs.
+//
+// A unit is up to 256 rows ((node, query head) pairs) of one KV head of one request; its keys are
+// chunks of 128. The units' chunks laid end to end (a unit weighs its chunks and one more for its
+// start and end) are cut into one range per CTA, so that a CTA takes pieces of units, whatever the
+// requests' lengths. A piece that is a whole unit is written as it is; the pieces of a cut unit leave
+// their rows' maximum, sum and unnormalised output in fp32 in the work area, and a second kernel joins
+// them in the order of the keys.
+//
+// In a CTA: four warps gather keys and values into a ring of 128-key blocks with cp.async (the slots of
+// neighbouring keys are anywhere, so there is no box for TMA to fetch), one warp issues the MMAs, and
+// two groups of four warps hold the softmax of one stream each. With more than 128 rows the streams are
+// the two halves of the rows, both on every chunk; with fewer they are the even and the odd chunks of
+// the same rows, each with its own maximum, sum and output, joined at the end. So the MMAs of one stream
+// run while the other's exponentials are taken. S = Q K^T comes from shared memory into TMEM; a thread
+// owns a row (a TMEM lane), takes its maximum and exponentials, and writes the weights back over S as the
+// bf16 A operand of O += P V (V as it lies, the keys as its k: an MN-major B operand).
+// A row's output is rescaled only where its maximum has grown by more than 2^8 over the one that its
+// exponentials refer to: any reference gives the same quotient.
+#include <algorithm>
+
+#include "tree.cuh"
+
+namespace aiosb {
+namespace {
+
+constexpr int kTile = 128;      // rows of a tile: UMMA M, TMEM lanes
+constexpr int kUnitRows = 256;  // two tiles
+constexpr int kKeys = 128;      // keys of a chunk
+constexpr int kSoftWarps = 8;
+constexpr int kMmaWarp = kSoftWarps;
+constexpr int kLoadWarps = 4;
+constexpr int kThreads = (kSoftWarps + 1 + kLoadWarps) * 32;
+constexpr int kAtomBytes = kKeys * 128;  // 128 rows of 64 values, 128-byte swizzled
+constexpr int kUnitCost = 1;             // a unit's start and end, in chunks
+constexpr int kMinShare = 3;             // weight below which a range is not worth a CTA
+constexpr int kMaxGrid = 1024;
+constexpr int kLag = 2;                  // blocks that a loading warp leaves in flight
+constexpr int kBadSlots = 8;
+constexpr float kRescaleAt = 8.f;
+
+template <int D>
+struct Shape {
+  static constexpr int kAtoms = (D + 63) / 64;
+  static constexpr int kBlockBytes = kAtoms * kAtomBytes;  // a block of keys or values; also a tile of Q
+  static constexpr int kStages = kAtoms == 1 ? 10 : 5;
+  static constexpr int kSmem = 2 * kBlockBytes + kStages * kBlockBytes + 1024;
+};
+
+// ---- the cut --------------------------------------------------------------------------------
+struct Cut {
+  int64_t total;  // weight of all units
+  int ctas;       // ranges in use
+  __device__ __forceinline__ int64_t begin(int c) const { return total * c / ctas; }
+  // the range that holds position p
+  __device__ __forceinline__ int owner(int64_t p) const { return (int)(((p + 1) * ctas - 1) / total); }
+};
+
+struct Piece {
+  TreeRequest t;
+  int h;
+  int row0, rows;  // rows of the unit, in the request's (node, head) pairs
+  int c0, c1, chunks;
+  int64_t first_at;  // position of the unit's first chunk
+  __device__ __forceinline__ bool whole() const { return c0 == 0 && c1 == chunks; }
+  __device__ __forceinline__ bool pair() const { return rows > kTile; }
+};
+
+__device__ __forceinline__ int64_t unit_weight(const TreeRequest& t) {
+  return max(1, (t.keys + kKeys - 1) / kKeys) + kUnitCost;
+}
+__device__ __forceinline__ int unit_blocks(const TreeAttnArgs& a, const TreeRequest& t) {
+  return (t.nodes * a.group + kUnitRows - 1) / kUnitRows;
+}
+
+// The pieces of a range, in order. Every warp walks its own: a few loads a piece, ahead of what uses it.
+struct Pieces {
+  int64_t pos, end, base;
+  int r;
+  TreeRequest t;
+  int64_t w, span;
+
+  __device__ __forceinline__ void request(const TreeAttnArgs& a) {
+    t = tree_request(a, r, false);
+    w = unit_weight(t);
+    span = w * unit_blocks(a, t) * a.hkv;
+  }
+  __device__ __forceinline__ bool next(const TreeAttnArgs& a, Piece& p) {
+    while (pos < end) {
+      while (pos >= base + span) {
+        base += span;
+        ++r;
+        request(a);
+      }
+      const int blocks = unit_blocks(a, t);
+      const int64_t unit = (pos - base) / w, at = base + unit * w;
+      const int64_t stop = min(end, at + w);
+      p.c0 = (int)max((int64_t)0, pos - at - kUnitCost);
+      p.c1 = (int)(stop - at - kUnitCost);
+      pos = stop;
+      if (p.c1 <= p.c0) continue;
+      p.t = t;
+      p.h = (int)(unit / blocks);
+      p.row0 = (int)(unit % blocks) * kUnitRows;
+      p.rows = min(kUnitRows, t.nodes * a.group - p.row0);
+      p.chunks = (int)w - kUnitCost;
+      p.first_at = at + kUnitCost;
+      return true;
+    }
+    return false;
+  }
+};
+
+// ---- work area ------------------------------------------------------------------------------
+// Per range a descriptor of the cut unit that starts in it, then two slots of partial rows: slot 2c holds
+// the piece that goes on from the range before, slot 2c + 1 the one that starts here.
+struct __align__(16) Join {
+  int start, row0, rows, h;  // rows 0: nothing to join
+  int last;                  // the range with the unit's end
+  int pad[3];
+};
+template <int D>
+__host__ __device__ constexpr size_t slot_floats(int unit_rows) {
+  return (size_t)unit_rows * (D + 2);
+}
+__device__ __forceinline__ float* slot_at(const TreeAttnArgs& a, int grid, size_t floats, int slot) {
+  return reinterpret_cast<float*>(reinterpret_cast<Join*>(a.work) + grid) + floats * slot;
+}
+
+// ---- tcgen05 pieces of this kernel ----------------------------------------------------------
+// D(tmem) (+)= A(tmem) * B(smem desc)
+__device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st2(uint32_t taddr, uint32_t x, uint32_t y) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1,%2};" ::"r"(taddr), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void tmem_ld2(uint32_t taddr, float2& v) {
+  uint32_t x, y;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0,%1}, [%2];" : "=r"(x), "=r"(y) : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(x), "+r"(y)::"memory");
+  v = make_float2(__uint_as_float(x), __uint_as_float(y));
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// MN-major B operand (values as they lie: a key to a 128-byte row of 64 columns): 8 keys 1024 bytes apart
+// along k, the next 64 columns an atom away.
+__device__ __forceinline__ uint64_t umma_desc_mn(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((smem_addr >> 4) & 0x3FFFu);
+  d |= (uint64_t)(kAtomBytes >> 4) << 16;
+  d |= (uint64_t)(1024u >> 4) << 32;
+  d |= (uint64_t)1u << 46;
+  d |= (uint64_t)2u << 61;
+  return d;
+}
+constexpr uint32_t kBMajorMn = 1u << 16;  // instruction descriptor: B is MN-major
+
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0)
+               : "memory");
+}
+
+// Bits of the 32 keys from kb on that a node with mask words `bits` sees.
+__device__ __forceinline__ uint32_t seen32(const int32_t* bits, int words, int kb, int cached, int keys) {
+  if (kb >= keys) return 0;
+  const int o = kb - cached;
+  uint32_t m;
+  if (o <= -32) {
+    m = 0xFFFFFFFFu;
+  } else if (o < 0) {
+    const uint32_t w = keys > cached ? (uint32_t)bits[0] : 0u;
+    m = (w << -o) | ((1u << -o) - 1u);
+  } else {
+    const int i = o >> 5;
+    const uint32_t w0 = i < words ? (uint32_t)bits[i] : 0u, w1 = i + 1 < words ? (uint32_t)bits[i + 1] : 0u;
+    m = __funnelshift_r(w0, w1, o & 31);
+  }
+  const int left = keys - kb;
+  return left >= 32 ? m : m & ((1u << left) - 1u);
+}
+
+struct Shared {
+  uint64_t full[10], empty[10];
+  uint64_t s_full[2], p_full[2], q_full, piece_done, state_full, drained;
+  uint32_t tmem_slot;
+  volatile int abort_flag;
+  int r0;
+  int64_t base0;
+  Cut cut;
+  uint32_t bad[kBadSlots][AIOSB_TREE_MAX_NODES / 32];  // per piece: tree keys whose V holds an infinity or a NaN
+};
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const TreeAttnArgs a, int unit_rows) {
+  using S = Shape<D>;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ Shared sh;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t q_smem = smem_u32(smem), ring = q_smem + 2 * S::kBlockBytes;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(&sh.full[i], kLoadWarps);
+      mbar_init(&sh.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], 4);
+    }
+    mbar_init(&sh.q_full, kSoftWarps);
+    mbar_init(&sh.piece_done, 1);
+    mbar_init(&sh.state_full, kSoftWarps);
+    mbar_init(&sh.drained, 1);
+    sh.abort_flag = 0;
+    fence_mbar_init();
+  }
+  for (int i = threadIdx.x; i < kBadSlots * (AIOSB_TREE_MAX_NODES / 32); i += kThreads)
+    (&sh.bad[0][0])[i] = 0;
+  if (warp == kMmaWarp) {
+    tmem_alloc(&sh.tmem_slot, 512);
+    tmem_relinquish();
+  }
+  pdl_wait();
+  if (warp == 0) {  // the weight of all units, and where this CTA's range starts
+    int64_t total = 0;
+    for (int r0 = 0; r0 < a.requests; r0 += 32) {
+      int64_t w = 0;
+      if (r0 + lane < a.requests) {
+        const TreeRequest t = tree_request(a, r0 + lane, blockIdx.x == 0);
+        w = unit_weight(t) * unit_blocks(a, t) * a.hkv;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+      total += w;
+    }
+    Cut cut;
+    cut.total = total;
+    cut.ctas = (int)max((int64_t)1, min((int64_t)gridDim.x, total / kMinShare));
+    const int64_t pos = (int)blockIdx.x < cut.ctas ? cut.begin(blockIdx.x) : total;
+    int64_t base = 0;
+    int found = a.requests;
+    for (int r0 = 0; r0 < a.requests && found == a.requests; r0 += 32) {
+      int64_t w = 0;
+      if (r0 + lane < a.requests) {
+        const TreeRequest t = tree_request(a, r0 + lane, false);
+        w = unit_weight(t) * unit_blocks(a, t) * a.hkv;
+      }
+      int64_t upto = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, base + upto > pos);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        found = r0 + l;
+        base += __shfl_sync(0xffffffffu, upto - w, l);
+      } else {
+        base += __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
+    if (lane == 0) {
+      sh.cut = cut;
+      sh.r0 = found;
+      sh.base0 = base;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_dependents();
+  const uint32_t tmem = sh.tmem_slot;
+  const Cut cut = sh.cut;
+  const int me = blockIdx.x;
+
+  Pieces it;
+  it.pos = it.end = 0;
+  if (me < cut.ctas && cut.total > 0) {
+    it.pos = cut.begin(me);
+    it.end = cut.begin(me + 1);
+    it.base = sh.base0;
+    it.r = sh.r0;
+    if (it.pos < it.end) it.request(a);
+  }
+  Piece p = {};
+
+  if (warp > kMmaWarp) {
+    // ---- gather. Block order of a piece: the order in which the MMAs want them.
+    const int lw = warp - kMmaWarp - 1;
+    const int64_t slot_bytes = (int64_t)a.hkv * D * 2;
+    int stage = 0, issued = 0, told = 0, turn = 0;
+    uint32_t phase = 1;
+    bool ok = true;
+    // makes blocks [told, upto) known to the MMA warp; `upto` blocks of this warp's copies have landed
+    auto tell = [&](int upto) {
+      if (told >= upto) return;
+      fence_proxy_async_shared();
+      for (; told < upto; ++told) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.full[told % S::kStages]);
+      }
+    };
+    auto load = [&](bool values, int chunk) {
+      if (!mbar_try_wait(&sh.empty[stage], phase)) {
+        cp_async_wait_all();
+        tell(issued);
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[stage], phase));
+        if (!ok) return;
+      }
+      __syncwarp();
+      const int k0 = chunk * kKeys + lw * 32;
+      int slot = 0;
+      const bool in = k0 + lane < p.t.keys;
+      if (in) {
+        slot = p.t.slots[k0 + lane];
+        if (slot < 0 || slot >= a.num_slots) {
+          if (!values) report(a.status, AIOSB_DEV_SLOT_RANGE);
+          slot = 0;
+        }
+      }
+      const char* const src =
+          reinterpret_cast<const char*>(values ? a.v_cache : a.k_cache) + (int64_t)p.h * D * 2;
+      const uint32_t dst = ring + stage * S::kBlockBytes + lw * 32 * 128;
+      constexpr int kCols = D / 8;  // 16-byte pieces of a key
+      if (values && (chunk + 1) * kKeys > p.t.cached) {
+        // a key that a node does not see gets weight 0, and 0 * inf is NaN: infinities and NaN of the tree's
+        // keys leave V here, and reach the nodes that see them at the end
+#pragma unroll 1
+        for (int i = lane; i < 32 * kCols; i += 32) {
+          const int row = i / kCols, c = i % kCols, key = k0 + row;
+          const int s = __shfl_sync(0xffffffffu, slot, row);
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (key < p.t.keys) v = *reinterpret_cast<const uint4*>(src + s * slot_bytes + c * 16);
+          if (key >= p.t.cached &&
+              !(finite_bf16x2(v.x) && finite_bf16x2(v.y) && finite_bf16x2(v.z) && finite_bf16x2(v.w))) {
+            v = make_uint4(drop_nonfinite_bf16x2(v.x), drop_nonfinite_bf16x2(v.y), drop_nonfinite_bf16x2(v.z),
+                           drop_nonfinite_bf16x2(v.w));
+            const int j = key - p.t.cached;
+            atomicOr(&sh.bad[turn][j >> 5], 1u << (j & 31));
+          }
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (c >> 3) * kAtomBytes + row * 128 +
+                                                                    (((c & 7) ^ (row & 7)) << 4)),
+                       "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                       : "memory");
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) {
+          const int at = i * 32 + lane, row = at / kCols, c = at % kCols;
+          const int s = __shfl_sync(0xffffffffu, slot, row);
+          cp_async16_or_zero(dst + (c >> 3) * kAtomBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4),
+                             src + s * slot_bytes + c * 16, k0 + row < p.t.keys);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      ++issued;
+      if (++stage == S::kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
+      tell(issued - kLag);
+    };
+    while (ok && it.next(a, p)) {
+      if (p.pair()) {
+        for (int c = p.c0; c < p.c1 && ok; ++c) {
+          load(false, c);
+          if (ok) load(true, c);
+        }
+      } else {
+        load(false, p.c0);
+        if (ok && p.c0 + 1 < p.c1) load(false, p.c0 + 1);
+        for (int c = p.c0; c < p.c1 && ok; ++c) {
+          load(true, c);
+          if (ok && c + 2 < p.c1) load(false, c + 2);
+        }
+      }
+      turn = (turn + 1) % kBadSlots;
+    }
+    cp_async_wait_all();
+    if (ok) {
+      tell(issued);
+    } else {
+      report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
+      sh.abort_flag = 1;
+    }
+  } else if (warp == kMmaWarp) {
+    // ---- MMAs: for each stream in turn O += P V of its last chunk, then S of its next one
+    constexpr uint32_t idesc_s = umma_idesc_bf16(kTile, kKeys), idesc_o = umma_idesc_bf16(kTile, D) | kBMajorMn;
+    uint32_t base = 0, q_phase = 0, p_phase[2] = {0, 0};
+    bool ok = true;
+    auto stage_of = [&](uint32_t block) { return block % S::kStages; };
+    auto wait_block = [&](uint32_t block) {
+      return mbar_wait(&sh.full[stage_of(block)], (block / S::kStages) & 1);
+    };
+    while (ok && it.next(a, p)) {
+      const int n = p.c1 - p.c0;
+      const bool pair = p.pair();
+      // blocks of chunk i's keys and values, as the gathering warps order them
+      auto k_block = [&](int i) { return base + (pair ? 2 * i : i < 2 ? i : 2 * i - 1); };
+      auto v_block = [&](int i) { return base + (pair ? 2 * i + 1 : i == n - 1 ? 2 * n - 1 : 2 * i + 2); };
+      const int step = pair ? 1 : 2;
+      ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full, q_phase));
+      q_phase ^= 1;
+      if (!ok) break;
+      tc_fence_after();
+      // turn i of a stream: P V of its chunk i - 1, S of its chunk i
+      for (int i = 0; ok; ++i) {
+        bool more = false;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const int first = pair ? 0 : s;
+          const int now = first + i * step, before = now - step;
+          if (i > 0 && before < n) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.p_full[s], p_phase[s]) && wait_block(v_block(before)));
+            p_phase[s] ^= 1;
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t st = stage_of(v_block(before));
+            if (elect_one()) {
+              const uint32_t v = ring + st * S::kBlockBytes;
+#pragma unroll
+              for (int k = 0; k < kKeys / 16; ++k)
+                tc_mma_bf16_ts(tmem + 256 + s * 128, tmem + s * 128 + k * 8, umma_desc_mn(v + k * 2048), idesc_o,
+                               i > 1 || k > 0);
+              if (!pair || s == 1) tc_commit(&sh.empty[st]);
+            }
+            __syncwarp();
+            more = true;
+          }
+          if (now < n) {
+            ok = __all_sync(0xffffffffu, wait_block(k_block(now)));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t st = stage_of(k_block(now));
+            if (elect_one()) {
+              const uint64_t kd = umma_desc_sw128(ring + st * S::kBlockBytes);
+              const uint64_t qd = umma_desc_sw128(q_smem + (pair ? s : 0) * S::kBlockBytes);
+#pragma unroll
+              for (int k = 0; k < D / 16; ++k) {
+                const uint32_t off = ((k >> 2) * kAtomBytes + (k & 3) * 32) >> 4;
+                tc_mma_bf16(tmem + s * 128, qd + off, kd + off, idesc_s, k > 0);
+              }
+              tc_commit(&sh.s_full[s]);
+              if (!pair || s == 1) tc_commit(&sh.empty[st]);
+            }
+            __syncwarp();
+            more = true;
+          }
+        }
+        if (!more) break;
+      }
+      if (!ok) break;
+      if (elect_one()) tc_commit(&sh.piece_done);
+      __syncwarp();
+      base += 2 * n;
+    }
+    if (!ok) {
+      report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
+      sh.abort_flag = 1;
+    }
+  } else {
+    // ---- softmax of stream s; a thread owns row `row` of the stream's tile
+    const int s = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t t_s = t_lane + s * 128;
+    uint32_t s_phase = 0, done_phase = 0, state_phase = 0;
+    int turn = 0, partial_of = -1;
+    bool ok = true;
+    Join join = {};
+    while (ok && it.next(a, p)) {
+      const bool pair = p.pair();
+      // Q: this group's tile (the second group's is not used by a narrow unit)
+      if (s == 0 || pair) {
+        const int wt = threadIdx.x & 127;
+        constexpr int kCols = D / 8;
+        for (int i = wt; i < kTile * kCols; i += 128) {
+          const int rr = i / kCols, c = i % kCols, g = p.row0 + s * kTile + rr;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (s * kTile + rr < p.rows)
+            v = *reinterpret_cast<const uint4*>(a.q + (int64_t)(p.t.start + g / a.group) * a.q_stride +
+                                                (int64_t)(p.h * a.group + g % a.group) * D + c * 8);
+          *reinterpret_cast<uint4*>(smem + s * S::kBlockBytes + (c >> 3) * kAtomBytes + rr * 128 +
+                                    (((c & 7) ^ (rr & 7)) << 4)) = v;
+        }
+        fence_proxy_async_shared();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.q_full);
+
+      const int my_row = (pair ? s * kTile : 0) + row;  // of the unit
+      const int rows_here = p.rows - (pair ? s * kTile : 0);
+      const bool warp_works = (warp & 3) * 32 < rows_here;
+      const int pair_row = p.row0 + min(my_row, p.rows - 1);
+      const int node = p.t.start + pair_row / a.group;
+      const int32_t* const bits = a.mask + (int64_t)node * a.words;
+      float ref = -INFINITY, sum = 0.f;
+      bool fresh = true;  // no output of this piece yet
+      for (int c = p.c0 + (pair ? 0 : s); c < p.c1; c += pair ? 1 : 2) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full[s], s_phase));
+        s_phase ^= 1;
+        if (!ok) break;
+        tc_fence_after();
+        if (warp_works) {
+          const bool masked = (c + 1) * kKeys > p.t.cached;
+          uint32_t v[32];
+          float top = -INFINITY;
+#pragma unroll 1
+          for (int j = 0; j < 4; ++j) {
+            tmem_ld(t_s + j * 32, v);
+            uint32_t seen = 0xFFFFFFFFu;
+            if (masked) seen = seen32(bits, a.words, c * kKeys + j * 32, p.t.cached, p.t.keys);
+            tmem_wait(v);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!masked || ((seen >> e) & 1)) top = fmaxf(top, __uint_as_float(v[e]) * a.scale_log2);
+          }
+          const bool grows = top > ref + kRescaleAt || (ref == -INFINITY && top > -INFINITY);
+          if (__any_sync(0xffffffffu, grows)) {
+            const float next = grows ? top : ref;
+            const float corr = grows ? exp2_fast(ref - top) : 1.f;
+            if (!fresh) {
+#pragma unroll 1
+              for (int j = 0; j < D / 32; ++j) {
+                tmem_ld(t_lane + 256 + s * 128 + j * 32, v);
+                tmem_wait(v);
+                uint32_t lo[16], hi[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                  lo[e] = __float_as_uint(__uint_as_float(v[e]) * corr);
+                  hi[e] = __float_as_uint(__uint_as_float(v[e + 16]) * corr);
+                }
+                tmem_st16(t_lane + 256 + s * 128 + j * 32, lo);
+                tmem_st16(t_lane + 256 + s * 128 + j * 32 + 16, hi);
+              }
+            }
+            sum *= corr;
+            ref = next;
+          }
+          const float minus = ref == -INFINITY ? 0.f : -ref;
+#pragma unroll 1
+          for (int j = 0; j < 4; ++j) {
+            tmem_ld(t_s + j * 32, v);
+            uint32_t seen = 0xFFFFFFFFu;
+            if (masked) seen = seen32(bits, a.words, c * kKeys + j * 32, p.t.cached, p.t.keys);
+            tmem_wait(v);
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              float x = exp2_fast(fmaf(__uint_as_float(v[e]), a.scale_log2, minus));
+              float y = exp2_fast(fmaf(__uint_as_float(v[e + 1]), a.scale_log2, minus));
+              if (masked) {
+                if (!((seen >> e) & 1)) x = 0.f;
+                if (!((seen >> (e + 1)) & 1)) y = 0.f;
+              }
+              sum += x + y;
+              w[e / 2] = pack_bf16x2(x, y);  // off by 2^-8 of each at most, as the result is by its own
+            }
+            tmem_st16(t_s + j * 16, w);  // over columns that have been read
+          }
+          tmem_wait_st();
+        }
+        fresh = false;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.p_full[s]);
+      }
+      if (!ok) break;
+      ok = __all_sync(0xffffffffu, mbar_wait(&sh.piece_done, done_phase));
+      done_phase ^= 1;
+      if (!ok) break;
+      tc_fence_after();
+
+      // ---- a narrow unit's streams are joined here: each group writes half of the columns
+      float weight[2] = {1.f, 0.f};
+      float m_all = ref, l_all = sum;
+      bool use[2] = {s == 0 || !pair, !pair && p.c1 - p.c0 > 1};
+      if (!pair) {
+        // through TMEM, where S was: the two warps with this row reach the same lane
+        tmem_st2(t_s, __float_as_uint(ref), __float_as_uint(sum));
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.state_full);
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.state_full, state_phase));
+        state_phase ^= 1;
+        if (!ok) break;
+        tc_fence_after();
+        float2 x, y;
+        tmem_ld2(t_lane, x);
+        tmem_ld2(t_lane + 128, y);
+        m_all = fmaxf(x.x, use[1] ? y.x : -INFINITY);
+        const float m = m_all == -INFINITY ? 0.f : m_all;
+        weight[0] = exp2_fast(x.x - m);
+        weight[1] = use[1] ? exp2_fast(y.x - m) : 0.f;
+        l_all = x.y * weight[0] + (use[1] ? y.y * weight[1] : 0.f);
+      }
+      const bool whole = p.whole();
+      const bool none = m_all == -INFINITY && l_all == 0.f;  // the row sees none of these keys
+      const float inv = !whole ? 1.f : none ? 0.f : 1.f / l_all;
+      const int slot = p.c0 == 0 ? 2 * me + 1 : 2 * me;
+      float* const part = whole ? nullptr : slot_at(a, gridDim.x, slot_floats<D>(unit_rows), slot);
+      const bool row_works = my_row < p.rows;
+      if (!whole && row_works && (pair || s == 0))
+        reinterpret_cast<float2*>(part)[my_row] = make_float2(m_all, l_all);
+      if (!whole && p.c0 == 0) {
+        partial_of = 1;
+        join.start = p.t.start;
+        join.row0 = p.row0;
+        join.rows = p.rows;
+        join.h = p.h;
+        join.last = cut.owner(p.first_at + p.chunks - 1);
+      }
+      uint32_t any_bad = 0;
+      if (p.c1 * kKeys > p.t.cached)
+        for (int w = 0; w < a.words; ++w) any_bad |= sh.bad[turn][w];
+      if (warp_works) {
+        const int g = p.row0 + my_row;
+        __nv_bfloat16* const dst = a.out + (int64_t)(p.t.start + g / a.group) * a.out_stride +
+                                   (int64_t)(p.h * a.group + g % a.group) * D;
+        const int j0 = pair ? 0 : s * (D / 32), j1 = pair ? D / 16 : (s + 1) * (D / 32);  // of 16 columns each
+#pragma unroll 1
+        for (int j = j0; j < j1; ++j) {
+          uint32_t v[16];
+          float o[16];
+          tmem_ld(t_lane + 256 + (pair ? s * 128 : 0) + j * 16, v);
+          tmem_wait(v);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = __uint_as_float(v[e]) * weight[0];
+          if (use[1]) {
+            tmem_ld(t_lane + 384 + j * 16, v);
+            tmem_wait(v);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = fmaf(__uint_as_float(v[e]), weight[1], o[e]);
+          }
+          if (!row_works) continue;
+          if (any_bad) {
+#pragma unroll 1
+            for (int w = 0; w < a.words; ++w) {
+              for (uint32_t hit = sh.bad[turn][w] & (uint32_t)bits[w]; hit; hit &= hit - 1) {
+                const int key = p.t.cached + w * 32 + __ffs(hit) - 1;
+                const __nv_bfloat16* x =
+                    a.v_cache + (tree_slot(a, p.t.slots[key]) * a.hkv + p.h) * D + j * 16;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                  const float y = bf16_to_f(x[e]);
+                  if (!(fabsf(y) < INFINITY)) o[e] += y;
+                }
+              }
+            }
+          }
+          if (whole) {
+            uint4 u[2];
+            uint32_t* const w = reinterpret_cast<uint32_t*>(u);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = pack_bf16x2(o[2 * e] * inv, o[2 * e + 1] * inv);
+            reinterpret_cast<uint4*>(dst + j * 16)[0] = u[0];
+            reinterpret_cast<uint4*>(dst + j * 16)[1] = u[1];
+          } else {  // a column of float4 for each row, so that neighbouring rows lie side by side
+            float4* const f = reinterpret_cast<float4*>(part + 2 * unit_rows) + my_row;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              f[(size_t)(j * 4 + e) * unit_rows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+        }
+      }
+      // every warp has started on this piece, so all are through with the one before it
+      if (warp == 0) sh.bad[(turn + kBadSlots - 1) % kBadSlots][lane] = 0;
+      turn = (turn + 1) % kBadSlots;
+      tc_fence_before();
+    }
+    if (!ok) {
+      report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
+      sh.abort_flag = 1;
+    }
+    if (threadIdx.x == 0) {
+      if (partial_of < 0) join.rows = 0;
+      reinterpret_cast<Join*>(a.work)[me] = join;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    if (sh.abort_flag) {  // MMAs may still run: their end is waited for, with a limit
+      if (elect_one()) tc_commit(&sh.drained);
+      __syncwarp();
+      mbar_wait(&sh.drained, 0);
+    }
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the pieces of the unit that starts in range blockIdx.x and goes on behind it: a thread takes every
+// eighth float4 of a row.
+template <int D>
+__global__ void __launch_bounds__(256) attn_tree_join_kernel(const TreeAttnArgs a, int grid, int unit_rows) {
+  pdl_enter();
+  const Join j = reinterpret_cast<const Join*>(a.work)[blockIdx.x];
+  const int row = blockIdx.y * 32 + (threadIdx.x & 31), c0 = threadIdx.x >> 5;
+  if (row >= j.rows) return;
+  const size_t floats = slot_floats<D>(unit_rows);
+  const int first = blockIdx.x;
+  auto slot = [&](int c) { return slot_at(a, grid, floats, c == first ? 2 * c + 1 : 2 * c); };
+  float m = -INFINITY;
+  for (int c = first; c <= j.last; ++c) m = fmaxf(m, reinterpret_cast<const float2*>(slot(c))[row].x);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float4 o[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c = first; c <= j.last; ++c) {
+    const float* const p = slot(c);
+    const float2 s = reinterpret_cast<const float2*>(p)[row];
+    const float w = exp2_fast(s.x - ref);
+    l = fmaf(s.y, w, l);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      const float4 v = reinterpret_cast<const float4*>(p + 2 * unit_rows)[(size_t)(c0 + 8 * i) * unit_rows + row];
+      o[i].x = fmaf(v.x, w, o[i].x);
+      o[i].y = fmaf(v.y, w, o[i].y);
+      o[i].z = fmaf(v.z, w, o[i].z);
+      o[i].w = fmaf(v.w, w, o[i].w);
+    }
+  }
+  const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
+  const int g = j.row0 + row;
+  __nv_bfloat16* const dst = a.out + (int64_t)(j.start + g / a.group) * a.out_stride +
+                             (int64_t)(j.h * a.group + g % a.group) * D;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+    reinterpret_cast<uint2*>(dst)[c0 + 8 * i] =
+        make_uint2(pack_bf16x2(o[i].x * inv, o[i].y * inv), pack_bf16x2(o[i].z * inv, o[i].w * inv));
+}
+
+template <int D>
+cudaError_t launch(const TreeAttnArgs& a, int grid, int unit_rows, cudaStream_t stream) {
+  const auto kernel = attn_tree_split_kernel<D>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
+  if (e != cudaSuccess) return e;
+  e = launch_pdl(kernel, dim3((unsigned)grid), dim3(kThreads), Shape<D>::kSmem, stream, a, unit_rows);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(attn_tree_join_kernel<D>, dim3((unsigned)grid, (unsigned)((unit_rows + 31) / 32)), dim3(256), 0,
+                    stream, a, grid, unit_rows);
+}
+
+}  // namespace
+
+int tree_split_grid() { return std::min(sm_count(), kMaxGrid); }
+
+int tree_split_unit_rows(int64_t max_rows) {
+  return (int)std::min<int64_t>(kUnitRows, (max_rows + 31) / 32 * 32);
+}
+
+int64_t tree_split_work_bytes(int grid, int unit_rows, int d) {
+  return (int64_t)grid * (sizeof(Join) + 2 * sizeof(float) * (int64_t)unit_rows * (d + 2));
+}
+
+cudaError_t launch_tree_split(const TreeAttnArgs& a, int d, int grid, int unit_rows, cudaStream_t stream) {
+  if (d == 64) return launch<64>(a, grid, unit_rows, stream);
+  if (d == 96) return launch<96>(a, grid, unit_rows, stream);
+  return launch<128>(a, grid, unit_rows, stream);
+}
+
+}  // namespace aiosb

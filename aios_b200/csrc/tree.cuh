@@ -44,14 +44,15 @@ __device__ __forceinline__ TreeRequest tree_request(const TreeAttnArgs& a, int r
   TreeRequest t;
   const int s = a.tree_start[r], e = a.tree_start[r + 1], c = a.cached_lens[r], row = a.row_table[r];
   t.start = min(max(s, 0), a.tokens);
-  t.nodes = min(max(e, t.start), a.tokens) - t.start;
+  const int nodes = min(max(e, t.start), a.tokens) - t.start;
+  t.nodes = min(nodes, 32 * a.words);
   const bool row_ok = row >= 0 && row < a.table_rows;
   t.cached = row_ok ? min(max(c, 0), a.table_width) : 0;
-  t.keys = row_ok ? t.cached + min(min(t.nodes, 32 * a.words), a.table_width - t.cached) : 0;
+  t.keys = row_ok ? t.cached + min(t.nodes, a.table_width - t.cached) : 0;
   t.slots = a.page_table + (row_ok ? row : 0) * a.table_stride;
-  if (tell && (t.start != s || t.start + t.nodes != e || t.cached != c || t.keys - t.cached != t.nodes) && t.nodes > 0)
+  if (tell && (s < 0 || e < s || e > a.tokens || t.nodes != nodes ||
+               (nodes > 0 && (t.cached != c || t.keys - t.cached != t.nodes))))
     report(a.status, AIOSB_DEV_TREE_RANGE);
-  if (tell && (s < 0 || e < s || e > a.tokens)) report(a.status, AIOSB_DEV_TREE_RANGE);
   return t;
 }
 
@@ -76,5 +77,11 @@ __device__ __forceinline__ uint32_t drop_nonfinite_bf16x2(uint32_t v) {
   if ((v & 0x7F80u) == 0x7F80u) v &= 0xFFFF0000u;
   return v;
 }
+
+// attn_tree_split.cu: the keys of all requests dealt over `grid` CTAs.
+int tree_split_grid();
+int tree_split_unit_rows(int64_t max_rows);
+int64_t tree_split_work_bytes(int grid, int unit_rows, int d);
+cudaError_t launch_tree_split(const TreeAttnArgs& a, int d, int grid, int unit_rows, cudaStream_t stream);
 
 }  // namespace aiosb

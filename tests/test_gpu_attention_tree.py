@@ -49,6 +49,11 @@ class Case:
         args.update(kw)
         return ops.attention_tree(**args)
 
+    def check_every_way(self):
+        """Whole requests to a CTA, and keys dealt over the SMs (the bound on the histories chooses)."""
+        for bound in (1, 1 << 20):
+            self.check(self.run(max_cached=bound))
+
     def check(self, got):
         n = sum(self.sizes)
         want, mag, top = ref.attention(self.q[:n], self.k, self.v, self.table, self.row_list, self.cached_list, self.sizes,
@@ -65,14 +70,14 @@ class Case:
 @pytest.mark.parametrize("page", [1, 16])
 def test_heads(cuda_device, d, heads, page) -> None:
     c = Case([5, 1, 13], [37, 0, 130], *heads, d, page=page, seed=d)
-    c.check(c.run())
+    c.check_every_way()
 
 
 @pytest.mark.parametrize("nodes", [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 128, 200])
 @pytest.mark.parametrize("cached", [0, 1, 63, 64, 65, 127, 128, 300])
 def test_sizes(cuda_device, nodes, cached) -> None:
     c = Case([nodes], [cached], 6, 2, 64, seed=nodes)
-    c.check(c.run())
+    c.check_every_way()
 
 
 @pytest.mark.parametrize("d", [64, 96, 128])
@@ -81,7 +86,7 @@ def test_ragged_batches(cuda_device, d, kind) -> None:
     sizes = [3, 0, 64, 1, 40, 7, 0, 17, 100]
     cached = [500, 20, 0, 1, 1000, 3, 0, 129, 64]
     c = Case(sizes, cached, 8, 2, d, kind=kind, page=16, seed=7)
-    c.check(c.run())
+    c.check_every_way()
 
 
 @pytest.mark.parametrize("d,heads,requests,nodes,cached", [
@@ -98,7 +103,7 @@ def test_long_histories(cuda_device, d, heads, requests, nodes, cached) -> None:
 
 def test_the_largest_tree(cuda_device) -> None:
     c = Case([1024, 1000], [70, 2000], 4, 2, 64, seed=2)
-    c.check(c.run())
+    c.check_every_way()
 
 
 def test_any_bits(cuda_device) -> None:
@@ -112,10 +117,11 @@ def test_any_bits(cuda_device) -> None:
     bits[62] = 0
     bits[10, 0], bits[10, 1] = 0, 1 << 30  # past the tree's 40 nodes: nothing
     c.mask[:n] = bits.to(torch.int32).cuda()
-    out = torch.full_like(c.q, 7.0)
-    c.run(out=out)
-    c.check(out)
-    assert (out[5] == 0).all() and (out[62] == 0).all() and (out[10] == 0).all() and (out[40] != 0).any()
+    for bound in (1, 1 << 20):
+        out = torch.full_like(c.q, 7.0)
+        c.run(out=out, max_cached=bound)
+        c.check(out)
+        assert (out[5] == 0).all() and (out[62] == 0).all() and (out[10] == 0).all() and (out[40] != 0).any()
 
 
 def test_rows_behind_the_last_tree_and_strides(cuda_device) -> None:
@@ -133,17 +139,18 @@ def test_rows_behind_the_last_tree_and_strides(cuda_device) -> None:
 @pytest.mark.parametrize("d", [64, 96, 128])
 @pytest.mark.parametrize("cached", [0, 30, 700])
 @pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
-def test_what_a_node_does_not_see_does_not_reach_it(cuda_device, d, cached, value) -> None:
+@pytest.mark.parametrize("bound", [1, 1 << 20])
+def test_what_a_node_does_not_see_does_not_reach_it(cuda_device, d, cached, value, bound) -> None:
     sizes = [20, 50]
     c = Case(sizes, [cached, cached], 4, 2, d, kind="star", seed=11)
-    clean = c.run()
+    clean = c.run(max_cached=bound)
     # node 7 of the first tree, nodes 3 and 45 of the second: only they see themselves
     hit = [(0, 7), (1, 3), (1, 45)]
     for r, j in hit:
         slot = int(c.table[c.row_list[r], cached + j])
         c.v[slot, :, 5] = value
         c.k[slot, 0, 2] = value
-    got = c.run()
+    got = c.run(max_cached=bound)
     touched = [r * 20 + j for r, j in hit]
     rest = [i for i in range(70) if i not in touched]
     assert torch.equal(got[rest], clean[rest])
@@ -163,16 +170,28 @@ def test_unused_pool_slots_and_table_entries_do_not_matter(cuda_device) -> None:
     used = torch.zeros(c.k.shape[0], dtype=torch.bool, device="cuda")
     for row, n, length in zip(c.row_list, c.sizes, c.cached_list):
         used[c.table[row, : length + n].long()] = True
+    dealt = c.run(max_cached=1 << 20)
     c.k[~used] = float("nan")
     c.v[~used] = float("nan")
-    assert torch.equal(c.run(), clean)
+    assert torch.equal(c.run(), clean) and torch.equal(c.run(max_cached=1 << 20), dealt)
 
 
 def test_a_large_score_and_equal_scores(cuda_device) -> None:
     c = Case([3], [200], 2, 1, 64, seed=9, spread=30.0)
-    c.check(c.run())
+    c.check_every_way()
     c.q.zero_()  # every key alike: a plain mean
-    c.check(c.run())
+    c.check_every_way()
+
+
+def test_a_history_that_grows_in_score(cuda_device) -> None:
+    """Every chunk of keys has larger scores than the one before: the rows' references move each time."""
+    c = Case([9], [1500], 4, 2, 128, seed=2)
+    order = c.table[c.row_list[0], :1500].long()
+    c.q.copy_(c.q.abs() + 1)
+    c.k[order] = (torch.arange(1500, device="cuda")[:, None, None] / 60).expand(1500, 2, 128).to(torch.bfloat16)
+    c.check_every_way()
+    c.k[order] = c.k[order.flip(0)]
+    c.check_every_way()
 
 
 def test_one_history_of_several_requests(cuda_device) -> None:
@@ -183,8 +202,9 @@ def test_one_history_of_several_requests(cuda_device) -> None:
     c.check(c.run())
 
 
+@pytest.mark.parametrize("bound", [1, 1 << 20])
 @pytest.mark.parametrize("what", ["slot", "row", "cached", "start", "width", "words"])
-def test_numbers_outside_their_arrays_are_reported(cuda_device, what) -> None:
+def test_numbers_outside_their_arrays_are_reported(cuda_device, what, bound) -> None:
     c = Case([4, 40], [100, 30], 4, 2, 64, seed=12)
     if what == "slot":
         c.table[c.row_list[0], 50] = c.k.shape[0]
@@ -198,7 +218,7 @@ def test_numbers_outside_their_arrays_are_reported(cuda_device, what) -> None:
         c.cached[1] = 1 << 30
     else:
         c.mask = c.mask[:, :1].contiguous()
-    out = c.run()
+    out = c.run(max_cached=bound)
     torch.cuda.synchronize()
     assert out.shape == c.q.shape
     with pytest.raises(RuntimeError, match="slot" if what == "slot" else "tree"):
