@@ -270,7 +270,7 @@ extern "C" int aiosb_attention_tree(const void* q, int64_t q_stride, int64_t tok
   AIOSB_REQUIRE(head_dim == 64 || head_dim == 96 || head_dim == 128, AIOSB_ERR_UNSUPPORTED,
                 "attention_tree: head_dim %lld unsupported (64, 96, 128)", (long long)head_dim);
   AIOSB_REQUIRE(tokens >= 0 && requests >= 0 && num_slots >= 0 && table_rows >= 0 && table_width >= 0 &&
-                    max_cached >= 0 && work_bytes >= 0 && scale == scale,
+                    max_cached >= 0 && work_bytes >= 0 && scale > 0 && scale < INFINITY,
                 AIOSB_ERR_INVALID_ARG, "attention_tree: bad sizes");
   AIOSB_REQUIRE(mask_words >= 1 && mask_words <= AIOSB_TREE_MAX_NODES / 32, AIOSB_ERR_UNSUPPORTED,
                 "attention_tree: %lld mask words; a tree has at most %d nodes", (long long)mask_words,

@@ -28,9 +28,13 @@ constexpr int kTile = 128;      // rows of a tile: UMMA M, TMEM lanes
 constexpr int kUnitRows = 256;  // two tiles
 constexpr int kKeys = 128;      // keys of a chunk
 constexpr int kSoftWarps = 8;
-constexpr int kMmaWarp = kSoftWarps;
 constexpr int kLoadWarps = 4;
-constexpr int kThreads = (kSoftWarps + 1 + kLoadWarps) * 32;
+constexpr int kMmaWarp = kSoftWarps + kLoadWarps;
+constexpr int kThreads = (kMmaWarp + 4) * 32;  // whole groups of four warps; three idle
+// Registers of a thread: a softmax thread holds a row's 128 scores. 2 x 176 + 96 + 64 = 4 x 128, what the
+// block is launched with.
+constexpr int kSoftRegs = 176, kLoadRegs = 96, kMmaRegs = 64;
+static_assert(2 * kSoftRegs + kLoadRegs + kMmaRegs <= 65536 / kThreads * 4, "more registers than the block has");
 constexpr int kAtomBytes = kKeys * 128;  // 128 rows of 64 values, 128-byte swizzled
 constexpr int kUnitCost = 1;             // a unit's start and end, in chunks
 constexpr int kMinShare = 3;             // weight below which a range is not worth a CTA
@@ -155,6 +159,11 @@ __device__ __forceinline__ void tmem_ld2(uint32_t taddr, float2& v) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(x), "+r"(y)::"memory");
   v = make_float2(__uint_as_float(x), __uint_as_float(y));
 }
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // MN-major B operand (values as they lie: a key to a 128-byte row of 64 columns): 8 keys 1024 bytes apart
@@ -192,6 +201,68 @@ __device__ __forceinline__ uint32_t seen32(const int32_t* bits, int words, int k
   }
   const int left = keys - kb;
   return left >= 32 ? m : m & ((1u << left) - 1u);
+}
+
+// One chunk of a row: S (128 columns at t_s) to weights in bf16 over it; the row's reference and sum, and
+// its output at t_o where the reference moves. `seen`: bits of the keys, if some are hidden.
+template <int D, bool MASKED>
+__device__ __forceinline__ void soft_chunk(uint32_t t_s, uint32_t t_o, const uint32_t (&seen)[4], float scale,
+                                           bool fresh, float& ref, float& sum) {
+  uint32_t v[4][32];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) tmem_ld(t_s + j * 32, v[j]);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) tmem_wait(v[j]);
+  if (MASKED) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if (!((seen[j] >> e) & 1)) v[j][e] = 0xFF800000u;  // -inf
+  }
+  float top[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    top[j] = __uint_as_float(v[j][0]);
+#pragma unroll
+    for (int e = 1; e < 31; e += 2) top[j] = max3(top[j], __uint_as_float(v[j][e]), __uint_as_float(v[j][e + 1]));
+    top[j] = fmaxf(top[j], __uint_as_float(v[j][31]));
+  }
+  const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+  const bool grows = most > ref + kRescaleAt;
+  if (__any_sync(0xffffffffu, grows)) {
+    const float corr = grows ? exp2_fast(ref - most) : 1.f;
+    if (!fresh) {
+#pragma unroll 1
+      for (int j = 0; j < D / 16; ++j) {
+        uint32_t o[16];
+        tmem_ld(t_o + j * 16, o);
+        tmem_wait(o);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+        tmem_st16(t_o + j * 16, o);
+      }
+    }
+    sum *= corr;
+    if (grows) ref = most;
+  }
+  const float minus = ref == -INFINITY ? 0.f : -ref;  // nothing seen yet: any finite reference will do
+  const float2 m2 = make_float2(minus, minus), s2 = make_float2(scale, scale);
+  float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t w[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      float2 x = __ffma2_rn(make_float2(__uint_as_float(v[j][2 * e]), __uint_as_float(v[j][2 * e + 1])), s2, m2);
+      x = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+      part[e & 1] = __fadd2_rn(part[e & 1], x);
+      w[e] = pack_bf16x2(x.x, x.y);  // off by 2^-8 of each at most, as the result is by its own
+    }
+    tmem_st16(t_s + j * 16, w);  // over columns that have been read
+  }
+  sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
+  tmem_wait_st();
 }
 
 struct Shared {
@@ -301,14 +372,44 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
   }
   Piece p = {};
 
-  if (warp > kMmaWarp) {
-    // ---- gather. Block order of a piece: the order in which the MMAs want them.
-    const int lw = warp - kMmaWarp - 1;
+  if (warp >= kSoftWarps && warp < kMmaWarp) {
+    // ---- gather
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
+    const int lw = warp - kSoftWarps;
     const int64_t slot_bytes = (int64_t)a.hkv * D * 2;
-    int stage = 0, issued = 0, told = 0, turn = 0;
+    int stage = 0, issued = 0, told = 0;
     uint32_t phase = 1;
     bool ok = true;
-    // makes blocks [told, upto) known to the MMA warp; `upto` blocks of this warp's copies have landed
+    // The blocks of this CTA's pieces, in the order in which the MMAs want them.
+    struct Block {
+      Piece p;
+      int i, n;  // block of the piece, chunks of the piece
+      int turn;
+      bool values;
+      int chunk;
+    } now = {}, next;
+    now.turn = -1;
+    auto advance = [&](Block& b) {
+      if (++b.i >= 2 * b.n) {
+        if (!it.next(a, b.p)) return false;
+        b.i = 0;
+        b.n = b.p.c1 - b.p.c0;
+        b.turn = (b.turn + 1) % kBadSlots;
+      }
+      if (b.p.pair() || b.n == 1) {  // K0 V0 K1 V1 ..
+        b.values = b.i & 1;
+        b.chunk = b.p.c0 + b.i / 2;
+      } else {  // K0 K1 V0 K2 V1 .. V(n-2) V(n-1)
+        b.values = b.i == 2 * b.n - 1 || (b.i >= 2 && !(b.i & 1));
+        b.chunk = b.p.c0 + (b.i < 2 ? b.i : b.i == 2 * b.n - 1 ? b.n - 1 : (b.i & 1) ? (b.i + 1) / 2 : b.i / 2 - 1);
+      }
+      return true;
+    };
+    auto slot_of = [&](const Block& b) {  // of this lane's key
+      const int key = b.chunk * kKeys + lw * 32 + lane;
+      return key < b.p.t.keys ? b.p.t.slots[key] : 0;
+    };
+    // makes blocks [told, upto) known to the MMA warp: this warp's copies of them have landed
     auto tell = [&](int upto) {
       if (told >= upto) return;
       fence_proxy_async_shared();
@@ -317,29 +418,30 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
         if (lane == 0) mbar_arrive(&sh.full[told % S::kStages]);
       }
     };
-    auto load = [&](bool values, int chunk) {
+    bool more = advance(now);
+    int slot = more ? slot_of(now) : 0;
+    while (more) {
+      next = now;
+      const bool more_next = advance(next);
+      const int slot_next = more_next ? slot_of(next) : 0;  // asked for a block ahead
       if (!mbar_try_wait(&sh.empty[stage], phase)) {
         cp_async_wait_all();
         tell(issued);
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[stage], phase));
-        if (!ok) return;
+        if (!ok) break;
       }
       __syncwarp();
-      const int k0 = chunk * kKeys + lw * 32;
-      int slot = 0;
-      const bool in = k0 + lane < p.t.keys;
-      if (in) {
-        slot = p.t.slots[k0 + lane];
-        if (slot < 0 || slot >= a.num_slots) {
-          if (!values) report(a.status, AIOSB_DEV_SLOT_RANGE);
-          slot = 0;
-        }
+      const Piece& p = now.p;
+      const int k0 = now.chunk * kKeys + lw * 32;
+      if (slot < 0 || slot >= a.num_slots) {
+        if (!now.values) report(a.status, AIOSB_DEV_SLOT_RANGE);
+        slot = 0;
       }
       const char* const src =
-          reinterpret_cast<const char*>(values ? a.v_cache : a.k_cache) + (int64_t)p.h * D * 2;
+          reinterpret_cast<const char*>(now.values ? a.v_cache : a.k_cache) + (int64_t)p.h * D * 2;
       const uint32_t dst = ring + stage * S::kBlockBytes + lw * 32 * 128;
       constexpr int kCols = D / 8;  // 16-byte pieces of a key
-      if (values && (chunk + 1) * kKeys > p.t.cached) {
+      if (now.values && (now.chunk + 1) * kKeys > p.t.cached) {
         // a key that a node does not see gets weight 0, and 0 * inf is NaN: infinities and NaN of the tree's
         // keys leave V here, and reach the nodes that see them at the end
 #pragma unroll 1
@@ -353,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
             v = make_uint4(drop_nonfinite_bf16x2(v.x), drop_nonfinite_bf16x2(v.y), drop_nonfinite_bf16x2(v.z),
                            drop_nonfinite_bf16x2(v.w));
             const int j = key - p.t.cached;
-            atomicOr(&sh.bad[turn][j >> 5], 1u << (j & 31));
+            atomicOr(&sh.bad[now.turn][j >> 5], 1u << (j & 31));
           }
           asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (c >> 3) * kAtomBytes + row * 128 +
                                                                     (((c & 7) ^ (row & 7)) << 4)),
@@ -377,22 +479,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       }
       asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
       tell(issued - kLag);
-    };
-    while (ok && it.next(a, p)) {
-      if (p.pair()) {
-        for (int c = p.c0; c < p.c1 && ok; ++c) {
-          load(false, c);
-          if (ok) load(true, c);
-        }
-      } else {
-        load(false, p.c0);
-        if (ok && p.c0 + 1 < p.c1) load(false, p.c0 + 1);
-        for (int c = p.c0; c < p.c1 && ok; ++c) {
-          load(true, c);
-          if (ok && c + 2 < p.c1) load(false, c + 2);
-        }
-      }
-      turn = (turn + 1) % kBadSlots;
+      now = next;
+      more = more_next;
+      slot = slot_next;
     }
     cp_async_wait_all();
     if (ok) {
@@ -401,7 +490,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
       sh.abort_flag = 1;
     }
-  } else if (warp == kMmaWarp) {
+  } else if (warp >= kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
+    if (warp == kMmaWarp) {
     // ---- MMAs: for each stream in turn O += P V of its last chunk, then S of its next one
     constexpr uint32_t idesc_s = umma_idesc_bf16(kTile, kKeys), idesc_o = umma_idesc_bf16(kTile, D) | kBMajorMn;
     uint32_t base = 0, q_phase = 0, p_phase[2] = {0, 0};
@@ -476,11 +567,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
       sh.abort_flag = 1;
     }
+    }
   } else {
     // ---- softmax of stream s; a thread owns row `row` of the stream's tile
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
     const int s = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t t_s = t_lane + s * 128;
+    const uint32_t t_s = t_lane + s * 128, t_o = t_lane + 256 + s * 128;
     uint32_t s_phase = 0, done_phase = 0, state_phase = 0;
     int turn = 0, partial_of = -1;
     bool ok = true;
@@ -519,63 +612,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
         if (!ok) break;
         tc_fence_after();
         if (warp_works) {
-          const bool masked = (c + 1) * kKeys > p.t.cached;
-          uint32_t v[32];
-          float top = -INFINITY;
-#pragma unroll 1
-          for (int j = 0; j < 4; ++j) {
-            tmem_ld(t_s + j * 32, v);
-            uint32_t seen = 0xFFFFFFFFu;
-            if (masked) seen = seen32(bits, a.words, c * kKeys + j * 32, p.t.cached, p.t.keys);
-            tmem_wait(v);
+          if ((c + 1) * kKeys > p.t.cached) {
+            uint32_t seen[4];
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!masked || ((seen >> e) & 1)) top = fmaxf(top, __uint_as_float(v[e]) * a.scale_log2);
+            for (int j = 0; j < 4; ++j) seen[j] = seen32(bits, a.words, c * kKeys + j * 32, p.t.cached, p.t.keys);
+            soft_chunk<D, true>(t_s, t_o, seen, a.scale_log2, fresh, ref, sum);
+          } else {
+            const uint32_t all[4] = {};
+            soft_chunk<D, false>(t_s, t_o, all, a.scale_log2, fresh, ref, sum);
           }
-          const bool grows = top > ref + kRescaleAt || (ref == -INFINITY && top > -INFINITY);
-          if (__any_sync(0xffffffffu, grows)) {
-            const float next = grows ? top : ref;
-            const float corr = grows ? exp2_fast(ref - top) : 1.f;
-            if (!fresh) {
-#pragma unroll 1
-              for (int j = 0; j < D / 32; ++j) {
-                tmem_ld(t_lane + 256 + s * 128 + j * 32, v);
-                tmem_wait(v);
-                uint32_t lo[16], hi[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                  lo[e] = __float_as_uint(__uint_as_float(v[e]) * corr);
-                  hi[e] = __float_as_uint(__uint_as_float(v[e + 16]) * corr);
-                }
-                tmem_st16(t_lane + 256 + s * 128 + j * 32, lo);
-                tmem_st16(t_lane + 256 + s * 128 + j * 32 + 16, hi);
-              }
-            }
-            sum *= corr;
-            ref = next;
-          }
-          const float minus = ref == -INFINITY ? 0.f : -ref;
-#pragma unroll 1
-          for (int j = 0; j < 4; ++j) {
-            tmem_ld(t_s + j * 32, v);
-            uint32_t seen = 0xFFFFFFFFu;
-            if (masked) seen = seen32(bits, a.words, c * kKeys + j * 32, p.t.cached, p.t.keys);
-            tmem_wait(v);
-            uint32_t w[16];
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              float x = exp2_fast(fmaf(__uint_as_float(v[e]), a.scale_log2, minus));
-              float y = exp2_fast(fmaf(__uint_as_float(v[e + 1]), a.scale_log2, minus));
-              if (masked) {
-                if (!((seen >> e) & 1)) x = 0.f;
-                if (!((seen >> (e + 1)) & 1)) y = 0.f;
-              }
-              sum += x + y;
-              w[e / 2] = pack_bf16x2(x, y);  // off by 2^-8 of each at most, as the result is by its own
-            }
-            tmem_st16(t_s + j * 16, w);  // over columns that have been read
-          }
-          tmem_wait_st();
         }
         fresh = false;
         tc_fence_before();

@@ -476,7 +476,7 @@ AIOSB_API int aiosb_draft_tree(const int32_t* parents, int64_t tokens, const int
  * page_table[row_table[r], 0 .. cached_lens[r]) and page_table[row_table[r],
  * cached_lens[r] + j] for each set bit j of its mask, any set of them; a node that sees
  * nothing gets 0, and what a node does not see does not reach it, infinities and NaN
- * included. head_dim 64, 96 or 128; at most AIOSB_TREE_MAX_GROUP query heads to a KV
+ * included. scale > 0; head_dim 64, 96 or 128; at most AIOSB_TREE_MAX_GROUP query heads to a KV
  * head; mask_words up to AIOSB_TREE_MAX_NODES / 32. max_cached: a bound on cached_lens
  * from which the split over the GPU is chosen (0: the page table's width); longer
  * histories are read all the same.

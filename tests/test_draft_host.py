@@ -47,7 +47,8 @@ def test_attention_tree_refuses() -> None:
     call(UNS, "head_dim", d=80)
     call(INV, "bad sizes", tokens=-1)
     call(INV, "bad sizes", max_cached=-1)
-    call(INV, "bad sizes", scale=float("nan"))
+    for scale in (0.0, -0.125, float("inf"), float("nan")):
+        call(INV, "bad sizes", scale=scale)
     call(UNS, "at most 1024", words=33)
     call(UNS, "at most 1024", words=0)
     call(UNS, "too many", hq=65 * 4, qs=65 * 256, os=65 * 256)
