@@ -39,7 +39,6 @@ constexpr int kAtomBytes = kKeys * 128;  // 128 rows of 64 values, 128-byte swiz
 constexpr int kUnitCost = 1;             // a unit's start and end, in chunks
 constexpr int kMinShare = 3;             // weight below which a range is not worth a CTA
 constexpr int kMaxGrid = 1024;
-constexpr int kLag = 2;                  // blocks that a loading warp leaves in flight
 constexpr int kBadSlots = 8;
 constexpr float kRescaleAt = 8.f;
 
@@ -287,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
-      mbar_init(&sh.full[i], kLoadWarps);
+      mbar_init(&sh.full[i], kLoadWarps * 32);
       mbar_init(&sh.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -377,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
     const int lw = warp - kSoftWarps;
     const int64_t slot_bytes = (int64_t)a.hkv * D * 2;
-    int stage = 0, issued = 0, told = 0;
+    int stage = 0;
     uint32_t phase = 1;
     bool ok = true;
     // The blocks of this CTA's pieces, in the order in which the MMAs want them.
@@ -409,28 +408,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       const int key = b.chunk * kKeys + lw * 32 + lane;
       return key < b.p.t.keys ? b.p.t.slots[key] : 0;
     };
-    // makes blocks [told, upto) known to the MMA warp: this warp's copies of them have landed
-    auto tell = [&](int upto) {
-      if (told >= upto) return;
-      fence_proxy_async_shared();
-      for (; told < upto; ++told) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.full[told % S::kStages]);
-      }
-    };
     bool more = advance(now);
     int slot = more ? slot_of(now) : 0;
     while (more) {
       next = now;
       const bool more_next = advance(next);
       const int slot_next = more_next ? slot_of(next) : 0;  // asked for a block ahead
-      if (!mbar_try_wait(&sh.empty[stage], phase)) {
-        cp_async_wait_all();
-        tell(issued);
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[stage], phase));
-        if (!ok) break;
-      }
-      __syncwarp();
+      ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[stage], phase));
+      if (!ok) break;
       const Piece& p = now.p;
       const int k0 = now.chunk * kKeys + lw * 32;
       if (slot < 0 || slot >= a.num_slots) {
@@ -462,6 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
                        "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
                        : "memory");
         }
+        mbar_arrive(&sh.full[stage]);
       } else {
 #pragma unroll
         for (int i = 0; i < kCols; ++i) {
@@ -470,23 +456,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
           cp_async16_or_zero(dst + (c >> 3) * kAtomBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4),
                              src + s * slot_bytes + c * 16, k0 + row < p.t.keys);
         }
+        // this thread arrives when its copies so far have landed
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&sh.full[stage]))
+                     : "memory");
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      ++issued;
       if (++stage == S::kStages) {
         stage = 0;
         phase ^= 1;
       }
-      asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
-      tell(issued - kLag);
       now = next;
       more = more_next;
       slot = slot_next;
     }
     cp_async_wait_all();
-    if (ok) {
-      tell(issued);
-    } else {
+    if (!ok) {
       report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
       sh.abort_flag = 1;
     }
@@ -499,7 +482,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
     bool ok = true;
     auto stage_of = [&](uint32_t block) { return block % S::kStages; };
     auto wait_block = [&](uint32_t block) {
-      return mbar_wait(&sh.full[stage_of(block)], (block / S::kStages) & 1);
+      const bool here = mbar_wait(&sh.full[stage_of(block)], (block / S::kStages) & 1);
+      fence_proxy_async_shared();  // the copies went through the generic proxy, the MMAs read through the other one
+      return here;
     };
     while (ok && it.next(a, p)) {
       const int n = p.c1 - p.c0;
