@@ -287,16 +287,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&sh.full[i], kLoadWarps * 32);
-      mbar_init(&sh.empty[i], 1);
+      mbar_init(&sh.empty[i], 2);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.p_full[i], 4);
     }
     mbar_init(&sh.q_full, kSoftWarps);
-    mbar_init(&sh.piece_done, 1);
+    mbar_init(&sh.piece_done, 2);
     mbar_init(&sh.state_full, kSoftWarps);
-    mbar_init(&sh.drained, 1);
+    mbar_init(&sh.drained, 2);
     sh.abort_flag = 0;
     fence_mbar_init();
   }
@@ -379,83 +379,78 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
     int stage = 0;
     uint32_t phase = 1;
     bool ok = true;
-    // The blocks of this CTA's pieces, in the order in which the MMAs want them.
-    struct Block {
-      Piece p;
-      int i, n;  // block of the piece, chunks of the piece
-      int turn;
-      bool values;
-      int chunk;
-    } now = {}, next;
-    now.turn = -1;
-    auto advance = [&](Block& b) {
-      if (++b.i >= 2 * b.n) {
-        if (!it.next(a, b.p)) return false;
-        b.i = 0;
-        b.n = b.p.c1 - b.p.c0;
-        b.turn = (b.turn + 1) % kBadSlots;
+    int turn = 0;
+    // Slots of this lane's key in eight chunks: four from `window` on, and the four behind them. They are asked
+    // for four to eight chunks ahead: a page table's line comes from DRAM, which takes as long as a chunk.
+    int window = 0, here[4], ahead[4];
+    auto ask = [&](int chunk, int (&out)[4]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = (chunk + j) * kKeys + lw * 32 + lane;
+        out[j] = key < min(p.t.keys, p.c1 * kKeys) ? p.t.slots[key] : 0;
       }
-      if (b.p.pair() || b.n == 1) {  // K0 V0 K1 V1 ..
-        b.values = b.i & 1;
-        b.chunk = b.p.c0 + b.i / 2;
-      } else {  // K0 K1 V0 K2 V1 .. V(n-2) V(n-1)
-        b.values = b.i == 2 * b.n - 1 || (b.i >= 2 && !(b.i & 1));
-        b.chunk = b.p.c0 + (b.i < 2 ? b.i : b.i == 2 * b.n - 1 ? b.n - 1 : (b.i & 1) ? (b.i + 1) / 2 : b.i / 2 - 1);
+    };
+    auto load = [&](bool values, int chunk) {
+      if (values && chunk >= window + 4) {
+        window += 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) here[j] = ahead[j];
+        ask(window + 4, ahead);
       }
-      return true;
-    };
-    auto slot_of = [&](const Block& b) {  // of this lane's key
-      const int key = b.chunk * kKeys + lw * 32 + lane;
-      return key < b.p.t.keys ? b.p.t.slots[key] : 0;
-    };
-    bool more = advance(now);
-    int slot = more ? slot_of(now) : 0;
-    while (more) {
-      next = now;
-      const bool more_next = advance(next);
-      const int slot_next = more_next ? slot_of(next) : 0;  // asked for a block ahead
+      const int at = chunk - window;
+      int slot = at < 4 ? here[0] : ahead[0];
+#pragma unroll
+      for (int j = 1; j < 4; ++j)
+        if ((at & 3) == j) slot = at < 4 ? here[j] : ahead[j];
       ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[stage], phase));
-      if (!ok) break;
-      const Piece& p = now.p;
-      const int k0 = now.chunk * kKeys + lw * 32;
+      if (!ok) return;
+      const int k0 = chunk * kKeys + lw * 32;
       if (slot < 0 || slot >= a.num_slots) {
-        if (!now.values) report(a.status, AIOSB_DEV_SLOT_RANGE);
+        if (!values) report(a.status, AIOSB_DEV_SLOT_RANGE);
         slot = 0;
       }
       const char* const src =
-          reinterpret_cast<const char*>(now.values ? a.v_cache : a.k_cache) + (int64_t)p.h * D * 2;
+          reinterpret_cast<const char*>(values ? a.v_cache : a.k_cache) + (int64_t)p.h * D * 2;
       const uint32_t dst = ring + stage * S::kBlockBytes + lw * 32 * 128;
       constexpr int kCols = D / 8;  // 16-byte pieces of a key
-      if (now.values && (now.chunk + 1) * kKeys > p.t.cached) {
+      int slots[kCols];  // every exchange before the first copy: one after another they take as long as the copies
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) slots[i] = __shfl_sync(0xffffffffu, slot, (i * 32 + lane) / kCols);
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) {
+        const int at = i * 32 + lane, row = at / kCols, c = at % kCols;
+        cp_async16_or_zero(dst + (c >> 3) * kAtomBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4),
+                           src + slots[i] * slot_bytes + c * 16, k0 + row < p.t.keys);
+      }
+      if (values && k0 + 32 > p.t.cached && k0 < p.t.keys) {
         // a key that a node does not see gets weight 0, and 0 * inf is NaN: infinities and NaN of the tree's
         // keys leave V here, and reach the nodes that see them at the end
-#pragma unroll 1
-        for (int i = lane; i < 32 * kCols; i += 32) {
-          const int row = i / kCols, c = i % kCols, key = k0 + row;
-          const int s = __shfl_sync(0xffffffffu, slot, row);
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (key < p.t.keys) v = *reinterpret_cast<const uint4*>(src + s * slot_bytes + c * 16);
-          if (key >= p.t.cached &&
-              !(finite_bf16x2(v.x) && finite_bf16x2(v.y) && finite_bf16x2(v.z) && finite_bf16x2(v.w))) {
-            v = make_uint4(drop_nonfinite_bf16x2(v.x), drop_nonfinite_bf16x2(v.y), drop_nonfinite_bf16x2(v.z),
-                           drop_nonfinite_bf16x2(v.w));
-            const int j = key - p.t.cached;
-            atomicOr(&sh.bad[now.turn][j >> 5], 1u << (j & 31));
+        cp_async_wait_all();
+        __syncwarp();
+        const int key = k0 + lane;
+        bool bad = false;
+        if (key >= p.t.cached && key < p.t.keys) {
+#pragma unroll 4
+          for (int c = 0; c < kCols; ++c) {
+            const uint32_t at = dst + (c >> 3) * kAtomBytes + lane * 128 + (((c & 7) ^ (lane & 7)) << 4);
+            uint4 v;
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                         : "r"(at)
+                         : "memory");
+            if (finite_bf16x2(v.x) && finite_bf16x2(v.y) && finite_bf16x2(v.z) && finite_bf16x2(v.w)) continue;
+            bad = true;
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(drop_nonfinite_bf16x2(v.x)),
+                         "r"(drop_nonfinite_bf16x2(v.y)), "r"(drop_nonfinite_bf16x2(v.z)),
+                         "r"(drop_nonfinite_bf16x2(v.w))
+                         : "memory");
           }
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (c >> 3) * kAtomBytes + row * 128 +
-                                                                    (((c & 7) ^ (row & 7)) << 4)),
-                       "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                       : "memory");
+          const int j = key - p.t.cached;
+          if (bad) atomicOr(&sh.bad[turn][j >> 5], 1u << (j & 31));
         }
+        fence_proxy_async_shared();
         mbar_arrive(&sh.full[stage]);
       } else {
-#pragma unroll
-        for (int i = 0; i < kCols; ++i) {
-          const int at = i * 32 + lane, row = at / kCols, c = at % kCols;
-          const int s = __shfl_sync(0xffffffffu, slot, row);
-          cp_async16_or_zero(dst + (c >> 3) * kAtomBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4),
-                             src + s * slot_bytes + c * 16, k0 + row < p.t.keys);
-        }
         // this thread arrives when its copies so far have landed
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&sh.full[stage]))
                      : "memory");
@@ -464,9 +459,26 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
         stage = 0;
         phase ^= 1;
       }
-      now = next;
-      more = more_next;
-      slot = slot_next;
+    };
+    // block order of a piece: the order in which the MMAs want them
+    while (ok && it.next(a, p)) {
+      window = p.c0;
+      ask(window, here);
+      ask(window + 4, ahead);
+      if (p.pair()) {
+        for (int c = p.c0; c < p.c1 && ok; ++c) {
+          load(false, c);
+          if (ok) load(true, c);
+        }
+      } else {
+        load(false, p.c0);
+        if (ok && p.c0 + 1 < p.c1) load(false, p.c0 + 1);
+        for (int c = p.c0; c < p.c1 && ok; ++c) {
+          load(true, c);
+          if (ok && c + 2 < p.c1) load(false, c + 2);
+        }
+      }
+      turn = (turn + 1) % kBadSlots;
     }
     cp_async_wait_all();
     if (!ok) {
@@ -475,83 +487,77 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
     }
   } else if (warp >= kMmaWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
-    if (warp == kMmaWarp) {
-    // ---- MMAs: for each stream in turn O += P V of its last chunk, then S of its next one
-    constexpr uint32_t idesc_s = umma_idesc_bf16(kTile, kKeys), idesc_o = umma_idesc_bf16(kTile, D) | kBMajorMn;
-    uint32_t base = 0, q_phase = 0, p_phase[2] = {0, 0};
-    bool ok = true;
-    auto stage_of = [&](uint32_t block) { return block % S::kStages; };
-    auto wait_block = [&](uint32_t block) {
-      const bool here = mbar_wait(&sh.full[stage_of(block)], (block / S::kStages) & 1);
-      fence_proxy_async_shared();  // the copies went through the generic proxy, the MMAs read through the other one
-      return here;
-    };
-    while (ok && it.next(a, p)) {
-      const int n = p.c1 - p.c0;
-      const bool pair = p.pair();
-      // blocks of chunk i's keys and values, as the gathering warps order them
-      auto k_block = [&](int i) { return base + (pair ? 2 * i : i < 2 ? i : 2 * i - 1); };
-      auto v_block = [&](int i) { return base + (pair ? 2 * i + 1 : i == n - 1 ? 2 * n - 1 : 2 * i + 2); };
-      const int step = pair ? 1 : 2;
-      ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full, q_phase));
-      q_phase ^= 1;
-      if (!ok) break;
-      tc_fence_after();
-      // turn i of a stream: P V of its chunk i - 1, S of its chunk i
-      for (int i = 0; ok; ++i) {
-        bool more = false;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const int first = pair ? 0 : s;
-          const int now = first + i * step, before = now - step;
-          if (i > 0 && before < n) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&sh.p_full[s], p_phase[s]) && wait_block(v_block(before)));
-            p_phase[s] ^= 1;
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t st = stage_of(v_block(before));
-            if (elect_one()) {
-              const uint32_t v = ring + st * S::kBlockBytes;
+    if (warp < kMmaWarp + 2) {
+      // ---- MMAs of stream s: O += P V of a chunk, then S of the stream's next one. A warp for each stream: a wait
+      // that is over and the issue behind it take some hundred clocks of a warp, four times a chunk.
+      constexpr uint32_t idesc_s = umma_idesc_bf16(kTile, kKeys), idesc_o = umma_idesc_bf16(kTile, D) | kBMajorMn;
+      const int s = warp - kMmaWarp;
+      const uint32_t t_s = tmem + s * 128, t_o = tmem + 256 + s * 128;
+      uint32_t base = 0, q_phase = 0, p_phase = 0;
+      bool ok = true;
+      while (ok && it.next(a, p)) {
+        const int n = p.c1 - p.c0;
+        const bool pair = p.pair();
+        // blocks of chunk i's keys and values, as the gathering warps order them
+        auto k_block = [&](int i) { return base + (pair ? 2 * i : i < 2 ? i : 2 * i - 1); };
+        auto v_block = [&](int i) { return base + (pair ? 2 * i + 1 : i == n - 1 ? 2 * n - 1 : 2 * i + 2); };
+        // a block is free when both streams are through with it, or the only one that uses it
+        auto release = [&](uint32_t stage) {
+          tc_commit(&sh.empty[stage]);
+          if (!pair) mbar_arrive(&sh.empty[stage]);
+        };
+        const uint32_t q_desc = q_smem + (pair ? s : 0) * S::kBlockBytes;
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full, q_phase));
+        q_phase ^= 1;
+        if (!ok) break;
+        const int step = pair ? 1 : 2;
+        int before = -1;
+        for (int now = pair ? 0 : s; now < n || before >= 0; now += step) {
+          const uint32_t vb = before >= 0 ? v_block(before) : 0, kb = now < n ? k_block(now) : 0;
+          const uint32_t v_stage = vb % S::kStages, k_stage = kb % S::kStages;
+          // the blocks first: they are there before the weights, as a rule
+          if (before >= 0) ok = mbar_wait(&sh.full[v_stage], (vb / S::kStages) & 1);
+          if (ok && now < n) ok = mbar_wait(&sh.full[k_stage], (kb / S::kStages) & 1);
+          if (ok && before >= 0) {
+            ok = mbar_wait(&sh.p_full[s], p_phase);
+            p_phase ^= 1;
+          }
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            fence_proxy_async_shared();  // the copies went through the generic proxy, the MMAs read through the other
+            if (before >= 0) {
+              const uint32_t v = ring + v_stage * S::kBlockBytes;
+              const bool first = before < step;
 #pragma unroll
               for (int k = 0; k < kKeys / 16; ++k)
-                tc_mma_bf16_ts(tmem + 256 + s * 128, tmem + s * 128 + k * 8, umma_desc_mn(v + k * 2048), idesc_o,
-                               i > 1 || k > 0);
-              if (!pair || s == 1) tc_commit(&sh.empty[st]);
+                tc_mma_bf16_ts(t_o, t_s + k * 8, umma_desc_mn(v + k * 2048), idesc_o, !first || k > 0);
+              release(v_stage);
             }
-            __syncwarp();
-            more = true;
-          }
-          if (now < n) {
-            ok = __all_sync(0xffffffffu, wait_block(k_block(now)));
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t st = stage_of(k_block(now));
-            if (elect_one()) {
-              const uint64_t kd = umma_desc_sw128(ring + st * S::kBlockBytes);
-              const uint64_t qd = umma_desc_sw128(q_smem + (pair ? s : 0) * S::kBlockBytes);
+            if (now < n) {
+              const uint64_t kd = umma_desc_sw128(ring + k_stage * S::kBlockBytes), qd = umma_desc_sw128(q_desc);
 #pragma unroll
               for (int k = 0; k < D / 16; ++k) {
                 const uint32_t off = ((k >> 2) * kAtomBytes + (k & 3) * 32) >> 4;
-                tc_mma_bf16(tmem + s * 128, qd + off, kd + off, idesc_s, k > 0);
+                tc_mma_bf16(t_s, qd + off, kd + off, idesc_s, k > 0);
               }
               tc_commit(&sh.s_full[s]);
-              if (!pair || s == 1) tc_commit(&sh.empty[st]);
+              release(k_stage);
             }
-            __syncwarp();
-            more = true;
           }
+          __syncwarp();
+          before = now < n ? now : -1;
         }
-        if (!more) break;
+        if (!ok) break;
+        if (elect_one()) tc_commit(&sh.piece_done);
+        __syncwarp();
+        base += 2 * n;
       }
-      if (!ok) break;
-      if (elect_one()) tc_commit(&sh.piece_done);
-      __syncwarp();
-      base += 2 * n;
-    }
-    if (!ok) {
-      report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
-      sh.abort_flag = 1;
-    }
+      if (!ok) {
+        report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
+        sh.abort_flag = 1;
+      }
     }
   } else {
     // ---- softmax of stream s; a thread owns row `row` of the stream's tile
@@ -569,14 +575,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       if (s == 0 || pair) {
         const int wt = threadIdx.x & 127;
         constexpr int kCols = D / 8;
-        for (int i = wt; i < kTile * kCols; i += 128) {
-          const int rr = i / kCols, c = i % kCols, g = p.row0 + s * kTile + rr;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (s * kTile + rr < p.rows)
-            v = *reinterpret_cast<const uint4*>(a.q + (int64_t)(p.t.start + g / a.group) * a.q_stride +
-                                                (int64_t)(p.h * a.group + g % a.group) * D + c * 8);
+        uint4 v[kCols];  // every load in flight before the first store: one round trip
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) {
+          const int at = i * 128 + wt, rr = s * kTile + at / kCols, g = p.row0 + rr;
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (rr < p.rows)
+            v[i] = *reinterpret_cast<const uint4*>(a.q + (int64_t)(p.t.start + g / a.group) * a.q_stride +
+                                                   (int64_t)(p.h * a.group + g % a.group) * D + at % kCols * 8);
+        }
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) {
+          const int at = i * 128 + wt, rr = at / kCols, c = at % kCols;
           *reinterpret_cast<uint4*>(smem + s * S::kBlockBytes + (c >> 3) * kAtomBytes + rr * 128 +
-                                    (((c & 7) ^ (rr & 7)) << 4)) = v;
+                                    (((c & 7) ^ (rr & 7)) << 4)) = v[i];
         }
         fence_proxy_async_shared();
       }
@@ -728,13 +740,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
 
   tc_fence_before();
   __syncthreads();
+  if (sh.abort_flag && warp >= kMmaWarp && warp < kMmaWarp + 2) {  // MMAs may still run: their end is waited for
+    if (elect_one()) tc_commit(&sh.drained);
+    __syncwarp();
+    mbar_wait(&sh.drained, 0);
+  }
   if (warp == kMmaWarp) {
     tc_fence_after();
-    if (sh.abort_flag) {  // MMAs may still run: their end is waited for, with a limit
-      if (elect_one()) tc_commit(&sh.drained);
-      __syncwarp();
-      mbar_wait(&sh.drained, 0);
-    }
     tmem_dealloc(tmem, 512);
   }
 }
