@@ -26,15 +26,12 @@ namespace {
 
 constexpr int kTile = 128;      // rows of a tile: UMMA M, TMEM lanes
 constexpr int kUnitRows = 256;  // two tiles
-constexpr int kKeys = 128;      // keys of a chunk
+constexpr int kKeys = 128;      // keys of a chunk: a block of keys and one of values
+constexpr int kStep = 64;       // keys of a softmax step, half a chunk
 constexpr int kSoftWarps = 8;
 constexpr int kLoadWarps = 4;
 constexpr int kMmaWarp = kSoftWarps + kLoadWarps;
-constexpr int kThreads = (kMmaWarp + 4) * 32;  // whole groups of four warps; three idle
-// Registers of a thread: a softmax thread holds a row's 128 scores. 2 x 176 + 96 + 64 = 4 x 128, what the
-// block is launched with.
-constexpr int kSoftRegs = 176, kLoadRegs = 96, kMmaRegs = 64;
-static_assert(2 * kSoftRegs + kLoadRegs + kMmaRegs <= 65536 / kThreads * 4, "more registers than the block has");
+constexpr int kThreads = (kMmaWarp + 1) * 32;
 constexpr int kAtomBytes = kKeys * 128;  // 128 rows of 64 values, 128-byte swizzled
 constexpr int kUnitCost = 1;             // a unit's start and end, in chunks
 constexpr int kMinShare = 3;             // weight below which a range is not worth a CTA
@@ -202,19 +199,21 @@ __device__ __forceinline__ uint32_t seen32(const int32_t* bits, int words, int k
   return left >= 32 ? m : m & ((1u << left) - 1u);
 }
 
-// One chunk of a row: S (128 columns at t_s) to weights in bf16 over it; the row's reference and sum, and
-// its output at t_o where the reference moves. `seen`: bits of the keys, if some are hidden.
-template <int D, bool MASKED>
-__device__ __forceinline__ void soft_chunk(uint32_t t_s, uint32_t t_o, const uint32_t (&seen)[4], float scale,
-                                           bool fresh, float& ref, float& sum) {
-  uint32_t v[4][32];
+// One step of a row: its 64 scores at t_s to weights in bf16 over them; the row's reference and sum, and its output
+// at t_o where the reference moves (behind `settled`: the products so far are in it). `seen`: bits of the keys, if
+// some are hidden. False: a wait ran out.
+template <int D, bool MASKED, typename Settled>
+__device__ __forceinline__ bool soft_step(uint32_t t_s, uint32_t t_o, const uint32_t (&seen)[2], float scale, bool fresh,
+                                          float& ref, float& sum, Settled settled) {
+  bool ok = true;
+  uint32_t v[2][32];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) tmem_ld(t_s + j * 32, v[j]);
+  for (int j = 0; j < 2; ++j) tmem_ld(t_s + j * 32, v[j]);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) tmem_wait(v[j]);
+  for (int j = 0; j < 2; ++j) tmem_wait(v[j]);
   if (MASKED) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int e = 0; e < 32; ++e)
         if (!((seen[j] >> e) & 1)) v[j][e] = 0xFF800000u;  // -inf
@@ -222,24 +221,27 @@ __device__ __forceinline__ void soft_chunk(uint32_t t_s, uint32_t t_o, const uin
   float top[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    top[j] = __uint_as_float(v[j][0]);
+    const uint32_t* const u = v[j / 2] + j % 2 * 16;
+    top[j] = fmaxf(__uint_as_float(u[0]), __uint_as_float(u[15]));
 #pragma unroll
-    for (int e = 1; e < 31; e += 2) top[j] = max3(top[j], __uint_as_float(v[j][e]), __uint_as_float(v[j][e + 1]));
-    top[j] = fmaxf(top[j], __uint_as_float(v[j][31]));
+    for (int e = 1; e < 15; e += 2) top[j] = max3(top[j], __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
   }
   const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
   const bool grows = most > ref + kRescaleAt;
   if (__any_sync(0xffffffffu, grows)) {
     const float corr = grows ? exp2_fast(ref - most) : 1.f;
     if (!fresh) {
+      ok = settled();
+      if (ok) {
 #pragma unroll 1
-      for (int j = 0; j < D / 16; ++j) {
-        uint32_t o[16];
-        tmem_ld(t_o + j * 16, o);
-        tmem_wait(o);
+        for (int j = 0; j < D / 16; ++j) {
+          uint32_t o[16];
+          tmem_ld(t_o + j * 16, o);
+          tmem_wait(o);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-        tmem_st16(t_o + j * 16, o);
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+          tmem_st16(t_o + j * 16, o);
+        }
       }
     }
     sum *= corr;
@@ -249,7 +251,7 @@ __device__ __forceinline__ void soft_chunk(uint32_t t_s, uint32_t t_o, const uin
   const float2 m2 = make_float2(minus, minus), s2 = make_float2(scale, scale);
   float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < 2; ++j) {
     uint32_t w[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
@@ -262,11 +264,12 @@ __device__ __forceinline__ void soft_chunk(uint32_t t_s, uint32_t t_o, const uin
   }
   sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
   tmem_wait_st();
+  return ok;
 }
 
 struct Shared {
   uint64_t full[10], empty[10];
-  uint64_t s_full[2], p_full[2], q_full, piece_done, state_full, drained;
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2], q_full, piece_done, state_full, drained;
   uint32_t tmem_slot;
   volatile int abort_flag;
   int r0;
@@ -287,16 +290,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&sh.full[i], kLoadWarps * 32);
-      mbar_init(&sh.empty[i], 2);
+      mbar_init(&sh.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.p_full[i], 4);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&sh.s_full[i][b], 1);
+        mbar_init(&sh.p_full[i][b], 4);
+      }
+      mbar_init(&sh.pv_done[i], 1);
     }
     mbar_init(&sh.q_full, kSoftWarps);
-    mbar_init(&sh.piece_done, 2);
+    mbar_init(&sh.piece_done, 1);
     mbar_init(&sh.state_full, kSoftWarps);
-    mbar_init(&sh.drained, 2);
+    mbar_init(&sh.drained, 1);
     sh.abort_flag = 0;
     fence_mbar_init();
   }
@@ -373,7 +379,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
 
   if (warp >= kSoftWarps && warp < kMmaWarp) {
     // ---- gather
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
     const int lw = warp - kSoftWarps;
     const int64_t slot_bytes = (int64_t)a.hkv * D * 2;
     int stage = 0;
@@ -485,87 +490,97 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
       sh.abort_flag = 1;
     }
-  } else if (warp >= kMmaWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
-    if (warp < kMmaWarp + 2) {
-      // ---- MMAs of stream s: O += P V of a chunk, then S of the stream's next one. A warp for each stream: a wait
-      // that is over and the issue behind it take some hundred clocks of a warp, four times a chunk.
-      constexpr uint32_t idesc_s = umma_idesc_bf16(kTile, kKeys), idesc_o = umma_idesc_bf16(kTile, D) | kBMajorMn;
-      const int s = warp - kMmaWarp;
-      const uint32_t t_s = tmem + s * 128, t_o = tmem + 256 + s * 128;
-      uint32_t base = 0, q_phase = 0, p_phase = 0;
-      bool ok = true;
-      while (ok && it.next(a, p)) {
-        const int n = p.c1 - p.c0;
-        const bool pair = p.pair();
-        // blocks of chunk i's keys and values, as the gathering warps order them
-        auto k_block = [&](int i) { return base + (pair ? 2 * i : i < 2 ? i : 2 * i - 1); };
-        auto v_block = [&](int i) { return base + (pair ? 2 * i + 1 : i == n - 1 ? 2 * n - 1 : 2 * i + 2); };
-        // a block is free when both streams are through with it, or the only one that uses it
-        auto release = [&](uint32_t stage) {
-          tc_commit(&sh.empty[stage]);
-          if (!pair) mbar_arrive(&sh.empty[stage]);
-        };
-        const uint32_t q_desc = q_smem + (pair ? s : 0) * S::kBlockBytes;
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full, q_phase));
-        q_phase ^= 1;
-        if (!ok) break;
-        const int step = pair ? 1 : 2;
-        int before = -1;
-        for (int now = pair ? 0 : s; now < n || before >= 0; now += step) {
-          const uint32_t vb = before >= 0 ? v_block(before) : 0, kb = now < n ? k_block(now) : 0;
-          const uint32_t v_stage = vb % S::kStages, k_stage = kb % S::kStages;
+  } else if (warp == kMmaWarp) {
+    // ---- MMAs: for each stream in turn O += P V of its last step, then S of the step after next, so that scores are
+    // there when a stream's softmax comes to them. One warp for both streams: it keeps them apart.
+    constexpr uint32_t idesc_s = umma_idesc_bf16(kTile, kStep), idesc_o = umma_idesc_bf16(kTile, D) | kBMajorMn;
+    uint32_t base = 0, q_phase = 0, steps[2] = {0, 0};  // of a stream, in all pieces so far
+    bool ok = true;
+    while (ok && it.next(a, p)) {
+      const int n = p.c1 - p.c0;
+      const bool pair = p.pair();
+      // blocks of chunk i's keys and values, as the gathering warps order them
+      auto k_block = [&](int i) { return base + (pair ? 2 * i : i < 2 ? i : 2 * i - 1); };
+      auto v_block = [&](int i) { return base + (pair ? 2 * i + 1 : i == n - 1 ? 2 * n - 1 : 2 * i + 2); };
+      auto wait_block = [&](uint32_t b) { return mbar_wait(&sh.full[b % S::kStages], (b / S::kStages) & 1); };
+      ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full, q_phase));
+      q_phase ^= 1;
+      if (!ok) break;
+      // S of step h of stream s (chunk `c` of the piece); the elected lane
+      auto score = [&](int s, int h, int c) {
+        const uint32_t stage = k_block(c) % S::kStages, buffer = (steps[s] + h) & 1;
+        const uint64_t kd = umma_desc_sw128(ring + stage * S::kBlockBytes + (h & 1) * (kStep * 128)),
+                       qd = umma_desc_sw128(q_smem + (pair ? s : 0) * S::kBlockBytes);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = ((k >> 2) * kAtomBytes + (k & 3) * 32) >> 4;
+          tc_mma_bf16(tmem + s * 128 + buffer * kStep, qd + off, kd + off, idesc_s, k > 0);
+        }
+        tc_commit(&sh.s_full[s][buffer]);
+        // the block's last reader: a wide unit's second stream, or the only one that has the chunk
+        if ((h & 1) && (!pair || s == 1)) tc_commit(&sh.empty[stage]);
+      };
+      // step h of stream s is half h & 1 of this chunk
+      auto chunk_of = [&](int s, int h) { return pair ? h >> 1 : 2 * (h >> 1) + s; };
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (chunk_of(s, 0) >= n) continue;
+        ok = ok && __all_sync(0xffffffffu, wait_block(k_block(chunk_of(s, 0))));
+        if (ok && elect_one()) {
+          fence_proxy_async_shared();  // the copies went through the generic proxy, the MMAs read through the other
+          score(s, 0, chunk_of(s, 0));
+          score(s, 1, chunk_of(s, 0));
+        }
+        __syncwarp();
+      }
+      bool more = ok;
+      for (int h = 0; more; ++h) {
+        more = false;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const int c = chunk_of(s, h), next = chunk_of(s, h + 2);
+          if (c >= n || !ok) continue;
+          more = true;
+          const uint32_t buffer = (steps[s] + h) & 1;
           // the blocks first: they are there before the weights, as a rule
-          if (before >= 0) ok = mbar_wait(&sh.full[v_stage], (vb / S::kStages) & 1);
-          if (ok && now < n) ok = mbar_wait(&sh.full[k_stage], (kb / S::kStages) & 1);
-          if (ok && before >= 0) {
-            ok = mbar_wait(&sh.p_full[s], p_phase);
-            p_phase ^= 1;
-          }
+          ok = wait_block(v_block(c)) && (next >= n || wait_block(k_block(next))) &&
+               mbar_wait(&sh.p_full[s][buffer], ((steps[s] + h) >> 1) & 1);
           ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
+          if (!ok) continue;
           tc_fence_after();
           if (elect_one()) {
-            fence_proxy_async_shared();  // the copies went through the generic proxy, the MMAs read through the other
-            if (before >= 0) {
-              const uint32_t v = ring + v_stage * S::kBlockBytes;
-              const bool first = before < step;
+            fence_proxy_async_shared();
+            const uint32_t stage = v_block(c) % S::kStages;
+            const uint32_t v = ring + stage * S::kBlockBytes + (h & 1) * (kStep * 128);
 #pragma unroll
-              for (int k = 0; k < kKeys / 16; ++k)
-                tc_mma_bf16_ts(t_o, t_s + k * 8, umma_desc_mn(v + k * 2048), idesc_o, !first || k > 0);
-              release(v_stage);
-            }
-            if (now < n) {
-              const uint64_t kd = umma_desc_sw128(ring + k_stage * S::kBlockBytes), qd = umma_desc_sw128(q_desc);
-#pragma unroll
-              for (int k = 0; k < D / 16; ++k) {
-                const uint32_t off = ((k >> 2) * kAtomBytes + (k & 3) * 32) >> 4;
-                tc_mma_bf16(t_s, qd + off, kd + off, idesc_s, k > 0);
-              }
-              tc_commit(&sh.s_full[s]);
-              release(k_stage);
-            }
+            for (int k = 0; k < kStep / 16; ++k)
+              tc_mma_bf16_ts(tmem + 256 + s * 128, tmem + s * 128 + buffer * kStep + k * 8, umma_desc_mn(v + k * 2048),
+                             idesc_o, h > 0 || k > 0);
+            tc_commit(&sh.pv_done[s]);
+            if ((h & 1) && (!pair || s == 1)) tc_commit(&sh.empty[stage]);
+            if (next < n) score(s, h + 2, next);
           }
           __syncwarp();
-          before = now < n ? now : -1;
         }
-        if (!ok) break;
-        if (elect_one()) tc_commit(&sh.piece_done);
-        __syncwarp();
-        base += 2 * n;
+        more = more && ok;
       }
-      if (!ok) {
-        report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
-        sh.abort_flag = 1;
-      }
+      if (!ok) break;
+      if (elect_one()) tc_commit(&sh.piece_done);
+      __syncwarp();
+      base += 2 * n;
+      steps[0] += pair ? 2 * n : 2 * ((n + 1) / 2);
+      steps[1] += pair ? 2 * n : 2 * (n / 2);
+    }
+    if (!ok) {
+      report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
+      sh.abort_flag = 1;
     }
   } else {
     // ---- softmax of stream s; a thread owns row `row` of the stream's tile
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
     const int s = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t t_s = t_lane + s * 128, t_o = t_lane + 256 + s * 128;
-    uint32_t s_phase = 0, done_phase = 0, state_phase = 0;
+    const uint32_t t_o = t_lane + 256 + s * 128;
+    uint32_t step = 0, done_phase = 0, state_phase = 0;  // steps of this stream, in all pieces so far
     int turn = 0, partial_of = -1;
     bool ok = true;
     Join join = {};
@@ -603,26 +618,34 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       const int32_t* const bits = a.mask + (int64_t)node * a.words;
       float ref = -INFINITY, sum = 0.f;
       bool fresh = true;  // no output of this piece yet
-      for (int c = p.c0 + (pair ? 0 : s); c < p.c1; c += pair ? 1 : 2) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full[s], s_phase));
-        s_phase ^= 1;
-        if (!ok) break;
-        tc_fence_after();
-        if (warp_works) {
-          if ((c + 1) * kKeys > p.t.cached) {
-            uint32_t seen[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) seen[j] = seen32(bits, a.words, c * kKeys + j * 32, p.t.cached, p.t.keys);
-            soft_chunk<D, true>(t_s, t_o, seen, a.scale_log2, fresh, ref, sum);
-          } else {
-            const uint32_t all[4] = {};
-            soft_chunk<D, false>(t_s, t_o, all, a.scale_log2, fresh, ref, sum);
+      for (int c = p.c0 + (pair ? 0 : s); c < p.c1 && ok; c += pair ? 1 : 2) {
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half, ++step) {
+          const uint32_t buffer = step & 1, t_s = t_lane + s * 128 + buffer * kStep;
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full[s][buffer], (step >> 1) & 1));
+          if (!ok) break;
+          tc_fence_after();
+          if (warp_works) {
+            const int k0 = c * kKeys + half * kStep;
+            auto settled = [&] {  // the products of the steps before this one are in the output
+              const bool there = __all_sync(0xffffffffu, mbar_wait(&sh.pv_done[s], (step - 1) & 1));
+              tc_fence_after();
+              return there;
+            };
+            if (k0 + kStep > p.t.cached) {
+              const uint32_t seen[2] = {seen32(bits, a.words, k0, p.t.cached, p.t.keys),
+                                        seen32(bits, a.words, k0 + 32, p.t.cached, p.t.keys)};
+              ok = soft_step<D, true>(t_s, t_o, seen, a.scale_log2, fresh, ref, sum, settled);
+            } else {
+              const uint32_t all[2] = {};
+              ok = soft_step<D, false>(t_s, t_o, all, a.scale_log2, fresh, ref, sum, settled);
+            }
           }
+          fresh = false;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.p_full[s][buffer]);
         }
-        fresh = false;
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.p_full[s]);
       }
       if (!ok) break;
       ok = __all_sync(0xffffffffu, mbar_wait(&sh.piece_done, done_phase));
@@ -636,7 +659,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       bool use[2] = {s == 0 || !pair, !pair && p.c1 - p.c0 > 1};
       if (!pair) {
         // through TMEM, where S was: the two warps with this row reach the same lane
-        tmem_st2(t_s, __float_as_uint(ref), __float_as_uint(sum));
+        tmem_st2(t_lane + s * 128, __float_as_uint(ref), __float_as_uint(sum));
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -740,7 +763,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
 
   tc_fence_before();
   __syncthreads();
-  if (sh.abort_flag && warp >= kMmaWarp && warp < kMmaWarp + 2) {  // MMAs may still run: their end is waited for
+  if (sh.abort_flag && warp == kMmaWarp) {  // MMAs may still run: their end is waited for
     if (elect_one()) tc_commit(&sh.drained);
     __syncwarp();
     mbar_wait(&sh.drained, 0);
