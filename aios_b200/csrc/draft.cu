@@ -50,7 +50,8 @@ __global__ void __launch_bounds__(kTreeThreads)
 // ---- verification ----------------------------------------------------------------------------
 constexpr int kVerifyThreads = 512;
 constexpr int kVerifyWarps = kVerifyThreads / 32;
-constexpr int kMaxRanks = 8;
+constexpr int kMaxRanks = 16;
+constexpr int kBlockIds = 256;  // ids that a warp takes at a time, eight to a lane
 
 struct VerifyArgs {
   const void* logits;
@@ -69,6 +70,7 @@ struct VerifyArgs {
   int32_t* order;
   int32_t* status;
   int ranks;  // CTAs of a cluster: they share a request's vocabulary
+  int run;    // ids of a warp, a multiple of kBlockIds
 };
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -76,231 +78,464 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ float load_logit(const __nv_bfloat16* p) { return bf16_to_f(*p); }
-__device__ __forceinline__ float load_logit(const float* p) { return *p; }
-
 __device__ __forceinline__ double warp_sum_f64(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+__device__ __forceinline__ float load_logit(const __nv_bfloat16* p) { return bf16_to_f(*p); }
+__device__ __forceinline__ float load_logit(const float* p) { return *p; }
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x[2 * j] = bf16_lo(w[j]);
+    x[2 * j + 1] = bf16_hi(w[j]);
+  }
+}
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
 
-// A cluster per request walks its tree from the root. The vocabulary is cut into one run of ids per
-// warp of the cluster, in ascending order: a pass over a row leaves each warp the sum of its run, each
-// CTA the sum of its warps', and a token is found by these sums from the outside in. Sums are taken in
-// a fixed order, in fp64: an accepted or drawn token hangs on comparisons of them.
-template <typename T, bool GREEDY, bool PROBS>
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs a) {
-  __shared__ int32_t path[AIOSB_TREE_MAX_NODES];
-  __shared__ uint32_t on_path[AIOSB_TREE_MAX_NODES / 32];
-  __shared__ int64_t rejected[AIOSB_TREE_MAX_NODES];  // without draft_probs: tokens that left r at this node
-  __shared__ double scale_by[AIOSB_TREE_MAX_NODES];   // with: 1 / sum(r) before each subtraction of q
-  __shared__ double run_sum[kVerifyWarps];
-  __shared__ float run_max[kVerifyWarps];
-  __shared__ int run_arg[kVerifyWarps];
-  __shared__ double peer_sum[2][kMaxRanks];
-  __shared__ float peer_max[2][kMaxRanks];
-  __shared__ int peer_arg[2][kMaxRanks];
-  __shared__ int next_child;
+// The eight ids of a lane in the block of kBlockIds from `base` on: consecutive ones where the row lies on 16
+// bytes, else every 32nd.
+struct Ids {
+  int base, end, first, step;
+  __device__ __forceinline__ Ids(int base, int end, bool vec, int lane)
+      : base(base), end(end), first(vec ? base + lane * 8 : base + lane), step(vec ? 1 : 32) {}
+  __device__ __forceinline__ int operator[](int j) const { return first + j * step; }
+  __device__ __forceinline__ bool whole() const { return step == 1 && first + 8 <= end; }
+};
+template <typename V>
+__device__ __forceinline__ void load_ids(const V* row, bool vec, const Ids& ids, float none, float (&x)[8]) {
+  if (vec && ids.whole()) {
+    load8(row + ids.first, x);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = ids[j] < ids.end ? load_logit(row + ids[j]) : none;
+  }
+}
+template <typename V>
+__device__ __forceinline__ bool lies_on_16(const V* row) {
+  return (reinterpret_cast<uintptr_t>(row) & 15u) == 0;
+}
 
+// 2^(i / 128) for the exponential below.
+constexpr int kExpTable = 128;
+// e^(d / T) in fp64 for d <= 0, off by about 2^-49: d / (T ln 2) = k / 128 + f / 128 with |f| <= 1/2, 2^(k / 128)
+// from the table and k's upper bits, and 2^(f / 128) by its series to the fourth power (table-driven exponentials:
+// P. T. P. Tang, ACM TOMS 15, 1989). Eleven fp64 instructions, where the general function takes some thirty and its
+// passes over the vocabulary bound the kernel. scale: 128 / (T ln 2). Below 2^-1000 it is 0.
+__device__ __forceinline__ double exp_table(double d, double scale, const double* table) {
+  const double t = d * scale;
+  if (!(t > -128000.0)) return 0.0;
+  const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are round(t)
+  const double s = t + magic, f = t - (s - magic);
+  const int k = __double2loint(s);
+  constexpr double c = 0.0054152123481245727;  // ln 2 / 128
+  double p = fma(f, c * c * c * c / 24, c * c * c / 6);
+  p = fma(f, p, c * c / 2);
+  p = fma(f, p, c);
+  const double b = table[k & (kExpTable - 1)];
+  const double r = fma(b, f * p, b);
+  return __hiloint2double(__double2hiint(r) + ((k >> 7) << 20), __double2loint(r));
+}
+
+// Values that the CTAs of a cluster hand to one another; the buffers take turns, so that one barrier an exchange is
+// enough: a CTA writes a buffer again only behind the next barrier, which all have reached after reading it.
+struct Exchange {
+  double sum[2][kMaxRanks];
+  float top[2][kMaxRanks];
+  int arg[2][kMaxRanks];
+};
+__device__ __forceinline__ void hand_out(Exchange& e, int turn, int rank, int to, double sum, float top, int arg) {
+  const uint32_t s = map_shared_rank(smem_u32(&e.sum[turn][rank]), to),
+                 t = map_shared_rank(smem_u32(&e.top[turn][rank]), to),
+                 a = map_shared_rank(smem_u32(&e.arg[turn][rank]), to);
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(s), "d"(sum) : "memory");
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(t), "f"(top) : "memory");
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(arg) : "memory");
+}
+
+// A request's tree in shared memory, and the path through it.
+struct Walk {
+  int32_t up[AIOSB_TREE_MAX_NODES];
+  int32_t path[AIOSB_TREE_MAX_NODES];
+  int32_t child[AIOSB_TREE_MAX_NODES];  // the current node's children
+  uint32_t on_path[AIOSB_TREE_MAX_NODES / 32];
+  int children;
+};
+__device__ __forceinline__ void list_children(Walk& w, int cur, int n) {  // one warp
+  const int lane = threadIdx.x & 31;
+  int count = 0;
+  for (int j0 = (cur + 1) & ~31; j0 < n; j0 += 32) {
+    const int j = j0 + lane;
+    const bool is = j > cur && j < n && w.up[j] == cur;
+    const unsigned some = __ballot_sync(0xffffffffu, is);
+    if (is) w.child[count + __popc(some & ((1u << lane) - 1))] = j;
+    count += __popc(some);
+  }
+  if (lane == 0) w.children = count;
+}
+// Writes the path, then the other nodes; one warp.
+__device__ __forceinline__ void write_order(const Walk& w, int depth, int n, int all, int32_t* order) {
+  const int lane = threadIdx.x & 31;
+  for (int i = lane; i <= depth; i += 32) order[i] = w.path[i];
+  int at = depth + 1;
+  for (int j0 = 0; j0 < all; j0 += 32) {
+    const int j = j0 + lane;
+    const bool rest = j < all && !(j < n && ((w.on_path[j >> 5] >> (j & 31)) & 1));
+    const unsigned some = __ballot_sync(0xffffffffu, rest);
+    if (rest) order[at + __popc(some & ((1u << lane) - 1))] = j;
+    at += __popc(some);
+  }
+}
+
+struct TreeRows {
+  int start, n, all;
+};
+// Request r's rows; false: it has none, and its outputs are written.
+__device__ __forceinline__ bool tree_rows(const VerifyArgs& a, int r, bool first, TreeRows& t) {
+  const int s = a.tree_start[r], e = a.tree_start[r + 1];
+  t.start = min(max(s, 0), a.tokens);
+  t.all = min(max(e, t.start), a.tokens) - t.start;
+  t.n = min(t.all, AIOSB_TREE_MAX_NODES);
+  if (first && (s < 0 || e < s || e > a.tokens || t.all > t.n)) report(a.status, AIOSB_DEV_TREE_RANGE);
+  if (t.n == 0 && first) {
+    a.accepted[r] = 0;
+    a.next_token[r] = -1;
+  }
+  return t.n > 0;
+}
+
+// Greedy: a node's argmax decides. A cluster per request; each warp looks through every (ranks x warps)th block.
+template <typename T>
+__global__ void __launch_bounds__(kVerifyThreads) verify_greedy_kernel(const VerifyArgs a) {
+  __shared__ Walk walk;
+  __shared__ Exchange ex;
+  __shared__ float warp_top[kVerifyWarps];
+  __shared__ int warp_arg[kVerifyWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int ranks = a.ranks, rank = (int)cluster_ctarank(), r = blockIdx.x / ranks;
   pdl_enter();
-
-  const int s0 = a.tree_start[r], e0 = a.tree_start[r + 1];
-  const int start = min(max(s0, 0), a.tokens), all = min(max(e0, start), a.tokens) - start;
-  const int n = min(all, AIOSB_TREE_MAX_NODES);
-  const bool first = rank == 0 && threadIdx.x == 0;
-  if (first && (s0 < 0 || e0 < s0 || e0 > a.tokens || all > n)) report(a.status, AIOSB_DEV_TREE_RANGE);
-  if (n == 0) {  // the whole cluster leaves
-    if (first) {
-      a.accepted[r] = 0;
-      a.next_token[r] = -1;
-    }
-    return;
-  }
-  const int32_t* const parents = a.parents + start;
-  const int run = (a.vocab + ranks * kVerifyWarps - 1) / (ranks * kVerifyWarps);
-  const int lo = min((rank * kVerifyWarps + warp) * run, a.vocab), hi = min(lo + run, a.vocab);
-
-  int turn = 0;
-  // Every CTA's value to every CTA; the buffers take turns, so that one barrier per exchange is enough:
-  // a CTA writes a buffer again only behind the next barrier, which all have reached after reading it.
-  auto exchange_max = [&](float v, int arg) {
-    if (threadIdx.x < ranks) {
-      const uint32_t m = map_shared_rank(smem_u32(&peer_max[turn][rank]), threadIdx.x);
-      const uint32_t g = map_shared_rank(smem_u32(&peer_arg[turn][rank]), threadIdx.x);
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(m), "f"(v) : "memory");
-      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(g), "r"(arg) : "memory");
-    }
-    cluster_sync();
-  };
-  // Sums each warp's `mine` within the CTA (in run_sum) and exchanges the CTAs' sums; the total.
-  auto exchange_sum = [&](double mine) {
-    mine = warp_sum_f64(mine);
-    __syncthreads();
-    if (lane == 0) run_sum[warp] = mine;
-    __syncthreads();
-    if (threadIdx.x < ranks) {
-      double v = 0;
-      for (int w = 0; w < kVerifyWarps; ++w) v += run_sum[w];
-      const uint32_t p = map_shared_rank(smem_u32(&peer_sum[turn][rank]), threadIdx.x);
-      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(p), "d"(v) : "memory");
-    }
-    cluster_sync();
-    double total = 0;
-    for (int c = 0; c < ranks; ++c) total += peer_sum[turn][c];
-    turn ^= 1;
-    return total;
-  };
-
-  int cur = 0, depth = 0;
-  int64_t token = -1;   // valid in the CTA (and by all of its threads) that writes it
-  bool writes = false;
-  if (threadIdx.x < AIOSB_TREE_MAX_NODES / 32) on_path[threadIdx.x] = threadIdx.x == 0 ? 1u : 0u;
-  if (threadIdx.x == 0) path[0] = 0;
+  TreeRows t;
+  if (!tree_rows(a, r, rank == 0 && threadIdx.x == 0, t)) return;  // the whole cluster leaves
+  for (int i = threadIdx.x; i < t.n; i += kVerifyThreads) walk.up[i] = a.parents[t.start + i];
+  if (threadIdx.x < AIOSB_TREE_MAX_NODES / 32) walk.on_path[threadIdx.x] = threadIdx.x == 0 ? 1u : 0u;
+  if (threadIdx.x == 0) walk.path[0] = 0;
   cluster_sync();  // every CTA runs: its shared memory may be written
 
+  int cur = 0, depth = 0, turn = 0;
+  int64_t token = -1;
   for (;;) {
-    const T* const row = reinterpret_cast<const T*>(a.logits) + (int64_t)(start + cur) * a.logits_stride;
-    const float* const q = PROBS ? a.probs + (int64_t)(start + cur) * a.probs_stride : nullptr;
-    // ---- the row's maximum (and where it is first)
+    const T* const row = reinterpret_cast<const T*>(a.logits) + (int64_t)(t.start + cur) * a.logits_stride;
+    const bool vec = lies_on_16(row);
     float top = -INFINITY;
     int arg = INT32_MAX;
-    for (int v = lo + lane; v < hi; v += 32) {
-      const float x = load_logit(row + v);
-      if (GREEDY && x > top) arg = v;
-      top = max_nan(top, x);
-    }
+    // ids ascend within a lane, so that the first of equal ones stays
+#pragma unroll 4
+    for (int base = (rank * kVerifyWarps + warp) * kBlockIds; base < a.vocab;
+         base += ranks * kVerifyWarps * kBlockIds) {
+      const Ids ids(base, a.vocab, vec, lane);
+      float x[8];
+      load_ids(row, vec, ids, -INFINITY, x);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float x = __shfl_xor_sync(0xffffffffu, top, o);
-      const int b = __shfl_xor_sync(0xffffffffu, arg, o);
-      if (GREEDY) arg = x > top ? b : x == top ? min(arg, b) : arg;
+      for (int j = 0; j < 8; ++j) {
+        if (x[j] > top) arg = ids[j];
+        top = max_nan(top, x[j]);
+      }
+    }
+    auto join = [&](float x, int b) {
+      arg = x > top ? b : x == top ? min(arg, b) : arg;
       top = max_nan(top, x);
-    }
-    __syncthreads();
+    };
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) join(__shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, arg, o));
     if (lane == 0) {
-      run_max[warp] = top;
-      run_arg[warp] = arg;
+      warp_top[warp] = top;
+      warp_arg[warp] = arg;
     }
     __syncthreads();
-    top = run_max[0];
-    arg = run_arg[0];
-    for (int w = 1; w < kVerifyWarps; ++w) {
-      if (run_max[w] > top) arg = run_arg[w];
-      top = max_nan(top, run_max[w]);
+    if (warp == 0) {
+      top = lane < kVerifyWarps ? warp_top[lane] : -INFINITY;
+      arg = lane < kVerifyWarps ? warp_arg[lane] : INT32_MAX;
+#pragma unroll
+      for (int o = kVerifyWarps / 2; o > 0; o >>= 1)
+        join(__shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, arg, o));
+      if (lane < ranks) hand_out(ex, turn, rank, lane, 0.0, top, arg);
+      list_children(walk, cur, t.n);
     }
-    exchange_max(top, arg);
-    top = peer_max[turn][0];
-    arg = peer_arg[turn][0];
-    for (int c = 1; c < ranks; ++c) {
-      if (peer_max[turn][c] > top) arg = peer_arg[turn][c];
-      top = max_nan(top, peer_max[turn][c]);
-    }
+    cluster_sync();
+    top = ex.top[turn][0];
+    arg = ex.arg[turn][0];
+    for (int c = 1; c < ranks; ++c) join(ex.top[turn][c], ex.arg[turn][c]);
     turn ^= 1;
-    if (!(top > -INFINITY) || (!GREEDY && top == INFINITY)) {  // NaN, -inf only, or +inf
-      if (first) report(a.status, AIOSB_DEV_NO_DISTRIBUTION);
-      writes = rank == 0;
+    if (!(top > -INFINITY)) {  // NaN, or -inf only
+      if (rank == 0 && threadIdx.x == 0) report(a.status, AIOSB_DEV_NO_DISTRIBUTION);
       break;
     }
-
-    // ---- r(v) as it stands: p(v) behind the subtractions so far
-    double inv_z = 1;
-    int cuts = 0;  // entries of scale_by or rejected
-    auto weight = [&](int v) {
-      double x = exp((double)(load_logit(row + v) - top) * a.inv_temperature) * inv_z;
-      if (PROBS) {
-        const double qv = cuts > 0 ? (double)q[v] : 0.0;
-        for (int i = 0; i < cuts; ++i) x = fmax(x * scale_by[i] - qv, 0.0);
-      } else {
-        for (int i = 0; i < cuts; ++i)
-          if (rejected[i] == v) x = 0;
+    int found = INT32_MAX;
+    for (int i = threadIdx.x & 31; i < walk.children; i += 32) {
+      const int64_t x = a.draft_tokens[t.start + walk.child[i]];
+      if (x < 0 || x >= a.vocab) {
+        if (rank == 0) report(a.status, AIOSB_DEV_TOKEN_RANGE);
+      } else if (x == arg) {
+        found = min(found, walk.child[i]);
       }
-      return x;
-    };
-    auto sum_run = [&]() {
-      double part = 0;
-      for (int v = lo + lane; v < hi; v += 32) part += weight(v);
-      return part;
-    };
-    double total = 1;
-    if (!GREEDY) {
-      const double z = exchange_sum(sum_run());
-      inv_z = 1.0 / z;
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) found = min(found, __shfl_xor_sync(0xffffffffu, found, o));
+    if (found == INT32_MAX) {
+      token = arg;
+      break;
+    }
+    cur = found;
+    ++depth;
+    __syncthreads();  // the children have been read
+    if (threadIdx.x == 0) {
+      walk.path[depth] = cur;
+      walk.on_path[cur >> 5] |= 1u << (cur & 31);
+    }
+  }
+  if (rank != 0 || warp != 0) return;
+  __syncwarp();
+  if (lane == 0) {
+    a.accepted[r] = depth;
+    a.next_token[r] = token;
+  }
+  write_order(walk, depth, t.n, t.all, a.order + t.start);
+}
 
-    // ---- its children, in ascending order
-    int found = -1, child = cur;
-    while (found < 0) {
-      __syncthreads();
-      if (warp == 0) {
-        int c = INT32_MAX;
-        for (int j = child + 1 + lane; j - lane < n; j += 32) {
-          const unsigned hit = __ballot_sync(0xffffffffu, j < n && parents[j] == cur);
-          if (hit) {
-            c = j - lane + __ffs(hit) - 1;
-            break;
+// Sampling. A cluster per request walks its tree from the root. The vocabulary is cut into one run of ids per warp
+// of the cluster, in ascending order, and a node's weights r stay in shared memory in fp64 while its children are
+// tried, so that a row is read once. A pass leaves each warp the sum of its run and each CTA the sum of its warps';
+// a token is found by these sums from the outside in. Sums are taken in a fixed order, in fp64: what is accepted or
+// drawn hangs on comparisons of them.
+template <typename T, bool PROBS>
+__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs a) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  double* const weights = reinterpret_cast<double*>(smem_raw);
+  __shared__ Walk walk;
+  __shared__ Exchange ex;
+  __shared__ double table[kExpTable];
+  __shared__ double child_r[AIOSB_TREE_MAX_NODES];  // the children's r, and what they were drawn with
+  __shared__ float child_q[AIOSB_TREE_MAX_NODES], child_u[AIOSB_TREE_MAX_NODES];
+  __shared__ int32_t child_x[AIOSB_TREE_MAX_NODES];  // their tokens; -1: none of the vocabulary
+  __shared__ double warp_sum_of[kVerifyWarps];
+  __shared__ float warp_top[kVerifyWarps];
+  __shared__ double factor[kMaxRanks];  // of the ranks' weights: they are stored over the rank's own maximum
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int ranks = a.ranks, rank = (int)cluster_ctarank(), r = blockIdx.x / ranks;
+  if (threadIdx.x < kExpTable) table[threadIdx.x] = exp2((double)threadIdx.x / kExpTable);
+  pdl_enter();
+  TreeRows t;
+  const bool first = rank == 0 && threadIdx.x == 0;
+  if (!tree_rows(a, r, first, t)) return;  // the whole cluster leaves
+  for (int i = threadIdx.x; i < t.n; i += kVerifyThreads) walk.up[i] = a.parents[t.start + i];
+  if (threadIdx.x < AIOSB_TREE_MAX_NODES / 32) walk.on_path[threadIdx.x] = threadIdx.x == 0 ? 1u : 0u;
+  if (threadIdx.x == 0) walk.path[0] = 0;
+  cluster_sync();  // every CTA runs: its shared memory may be written
+
+  const double scale = a.inv_temperature * (1.4426950408889634 * kExpTable);
+  const int per_rank = a.run * kVerifyWarps, rank_lo = rank * per_rank;
+  const int lo = min(rank_lo + warp * a.run, a.vocab), hi = min(rank_lo + (warp + 1) * a.run, a.vocab);
+  // one place of padding to eight keeps a lane's eight consecutive ids off one bank
+  auto at = [&](int v) -> double& { return weights[(v - rank_lo) + ((v - rank_lo) >> 3)]; };
+
+  int turn = 0, cur = 0, depth = 0, last_turn = 0;
+  // The sums of the warps' runs within the CTA, then of the CTAs (ex.sum, in rank order); `top` goes along.
+  auto exchange = [&](double mine, float top) {
+    mine = warp_sum_f64(mine);
+    __syncthreads();
+    if (lane == 0) warp_sum_of[warp] = mine;
+    __syncthreads();
+    if (warp == 0) {
+      double v = 0;
+#pragma unroll
+      for (int w = 0; w < kVerifyWarps; ++w) v += warp_sum_of[w];
+      if (lane < ranks) hand_out(ex, turn, rank, lane, v, top, 0);
+    }
+    cluster_sync();
+    last_turn = turn;
+    turn ^= 1;
+  };
+  auto total_sum = [&] {
+    double v = 0;
+    for (int c = 0; c < ranks; ++c) v += ex.sum[last_turn][c];
+    return v;
+  };
+
+  for (;;) {
+    const T* const row = reinterpret_cast<const T*>(a.logits) + (int64_t)(t.start + cur) * a.logits_stride;
+    const float* const q = PROBS ? a.probs + (int64_t)(t.start + cur) * a.probs_stride : nullptr;
+    const bool vec = lies_on_16(row), vec_q = PROBS && vec && lies_on_16(q);
+    if (warp == 0) list_children(walk, cur, t.n);
+    // ---- the row, as it is, to its place; its maximum
+    float top = -INFINITY;
+#pragma unroll 2
+    for (int base = lo; base < hi; base += kBlockIds) {
+      const Ids ids(base, hi, vec, lane);
+      float x[8];
+      load_ids(row, vec, ids, -INFINITY, x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        top = max_nan(top, x[j]);
+        if (ids[j] < hi) *reinterpret_cast<float*>(&at(ids[j])) = x[j];
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) warp_top[warp] = top;
+    __syncthreads();
+    top = lane < kVerifyWarps ? warp_top[lane] : -INFINITY;
+#pragma unroll
+    for (int o = kVerifyWarps / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = __shfl_sync(0xffffffffu, top, 0);
+    // ---- the children's logits and probabilities are asked for meanwhile
+    const int children = walk.children;
+    for (int i = threadIdx.x; i < children; i += kVerifyThreads) {
+      const int64_t x = a.draft_tokens[t.start + walk.child[i]];
+      const bool in = x >= 0 && x < a.vocab;
+      if (!in && rank == 0) report(a.status, AIOSB_DEV_TOKEN_RANGE);
+      *reinterpret_cast<float*>(&child_r[i]) = in ? load_logit(row + x) : -INFINITY;
+      child_x[i] = in ? (int32_t)x : -1;
+      child_u[i] = a.accept_u[t.start + walk.child[i]];
+      if (PROBS) child_q[i] = in ? q[x] : 0.f;
+    }
+    // ---- weights over this CTA's maximum
+    double part = 0;
+    const double mine = top;
+#pragma unroll 1
+    for (int base = lo; base < hi; base += kBlockIds) {
+      const Ids ids(base, hi, vec, lane);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (ids[j] >= hi) continue;
+        double& w = at(ids[j]);
+        const float x = *reinterpret_cast<const float*>(&w);
+        // a CTA whose maximum is no number or infinite ends the walk below
+        const double e = x == -INFINITY ? 0.0 : exp_table((double)x - mine, scale, table);
+        w = e;
+        part += e;
+      }
+    }
+    exchange(part, top);
+    float most = -INFINITY;
+    for (int c = 0; c < ranks; ++c) most = max_nan(most, ex.top[last_turn][c]);
+    if (!(fabsf(most) < INFINITY)) {  // NaN, -inf only, or +inf
+      if (first) {
+        report(a.status, AIOSB_DEV_NO_DISTRIBUTION);
+        a.next_token[r] = -1;
+      }
+      break;
+    }
+    if (warp == 0) {
+      double f = 0, z = 0;
+      if (lane < ranks && ex.top[last_turn][lane] > -INFINITY) {
+        f = exp_table((double)ex.top[last_turn][lane] - (double)most, scale, table);
+        z = f * ex.sum[last_turn][lane];
+      }
+      z = warp_sum_f64(z);
+      if (lane < ranks) factor[lane] = f / z;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < children; i += kVerifyThreads) {
+      const float x = *reinterpret_cast<const float*>(&child_r[i]);
+      double p = 0;
+      if (x != -INFINITY) {
+        const int owner = child_x[i] / per_rank;
+        p = exp_table((double)x - (double)ex.top[last_turn][owner], scale, table) * factor[owner];
+      }
+      child_r[i] = p;
+    }
+    __syncthreads();
+
+    // ---- the children, in ascending order. r(v) is weights(v) * mult, behind `pending`, the last subtraction
+    double mult = factor[rank], pending = 0, total = 1;
+    bool stale = false;  // the runs' sums are not r's
+    int found = -1;
+    for (int i = 0; i < children; ++i) {
+      const double rx = child_r[i], qx = PROBS ? (double)child_q[i] : 1.0;
+      if ((double)child_u[i] * qx * total < rx) {
+        found = walk.child[i];
+        break;
+      }
+      const int x = child_x[i];
+      if (x < 0) continue;
+      if (PROBS) {
+        const double inv = 1.0 / total;
+        part = 0;
+#pragma unroll 1
+        for (int base = lo; base < hi; base += kBlockIds) {
+          const Ids ids(base, hi, vec, lane);
+          float qv[8];
+          load_ids(q, vec_q, ids, 0.f, qv);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (ids[j] >= hi) continue;
+            double& w = at(ids[j]);
+            double v = w * mult;
+            if (pending != 0) v = fmax(fma(v, pending, -(double)qv[j]), 0.0);
+            w = v;
+            part += fmax(fma(v, inv, -(double)qv[j]), 0.0);
           }
         }
-        if (lane == 0) next_child = c;
-      }
-      __syncthreads();
-      child = next_child;
-      if (child >= n) break;
-      const int64_t x = a.draft_tokens[start + child];
-      if (x < 0 || x >= a.vocab) {
-        if (first) report(a.status, AIOSB_DEV_TOKEN_RANGE);
-        continue;
-      }
-      if (GREEDY) {
-        if (x == arg) found = child;
-        continue;
-      }
-      const double rx = weight((int)x), qx = PROBS ? (double)q[x] : 1.0;
-      if ((double)a.accept_u[start + child] * qx * total < rx) {
-        found = child;
-      } else if (PROBS) {
-        __syncthreads();
-        if (threadIdx.x == 0) scale_by[cuts] = 1.0 / total;
-        __syncthreads();
-        ++cuts;
-        const double left = exchange_sum(sum_run());
-        if (left > 0) total = left;
-        else --cuts;
-      } else {
-        __syncthreads();
-        if (threadIdx.x == 0) rejected[cuts] = x;
-        __syncthreads();
-        if (rx > 0) {
-          ++cuts;
-          total -= rx;
+        mult = 1;
+        exchange(part, 0.f);
+        const double left = total_sum();
+        pending = left > 0 ? inv : 0;  // where nothing is left r stays
+        stale = !(left > 0);
+        if (left > 0) {
+          total = left;
+          for (int c = threadIdx.x; c < children; c += kVerifyThreads)
+            child_r[c] = fmax(fma(child_r[c], inv, -(double)child_q[c]), 0.0);
+          __syncthreads();
         }
+      } else if (rx > 0) {
+        __syncthreads();
+        for (int c = threadIdx.x; c < children; c += kVerifyThreads)
+          if (child_x[c] == x) child_r[c] = 0;
+        if (threadIdx.x == 0 && x >= rank_lo && x < rank_lo + per_rank) at(x) = 0;
+        total -= rx;
+        stale = true;
+        __syncthreads();
       }
     }
     if (found >= 0) {
       cur = found;
       ++depth;
+      __syncthreads();  // the children have been read
       if (threadIdx.x == 0) {
-        path[depth] = cur;
-        on_path[cur >> 5] |= 1u << (cur & 31);
+        walk.path[depth] = cur;
+        walk.on_path[cur >> 5] |= 1u << (cur & 31);
       }
       continue;
     }
 
     // ---- the next token
-    if (GREEDY) {
-      token = arg;
-      writes = rank == 0;
-      break;
+    auto weight = [&](int v) {
+      double w = at(v) * mult;
+      if (PROBS && pending != 0) w = fmax(fma(w, pending, -(double)q[v]), 0.0);
+      return w;
+    };
+    if (stale) {
+      part = 0;
+      for (int v = lo + lane; v < hi; v += 32) part += weight(v);
+      exchange(part, 0.f);
     }
-    total = exchange_sum(sum_run());  // in the order of the search below
-    const double target = (double)a.sample_u[r] * total;
-    double before = 0;
+    // the first pass's sums are over the ranks' own maxima, later ones are r's
+    const bool direct = stale || pending != 0;
+    auto rank_sum = [&](int c) { return ex.sum[last_turn][c] * (direct ? 1.0 : factor[c]); };
+    double target = 0, before = 0, owner_before = 0;
+    for (int c = 0; c < ranks; ++c) target += rank_sum(c);
+    target *= (double)a.sample_u[r];
+    // the first whose end lies past the target; the last with any weight, should rounding leave none
     int owner = -1;
-    double owner_before = 0;
     for (int c = 0; c < ranks; ++c) {
-      const double w = peer_sum[turn ^ 1][c];
+      const double w = rank_sum(c);
       if (w > 0) {
         owner = c;
         owner_before = before;
@@ -308,69 +543,79 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
       }
       before += w;
     }
-    writes = owner == rank;
-    if (writes) {
-      before = owner_before;
+    if (owner == rank) {
       int own_warp = -1;
-      double warp_before = before;
+      double warp_before = owner_before;
+      before = owner_before;
       for (int w = 0; w < kVerifyWarps; ++w) {
-        if (run_sum[w] > 0) {
+        const double x = warp_sum_of[w] * (direct ? 1.0 : mult);
+        if (x > 0) {
           own_warp = w;
           warp_before = before;
-          if (before + run_sum[w] > target) break;
+          if (before + x > target) break;
         }
-        before += run_sum[w];
+        before += x;
       }
       if (warp == own_warp) {
         before = warp_before;
         int pick = -1;
-        for (int v0 = lo; v0 < hi; v0 += 32) {
-          const double x = v0 + lane < hi ? weight(v0 + lane) : 0.0;
-          double c = x;
+        for (int base = lo; base < hi; base += kBlockIds) {
+          const Ids ids(base, hi, true, lane);
+          double sum = 0;
+          int last = -1;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const double w = ids[j] < hi ? weight(ids[j]) : 0.0;
+            if (w > 0) last = ids[j];
+            sum += w;
+          }
+          double upto = sum;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
-            const double y = __shfl_up_sync(0xffffffffu, c, o);
-            if (lane >= o) c += y;
+            const double y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
           }
-          const unsigned some = __ballot_sync(0xffffffffu, x > 0);
-          const unsigned past = __ballot_sync(0xffffffffu, x > 0 && before + c > target);
+          const unsigned some = __ballot_sync(0xffffffffu, last >= 0);
+          const unsigned past = __ballot_sync(0xffffffffu, last >= 0 && before + upto > target);
           if (past) {
-            pick = v0 + __ffs(past) - 1;
+            const int l = __ffs(past) - 1;
+            if (lane == l) {
+              double c = before + (upto - sum);
+              pick = last;
+              for (int j = 7; j >= 0; --j) {  // the first one past the target, from the back
+                double e = c;
+                for (int i = 0; i <= j; ++i) e += ids[i] < hi ? weight(ids[i]) : 0.0;
+                if (ids[j] < hi && weight(ids[j]) > 0 && e > target) pick = ids[j];
+              }
+            }
+            pick = __shfl_sync(0xffffffffu, pick, l);
             break;
           }
-          if (some) pick = v0 + 31 - __clz(some);  // the last one, should rounding leave the target past it
-          before += __shfl_sync(0xffffffffu, c, 31);
+          if (some) pick = __shfl_sync(0xffffffffu, last, 31 - __clz(some));
+          before += __shfl_sync(0xffffffffu, upto, 31);
         }
         if (lane == 0) a.next_token[r] = pick;
       }
     }
-    token = -2;  // written above
     break;
   }
 
   __syncthreads();
-  if (writes && token != -2 && threadIdx.x == 0) a.next_token[r] = token;
-  if (rank != 0) return;
-  if (threadIdx.x == 0) a.accepted[r] = depth;
-  if (warp == 0) {
-    int32_t* const order = a.order + start;
-    for (int i = lane; i <= depth; i += 32) order[i] = path[i];
-    int at = depth + 1;
-    for (int j0 = 0; j0 < all; j0 += 32) {
-      const int j = j0 + lane;
-      const bool rest = j < all && !(j < n && ((on_path[j >> 5] >> (j & 31)) & 1));
-      const unsigned some = __ballot_sync(0xffffffffu, rest);
-      if (rest) order[at + __popc(some & ((1u << lane) - 1))] = j;
-      at += __popc(some);
-    }
-  }
+  if (rank != 0 || warp != 0) return;
+  if (lane == 0) a.accepted[r] = depth;
+  write_order(walk, depth, t.n, t.all, a.order + t.start);
 }
 
-template <typename T, bool GREEDY, bool PROBS>
-cudaError_t launch_verify(const VerifyArgs& a, int requests, cudaStream_t stream) {
+template <typename Kernel>
+cudaError_t launch_cluster(Kernel kernel, const VerifyArgs& a, int requests, size_t smem, cudaStream_t stream) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess && a.ranks > 8)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(requests * a.ranks));
   cfg.blockDim = dim3(kVerifyThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -381,14 +626,32 @@ cudaError_t launch_verify(const VerifyArgs& a, int requests, cudaStream_t stream
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, verify_kernel<T, GREEDY, PROBS>, a);
+  return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
+constexpr size_t kWeightBytes = 190 * 1024;  // beside the static shared memory
+constexpr int kMaxSampleVocab = 327680;
+
+int warp_run(int vocab, int ranks) {
+  const int blocks = (vocab + kBlockIds - 1) / kBlockIds, warps = ranks * kVerifyWarps;
+  return (blocks + warps - 1) / warps * kBlockIds;
+}
+size_t weight_bytes(int run) { return (size_t)run * kVerifyWarps * 9; }
+
 template <typename T>
-cudaError_t launch_verify(const VerifyArgs& a, int requests, bool greedy, cudaStream_t stream) {
-  if (greedy) return launch_verify<T, true, false>(a, requests, stream);
-  if (a.probs != nullptr) return launch_verify<T, false, true>(a, requests, stream);
-  return launch_verify<T, false, false>(a, requests, stream);
+cudaError_t launch_verify(VerifyArgs a, int requests, bool greedy, cudaStream_t stream) {
+  a.ranks = 1;
+  const int sms = sm_count();
+  // more CTAs to a request while they find SMs, and two blocks to each of their warps
+  while (a.ranks < 8 && (int64_t)requests * a.ranks * 2 <= sms && a.vocab >= a.ranks * 2 * kVerifyWarps * kBlockIds)
+    a.ranks *= 2;
+  if (greedy) return launch_cluster(verify_greedy_kernel<T>, a, requests, 0, stream);
+  // two CTAs to an SM if the weights allow it
+  while (a.ranks < kMaxRanks && weight_bytes(warp_run(a.vocab, a.ranks)) > kWeightBytes / 2) a.ranks *= 2;
+  a.run = warp_run(a.vocab, a.ranks);
+  const size_t smem = weight_bytes(a.run);
+  if (a.probs != nullptr) return launch_cluster(verify_kernel<T, true>, a, requests, smem, stream);
+  return launch_cluster(verify_kernel<T, false>, a, requests, smem, stream);
 }
 
 }  // namespace
@@ -418,7 +681,8 @@ extern "C" int aiosb_verify_draft(const void* logits, int logits_fp32, int64_t l
                                   int64_t* next_token, int32_t* order, int32_t* status, void* stream) {
   AIOSB_REQUIRE(tokens >= 0 && requests >= 0 && vocab >= 1 && tokens <= INT32_MAX && requests <= INT32_MAX / kMaxRanks,
                 AIOSB_ERR_INVALID_ARG, "verify_draft: bad sizes");
-  AIOSB_REQUIRE(vocab <= (1 << 30), AIOSB_ERR_UNSUPPORTED, "verify_draft: vocabulary too large");
+  AIOSB_REQUIRE(vocab <= (greedy ? 1 << 30 : kMaxSampleVocab), AIOSB_ERR_UNSUPPORTED,
+                "verify_draft: vocabulary too large (sampling: at most %d)", kMaxSampleVocab);
   AIOSB_REQUIRE(logits_stride >= vocab || tokens <= 1, AIOSB_ERR_INVALID_ARG,
                 "verify_draft: logits row stride below the vocabulary");
   AIOSB_REQUIRE(greedy || (temperature > 0 && 1.0 / temperature > 0 && 1.0 / temperature < 1e30),
@@ -450,7 +714,6 @@ extern "C" int aiosb_verify_draft(const void* logits, int logits_fp32, int64_t l
   a.next_token = next_token;
   a.order = order;
   a.status = status;
-  a.ranks = kMaxRanks;
   cudaStream_t s = as_stream(stream);
   return check_launch("verify_draft", logits_fp32 ? launch_verify<float>(a, (int)requests, greedy != 0, s)
                                                   : launch_verify<__nv_bfloat16>(a, (int)requests, greedy != 0, s));

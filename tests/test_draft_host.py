@@ -76,7 +76,8 @@ def test_verify_draft_refuses() -> None:
     _refused(name, good, INV, "bad sizes", tokens=-1)
     _refused(name, good, INV, "bad sizes", vocab=0)
     _refused(name, good, INV, "bad sizes", requests=1 << 29)
-    _refused(name, good, UNS, "too large", vocab=1 << 31, ls=1 << 31)
+    _refused(name, good, UNS, "too large", vocab=327681, ls=327681)
+    _refused(name, good, UNS, "too large", vocab=1 << 31, ls=1 << 31, greedy=1)
     _refused(name, good, INV, "logits row stride", ls=99)
     _refused(name, good, INV, "temperature", temperature=0.0)
     _refused(name, good, INV, "temperature", temperature=-1.0)

@@ -130,7 +130,7 @@ def test_verify(cuda_device, sizes, vocab: int, mode: str) -> None:
     ops.check_status(cuda_device)
 
 
-@pytest.mark.parametrize("vocab", [50021, 131072, 151111])
+@pytest.mark.parametrize("vocab", [50021, 131072, 151111, 262144, 327680])
 @pytest.mark.parametrize("probs", [False, True])
 def test_verify_large_vocabularies(cuda_device, vocab: int, probs: bool) -> None:
     sizes = [12, 7, 1]
