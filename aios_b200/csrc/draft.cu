@@ -122,25 +122,36 @@ __device__ __forceinline__ bool lies_on_16(const V* row) {
   return (reinterpret_cast<uintptr_t>(row) & 15u) == 0;
 }
 
-// 2^(i / 128) for the exponential below.
-constexpr int kExpTable = 128;
-// e^(d / T) in fp64 for d <= 0, off by about 2^-49: d / (T ln 2) = k / 128 + f / 128 with |f| <= 1/2, 2^(k / 128)
-// from the table and k's upper bits, and 2^(f / 128) by its series to the fourth power (table-driven exponentials:
-// P. T. P. Tang, ACM TOMS 15, 1989). Eleven fp64 instructions, where the general function takes some thirty and its
-// passes over the vocabulary bound the kernel. scale: 128 / (T ln 2). Below 2^-1000 it is 0.
-__device__ __forceinline__ double exp_table(double d, double scale, const double* table) {
-  const double t = d * scale;
-  if (!(t > -128000.0)) return 0.0;
+// An fp32 value's bits as an fp64 one: the conversion instruction runs at an eighth of the fp64 rate. 0 and subnormals
+// come out as values of 2^-127 or so, infinities and NaN as ones of 2^128.
+__device__ __forceinline__ double widen(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return __hiloint2double((int)((((u >> 3) & 0x0FFFFFFFu) + 0x38000000u) | (u & 0x80000000u)), (int)(u << 29));
+}
+
+// 2^(i / 16) for the exponential below: sixteen doubles are all of the banks once, so that no two lanes' entries
+// conflict (a table of 128 cost as much as the arithmetic).
+constexpr int kExpTable = 16;
+// e^((x - m) / T) in fp64 for x <= m, off by about 2^-50: (x - m) / (T ln 2) = (k + f) / 16 with |f| <= 1/2, 2^(k / 16)
+// from the table and k's upper bits, and 2^(f / 16) by its series to the sixth power (table-driven exponentials:
+// P. T. P. Tang, ACM TOMS 15, 1989). Eleven fp64 instructions, where the general function takes some thirty.
+// scale: 16 / (T ln 2); base: m * scale. Below 2^-1000, and for x of -inf, it is 0.
+__device__ __forceinline__ double exp_table(double x, double scale, double base, const double* table) {
+  double t = fma(x, scale, -base);
+  const bool none = (uint32_t)__double2hiint(t) >= 0xC0CF4000u;  // t <= -16000
+  if (none) t = 0;
   const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are round(t)
   const double s = t + magic, f = t - (s - magic);
   const int k = __double2loint(s);
-  constexpr double c = 0.0054152123481245727;  // ln 2 / 128
-  double p = fma(f, c * c * c * c / 24, c * c * c / 6);
+  constexpr double c = 0.043321698784996581;  // ln 2 / 16
+  double p = fma(f, c * c * c * c * c * c / 720, c * c * c * c * c / 120);
+  p = fma(f, p, c * c * c * c / 24);
+  p = fma(f, p, c * c * c / 6);
   p = fma(f, p, c * c / 2);
   p = fma(f, p, c);
   const double b = table[k & (kExpTable - 1)];
   const double r = fma(b, f * p, b);
-  return __hiloint2double(__double2hiint(r) + ((k >> 7) << 20), __double2loint(r));
+  return none ? 0.0 : __hiloint2double(__double2hiint(r) + ((k >> 4) << 20), __double2loint(r));
 }
 
 // Values that the CTAs of a cluster hand to one another; the buffers take turns, so that one barrier an exchange is
@@ -321,11 +332,12 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
   __shared__ Exchange ex;
   __shared__ double table[kExpTable];
   __shared__ double child_r[AIOSB_TREE_MAX_NODES];  // the children's r, and what they were drawn with
-  __shared__ float child_q[AIOSB_TREE_MAX_NODES], child_u[AIOSB_TREE_MAX_NODES];
-  __shared__ int32_t child_x[AIOSB_TREE_MAX_NODES];  // their tokens; -1: none of the vocabulary
+  __shared__ float child_q[AIOSB_TREE_MAX_NODES], node_u[AIOSB_TREE_MAX_NODES];
+  __shared__ int32_t node_x[AIOSB_TREE_MAX_NODES];  // the nodes' tokens; -1: none of the vocabulary
   __shared__ double warp_sum_of[kVerifyWarps];
   __shared__ float warp_top[kVerifyWarps];
   __shared__ double factor[kMaxRanks];  // of the ranks' weights: they are stored over the rank's own maximum
+  __shared__ double all_weights;
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int ranks = a.ranks, rank = (int)cluster_ctarank(), r = blockIdx.x / ranks;
@@ -334,7 +346,12 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
   TreeRows t;
   const bool first = rank == 0 && threadIdx.x == 0;
   if (!tree_rows(a, r, first, t)) return;  // the whole cluster leaves
-  for (int i = threadIdx.x; i < t.n; i += kVerifyThreads) walk.up[i] = a.parents[t.start + i];
+  for (int i = threadIdx.x; i < t.n; i += kVerifyThreads) {
+    const int64_t x = a.draft_tokens[t.start + i];
+    walk.up[i] = a.parents[t.start + i];
+    node_x[i] = x >= 0 && x < a.vocab ? (int32_t)x : -1;
+    node_u[i] = a.accept_u[t.start + i];
+  }
   if (threadIdx.x < AIOSB_TREE_MAX_NODES / 32) walk.on_path[threadIdx.x] = threadIdx.x == 0 ? 1u : 0u;
   if (threadIdx.x == 0) walk.path[0] = 0;
   cluster_sync();  // every CTA runs: its shared memory may be written
@@ -353,9 +370,9 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
     if (lane == 0) warp_sum_of[warp] = mine;
     __syncthreads();
     if (warp == 0) {
-      double v = 0;
+      double v = warp_sum_of[lane & (kVerifyWarps - 1)];
 #pragma unroll
-      for (int w = 0; w < kVerifyWarps; ++w) v += warp_sum_of[w];
+      for (int o = kVerifyWarps / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
       if (lane < ranks) hand_out(ex, turn, rank, lane, v, top, 0);
     }
     cluster_sync();
@@ -372,7 +389,16 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
     const T* const row = reinterpret_cast<const T*>(a.logits) + (int64_t)(t.start + cur) * a.logits_stride;
     const float* const q = PROBS ? a.probs + (int64_t)(t.start + cur) * a.probs_stride : nullptr;
     const bool vec = lies_on_16(row), vec_q = PROBS && vec && lies_on_16(q);
-    if (warp == 0) list_children(walk, cur, t.n);
+    if (warp == 0) {  // the children; their logits and probabilities are asked for ahead of the row's
+      list_children(walk, cur, t.n);
+      __syncwarp();
+      for (int i = lane; i < walk.children; i += 32) {
+        const int x = node_x[walk.child[i]];
+        if (x < 0 && rank == 0) report(a.status, AIOSB_DEV_TOKEN_RANGE);
+        *reinterpret_cast<float*>(&child_r[i]) = x >= 0 ? load_logit(row + x) : -INFINITY;
+        if (PROBS) child_q[i] = x >= 0 ? q[x] : 0.f;
+      }
+    }
     // ---- the row, as it is, to its place; its maximum
     float top = -INFINITY;
 #pragma unroll 2
@@ -394,32 +420,27 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
 #pragma unroll
     for (int o = kVerifyWarps / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     top = __shfl_sync(0xffffffffu, top, 0);
-    // ---- the children's logits and probabilities are asked for meanwhile
     const int children = walk.children;
-    for (int i = threadIdx.x; i < children; i += kVerifyThreads) {
-      const int64_t x = a.draft_tokens[t.start + walk.child[i]];
-      const bool in = x >= 0 && x < a.vocab;
-      if (!in && rank == 0) report(a.status, AIOSB_DEV_TOKEN_RANGE);
-      *reinterpret_cast<float*>(&child_r[i]) = in ? load_logit(row + x) : -INFINITY;
-      child_x[i] = in ? (int32_t)x : -1;
-      child_u[i] = a.accept_u[t.start + walk.child[i]];
-      if (PROBS) child_q[i] = in ? q[x] : 0.f;
-    }
     // ---- weights over this CTA's maximum
     double part = 0;
-    const double mine = top;
+    const double mine = widen(top) * scale;
 #pragma unroll 1
     for (int base = lo; base < hi; base += kBlockIds) {
       const Ids ids(base, hi, vec, lane);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (ids[j] >= hi) continue;
-        double& w = at(ids[j]);
-        const float x = *reinterpret_cast<const float*>(&w);
-        // a CTA whose maximum is no number or infinite ends the walk below
-        const double e = x == -INFINITY ? 0.0 : exp_table((double)x - mine, scale, table);
-        w = e;
-        part += e;
+      for (int j0 = 0; j0 < 8; j0 += 4) {
+        double e[4];  // four at once, without branches: they are chains of dependent fp64 instructions
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x = ids[j0 + j] < hi ? *reinterpret_cast<const float*>(&at(ids[j0 + j])) : -INFINITY;
+          // -inf gives 0; a CTA whose maximum is NaN or +inf ends the walk below
+          e[j] = exp_table(widen(x), scale, mine, table);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (ids[j0 + j] < hi) at(ids[j0 + j]) = e[j];
+          part += e[j];
+        }
       }
     }
     exchange(part, top);
@@ -433,37 +454,33 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
       break;
     }
     if (warp == 0) {
-      double f = 0, z = 0;
-      if (lane < ranks && ex.top[last_turn][lane] > -INFINITY) {
-        f = exp_table((double)ex.top[last_turn][lane] - (double)most, scale, table);
-        z = f * ex.sum[last_turn][lane];
+      const int c = lane & (kMaxRanks - 1);
+      const double f = c < ranks ? exp_table(widen(ex.top[last_turn][c]), scale, widen(most) * scale, table) : 0.0;
+      double z = c < ranks ? f * ex.sum[last_turn][c] : 0.0;
+#pragma unroll
+      for (int o = kMaxRanks / 2; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+      if (lane < ranks) factor[lane] = f;
+      if (lane == 0) all_weights = z;
+      __syncwarp();
+      for (int i = lane; i < children; i += 32) {
+        const float x = *reinterpret_cast<const float*>(&child_r[i]);
+        const int owner = max(node_x[walk.child[i]], 0) / per_rank;
+        child_r[i] = exp_table(widen(x), scale, widen(ex.top[last_turn][owner]) * scale, table) * factor[owner];
       }
-      z = warp_sum_f64(z);
-      if (lane < ranks) factor[lane] = f / z;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < children; i += kVerifyThreads) {
-      const float x = *reinterpret_cast<const float*>(&child_r[i]);
-      double p = 0;
-      if (x != -INFINITY) {
-        const int owner = child_x[i] / per_rank;
-        p = exp_table((double)x - (double)ex.top[last_turn][owner], scale, table) * factor[owner];
-      }
-      child_r[i] = p;
     }
     __syncthreads();
 
     // ---- the children, in ascending order. r(v) is weights(v) * mult, behind `pending`, the last subtraction
-    double mult = factor[rank], pending = 0, total = 1;
+    double mult = factor[rank], pending = 0, total = all_weights;
     bool stale = false;  // the runs' sums are not r's
     int found = -1;
     for (int i = 0; i < children; ++i) {
       const double rx = child_r[i], qx = PROBS ? (double)child_q[i] : 1.0;
-      if ((double)child_u[i] * qx * total < rx) {
-        found = walk.child[i];
+      const int child = walk.child[i], x = node_x[child];
+      if ((double)node_u[child] * qx * total < rx) {
+        found = child;
         break;
       }
-      const int x = child_x[i];
       if (x < 0) continue;
       if (PROBS) {
         const double inv = 1.0 / total;
@@ -475,12 +492,11 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
           load_ids(q, vec_q, ids, 0.f, qv);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            if (ids[j] >= hi) continue;
-            double& w = at(ids[j]);
-            double v = w * mult;
-            if (pending != 0) v = fmax(fma(v, pending, -(double)qv[j]), 0.0);
-            w = v;
-            part += fmax(fma(v, inv, -(double)qv[j]), 0.0);
+            double v = ids[j] < hi ? at(ids[j]) * mult : 0.0;
+            const double qj = widen(qv[j]);
+            if (pending != 0) v = fmax(fma(v, pending, -qj), 0.0);
+            if (ids[j] < hi) at(ids[j]) = v;
+            part += fmax(fma(v, inv, -qj), 0.0);
           }
         }
         mult = 1;
@@ -491,13 +507,13 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
         if (left > 0) {
           total = left;
           for (int c = threadIdx.x; c < children; c += kVerifyThreads)
-            child_r[c] = fmax(fma(child_r[c], inv, -(double)child_q[c]), 0.0);
+            child_r[c] = fmax(fma(child_r[c], inv, -widen(child_q[c])), 0.0);
           __syncthreads();
         }
       } else if (rx > 0) {
         __syncthreads();
         for (int c = threadIdx.x; c < children; c += kVerifyThreads)
-          if (child_x[c] == x) child_r[c] = 0;
+          if (node_x[walk.child[c]] == x) child_r[c] = 0;
         if (threadIdx.x == 0 && x >= rank_lo && x < rank_lo + per_rank) at(x) = 0;
         total -= rx;
         stale = true;
@@ -518,7 +534,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
     // ---- the next token
     auto weight = [&](int v) {
       double w = at(v) * mult;
-      if (PROBS && pending != 0) w = fmax(fma(w, pending, -(double)q[v]), 0.0);
+      if (PROBS && pending != 0) w = fmax(fma(w, pending, -widen(q[v])), 0.0);
       return w;
     };
     if (stale) {
@@ -561,13 +577,13 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
         int pick = -1;
         for (int base = lo; base < hi; base += kBlockIds) {
           const Ids ids(base, hi, true, lane);
-          double sum = 0;
+          double w[8], sum = 0;
           int last = -1;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const double w = ids[j] < hi ? weight(ids[j]) : 0.0;
-            if (w > 0) last = ids[j];
-            sum += w;
+            w[j] = ids[j] < hi ? weight(ids[j]) : 0.0;
+            if (w[j] > 0) last = ids[j];
+            sum += w[j];
           }
           double upto = sum;
 #pragma unroll
@@ -579,13 +595,14 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
           const unsigned past = __ballot_sync(0xffffffffu, last >= 0 && before + upto > target);
           if (past) {
             const int l = __ffs(past) - 1;
-            if (lane == l) {
-              double c = before + (upto - sum);
-              pick = last;
-              for (int j = 7; j >= 0; --j) {  // the first one past the target, from the back
-                double e = c;
-                for (int i = 0; i <= j; ++i) e += ids[i] < hi ? weight(ids[i]) : 0.0;
-                if (ids[j] < hi && weight(ids[j]) > 0 && e > target) pick = ids[j];
+            double c = before + (upto - sum);
+            pick = last;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {  // the first one past the target
+              c += w[j];
+              if (w[j] > 0 && c > target) {
+                pick = ids[j];
+                c = -INFINITY;
               }
             }
             pick = __shfl_sync(0xffffffffu, pick, l);
