@@ -31,7 +31,7 @@ constexpr int kStep = 64;       // keys of a softmax step, half a chunk
 constexpr int kSoftWarps = 8;
 constexpr int kLoadWarps = 4;
 constexpr int kMmaWarp = kSoftWarps + kLoadWarps;
-constexpr int kThreads = (kMmaWarp + 1) * 32;
+constexpr int kThreads = (kMmaWarp + 2) * 32;
 constexpr int kAtomBytes = kKeys * 128;  // 128 rows of 64 values, 128-byte swizzled
 constexpr int kUnitCost = 1;             // a unit's start and end, in chunks
 constexpr int kMinShare = 3;             // weight below which a range is not worth a CTA
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&sh.full[i], kLoadWarps * 32);
-      mbar_init(&sh.empty[i], 1);
+      mbar_init(&sh.empty[i], 2);
     }
     for (int i = 0; i < 2; ++i) {
       for (int b = 0; b < 2; ++b) {
@@ -300,9 +300,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       mbar_init(&sh.pv_done[i], 1);
     }
     mbar_init(&sh.q_full, kSoftWarps);
-    mbar_init(&sh.piece_done, 1);
+    mbar_init(&sh.piece_done, 2);
     mbar_init(&sh.state_full, kSoftWarps);
-    mbar_init(&sh.drained, 1);
+    mbar_init(&sh.drained, 2);
     sh.abort_flag = 0;
     fence_mbar_init();
   }
@@ -490,11 +490,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
       sh.abort_flag = 1;
     }
-  } else if (warp == kMmaWarp) {
-    // ---- MMAs: for each stream in turn O += P V of its last step, then S of the step after next, so that scores are
-    // there when a stream's softmax comes to them. One warp for both streams: it keeps them apart.
+  } else if (warp >= kMmaWarp) {
+    // ---- MMAs of stream s: O += P V of its last step, then S of the step after next, so that scores are there when
+    // the softmax comes to them. A warp for each stream: a wait that is over and the issue behind it take some
+    // hundred clocks of a warp, in which the other's MMAs run.
     constexpr uint32_t idesc_s = umma_idesc_bf16(kTile, kStep), idesc_o = umma_idesc_bf16(kTile, D) | kBMajorMn;
-    uint32_t base = 0, q_phase = 0, steps[2] = {0, 0};  // of a stream, in all pieces so far
+    const int s = warp - kMmaWarp;
+    uint32_t base = 0, q_phase = 0, steps = 0;  // of the stream, in all pieces so far
     bool ok = true;
     while (ok && it.next(a, p)) {
       const int n = p.c1 - p.c0;
@@ -503,73 +505,66 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       auto k_block = [&](int i) { return base + (pair ? 2 * i : i < 2 ? i : 2 * i - 1); };
       auto v_block = [&](int i) { return base + (pair ? 2 * i + 1 : i == n - 1 ? 2 * n - 1 : 2 * i + 2); };
       auto wait_block = [&](uint32_t b) { return mbar_wait(&sh.full[b % S::kStages], (b / S::kStages) & 1); };
-      ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full, q_phase));
-      q_phase ^= 1;
-      if (!ok) break;
-      // S of step h of stream s (chunk `c` of the piece); the elected lane
-      auto score = [&](int s, int h, int c) {
-        const uint32_t stage = k_block(c) % S::kStages, buffer = (steps[s] + h) & 1;
-        const uint64_t kd = umma_desc_sw128(ring + stage * S::kBlockBytes + (h & 1) * (kStep * 128)),
-                       qd = umma_desc_sw128(q_smem + (pair ? s : 0) * S::kBlockBytes);
+      // a block is free when both streams are through with it, or the only one that uses it
+      auto release = [&](uint32_t stage) {
+        tc_commit(&sh.empty[stage]);
+        if (!pair) mbar_arrive(&sh.empty[stage]);
+      };
+      // step h is half h & 1 of this chunk of the piece
+      auto chunk_of = [&](int h) { return pair ? h >> 1 : 2 * (h >> 1) + s; };
+      const uint64_t q_desc = umma_desc_sw128(q_smem + (pair ? s : 0) * S::kBlockBytes);
+      auto score = [&](int h) {  // S of step h; the elected lane
+        const uint32_t stage = k_block(chunk_of(h)) % S::kStages, buffer = (steps + h) & 1;
+        const uint64_t kd = umma_desc_sw128(ring + stage * S::kBlockBytes + (h & 1) * (kStep * 128));
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t off = ((k >> 2) * kAtomBytes + (k & 3) * 32) >> 4;
-          tc_mma_bf16(tmem + s * 128 + buffer * kStep, qd + off, kd + off, idesc_s, k > 0);
+          tc_mma_bf16(tmem + s * 128 + buffer * kStep, q_desc + off, kd + off, idesc_s, k > 0);
         }
         tc_commit(&sh.s_full[s][buffer]);
-        // the block's last reader: a wide unit's second stream, or the only one that has the chunk
-        if ((h & 1) && (!pair || s == 1)) tc_commit(&sh.empty[stage]);
+        if (h & 1) release(stage);
       };
-      // step h of stream s is half h & 1 of this chunk
-      auto chunk_of = [&](int s, int h) { return pair ? h >> 1 : 2 * (h >> 1) + s; };
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if (chunk_of(s, 0) >= n) continue;
-        ok = ok && __all_sync(0xffffffffu, wait_block(k_block(chunk_of(s, 0))));
+      ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full, q_phase));
+      q_phase ^= 1;
+      if (!ok) break;
+      if (chunk_of(0) < n) {
+        ok = __all_sync(0xffffffffu, wait_block(k_block(chunk_of(0))));
         if (ok && elect_one()) {
           fence_proxy_async_shared();  // the copies went through the generic proxy, the MMAs read through the other
-          score(s, 0, chunk_of(s, 0));
-          score(s, 1, chunk_of(s, 0));
+          score(0);
+          score(1);
         }
         __syncwarp();
       }
-      bool more = ok;
-      for (int h = 0; more; ++h) {
-        more = false;
+      int h = 0;
+      for (; ok && chunk_of(h) < n; ++h) {
+        const int next = chunk_of(h + 2);
+        const uint32_t buffer = (steps + h) & 1, vb = v_block(chunk_of(h));
+        // the blocks first: they are there before the weights, as a rule
+        ok = wait_block(vb) && (next >= n || wait_block(k_block(next))) &&
+             mbar_wait(&sh.p_full[s][buffer], ((steps + h) >> 1) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          fence_proxy_async_shared();
+          const uint32_t stage = vb % S::kStages;
+          const uint32_t v = ring + stage * S::kBlockBytes + (h & 1) * (kStep * 128);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const int c = chunk_of(s, h), next = chunk_of(s, h + 2);
-          if (c >= n || !ok) continue;
-          more = true;
-          const uint32_t buffer = (steps[s] + h) & 1;
-          // the blocks first: they are there before the weights, as a rule
-          ok = wait_block(v_block(c)) && (next >= n || wait_block(k_block(next))) &&
-               mbar_wait(&sh.p_full[s][buffer], ((steps[s] + h) >> 1) & 1);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) continue;
-          tc_fence_after();
-          if (elect_one()) {
-            fence_proxy_async_shared();
-            const uint32_t stage = v_block(c) % S::kStages;
-            const uint32_t v = ring + stage * S::kBlockBytes + (h & 1) * (kStep * 128);
-#pragma unroll
-            for (int k = 0; k < kStep / 16; ++k)
-              tc_mma_bf16_ts(tmem + 256 + s * 128, tmem + s * 128 + buffer * kStep + k * 8, umma_desc_mn(v + k * 2048),
-                             idesc_o, h > 0 || k > 0);
-            tc_commit(&sh.pv_done[s]);
-            if ((h & 1) && (!pair || s == 1)) tc_commit(&sh.empty[stage]);
-            if (next < n) score(s, h + 2, next);
-          }
-          __syncwarp();
+          for (int k = 0; k < kStep / 16; ++k)
+            tc_mma_bf16_ts(tmem + 256 + s * 128, tmem + s * 128 + buffer * kStep + k * 8, umma_desc_mn(v + k * 2048),
+                           idesc_o, h > 0 || k > 0);
+          tc_commit(&sh.pv_done[s]);
+          if (h & 1) release(stage);
+          if (next < n) score(h + 2);
         }
-        more = more && ok;
+        __syncwarp();
       }
       if (!ok) break;
       if (elect_one()) tc_commit(&sh.piece_done);
       __syncwarp();
       base += 2 * n;
-      steps[0] += pair ? 2 * n : 2 * ((n + 1) / 2);
-      steps[1] += pair ? 2 * n : 2 * (n / 2);
+      steps += h;
     }
     if (!ok) {
       report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
@@ -763,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
 
   tc_fence_before();
   __syncthreads();
-  if (sh.abort_flag && warp == kMmaWarp) {  // MMAs may still run: their end is waited for
+  if (sh.abort_flag && warp >= kMmaWarp) {  // MMAs may still run: their end is waited for
     if (elect_one()) tc_commit(&sh.drained);
     __syncwarp();
     mbar_wait(&sh.drained, 0);
