@@ -35,7 +35,7 @@ constexpr int kThreads = (kMmaWarp + 2) * 32;
 constexpr int kAtomBytes = kKeys * 128;  // 128 rows of 64 values, 128-byte swizzled
 constexpr int kUnitCost = 1;             // a unit's start and end, in chunks
 constexpr int kMinShare = 3;             // weight below which a range is not worth a CTA
-constexpr int kMaxGrid = 1024;
+constexpr int kMaxGrid = 256;            // ranges: the join holds a weight for each of a unit's pieces and 32 rows
 constexpr int kBadSlots = 8;
 constexpr float kRescaleAt = 8.f;
 
@@ -66,6 +66,10 @@ struct Piece {
   __device__ __forceinline__ bool pair() const { return rows > kTile; }
 };
 
+// x / group for the rows of a tree (below 2^17): (x + 1/2) / group is 1/128 or more away from a whole number, and
+// fp32 is off by 2^-23 of it.
+__device__ __forceinline__ int node_of(int x, float inv_group) { return (int)(((float)x + 0.5f) * inv_group); }
+
 __device__ __forceinline__ int64_t unit_weight(const TreeRequest& t) {
   return max(1, (t.keys + kKeys - 1) / kKeys) + kUnitCost;
 }
@@ -93,15 +97,17 @@ struct Pieces {
         request(a);
       }
       const int blocks = unit_blocks(a, t);
-      const int64_t unit = (pos - base) / w, at = base + unit * w;
+      // (64-bit divisions only for what no memory holds)
+      const int64_t unit = span >> 32 ? (pos - base) / w : (int64_t)((uint32_t)(pos - base) / (uint32_t)w);
+      const int64_t at = base + unit * w;
       const int64_t stop = min(end, at + w);
       p.c0 = (int)max((int64_t)0, pos - at - kUnitCost);
       p.c1 = (int)(stop - at - kUnitCost);
       pos = stop;
       if (p.c1 <= p.c0) continue;
       p.t = t;
-      p.h = (int)(unit / blocks);
-      p.row0 = (int)(unit % blocks) * kUnitRows;
+      p.h = (int)((uint32_t)unit / (uint32_t)blocks);
+      p.row0 = (int)((uint32_t)unit % (uint32_t)blocks) * kUnitRows;
       p.rows = min(kUnitRows, t.nodes * a.group - p.row0);
       p.chunks = (int)w - kUnitCost;
       p.first_at = at + kUnitCost;
@@ -273,7 +279,7 @@ struct Shared {
   uint32_t tmem_slot;
   volatile int abort_flag;
   int r0;
-  int64_t base0;
+  int64_t pos, end, base;  // this CTA's range, and where the first request of it starts
   Cut cut;
   uint32_t bad[kBadSlots][AIOSB_TREE_MAX_NODES / 32];  // per piece: tree keys whose V holds an infinity or a NaN
 };
@@ -314,31 +320,27 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
   }
   pdl_wait();
   if (warp == 0) {  // the weight of all units, and where this CTA's range starts
-    int64_t total = 0;
-    for (int r0 = 0; r0 < a.requests; r0 += 32) {
-      int64_t w = 0;
-      if (r0 + lane < a.requests) {
-        const TreeRequest t = tree_request(a, r0 + lane, blockIdx.x == 0);
-        w = unit_weight(t) * unit_blocks(a, t) * a.hkv;
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-      total += w;
-    }
+    auto weight_of = [&](int r, bool tell) {
+      if (r >= a.requests) return (int64_t)0;
+      const TreeRequest t = tree_request(a, r, tell);
+      return unit_weight(t) * unit_blocks(a, t) * a.hkv;
+    };
+    const int64_t first = weight_of(lane, blockIdx.x == 0);
+    int64_t total = first;
+    for (int r = 32 + lane; r - lane < a.requests; r += 32) total += weight_of(r, blockIdx.x == 0);
+#pragma unroll 1
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     Cut cut;
     cut.total = total;
     cut.ctas = (int)max((int64_t)1, min((int64_t)gridDim.x, total / kMinShare));
-    const int64_t pos = (int)blockIdx.x < cut.ctas ? cut.begin(blockIdx.x) : total;
+    const bool used = (int)blockIdx.x < cut.ctas && total > 0;
+    const int64_t pos = used ? cut.begin(blockIdx.x) : 0, end = used ? cut.begin(blockIdx.x + 1) : 0;
     int64_t base = 0;
-    int found = a.requests;
-    for (int r0 = 0; r0 < a.requests && found == a.requests; r0 += 32) {
-      int64_t w = 0;
-      if (r0 + lane < a.requests) {
-        const TreeRequest t = tree_request(a, r0 + lane, false);
-        w = unit_weight(t) * unit_blocks(a, t) * a.hkv;
-      }
+    int found = 0;
+    for (int r0 = 0; used; r0 += 32) {
+      const int64_t w = r0 == 0 ? first : weight_of(r0 + lane, false);
       int64_t upto = w;
-#pragma unroll
+#pragma unroll 1
       for (int o = 1; o < 32; o <<= 1) {
         const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += v;
@@ -348,14 +350,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
         const int l = __ffs(hit) - 1;
         found = r0 + l;
         base += __shfl_sync(0xffffffffu, upto - w, l);
-      } else {
-        base += __shfl_sync(0xffffffffu, upto, 31);
+        break;
       }
+      base += __shfl_sync(0xffffffffu, upto, 31);
     }
     if (lane == 0) {
       sh.cut = cut;
       sh.r0 = found;
-      sh.base0 = base;
+      sh.pos = pos;
+      sh.end = end;
+      sh.base = base;
     }
   }
   tc_fence_before();
@@ -363,18 +367,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
   tc_fence_after();
   pdl_launch_dependents();
   const uint32_t tmem = sh.tmem_slot;
-  const Cut cut = sh.cut;
   const int me = blockIdx.x;
+  const float inv_group = 1.f / (float)a.group;
 
   Pieces it;
-  it.pos = it.end = 0;
-  if (me < cut.ctas && cut.total > 0) {
-    it.pos = cut.begin(me);
-    it.end = cut.begin(me + 1);
-    it.base = sh.base0;
-    it.r = sh.r0;
-    if (it.pos < it.end) it.request(a);
-  }
+  it.pos = sh.pos;
+  it.end = sh.end;
+  it.base = sh.base;
+  it.r = sh.r0;
+  if (it.pos < it.end) it.request(a);
   Piece p = {};
 
   if (warp >= kSoftWarps && warp < kMmaWarp) {
@@ -585,21 +586,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       if (s == 0 || pair) {
         const int wt = threadIdx.x & 127;
         constexpr int kCols = D / 8;
-        uint4 v[kCols];  // every load in flight before the first store: one round trip
-#pragma unroll
-        for (int i = 0; i < kCols; ++i) {
-          const int at = i * 128 + wt, rr = s * kTile + at / kCols, g = p.row0 + rr;
-          v[i] = make_uint4(0, 0, 0, 0);
-          if (rr < p.rows)
-            v[i] = *reinterpret_cast<const uint4*>(a.q + (int64_t)(p.t.start + g / a.group) * a.q_stride +
-                                                   (int64_t)(p.h * a.group + g % a.group) * D + at % kCols * 8);
-        }
-#pragma unroll
+        const uint32_t dst = q_smem + s * S::kBlockBytes;
+#pragma unroll 4
         for (int i = 0; i < kCols; ++i) {
           const int at = i * 128 + wt, rr = at / kCols, c = at % kCols;
-          *reinterpret_cast<uint4*>(smem + s * S::kBlockBytes + (c >> 3) * kAtomBytes + rr * 128 +
-                                    (((c & 7) ^ (rr & 7)) << 4)) = v[i];
+          const int g = min(p.row0 + s * kTile + rr, p.row0 + p.rows - 1), node = node_of(g, inv_group);
+          cp_async16_or_zero(dst + (c >> 3) * kAtomBytes + rr * 128 + (((c & 7) ^ (rr & 7)) << 4),
+                             a.q + (int64_t)(p.t.start + node) * a.q_stride +
+                                 (int64_t)(p.h * a.group + g - node * a.group) * D + c * 8,
+                             s * kTile + rr < p.rows);
         }
+        cp_async_wait_all();
         fence_proxy_async_shared();
       }
       __syncwarp();
@@ -609,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       const int rows_here = p.rows - (pair ? s * kTile : 0);
       const bool warp_works = (warp & 3) * 32 < rows_here;
       const int pair_row = p.row0 + min(my_row, p.rows - 1);
-      const int node = p.t.start + pair_row / a.group;
+      const int node = p.t.start + node_of(pair_row, inv_group);
       const int32_t* const bits = a.mask + (int64_t)node * a.words;
       float ref = -INFINITY, sum = 0.f;
       bool fresh = true;  // no output of this piece yet
@@ -686,15 +683,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
         join.row0 = p.row0;
         join.rows = p.rows;
         join.h = p.h;
-        join.last = cut.owner(p.first_at + p.chunks - 1);
+        if (threadIdx.x == 0) join.last = sh.cut.owner(p.first_at + p.chunks - 1);
       }
       uint32_t any_bad = 0;
       if (p.c1 * kKeys > p.t.cached)
         for (int w = 0; w < a.words; ++w) any_bad |= sh.bad[turn][w];
       if (warp_works) {
-        const int g = p.row0 + my_row;
-        __nv_bfloat16* const dst = a.out + (int64_t)(p.t.start + g / a.group) * a.out_stride +
-                                   (int64_t)(p.h * a.group + g % a.group) * D;
+        __nv_bfloat16* const dst = a.out + (int64_t)node * a.out_stride +
+                                   (int64_t)(p.h * a.group + pair_row - (node - p.t.start) * a.group) * D;
         const int j0 = pair ? 0 : s * (D / 32), j1 = pair ? D / 16 : (s + 1) * (D / 32);  // of 16 columns each
 #pragma unroll 1
         for (int j = j0; j < j1; ++j) {
@@ -769,46 +765,62 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
   }
 }
 
-// Joins the pieces of the unit that starts in range blockIdx.x and goes on behind it: a thread takes every
-// eighth float4 of a row.
+// Joins the pieces of the unit that starts in range blockIdx.x and goes on behind it. A CTA takes 32 rows and D / 4
+// columns: first every piece's maxima and sums, then the pieces' outputs, four loads in flight to a thread.
+constexpr int kJoinRows = 32, kJoinParts = 4;
+
 template <int D>
 __global__ void __launch_bounds__(256) attn_tree_join_kernel(const TreeAttnArgs a, int grid, int unit_rows) {
+  extern __shared__ float weight[];  // [pieces, rows]
   pdl_enter();
   const Join j = reinterpret_cast<const Join*>(a.work)[blockIdx.x];
-  const int row = blockIdx.y * 32 + (threadIdx.x & 31), c0 = threadIdx.x >> 5;
-  if (row >= j.rows) return;
+  const int r = threadIdx.x & 31, sub = threadIdx.x >> 5, row = blockIdx.y * kJoinRows + r;
+  if ((int)blockIdx.y * kJoinRows >= j.rows) return;
   const size_t floats = slot_floats<D>(unit_rows);
-  const int first = blockIdx.x;
-  auto slot = [&](int c) { return slot_at(a, grid, floats, c == first ? 2 * c + 1 : 2 * c); };
+  const int first = blockIdx.x, pieces = j.last - first + 1;
+  auto slot = [&](int i) { return slot_at(a, grid, floats, i == 0 ? 2 * first + 1 : 2 * (first + i)); };
+  const bool in = row < j.rows;
+  __shared__ float top[8][kJoinRows], total[8][kJoinRows];
   float m = -INFINITY;
-  for (int c = first; c <= j.last; ++c) m = fmaxf(m, reinterpret_cast<const float2*>(slot(c))[row].x);
+#pragma unroll 4
+  for (int i = sub; i < pieces; i += 8) m = fmaxf(m, in ? reinterpret_cast<const float2*>(slot(i))[row].x : -INFINITY);
+  top[sub][r] = m;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 8; ++k) m = fmaxf(m, top[k][r]);
   const float ref = m == -INFINITY ? 0.f : m;
   float l = 0.f;
-  float4 o[D / 32];
+#pragma unroll 4
+  for (int i = sub; i < pieces; i += 8) {
+    const float2 x = in ? reinterpret_cast<const float2*>(slot(i))[row] : make_float2(-INFINITY, 0.f);
+    const float w = exp2_fast(x.x - ref);
+    weight[i * kJoinRows + r] = w;
+    l = fmaf(x.y, w, l);
+  }
+  total[sub][r] = l;
+  __syncthreads();
+  if (!in) return;
+  l = 0.f;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c = first; c <= j.last; ++c) {
-    const float* const p = slot(c);
-    const float2 s = reinterpret_cast<const float2*>(p)[row];
-    const float w = exp2_fast(s.x - ref);
-    l = fmaf(s.y, w, l);
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      const float4 v = reinterpret_cast<const float4*>(p + 2 * unit_rows)[(size_t)(c0 + 8 * i) * unit_rows + row];
-      o[i].x = fmaf(v.x, w, o[i].x);
-      o[i].y = fmaf(v.y, w, o[i].y);
-      o[i].z = fmaf(v.z, w, o[i].z);
-      o[i].w = fmaf(v.w, w, o[i].w);
-    }
+  for (int k = 0; k < 8; ++k) l += total[k][r];
+  // D / 16 columns of float4 a CTA: the first D / 16 groups of threads take one each
+  if (sub >= D / 4 / kJoinParts) return;
+  const int c = blockIdx.z * (D / 4 / kJoinParts) + sub;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < pieces; ++i) {
+    const float4 v = reinterpret_cast<const float4*>(slot(i) + 2 * unit_rows)[(size_t)c * unit_rows + row];
+    const float w = weight[i * kJoinRows + r];
+    o.x = fmaf(v.x, w, o.x);
+    o.y = fmaf(v.y, w, o.y);
+    o.z = fmaf(v.z, w, o.z);
+    o.w = fmaf(v.w, w, o.w);
   }
   const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
   const int g = j.row0 + row;
   __nv_bfloat16* const dst = a.out + (int64_t)(j.start + g / a.group) * a.out_stride +
                              (int64_t)(j.h * a.group + g % a.group) * D;
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i)
-    reinterpret_cast<uint2*>(dst)[c0 + 8 * i] =
-        make_uint2(pack_bf16x2(o[i].x * inv, o[i].y * inv), pack_bf16x2(o[i].z * inv, o[i].w * inv));
+  reinterpret_cast<uint2*>(dst)[c] = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
 }
 
 template <int D>
@@ -818,8 +830,9 @@ cudaError_t launch(const TreeAttnArgs& a, int grid, int unit_rows, cudaStream_t 
   if (e != cudaSuccess) return e;
   e = launch_pdl(kernel, dim3((unsigned)grid), dim3(kThreads), Shape<D>::kSmem, stream, a, unit_rows);
   if (e != cudaSuccess) return e;
-  return launch_pdl(attn_tree_join_kernel<D>, dim3((unsigned)grid, (unsigned)((unit_rows + 31) / 32)), dim3(256), 0,
-                    stream, a, grid, unit_rows);
+  return launch_pdl(attn_tree_join_kernel<D>,
+                    dim3((unsigned)grid, (unsigned)((unit_rows + kJoinRows - 1) / kJoinRows), kJoinParts), dim3(256),
+                    (size_t)grid * kJoinRows * sizeof(float), stream, a, grid, unit_rows);
 }
 
 }  // namespace
