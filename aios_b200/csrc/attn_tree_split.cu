@@ -26,6 +26,7 @@ namespace {
 
 constexpr int kTile = 128;      // rows of a tile: UMMA M, TMEM lanes
 constexpr int kUnitRows = 256;  // two tiles
+constexpr int kFewRows = 32;    // up to here on mma.sync
 constexpr int kKeys = 128;      // keys of a chunk: a block of keys and one of values
 constexpr int kStep = 64;       // keys of a softmax step, half a chunk
 constexpr int kSoftWarps = 8;
@@ -44,7 +45,7 @@ struct Shape {
   static constexpr int kAtoms = (D + 63) / 64;
   static constexpr int kBlockBytes = kAtoms * kAtomBytes;  // a block of keys or values; also a tile of Q
   static constexpr int kStages = kAtoms == 1 ? 10 : 5;
-  static constexpr int kSmem = 2 * kBlockBytes + kStages * kBlockBytes + 1024;
+  static constexpr int kBlocks = (2 + kStages) * kBlockBytes;  // two tiles of Q, the ring
 };
 
 // ---- the cut --------------------------------------------------------------------------------
@@ -64,6 +65,7 @@ struct Piece {
   int64_t first_at;  // position of the unit's first chunk
   __device__ __forceinline__ bool whole() const { return c0 == 0 && c1 == chunks; }
   __device__ __forceinline__ bool pair() const { return rows > kTile; }
+  __device__ __forceinline__ bool few() const { return rows <= kFewRows; }
 };
 
 // x / group for the rows of a tree (below 2^17): (x + 1/2) / group is 1/128 or more away from a whole number, and
@@ -160,6 +162,9 @@ __device__ __forceinline__ void tmem_ld2(uint32_t taddr, float2& v) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0,%1}, [%2];" : "=r"(x), "=r"(y) : "r"(taddr));
   asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(x), "+r"(y)::"memory");
   v = make_float2(__uint_as_float(x), __uint_as_float(y));
+}
+__device__ __forceinline__ void mbar_arrive_count(uint64_t* bar, uint32_t count) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
 }
 __device__ __forceinline__ float max3(float x, float y, float z) {
   float r;
@@ -275,28 +280,33 @@ __device__ __forceinline__ bool soft_step(uint32_t t_s, uint32_t t_o, const uint
 
 struct Shared {
   uint64_t full[10], empty[10];
-  uint64_t s_full[2][2], p_full[2][2], pv_done[2], q_full, piece_done, state_full, drained;
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2], q_full, piece_done, met, drained;
   uint32_t tmem_slot;
   volatile int abort_flag;
   int r0;
   int64_t pos, end, base;  // this CTA's range, and where the first request of it starts
   Cut cut;
+  float2 few_state[kSoftWarps][16];  // (reference, sum) of the warps' rows, in a piece of few rows
   uint32_t bad[kBadSlots][AIOSB_TREE_MAX_NODES / 32];  // per piece: tree keys whose V holds an infinity or a NaN
 };
 
 template <int D>
+constexpr int kSmem = Shape<D>::kBlocks + (int)sizeof(Shared);
+static_assert(kSmem<128> <= 232448 && kSmem<96> <= 232448 && kSmem<64> <= 232448, "shared memory of a CTA");
+
+template <int D>
 __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const TreeAttnArgs a, int unit_rows) {
   using S = Shape<D>;
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ Shared sh;
+  // No static shared memory: the blocks start where dynamic shared memory does, on 1024 bytes.
+  extern __shared__ __align__(1024) uint8_t smem[];
+  Shared& sh = *reinterpret_cast<Shared*>(smem + S::kBlocks);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t q_smem = smem_u32(smem), ring = q_smem + 2 * S::kBlockBytes;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&sh.full[i], kLoadWarps * 32);
-      mbar_init(&sh.empty[i], 2);
+      mbar_init(&sh.empty[i], kSoftWarps);
     }
     for (int i = 0; i < 2; ++i) {
       for (int b = 0; b < 2; ++b) {
@@ -307,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
     }
     mbar_init(&sh.q_full, kSoftWarps);
     mbar_init(&sh.piece_done, 2);
-    mbar_init(&sh.state_full, kSoftWarps);
+    mbar_init(&sh.met, kSoftWarps);
     mbar_init(&sh.drained, 2);
     sh.abort_flag = 0;
     fence_mbar_init();
@@ -471,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       window = p.c0;
       ask(window, here);
       ask(window + 4, ahead);
-      if (p.pair()) {
+      if (p.pair() || p.few()) {
         for (int c = p.c0; c < p.c1 && ok; ++c) {
           load(false, c);
           if (ok) load(true, c);
@@ -501,6 +511,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
     bool ok = true;
     while (ok && it.next(a, p)) {
       const int n = p.c1 - p.c0;
+      if (p.few()) {
+        base += 2 * n;
+        continue;
+      }
       const bool pair = p.pair();
       // blocks of chunk i's keys and values, as the gathering warps order them
       auto k_block = [&](int i) { return base + (pair ? 2 * i : i < 2 ? i : 2 * i - 1); };
@@ -508,8 +522,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       auto wait_block = [&](uint32_t b) { return mbar_wait(&sh.full[b % S::kStages], (b / S::kStages) & 1); };
       // a block is free when both streams are through with it, or the only one that uses it
       auto release = [&](uint32_t stage) {
+        // (eight arrivals: in a piece of few rows the softmax warps read the blocks)
         tc_commit(&sh.empty[stage]);
-        if (!pair) mbar_arrive(&sh.empty[stage]);
+        mbar_arrive_count(&sh.empty[stage], pair ? kSoftWarps / 2 - 1 : kSoftWarps - 1);
       };
       // step h is half h & 1 of this chunk of the piece
       auto chunk_of = [&](int h) { return pair ? h >> 1 : 2 * (h >> 1) + s; };
@@ -576,27 +591,242 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
     const int s = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t t_o = t_lane + 256 + s * 128;
-    uint32_t step = 0, done_phase = 0, state_phase = 0;  // steps of this stream, in all pieces so far
+    uint32_t step = 0, base = 0, done_phase = 0, met_phase = 0;  // steps of this stream and blocks, in all pieces so far
     int turn = 0, partial_of = -1;
     bool ok = true;
     Join join = {};
+    // all softmax warps
+    auto meet = [&] {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.met);
+      const bool all = __all_sync(0xffffffffu, mbar_wait(&sh.met, met_phase));
+      met_phase ^= 1;
+      return all;
+    };
+    auto start_join = [&] {
+      partial_of = 1;
+      join.start = p.t.start;
+      join.row0 = p.row0;
+      join.rows = p.rows;
+      join.h = p.h;
+      if (threadIdx.x == 0) join.last = sh.cut.owner(p.first_at + p.chunks - 1);
+    };
+    // Up to 32 rows: 16 to a warp on mma.sync, each warp with its share of every chunk's keys and its own maximum,
+    // sum and output, joined at the end. The tensor pipe is idle here, but a TMEM round trip per step (scores out,
+    // weights back) took longer than the chunk's bytes: 64 x 8192 keys, 15 rows 148 -> KEEP us.
+    auto few_rows = [&](auto load_q) {
+      const int tiles = p.rows > 16 ? 2 : 1, tile = warp & (tiles - 1), part = warp / tiles;
+      if (s == 0) load_q(0, 16 * tiles);
+      if (!meet()) return false;
+      const int row[2] = {tile * 16 + lane / 4, tile * 16 + lane / 4 + 8};
+      const int32_t* bits[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        bits[i] = a.mask + (int64_t)(p.t.start + node_of(p.row0 + min(row[i], p.rows - 1), inv_group)) * a.words;
+      float o[D / 8][4];
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+      float ref[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+      const bool works = tile * 16 < p.rows;
+      // 16-byte piece `col` of row `r` of a block or of Q
+      auto piece_at = [](uint32_t block, int r, int col) {
+        return block + (col >> 3) * kAtomBytes + r * 128 + (((col & 7) ^ (r & 7)) << 4);
+      };
+      for (int c = p.c0; c < p.c1; ++c) {
+        const uint32_t kb = base + 2 * (c - p.c0), vb = kb + 1;
+        const uint32_t ks = kb % S::kStages, vs = vb % S::kStages;
+        const uint32_t k_mem = ring + ks * S::kBlockBytes, v_mem = ring + vs * S::kBlockBytes;
+        if (!__all_sync(0xffffffffu, mbar_wait(&sh.full[ks], (kb / S::kStages) & 1))) return false;
+        uint32_t w[2][4];  // weights as A operands, 16 keys each
+        if (works) {
+          float x[2][2][4];  // scores: 16 keys, 8 keys, the accumulator's values
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[g][n][e] = g < tiles ? 0.f : -INFINITY;
+            if (g >= tiles) continue;
+            const int key = (part * tiles + g) * 16;
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              uint32_t q[4], b[4];
+              ldmatrix4(q, piece_at(q_smem, tile * 16 + (lane & 15), 2 * k + (lane >> 4)));
+              ldmatrix4(b, piece_at(k_mem, key + (lane & 7) + (lane & 16 ? 8 : 0), 2 * k + (lane & 8 ? 1 : 0)));
+              mma_16816(x[g][0], q, b[0], b[1]);
+              mma_16816(x[g][1], q, b[2], b[3]);
+            }
+            if ((c + 1) * kKeys > p.t.cached) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t seen =
+                    seen32(bits[i], a.words, c * kKeys + key, p.t.cached, p.t.keys) >> (2 * (lane & 3));
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (!((seen >> ((e >> 1) * 8 + (e & 1))) & 1)) x[g][e >> 1][2 * i + (e & 1)] = -INFINITY;
+              }
+            }
+          }
+          float most[2];
+          bool grows[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            most[i] = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+              for (int n = 0; n < 2; ++n) most[i] = max3(most[i], x[g][n][2 * i], x[g][n][2 * i + 1]);
+            most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], 1));
+            most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], 2)) * a.scale_log2;
+            grows[i] = most[i] > ref[i] + kRescaleAt;
+          }
+          if (__any_sync(0xffffffffu, grows[0] || grows[1])) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float corr = grows[i] ? exp2_fast(ref[i] - most[i]) : 1.f;
+              if (grows[i]) ref[i] = most[i];
+              sum[i] *= corr;
+#pragma unroll
+              for (int n = 0; n < D / 8; ++n) {
+                o[n][2 * i] *= corr;
+                o[n][2 * i + 1] *= corr;
+              }
+            }
+          }
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (g >= tiles) continue;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float minus = ref[i] == -INFINITY ? 0.f : -ref[i];
+#pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                const float y = exp2_fast(fmaf(x[g][n][2 * i], a.scale_log2, minus)),
+                            z = exp2_fast(fmaf(x[g][n][2 * i + 1], a.scale_log2, minus));
+                sum[i] += y + z;
+                w[g][2 * n + i] = pack_bf16x2(y, z);  // off by 2^-8 of each at most, as the result is by its own
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.empty[ks]);
+        if (!__all_sync(0xffffffffu, mbar_wait(&sh.full[vs], (vb / S::kStages) & 1))) return false;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          if (g >= tiles || !works) continue;
+          const int key = (part * tiles + g) * 16;
+#pragma unroll
+          for (int n = 0; n < D / 16; ++n) {
+            uint32_t b[4];
+            ldmatrix4_trans(b, piece_at(v_mem, key + (lane & 15), 2 * n + (lane >> 4)));
+            mma_16816(o[2 * n], w[g], b[0], b[1]);
+            mma_16816(o[2 * n + 1], w[g], b[2], b[3]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.empty[vs]);
+      }
+      // ---- the warps' outputs, in Q's place: a row's columns are turned by 8 a row against bank conflicts
+      if (!meet()) return false;
+      float* const all = reinterpret_cast<float*>(smem);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+        const int r = lane / 4 + 8 * i;
+        if ((lane & 3) == 0) sh.few_state[warp][r] = make_float2(ref[i], sum[i]);
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+          *reinterpret_cast<float2*>(all + (warp * 16 + r) * D + (n * 8 + r * 8) % D + (lane & 3) * 2) =
+              make_float2(o[n][2 * i], o[n][2 * i + 1]);
+      }
+      if (!meet()) return false;
+      const bool whole = p.whole();
+      float* const slot = whole ? nullptr
+                                : slot_at(a, gridDim.x, slot_floats<D>(unit_rows), p.c0 == 0 ? 2 * me + 1 : 2 * me);
+      if (!whole && p.c0 == 0) start_join();
+      uint32_t any_bad = 0;
+      if (p.c1 * kKeys > p.t.cached)
+        for (int i = 0; i < a.words; ++i) any_bad |= sh.bad[turn][i];
+      for (int i = threadIdx.x; i < p.rows * (D / 4); i += kSoftWarps * 32) {
+        const int my = i / (D / 4), c4 = i % (D / 4), my_tile = my / 16, r = my & 15;
+        float m = -INFINITY, l = 0.f;
+        for (int q = 0; q < kSoftWarps / tiles; ++q) m = fmaxf(m, sh.few_state[q * tiles + my_tile][r].x);
+        const float from = m == -INFINITY ? 0.f : m;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int q = 0; q < kSoftWarps / tiles; ++q) {
+          const int from_warp = q * tiles + my_tile;
+          const float2 st = sh.few_state[from_warp][r];
+          const float f = exp2_fast(st.x - from);
+          const float4 y = *reinterpret_cast<const float4*>(all + (from_warp * 16 + r) * D + (c4 * 4 + r * 8) % D);
+          l = fmaf(st.y, f, l);
+          v.x = fmaf(y.x, f, v.x);
+          v.y = fmaf(y.y, f, v.y);
+          v.z = fmaf(y.z, f, v.z);
+          v.w = fmaf(y.w, f, v.w);
+        }
+        const int g = p.row0 + my, node = node_of(g, inv_group);
+        if (any_bad) {
+          const int32_t* const own = a.mask + (int64_t)(p.t.start + node) * a.words;
+#pragma unroll 1
+          for (int j = 0; j < a.words; ++j) {
+            for (uint32_t hit = sh.bad[turn][j] & (uint32_t)own[j]; hit; hit &= hit - 1) {
+              const int key = p.t.cached + j * 32 + __ffs(hit) - 1;
+              const __nv_bfloat16* x = a.v_cache + (tree_slot(a, p.t.slots[key]) * a.hkv + p.h) * D + c4 * 4;
+              float* const e = &v.x;
+              for (int z = 0; z < 4; ++z) {
+                const float y = bf16_to_f(x[z]);
+                if (!(fabsf(y) < INFINITY)) e[z] += y;
+              }
+            }
+          }
+        }
+        if (whole) {
+          const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
+          __nv_bfloat16* const dst = a.out + (int64_t)(p.t.start + node) * a.out_stride +
+                                     (int64_t)(p.h * a.group + g - node * a.group) * D;
+          reinterpret_cast<uint2*>(dst)[c4] =
+              make_uint2(pack_bf16x2(v.x * inv, v.y * inv), pack_bf16x2(v.z * inv, v.w * inv));
+        } else {
+          if (c4 == 0) reinterpret_cast<float2*>(slot)[my] = make_float2(m, l);
+          reinterpret_cast<float4*>(slot + 2 * unit_rows)[(size_t)c4 * unit_rows + my] = v;
+        }
+      }
+      // before Q of the next piece
+      if (!meet()) return false;
+      if (warp == 0) sh.bad[(turn + kBadSlots - 1) % kBadSlots][lane] = 0;
+      return true;
+    };
     while (ok && it.next(a, p)) {
       const bool pair = p.pair();
-      // Q: this group's tile (the second group's is not used by a narrow unit)
-      if (s == 0 || pair) {
+      // `tile` of Q's `count` rows, by 128 threads
+      auto load_q = [&](int tile, int count) {
         const int wt = threadIdx.x & 127;
         constexpr int kCols = D / 8;
-        const uint32_t dst = q_smem + s * S::kBlockBytes;
+        const uint32_t dst = q_smem + tile * S::kBlockBytes;
 #pragma unroll 4
-        for (int i = 0; i < kCols; ++i) {
+        for (int i = 0; i * 128 < count * kCols; ++i) {
           const int at = i * 128 + wt, rr = at / kCols, c = at % kCols;
-          const int g = min(p.row0 + s * kTile + rr, p.row0 + p.rows - 1), node = node_of(g, inv_group);
+          const int g = min(p.row0 + tile * kTile + rr, p.row0 + p.rows - 1), node = node_of(g, inv_group);
           cp_async16_or_zero(dst + (c >> 3) * kAtomBytes + rr * 128 + (((c & 7) ^ (rr & 7)) << 4),
                              a.q + (int64_t)(p.t.start + node) * a.q_stride +
                                  (int64_t)(p.h * a.group + g - node * a.group) * D + c * 8,
-                             s * kTile + rr < p.rows);
+                             tile * kTile + rr < p.rows);
         }
         cp_async_wait_all();
+      };
+      if (p.few()) {
+        ok = few_rows(load_q);
+        base += 2 * (p.c1 - p.c0);
+        turn = (turn + 1) % kBadSlots;
+        continue;
+      }
+      // this group's tile (the second group's is not used by a narrow unit)
+      if (s == 0 || pair) {
+        load_q(s, kTile);
         fence_proxy_async_shared();
       }
       __syncwarp();
@@ -654,10 +884,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
         tmem_st2(t_lane + s * 128, __float_as_uint(ref), __float_as_uint(sum));
         tmem_wait_st();
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.state_full);
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh.state_full, state_phase));
-        state_phase ^= 1;
+        ok = meet();
         if (!ok) break;
         tc_fence_after();
         float2 x, y;
@@ -677,14 +904,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       const bool row_works = my_row < p.rows;
       if (!whole && row_works && (pair || s == 0))
         reinterpret_cast<float2*>(part)[my_row] = make_float2(m_all, l_all);
-      if (!whole && p.c0 == 0) {
-        partial_of = 1;
-        join.start = p.t.start;
-        join.row0 = p.row0;
-        join.rows = p.rows;
-        join.h = p.h;
-        if (threadIdx.x == 0) join.last = sh.cut.owner(p.first_at + p.chunks - 1);
-      }
+      if (!whole && p.c0 == 0) start_join();
       uint32_t any_bad = 0;
       if (p.c1 * kKeys > p.t.cached)
         for (int w = 0; w < a.words; ++w) any_bad |= sh.bad[turn][w];
@@ -740,6 +960,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       // every warp has started on this piece, so all are through with the one before it
       if (warp == 0) sh.bad[(turn + kBadSlots - 1) % kBadSlots][lane] = 0;
       turn = (turn + 1) % kBadSlots;
+      base += 2 * (p.c1 - p.c0);
       tc_fence_before();
     }
     if (!ok) {
@@ -826,9 +1047,9 @@ __global__ void __launch_bounds__(256) attn_tree_join_kernel(const TreeAttnArgs 
 template <int D>
 cudaError_t launch(const TreeAttnArgs& a, int grid, int unit_rows, cudaStream_t stream) {
   const auto kernel = attn_tree_split_kernel<D>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem<D>);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(kernel, dim3((unsigned)grid), dim3(kThreads), Shape<D>::kSmem, stream, a, unit_rows);
+  e = launch_pdl(kernel, dim3((unsigned)grid), dim3(kThreads), kSmem<D>, stream, a, unit_rows);
   if (e != cudaSuccess) return e;
   return launch_pdl(attn_tree_join_kernel<D>,
                     dim3((unsigned)grid, (unsigned)((unit_rows + kJoinRows - 1) / kJoinRows), kJoinParts), dim3(256),
