@@ -22,6 +22,19 @@ inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s
 // Number of SMs of the current device (cached per device).
 int sm_count();
 
+// Opts `kernel` into `bytes` of dynamic shared memory (and clusters of more than eight CTAs), once per device:
+// `done` is the kernel's own.
+template <typename Kernel>
+inline cudaError_t allow_shared(Kernel kernel, int bytes, bool (&done)[64], bool wide_clusters = false) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && done[dev])) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && wide_clusters) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess && dev < 64) done[dev] = true;
+  return e;
+}
+
 // Launches `kernel` with programmatic dependent launch enabled, so it may start
 // while the previous kernel on the stream drains. Every kernel launched this way
 // executes griddepcontrol.wait in every block before it touches memory that an

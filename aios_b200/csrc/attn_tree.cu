@@ -216,7 +216,8 @@ __global__ void __launch_bounds__(kThreads) attn_tree_small_kernel(const TreeAtt
 template <int D>
 cudaError_t launch_small(const TreeAttnArgs& a, int64_t max_nodes, cudaStream_t stream) {
   const auto kernel = attn_tree_small_kernel<D>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmallSmem<D>);
+  static bool configured[64] = {false};
+  cudaError_t e = allow_shared(kernel, (int)kSmallSmem<D>, configured);
   if (e != cudaSuccess) return e;
   const dim3 grid((unsigned)((max_nodes * a.group + kRows - 1) / kRows), (unsigned)a.hkv, (unsigned)a.requests);
   return launch_pdl(kernel, grid, dim3(kThreads), kSmallSmem<D>, stream, a);

@@ -1047,7 +1047,8 @@ __global__ void __launch_bounds__(256) attn_tree_join_kernel(const TreeAttnArgs 
 template <int D>
 cudaError_t launch(const TreeAttnArgs& a, int grid, int unit_rows, cudaStream_t stream) {
   const auto kernel = attn_tree_split_kernel<D>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem<D>);
+  static bool configured[64] = {false};
+  cudaError_t e = allow_shared(kernel, kSmem<D>, configured);
   if (e != cudaSuccess) return e;
   e = launch_pdl(kernel, dim3((unsigned)grid), dim3(kThreads), kSmem<D>, stream, a, unit_rows);
   if (e != cudaSuccess) return e;

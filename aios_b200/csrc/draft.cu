@@ -633,11 +633,13 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
   write_order(walk, depth, t.n, t.all, a.order + t.start);
 }
 
+constexpr size_t kWeightBytes = 190 * 1024;  // beside the static shared memory
+constexpr int kMaxSampleVocab = 327680;
+
 template <typename Kernel>
-cudaError_t launch_cluster(Kernel kernel, const VerifyArgs& a, int requests, size_t smem, cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e == cudaSuccess && a.ranks > 8)
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+cudaError_t launch_cluster(Kernel kernel, const VerifyArgs& a, int requests, size_t smem, bool (&configured)[64],
+                           cudaStream_t stream) {
+  const cudaError_t e = allow_shared(kernel, smem > 0 ? (int)kWeightBytes : 0, configured, true);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(requests * a.ranks));
@@ -656,9 +658,6 @@ cudaError_t launch_cluster(Kernel kernel, const VerifyArgs& a, int requests, siz
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-constexpr size_t kWeightBytes = 190 * 1024;  // beside the static shared memory
-constexpr int kMaxSampleVocab = 327680;
-
 int warp_run(int vocab, int ranks) {
   const int blocks = (vocab + kBlockIds - 1) / kBlockIds, warps = ranks * kVerifyWarps;
   return (blocks + warps - 1) / warps * kBlockIds;
@@ -672,13 +671,14 @@ cudaError_t launch_verify(VerifyArgs a, int requests, bool greedy, cudaStream_t 
   // more CTAs to a request while they find SMs, and two blocks to each of their warps
   while (a.ranks < 8 && (int64_t)requests * a.ranks * 2 <= sms && a.vocab >= a.ranks * 2 * kVerifyWarps * kBlockIds)
     a.ranks *= 2;
-  if (greedy) return launch_cluster(verify_greedy_kernel<T>, a, requests, 0, stream);
+  static bool configured[3][64] = {};
+  if (greedy) return launch_cluster(verify_greedy_kernel<T>, a, requests, 0, configured[0], stream);
   // two CTAs to an SM if the weights allow it
   while (a.ranks < kMaxRanks && weight_bytes(warp_run(a.vocab, a.ranks)) > kWeightBytes / 2) a.ranks *= 2;
   a.run = warp_run(a.vocab, a.ranks);
   const size_t smem = weight_bytes(a.run);
-  if (a.probs != nullptr) return launch_cluster(verify_kernel<T, true>, a, requests, smem, stream);
-  return launch_cluster(verify_kernel<T, false>, a, requests, smem, stream);
+  if (a.probs != nullptr) return launch_cluster(verify_kernel<T, true>, a, requests, smem, configured[1], stream);
+  return launch_cluster(verify_kernel<T, false>, a, requests, smem, configured[2], stream);
 }
 
 }  // namespace

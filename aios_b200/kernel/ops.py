@@ -606,6 +606,13 @@ def _launch(index: int, name: str, *args) -> None:
 _new_cuda = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
 
 
+def _empty_vector(x: torch.Tensor, size: int, dtype: torch.dtype) -> torch.Tensor:
+    """An uninitialised [size] tensor on x's device."""
+    if _new_cuda is not None and x.get_device() == torch._C._cuda_getDevice():
+        return _new_cuda((size,), (1,), dtype)
+    return x.new_empty(size, dtype=dtype)
+
+
 def _empty_rows(x: torch.Tensor, rows: int, cols: int, dtype: torch.dtype) -> torch.Tensor:
     """An uninitialised contiguous [rows, cols] tensor on x's device."""
     if _new_cuda is not None and x.get_device() == torch._C._cuda_getDevice():
@@ -1034,17 +1041,18 @@ TREE_MAX_NODES = 1024  # nodes of a tree
 
 
 def _check_ints(what: str, name: str, t: torch.Tensor, size: int, index: int, dtype: torch.dtype = torch.int32) -> None:
-    if t.dtype is not dtype or t.ndim != 1 or t.shape[0] != size or t.get_device() != index or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != (size,) or t.get_device() != index or not t.is_contiguous():
         raise ValueError(f"{what}: {name} must be a contiguous {dtype} tensor of {size} on cuda:{index}")
 
 
-def _check_trees(what: str, tokens: int, tree_start: torch.Tensor, index: int) -> int:
+def _check_trees(what: str, tree_start: torch.Tensor, index: int) -> int:
     """The number of trees."""
     if tree_start.ndim != 1 or tree_start.shape[0] < 1:
         raise ValueError(f"{what}: tree_start must have shape [requests + 1]")
-    requests = tree_start.shape[0] - 1
-    _check_ints(what, "tree_start", tree_start, requests + 1, index)
-    return requests
+    size = tree_start.shape[0]
+    if tree_start.dtype is not torch.int32 or tree_start.get_device() != index or not tree_start.is_contiguous():
+        raise ValueError(f"{what}: tree_start must be a contiguous int32 tensor on cuda:{index}")
+    return size - 1
 
 
 def draft_tree(
@@ -1072,7 +1080,7 @@ def draft_tree(
         raise ValueError(f"draft_tree: max_nodes must be in [1, {TREE_MAX_NODES}]")
     tokens, index, words = parents.shape[0], parents.get_device(), (max_nodes + 31) // 32
     _check_ints("draft_tree", "parents", parents, tokens, index)
-    requests = _check_trees("draft_tree", tokens, tree_start, index)
+    requests = _check_trees("draft_tree", tree_start, index)
     if cached_lens is not None:
         _check_ints("draft_tree", "cached_lens", cached_lens, requests, index)
     if mask is None:
@@ -1080,7 +1088,7 @@ def draft_tree(
     else:
         _check_dense("draft_tree", "mask", mask, (tokens, words), torch.int32, index)
     if positions is None:
-        positions = parents.new_empty(tokens)
+        positions = _empty_vector(parents, tokens, torch.int32)
     else:
         _check_ints("draft_tree", "positions", positions, tokens, index)
     if tokens and requests:
@@ -1125,32 +1133,54 @@ def attention_tree(
         if rows != tokens or cols != width or out.get_device() != index:
             raise ValueError("attention_tree: out must match q")
     slots = k_cache.shape[0]
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if (t.dtype is not torch.bfloat16 or t.shape != (slots, num_kv_heads, head_dim) or t.get_device() != index
-                or not t.is_contiguous()):
-            raise ValueError(f"attention_tree: {name} must be a contiguous bf16 [slots, num_kv_heads, head_dim] tensor "
-                             f"on cuda:{index}")
-    requests = _check_trees("attention_tree", tokens, tree_start, index)
-    _check_ints("attention_tree", "row_table", row_table, requests, index)
-    _check_ints("attention_tree", "cached_lens", cached_lens, requests, index)
-    if (page_table.dtype is not torch.int32 or page_table.ndim != 2 or page_table.get_device() != index
-            or (page_table.shape[1] > 1 and page_table.stride(1) != 1)):
-        raise ValueError("attention_tree: page_table must be an int32 tensor of contiguous rows")
+    cache = (slots, num_kv_heads, head_dim)
+    requests = tree_start.shape[0] - 1 if tree_start.ndim == 1 else -1
+    words = tree_mask.shape[1] if tree_mask.ndim == 2 else -1
+    if not (k_cache.dtype is v_cache.dtype is torch.bfloat16 and k_cache.shape == cache and v_cache.shape == cache
+            and k_cache.is_contiguous() and v_cache.is_contiguous() and requests >= 0 and words >= 0
+            and tree_start.dtype is row_table.dtype is cached_lens.dtype is tree_mask.dtype is page_table.dtype
+            is torch.int32 and row_table.shape == (requests,) and cached_lens.shape == (requests,)
+            and tree_mask.shape == (tokens, words) and page_table.ndim == 2
+            and (page_table.stride(1) == 1 or page_table.shape[1] <= 1) and tree_start.is_contiguous()
+            and row_table.is_contiguous() and cached_lens.is_contiguous() and tree_mask.is_contiguous()
+            and k_cache.get_device() == v_cache.get_device() == tree_start.get_device() == row_table.get_device()
+            == cached_lens.get_device() == tree_mask.get_device() == page_table.get_device() == index):
+        _refuse_attention_tree(index, tokens, cache, k_cache, v_cache, page_table, row_table, cached_lens, tree_start,
+                               tree_mask)
     table_rows, table_width = page_table.shape
-    if tree_mask.ndim != 2:
-        raise ValueError("attention_tree: tree_mask must have shape [tokens, words]")
-    words = tree_mask.shape[1]
-    _check_dense("attention_tree", "tree_mask", tree_mask, (tokens, words), torch.int32, index)
     if tokens and requests:
-        size = _lib.load().aiosb_attention_tree_work_bytes(tokens, requests, words, max_cached or table_width,
-                                                           num_qo_heads, num_kv_heads, head_dim)
-        work = _empty_rows(q, 1, size, torch.uint8) if size else None
+        work, size = None, 0
+        if (max_cached or table_width) > ATTENTION_TREE_WHOLE_KEYS:
+            size = _lib.load().aiosb_attention_tree_work_bytes(tokens, requests, words, max_cached or table_width,
+                                                               num_qo_heads, num_kv_heads, head_dim)
+            work = _empty_vector(q, size, torch.uint8)
         _launch(index, "aiosb_attention_tree", q.data_ptr(), q_stride, tokens, k_cache.data_ptr(), v_cache.data_ptr(),
                 slots, page_table.data_ptr(), page_table.stride(0) if table_rows > 1 else table_width, table_rows,
                 table_width, row_table.data_ptr(), cached_lens.data_ptr(), tree_start.data_ptr(), requests,
-                tree_mask.data_ptr(), words, max_cached, num_qo_heads, num_kv_heads, head_dim, float(scale),
+                tree_mask.data_ptr(), words, max_cached, num_qo_heads, num_kv_heads, head_dim, scale,
                 out.data_ptr(), out_stride, _ptr(work), size, _status_pointer(index))
     return out
+
+
+# Histories up to here are attended whole by a CTA, without a work area (aiosb_attention_tree_work_bytes gives 0)
+ATTENTION_TREE_WHOLE_KEYS = 256
+
+
+def _refuse_attention_tree(index, tokens, cache, k_cache, v_cache, page_table, row_table, cached_lens, tree_start,
+                           tree_mask) -> None:
+    """Names the argument that attention_tree does not take."""
+    what = "attention_tree"
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if t.dtype is not torch.bfloat16 or t.shape != cache or t.get_device() != index or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be a contiguous bf16 [slots, num_kv_heads, head_dim] tensor on "
+                             f"cuda:{index}")
+    requests = _check_trees(what, tree_start, index)
+    _check_ints(what, "row_table", row_table, requests, index)
+    _check_ints(what, "cached_lens", cached_lens, requests, index)
+    if tree_mask.ndim != 2:
+        raise ValueError(f"{what}: tree_mask must have shape [tokens, words]")
+    _check_dense(what, "tree_mask", tree_mask, (tokens, tree_mask.shape[1]), torch.int32, index)
+    raise ValueError(f"{what}: page_table must be an int32 tensor of contiguous rows on cuda:{index}")
 
 
 def verify_draft(
@@ -1183,39 +1213,40 @@ def verify_draft(
     [tokens]: each tree's node numbers, the path from the root first, then the others)."""
     if not logits.is_cuda:
         raise ValueError("verify_draft requires CUDA tensors")
-    if logits.ndim != 2 or logits.dtype not in (torch.bfloat16, torch.float32):
+    fp32 = logits.dtype is torch.float32
+    if logits.ndim != 2 or not (fp32 or logits.dtype is torch.bfloat16):
         raise ValueError("verify_draft: logits must be a bf16 or fp32 tensor of shape [tokens, vocab]")
     tokens, vocab = logits.shape
     index = logits.get_device()
-    if vocab > 1 and logits.stride(1) != 1:
+    stride, inner = logits.stride()
+    if vocab > 1 and inner != 1:
         raise ValueError("verify_draft: logits rows must be contiguous")
     _check_ints("verify_draft", "draft_tokens", draft_tokens, tokens, index, torch.int64)
     _check_ints("verify_draft", "parents", parents, tokens, index)
-    requests = _check_trees("verify_draft", tokens, tree_start, index)
-    if greedy:
-        if draft_probs is not None:
-            raise ValueError("verify_draft: greedy verification takes no draft_probs")
-        accept_uniforms = sample_uniforms = None
-    else:
+    requests = _check_trees("verify_draft", tree_start, index)
+    accept = sample = probs = None
+    probs_stride = 0
+    if not greedy:
         if accept_uniforms is None or sample_uniforms is None:
             raise ValueError("verify_draft: sampling needs accept_uniforms and sample_uniforms")
         _check_ints("verify_draft", "accept_uniforms", accept_uniforms, tokens, index, torch.float32)
         _check_ints("verify_draft", "sample_uniforms", sample_uniforms, requests, index, torch.float32)
-    probs_stride = 0
+        accept, sample = accept_uniforms.data_ptr(), sample_uniforms.data_ptr()
     if draft_probs is not None:
+        if greedy:
+            raise ValueError("verify_draft: greedy verification takes no draft_probs")
         if (draft_probs.dtype is not torch.float32 or draft_probs.shape != (tokens, vocab)
                 or draft_probs.get_device() != index or (vocab > 1 and draft_probs.stride(1) != 1)):
             raise ValueError("verify_draft: draft_probs must be an fp32 [tokens, vocab] tensor with contiguous rows "
                              f"on cuda:{index}")
-        probs_stride = draft_probs.stride(0) if tokens > 1 else vocab
-    accepted = parents.new_empty(requests)
-    next_token = draft_tokens.new_empty(requests)
-    order = parents.new_empty(tokens)
+        probs, probs_stride = draft_probs.data_ptr(), draft_probs.stride(0) if tokens > 1 else vocab
+    accepted = _empty_vector(logits, requests, torch.int32)
+    next_token = _empty_vector(logits, requests, torch.int64)
+    order = _empty_vector(logits, tokens, torch.int32)
     if requests:
-        _launch(index, "aiosb_verify_draft", logits.data_ptr(), int(logits.dtype is torch.float32),
-                logits.stride(0) if tokens > 1 else vocab, tokens, vocab, draft_tokens.data_ptr(), parents.data_ptr(),
-                tree_start.data_ptr(), requests, _ptr(accept_uniforms), _ptr(sample_uniforms), float(temperature),
-                int(bool(greedy)), _ptr(draft_probs), probs_stride, accepted.data_ptr(), next_token.data_ptr(),
+        _launch(index, "aiosb_verify_draft", logits.data_ptr(), fp32, stride if tokens > 1 else vocab, tokens, vocab,
+                draft_tokens.data_ptr(), parents.data_ptr(), tree_start.data_ptr(), requests, accept, sample,
+                temperature, bool(greedy), probs, probs_stride, accepted.data_ptr(), next_token.data_ptr(),
                 order.data_ptr(), _status_pointer(index))
     return accepted, next_token, order
 
