@@ -142,26 +142,31 @@ __device__ __forceinline__ double widen(float x) {
 // 2^(i / 16) for the exponential below: sixteen doubles are all of the banks once, so that no two lanes' entries
 // conflict (a table of 128 cost as much as the arithmetic).
 constexpr int kExpTable = 16;
-// e^((x - m) / T) in fp64 for x <= m, off by about 2^-50: (x - m) / (T ln 2) = (k + f) / 16 with |f| <= 1/2, 2^(k / 16)
-// from the table and k's upper bits, and 2^(f / 16) by its series to the sixth power (table-driven exponentials:
-// P. T. P. Tang, ACM TOMS 15, 1989). Eleven fp64 instructions, where the general function takes some thirty.
-// scale: 16 / (T ln 2); base: m * scale. Below 2^-1000, and for x of -inf, it is 0.
-__device__ __forceinline__ double exp_table(double x, double scale, double base, const double* table) {
-  double t = fma(x, scale, -base);
-  const bool none = (uint32_t)__double2hiint(t) >= 0xC0CF4000u;  // t <= -16000
-  if (none) t = 0;
+// e^((x - m) / T) in fp64 for x <= m, off by about 2^-42: (x - m) / (T ln 2) = (k + f) / 16 with |f| <= 1/2, 2^(k / 16)
+// from the table and k's upper bits, and 2^(f / 16) by its series to the fifth power (table-driven exponentials:
+// P. T. P. Tang, ACM TOMS 15, 1989). Eleven fp64 instructions, where the general function takes some thirty. A sum's
+// borders are off by 2^-42 of it at most, so that a draw among 2^18 tokens differs from the exact one's once in 2^24.
+// scale: 16 / (T ln 2); base: m * scale (its rounding is a factor of all weights). Below m - 600 T, and for x of -inf,
+// it is 2^-865, as nothing against 1: at or below kNothing a weight counts as 0.
+constexpr double kNothing = 0x1p-800;
+__device__ __forceinline__ double exp_table(float x, double scale, double base, const double* table) {
+  double t = fma(widen(x), scale, -base);
+  t = __hiloint2double((int)min((uint32_t)__double2hiint(t), 0xC0CB0D00u), __double2loint(t));  // max(t, -13850)
   const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are round(t)
   const double s = t + magic, f = t - (s - magic);
   const int k = __double2loint(s);
   constexpr double c = 0.043321698784996581;  // ln 2 / 16
-  double p = fma(f, c * c * c * c * c * c / 720, c * c * c * c * c / 120);
-  p = fma(f, p, c * c * c * c / 24);
+  double p = fma(f, c * c * c * c * c / 120, c * c * c * c / 24);
   p = fma(f, p, c * c * c / 6);
   p = fma(f, p, c * c / 2);
   p = fma(f, p, c);
   const double b = table[k & (kExpTable - 1)];
   const double r = fma(b, f * p, b);
-  return none ? 0.0 : __hiloint2double(__double2hiint(r) + ((k >> 4) << 20), __double2loint(r));
+  return __hiloint2double(__double2hiint(r) + ((k >> 4) << 20), __double2loint(r));
+}
+__device__ __forceinline__ double positive(double x) {  // max(x, 0) of a number
+  const int keep = ~(__double2hiint(x) >> 31);
+  return __hiloint2double(__double2hiint(x) & keep, __double2loint(x) & keep);
 }
 
 // Values that the CTAs of a cluster hand to one another; the buffers take turns, so that one barrier an exchange is
@@ -182,9 +187,9 @@ __device__ __forceinline__ void hand_out(Exchange& e, int turn, int rank, int to
 
 // A request's tree in shared memory, and the path through it.
 struct Walk {
-  int32_t up[AIOSB_TREE_MAX_NODES];
-  int32_t path[AIOSB_TREE_MAX_NODES];
-  int32_t child[AIOSB_TREE_MAX_NODES];  // the current node's children
+  int16_t up[AIOSB_TREE_MAX_NODES];
+  int16_t path[AIOSB_TREE_MAX_NODES];
+  int16_t child[AIOSB_TREE_MAX_NODES];  // the current node's children
   uint32_t on_path[AIOSB_TREE_MAX_NODES / 32];
   int children;
 };
@@ -195,7 +200,7 @@ __device__ __forceinline__ void list_children(Walk& w, int cur, int n) {  // one
     const int j = j0 + lane;
     const bool is = j > cur && j < n && w.up[j] == cur;
     const unsigned some = __ballot_sync(0xffffffffu, is);
-    if (is) w.child[count + __popc(some & ((1u << lane) - 1))] = j;
+    if (is) w.child[count + __popc(some & ((1u << lane) - 1))] = (int16_t)j;
     count += __popc(some);
   }
   if (lane == 0) w.children = count;
@@ -212,6 +217,12 @@ __device__ __forceinline__ void write_order(const Walk& w, int depth, int n, int
     if (rest) order[at + __popc(some & ((1u << lane) - 1))] = j;
     at += __popc(some);
   }
+}
+
+// (-1 for what is no node's number)
+__device__ __forceinline__ int16_t parent_of(const VerifyArgs& a, int row) {
+  const int p = a.parents[row];
+  return (int16_t)(p >= 0 && p < AIOSB_TREE_MAX_NODES ? p : -1);
 }
 
 struct TreeRows {
@@ -243,7 +254,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_greedy_kernel(const Ver
   pdl_enter();
   TreeRows t;
   if (!tree_rows(a, r, rank == 0 && threadIdx.x == 0, t)) return;  // the whole cluster leaves
-  for (int i = threadIdx.x; i < t.n; i += kVerifyThreads) walk.up[i] = a.parents[t.start + i];
+  for (int i = threadIdx.x; i < t.n; i += kVerifyThreads) walk.up[i] = parent_of(a, t.start + i);
   if (threadIdx.x < AIOSB_TREE_MAX_NODES / 32) walk.on_path[threadIdx.x] = threadIdx.x == 0 ? 1u : 0u;
   if (threadIdx.x == 0) walk.path[0] = 0;
   cluster_sync();  // every CTA runs: its shared memory may be written
@@ -316,7 +327,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_greedy_kernel(const Ver
     ++depth;
     __syncthreads();  // the children have been read
     if (threadIdx.x == 0) {
-      walk.path[depth] = cur;
+      walk.path[depth] = (int16_t)cur;
       walk.on_path[cur >> 5] |= 1u << (cur & 31);
     }
   }
@@ -334,10 +345,13 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_greedy_kernel(const Ver
 // tried, so that a row is read once. A pass leaves each warp the sum of its run and each CTA the sum of its warps';
 // a token is found by these sums from the outside in. Sums are taken in a fixed order, in fp64: what is accepted or
 // drawn hangs on comparisons of them.
+// Weights lie in groups of eight ids, ten places to a group: a lane's 16-byte accesses to its group then fall on
+// different banks. A row comes as fp32 into its group's first places.
+constexpr int kGroupPlaces = 10;
+
 template <typename T, bool PROBS>
 __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs a) {
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  double* const weights = reinterpret_cast<double*>(smem_raw);
+  extern __shared__ __align__(16) double weights[];
   __shared__ Walk walk;
   __shared__ Exchange ex;
   __shared__ double table[kExpTable];
@@ -358,7 +372,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
   if (!tree_rows(a, r, first, t)) return;  // the whole cluster leaves
   for (int i = threadIdx.x; i < t.n; i += kVerifyThreads) {
     const int64_t x = a.draft_tokens[t.start + i];
-    walk.up[i] = a.parents[t.start + i];
+    walk.up[i] = parent_of(a, t.start + i);
     node_x[i] = x >= 0 && x < a.vocab ? (int32_t)x : -1;
     node_u[i] = a.accept_u[t.start + i];
   }
@@ -369,8 +383,22 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
   const double scale = a.inv_temperature * (1.4426950408889634 * kExpTable);
   const int per_rank = a.run * kVerifyWarps, rank_lo = rank * per_rank;
   const int lo = min(rank_lo + warp * a.run, a.vocab), hi = min(rank_lo + (warp + 1) * a.run, a.vocab);
-  // one place of padding to eight keeps a lane's eight consecutive ids off one bank
-  auto at = [&](int v) -> double& { return weights[(v - rank_lo) + ((v - rank_lo) >> 3)]; };
+  auto group_of = [&](int v) { return weights + ((v - rank_lo) >> 3) * kGroupPlaces; };
+  auto at = [&](int v) -> double& { return group_of(v)[(v - rank_lo) & 7]; };
+  auto load_group = [](const double* g, double (&w)[8]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const double2 d = reinterpret_cast<const double2*>(g)[j];
+      w[2 * j] = d.x;
+      w[2 * j + 1] = d.y;
+    }
+  };
+  auto store_group = [](double* g, const double (&w)[8]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) reinterpret_cast<double2*>(g)[j] = make_double2(w[2 * j], w[2 * j + 1]);
+  };
+  // ids of a lane's group that are none of this warp's hold 0 at all times
+  const int last_block = lo + (hi - lo + kBlockIds - 1) / kBlockIds * kBlockIds;
 
   int turn = 0, cur = 0, depth = 0, last_turn = 0;
   // The sums of the warps' runs within the CTA, then of the CTAs (ex.sum, in rank order); `top` goes along.
@@ -398,15 +426,18 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
   for (;;) {
     const T* const row = reinterpret_cast<const T*>(a.logits) + (int64_t)(t.start + cur) * a.logits_stride;
     const float* const q = PROBS ? a.probs + (int64_t)(t.start + cur) * a.probs_stride : nullptr;
-    const bool vec = lies_on_16(row), vec_q = PROBS && vec && lies_on_16(q);
-    if (warp == 0) {  // the children; their logits and probabilities are asked for ahead of the row's
+    const bool vec = lies_on_16(row), vec_q = PROBS && lies_on_16(q);
+    // the children; their logits and probabilities are asked for ahead of the row's, a lane each
+    float child_l = -INFINITY, child_p = 0.f;
+    if (warp == 0) {
       list_children(walk, cur, t.n);
       __syncwarp();
-      for (int i = lane; i < walk.children; i += 32) {
-        const int x = node_x[walk.child[i]];
-        if (x < 0 && rank == 0) report(a.status, AIOSB_DEV_TOKEN_RANGE);
-        *reinterpret_cast<float*>(&child_r[i]) = x >= 0 ? load_logit(row + x) : -INFINITY;
-        if (PROBS) child_q[i] = x >= 0 ? q[x] : 0.f;
+      if (lane < walk.children) {
+        const int x = node_x[walk.child[lane]];
+        if (x >= 0) {
+          child_l = load_logit(row + x);
+          if (PROBS) child_p = q[x];
+        }
       }
     }
     // ---- the row, as it is, to its place; its maximum
@@ -417,41 +448,56 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
       float x[8];
       load_ids(row, vec, ids, -INFINITY, x);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        top = max_nan(top, x[j]);
-        if (ids[j] < hi) *reinterpret_cast<float*>(&at(ids[j])) = x[j];
+      for (int j = 0; j < 8; ++j) top = max_nan(top, x[j]);
+      if (vec) {
+        float4* const g = reinterpret_cast<float4*>(group_of(ids.first));
+        g[0] = make_float4(x[0], x[1], x[2], x[3]);
+        g[1] = make_float4(x[4], x[5], x[6], x[7]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) reinterpret_cast<float*>(group_of(ids[j]))[(ids[j] - rank_lo) & 7] = x[j];
       }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (lane == 0) warp_top[warp] = top;
+    if (warp == 0) {
+      for (int i = lane; i < walk.children; i += 32) {
+        const int x = node_x[walk.child[i]];
+        if (x < 0 && rank == 0) report(a.status, AIOSB_DEV_TOKEN_RANGE);
+        if (i >= 32) {
+          child_l = x >= 0 ? load_logit(row + x) : -INFINITY;
+          if (PROBS) child_p = x >= 0 ? q[x] : 0.f;
+        }
+        *reinterpret_cast<float*>(&child_r[i]) = child_l;
+        if (PROBS) child_q[i] = child_p;
+      }
+    }
     __syncthreads();
     top = lane < kVerifyWarps ? warp_top[lane] : -INFINITY;
 #pragma unroll
     for (int o = kVerifyWarps / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     top = __shfl_sync(0xffffffffu, top, 0);
     const int children = walk.children;
-    // ---- weights over this CTA's maximum
+    // ---- weights over this CTA's maximum (one that is NaN or +inf ends the walk below; -inf leaves nothing)
     double part = 0;
-    const double mine = widen(top) * scale;
+    const double mine = widen(top > -INFINITY ? top : 0.f) * scale;
 #pragma unroll 1
-    for (int base = lo; base < hi; base += kBlockIds) {
-      const Ids ids(base, hi, vec, lane);
+    for (int base = lo; base < last_block; base += kBlockIds) {
+      const int v = base + lane * 8;
+      double* const g = group_of(v);
+      const float4 x0 = reinterpret_cast<const float4*>(g)[0], x1 = reinterpret_cast<const float4*>(g)[1];
+      const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+      double e[8];
 #pragma unroll
-      for (int j0 = 0; j0 < 8; j0 += 4) {
-        double e[4];  // four at once, without branches: they are chains of dependent fp64 instructions
+      for (int j = 0; j < 8; ++j) e[j] = exp_table(x[j], scale, mine, table);
+      if (v + 8 > hi) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float x = ids[j0 + j] < hi ? *reinterpret_cast<const float*>(&at(ids[j0 + j])) : -INFINITY;
-          // -inf gives 0; a CTA whose maximum is NaN or +inf ends the walk below
-          e[j] = exp_table(widen(x), scale, mine, table);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (ids[j0 + j] < hi) at(ids[j0 + j]) = e[j];
-          part += e[j];
-        }
+        for (int j = 0; j < 8; ++j)
+          if (v + j >= hi) e[j] = 0;
       }
+      store_group(g, e);
+      part += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
     }
     exchange(part, top);
     float most = -INFINITY;
@@ -463,19 +509,32 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
       }
       break;
     }
+    // ---- what the ranks' weights count, and the children's r
+    const double all = widen(most) * scale;
+    auto factor_of = [&](int c) {
+      const float m = ex.top[last_turn][c];
+      return m > -INFINITY ? exp_table(m, scale, all, table) : 0.0;
+    };
     if (warp == 0) {
       const int c = lane & (kMaxRanks - 1);
-      const double f = c < ranks ? exp_table(widen(ex.top[last_turn][c]), scale, widen(most) * scale, table) : 0.0;
+      const double f = c < ranks ? factor_of(c) : 0.0;
       double z = c < ranks ? f * ex.sum[last_turn][c] : 0.0;
 #pragma unroll
       for (int o = kMaxRanks / 2; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
       if (lane < ranks) factor[lane] = f;
       if (lane == 0) all_weights = z;
-      __syncwarp();
+    } else if (warp == 1) {
       for (int i = lane; i < children; i += 32) {
-        const float x = *reinterpret_cast<const float*>(&child_r[i]);
-        const int owner = max(node_x[walk.child[i]], 0) / per_rank;
-        child_r[i] = exp_table(widen(x), scale, widen(ex.top[last_turn][owner]) * scale, table) * factor[owner];
+        const int x = node_x[walk.child[i]];
+        double p = 0;
+        if (x >= 0) {
+          const int owner = x / per_rank;
+          const float m = ex.top[last_turn][owner];
+          if (m > -INFINITY)
+            p = exp_table(*reinterpret_cast<const float*>(&child_r[i]), scale, widen(m) * scale, table) *
+                factor_of(owner);
+        }
+        child_r[i] = p;
       }
     }
     __syncthreads();
@@ -485,9 +544,9 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
     bool stale = false;  // the runs' sums are not r's
     int found = -1;
     for (int i = 0; i < children; ++i) {
-      const double rx = child_r[i], qx = PROBS ? (double)child_q[i] : 1.0;
+      const double rx = child_r[i], qx = PROBS ? widen(child_q[i]) : 1.0;
       const int child = walk.child[i], x = node_x[child];
-      if ((double)node_u[child] * qx * total < rx) {
+      if (rx > kNothing && (double)node_u[child] * qx * total < rx) {
         found = child;
         break;
       }
@@ -496,18 +555,22 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
         const double inv = 1.0 / total;
         part = 0;
 #pragma unroll 1
-        for (int base = lo; base < hi; base += kBlockIds) {
-          const Ids ids(base, hi, vec, lane);
+        for (int base = lo; base < last_block; base += kBlockIds) {
+          const Ids ids(base, hi, true, lane);
+          double* const g = group_of(ids.first);
           float qv[8];
           load_ids(q, vec_q, ids, 0.f, qv);
+          double w[8], sum = 0;
+          load_group(g, w);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            double v = ids[j] < hi ? at(ids[j]) * mult : 0.0;
             const double qj = widen(qv[j]);
-            if (pending != 0) v = fmax(fma(v, pending, -qj), 0.0);
-            if (ids[j] < hi) at(ids[j]) = v;
-            part += fmax(fma(v, inv, -qj), 0.0);
+            w[j] *= mult;
+            if (pending != 0) w[j] = positive(fma(w[j], pending, -qj));
+            sum += positive(fma(w[j], inv, -qj));
           }
+          store_group(g, w);
+          part += sum;
         }
         mult = 1;
         exchange(part, 0.f);
@@ -517,10 +580,10 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
         if (left > 0) {
           total = left;
           for (int c = threadIdx.x; c < children; c += kVerifyThreads)
-            child_r[c] = fmax(fma(child_r[c], inv, -widen(child_q[c])), 0.0);
+            child_r[c] = positive(fma(child_r[c], inv, -widen(child_q[c])));
           __syncthreads();
         }
-      } else if (rx > 0) {
+      } else if (rx > kNothing) {
         __syncthreads();
         for (int c = threadIdx.x; c < children; c += kVerifyThreads)
           if (node_x[walk.child[c]] == x) child_r[c] = 0;
@@ -535,21 +598,31 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
       ++depth;
       __syncthreads();  // the children have been read
       if (threadIdx.x == 0) {
-        walk.path[depth] = cur;
+        walk.path[depth] = (int16_t)cur;
         walk.on_path[cur >> 5] |= 1u << (cur & 31);
       }
       continue;
     }
 
     // ---- the next token
-    auto weight = [&](int v) {
-      double w = at(v) * mult;
-      if (PROBS && pending != 0) w = fmax(fma(w, pending, -widen(q[v])), 0.0);
-      return w;
+    auto group_weights = [&](const Ids& ids, double (&w)[8]) {  // r of a lane's group
+      load_group(group_of(ids.first), w);
+      float qv[8];
+      if (PROBS && pending != 0) load_ids(q, vec_q, ids, 0.f, qv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        w[j] *= mult;
+        if (PROBS && pending != 0) w[j] = positive(fma(w[j], pending, -widen(qv[j])));
+      }
     };
     if (stale) {
       part = 0;
-      for (int v = lo + lane; v < hi; v += 32) part += weight(v);
+      for (int base = lo; base < last_block; base += kBlockIds) {
+        double w[8];
+        group_weights(Ids(base, hi, true, lane), w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) part += w[j];
+      }
       exchange(part, 0.f);
     }
     // the first pass's sums are over the ranks' own maxima, later ones are r's
@@ -562,7 +635,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
     int owner = -1;
     for (int c = 0; c < ranks; ++c) {
       const double w = rank_sum(c);
-      if (w > 0) {
+      if (w > kNothing) {
         owner = c;
         owner_before = before;
         if (before + w > target) break;
@@ -575,7 +648,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
       before = owner_before;
       for (int w = 0; w < kVerifyWarps; ++w) {
         const double x = warp_sum_of[w] * (direct ? 1.0 : mult);
-        if (x > 0) {
+        if (x > kNothing) {
           own_warp = w;
           warp_before = before;
           if (before + x > target) break;
@@ -585,14 +658,14 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
       if (warp == own_warp) {
         before = warp_before;
         int pick = -1;
-        for (int base = lo; base < hi; base += kBlockIds) {
+        for (int base = lo; base < last_block; base += kBlockIds) {
           const Ids ids(base, hi, true, lane);
           double w[8], sum = 0;
+          group_weights(ids, w);
           int last = -1;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            w[j] = ids[j] < hi ? weight(ids[j]) : 0.0;
-            if (w[j] > 0) last = ids[j];
+            if (w[j] > kNothing) last = ids[j];
             sum += w[j];
           }
           double upto = sum;
@@ -610,7 +683,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
 #pragma unroll
             for (int j = 0; j < 8; ++j) {  // the first one past the target
               c += w[j];
-              if (w[j] > 0 && c > target) {
+              if (w[j] > kNothing && c > target) {
                 pick = ids[j];
                 c = -INFINITY;
               }
@@ -634,7 +707,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
 }
 
 constexpr size_t kWeightBytes = 190 * 1024;  // beside the static shared memory
-constexpr int kMaxSampleVocab = 327680;
+constexpr int kMaxSampleVocab = 262144;
 
 template <typename Kernel>
 cudaError_t launch_cluster(Kernel kernel, const VerifyArgs& a, int requests, size_t smem, bool (&configured)[64],
@@ -662,7 +735,7 @@ int warp_run(int vocab, int ranks) {
   const int blocks = (vocab + kBlockIds - 1) / kBlockIds, warps = ranks * kVerifyWarps;
   return (blocks + warps - 1) / warps * kBlockIds;
 }
-size_t weight_bytes(int run) { return (size_t)run * kVerifyWarps * 9; }
+size_t weight_bytes(int run) { return (size_t)run * kVerifyWarps / 8 * kGroupPlaces * sizeof(double); }
 
 template <typename T>
 cudaError_t launch_verify(VerifyArgs a, int requests, bool greedy, cudaStream_t stream) {
@@ -712,8 +785,8 @@ extern "C" int aiosb_verify_draft(const void* logits, int logits_fp32, int64_t l
                 "verify_draft: vocabulary too large (sampling: at most %d)", kMaxSampleVocab);
   AIOSB_REQUIRE(logits_stride >= vocab || tokens <= 1, AIOSB_ERR_INVALID_ARG,
                 "verify_draft: logits row stride below the vocabulary");
-  AIOSB_REQUIRE(greedy || (temperature > 0 && 1.0 / temperature > 0 && 1.0 / temperature < 1e30),
-                AIOSB_ERR_INVALID_ARG, "verify_draft: the temperature must be positive");
+  AIOSB_REQUIRE(greedy || (temperature >= 1e-6 && temperature <= 1e6), AIOSB_ERR_INVALID_ARG,
+                "verify_draft: the temperature must be in [1e-6, 1e6]");
   AIOSB_REQUIRE(!(greedy && draft_probs != nullptr), AIOSB_ERR_INVALID_ARG,
                 "verify_draft: greedy verification takes no draft_probs");
   AIOSB_REQUIRE(draft_probs == nullptr || probs_stride >= vocab || tokens <= 1, AIOSB_ERR_INVALID_ARG,

@@ -1205,8 +1205,8 @@ def verify_draft(
     drawn from, independently) or 1 without it (distinct proposals). With no child left the next
     token is drawn from r by inverse CDF with ``sample_uniforms``. What is kept has the target's
     distribution. ``greedy``: children and next token by argmax (the lowest id of equal ones).
-    A sampler's filters (top-k, forbidden ids) go in as logits of -inf. Sampling takes up to 327680
-    ids.
+    A sampler's filters (top-k, forbidden ids) go in as logits of -inf. Sampling takes up to 262144
+    ids and temperatures in [1e-6, 1e6].
 
     Returns ``accepted`` (int32 [requests]: nodes behind the root that stay), ``next_token``
     (int64 [requests]; -1 where there is no tree or no distribution) and ``order`` (int32

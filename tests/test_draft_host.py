@@ -76,14 +76,15 @@ def test_verify_draft_refuses() -> None:
     _refused(name, good, INV, "bad sizes", tokens=-1)
     _refused(name, good, INV, "bad sizes", vocab=0)
     _refused(name, good, INV, "bad sizes", requests=1 << 29)
-    _refused(name, good, UNS, "too large", vocab=327681, ls=327681)
+    _refused(name, good, UNS, "too large", vocab=262145, ls=262145)
     _refused(name, good, UNS, "too large", vocab=1 << 31, ls=1 << 31, greedy=1)
     _refused(name, good, INV, "logits row stride", ls=99)
     _refused(name, good, INV, "temperature", temperature=0.0)
     _refused(name, good, INV, "temperature", temperature=-1.0)
     _refused(name, good, INV, "temperature", temperature=float("nan"))
     _refused(name, good, INV, "temperature", temperature=float("inf"))
-    _refused(name, good, INV, "temperature", temperature=1e-31)
+    _refused(name, good, INV, "temperature", temperature=0.9e-6)
+    _refused(name, good, INV, "temperature", temperature=1.1e6)
     _refused(name, good, INV, "greedy", greedy=1, probs=P, ps=100)
     _refused(name, good, INV, "draft_probs row stride", probs=P, ps=99)
     _refused(name, good, INV, "uniforms", au=None)

@@ -130,7 +130,7 @@ def test_verify(cuda_device, sizes, vocab: int, mode: str) -> None:
     ops.check_status(cuda_device)
 
 
-@pytest.mark.parametrize("vocab", [50021, 131072, 151111, 262144, 327680])
+@pytest.mark.parametrize("vocab", [50021, 131072, 151111, 160001, 262144])
 @pytest.mark.parametrize("probs", [False, True])
 def test_verify_large_vocabularies(cuda_device, vocab: int, probs: bool) -> None:
     sizes = [12, 7, 1]
@@ -182,6 +182,18 @@ def test_a_draft_equal_to_the_target_leaves_nothing(cuda_device) -> None:
             torch.tensor([0.6]).cuda())
     accepted, token, order = ops.verify_draft(*args, draft_probs=q.cuda())
     assert accepted.tolist() == [0] and token.tolist() == [2] and order.tolist() == [0, 1]
+
+
+@pytest.mark.parametrize("temperature", [1e-6, 1e-3, 0.02, 30.0, 1e6])
+@pytest.mark.parametrize("spread", [1e-3, 3.0, 3e4])
+def test_temperatures(cuda_device, temperature: float, spread: float) -> None:
+    sizes = [9, 4]
+    for probs in (False, True):
+        case = _case(sizes, 1200, probs=probs, seed=8, dtype=torch.float32, spread=spread)
+        case[1][:, 1000:1100] = -float("inf")
+        want = ref.verify(case[1], case[2], case[0], case[3], case[4], temperature=temperature, probs=case[5])
+        assert _run(case, sizes, temperature=temperature) == [list(w) for w in want]
+    ops.check_status(cuda_device)
 
 
 def test_masked_logits(cuda_device) -> None:
