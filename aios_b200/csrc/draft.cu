@@ -11,49 +11,58 @@ namespace {
 // ---- ancestors' bits -------------------------------------------------------------------------
 constexpr int kTreeThreads = 256;
 
-// A CTA per tree, a thread per node: it walks from the node to its root through the parents in shared memory. The
-// numbers fall on the way, so that one word of bits is held at a time. Bound by the walk's dependent loads, some 30
-// clocks a level: 256 trees of up to 256 nodes, up to 57 deep, take 7 us (with a warp per node, 32 words at a time,
-// 79).
+// A CTA per tree, by doubling: with every node's bits of its 2^k nearest ancestors (itself among them) and its 2^k-th
+// ancestor known, the ancestor's bits or-ed into its own are those of 2^(k + 1). So a chain of 256 takes eight rounds,
+// where a walk from each node to its root takes 256 dependent loads (63 us; 256 mixed trees of up to 256 nodes 13.5).
+// Bits may be or-ed while their owner adds to them: what it adds are ancestors as well. The ancestors' numbers have
+// two buffers.
 __global__ void __launch_bounds__(kTreeThreads)
     draft_tree_kernel(const int32_t* parents, const int32_t* tree_start, int tokens, int words,
                       const int32_t* cached_lens, int32_t* mask, int32_t* positions, int32_t* status) {
-  __shared__ int16_t up[AIOSB_TREE_MAX_NODES];
-  const int r = blockIdx.x;
+  extern __shared__ uint32_t bits[];  // [words, 32 * words]: a word of all nodes side by side
+  __shared__ int16_t up[2][AIOSB_TREE_MAX_NODES], depth[2][AIOSB_TREE_MAX_NODES];
+  const int r = blockIdx.x, most = 32 * words;
   pdl_enter();
   const int s = tree_start[r], e = tree_start[r + 1];
   const int base = cached_lens != nullptr ? cached_lens[r] : 0;
-  const int start = min(max(s, 0), tokens), n = min(max(e, start), tokens) - start;
-  if (threadIdx.x == 0 && (s < 0 || e < s || e > tokens || n > words * 32)) report(status, AIOSB_DEV_TREE_RANGE);
-  const int staged = min(n, AIOSB_TREE_MAX_NODES);
-  for (int i = threadIdx.x; i < staged; i += kTreeThreads) {
+  const int start = min(max(s, 0), tokens), all = min(max(e, start), tokens) - start, n = min(all, most);
+  if (threadIdx.x == 0 && (s < 0 || e < s || e > tokens || all > n)) report(status, AIOSB_DEV_TREE_RANGE);
+  int open = 0;
+  for (int i = threadIdx.x; i < n; i += kTreeThreads) {
     int p = parents[start + i];
     if (p < -1 || p >= i) {
       report(status, AIOSB_DEV_TREE_RANGE);
       p = -1;
     }
-    up[i] = (int16_t)p;
+    up[0][i] = (int16_t)p;
+    depth[0][i] = p >= 0;
+    for (int w = 0; w < words; ++w) bits[w * most + i] = w == i >> 5 ? 1u << (i & 31) : 0u;
+    open |= p >= 0;
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kTreeThreads) {
-    int32_t* const row = mask + (int64_t)(start + i) * words;
-    int depth = -1, word = words - 1;
-    uint32_t bits = 0;
-    // a node behind the staged ones (reported above) has itself alone
-    for (int j = i; j >= 0; j = j < staged ? up[j] : -1) {
-      const int w = j >> 5;
-      for (; word > w; --word) {
-        row[word] = (int32_t)bits;
-        bits = 0;
+  int now = 0;
+  while (__syncthreads_or(open)) {
+    open = 0;
+    for (int i = threadIdx.x; i < n; i += kTreeThreads) {
+      const int a = up[now][i], d = depth[now][i];
+      int next = -1, far = d;
+      if (a >= 0) {
+        next = up[now][a];
+        far += depth[now][a];
+        for (int w = 0; w <= a >> 5; ++w) bits[w * most + i] |= bits[w * most + a];  // ancestors' numbers are lower
       }
-      if (w == word) bits |= 1u << (j & 31);  // bits that the words do not hold are left out
-      ++depth;
+      up[now ^ 1][i] = (int16_t)next;
+      depth[now ^ 1][i] = (int16_t)far;
+      open |= next >= 0;
     }
-    for (; word >= 0; --word) {
-      row[word] = (int32_t)bits;
-      bits = 0;
-    }
-    positions[start + i] = base + depth;
+    now ^= 1;
+  }
+  for (int i = threadIdx.x; i < n * words; i += kTreeThreads)
+    mask[(int64_t)start * words + i] = (int32_t)bits[i % words * most + i / words];
+  for (int i = threadIdx.x; i < n; i += kTreeThreads) positions[start + i] = base + depth[now][i];
+  // nodes behind those that the words hold (reported above): nothing known
+  for (int i = n + threadIdx.x; i < all; i += kTreeThreads) {
+    for (int w = 0; w < words; ++w) mask[(int64_t)(start + i) * words + w] = 0;
+    positions[start + i] = base;
   }
 }
 
@@ -768,9 +777,14 @@ extern "C" int aiosb_draft_tree(const int32_t* parents, int64_t tokens, const in
                 "draft_tree: %lld mask words; a tree has at most %d nodes", (long long)words, AIOSB_TREE_MAX_NODES);
   if (tokens == 0 || requests == 0) return AIOSB_OK;
   AIOSB_REQUIRE(parents && tree_start && mask && positions, AIOSB_ERR_INVALID_ARG, "draft_tree: null pointer");
-  return check_launch("draft_tree", launch_pdl(draft_tree_kernel, dim3((unsigned)requests), dim3(kTreeThreads), 0,
-                                               as_stream(stream), parents, tree_start, (int)tokens, (int)words,
-                                               cached_lens, mask, positions, status));
+  static bool configured[64] = {false};
+  constexpr int most = AIOSB_TREE_MAX_NODES / 32 * (AIOSB_TREE_MAX_NODES / 32) * 128;  // bytes of `bits`
+  cudaError_t result = allow_shared(draft_tree_kernel, most, configured);
+  if (result == cudaSuccess)
+    result = launch_pdl(draft_tree_kernel, dim3((unsigned)requests), dim3(kTreeThreads), (size_t)(words * words * 128),
+                        as_stream(stream), parents, tree_start, (int)tokens, (int)words, cached_lens, mask, positions,
+                        status);
+  return check_launch("draft_tree", result);
 }
 
 extern "C" int aiosb_verify_draft(const void* logits, int logits_fp32, int64_t logits_stride, int64_t tokens,

@@ -465,7 +465,7 @@ AIOSB_API int aiosb_stateless_uniforms(const int64_t* seeds, int64_t rows, int64
 /* mask[i] ([tokens, words] int32): bit j % 32 of word j / 32 is set if node j of the
  * same tree is node i or an ancestor of it; positions[i] = cached_lens[r] (or 0, if
  * NULL) + the number of its ancestors. A node that does not fit the words
- * (32 * words nodes a tree) gets its earlier ancestors only. */
+ * (32 * words nodes a tree) gets no bits and position cached_lens[r]. */
 AIOSB_API int aiosb_draft_tree(const int32_t* parents, int64_t tokens, const int32_t* tree_start, int64_t requests,
                                int64_t words, const int32_t* cached_lens, int32_t* mask, int32_t* positions,
                                int32_t* status, void* stream);
