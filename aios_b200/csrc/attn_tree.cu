@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(kThreads) attn_tree_small_kernel(const TreeAtt
     for (int i = threadIdx.x; i < kChunk * (D / 8); i += kThreads) {
       const int j = i / (D / 8), c = i % (D / 8);
       if (k0 + j < t.keys) {
-        const int64_t at = (tree_slot(a, t.slots[k0 + j]) * a.hkv + h) * D + c * 8;
+        const int64_t at = (tree_slot(a, a.page_table[t.table + k0 + j]) * a.hkv + h) * D + c * 8;
         cp_async16(ks + j * kPitch<D> + c * 8, a.k_cache + at);
         cp_async16(vs + j * kPitch<D> + c * 8, a.v_cache + at);
       } else {  // weights of keys past the end are 0, and 0 times what lies there must be 0
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kThreads) attn_tree_small_kernel(const TreeAtt
         for (int j = 0; j < kChunk; ++j) {
           if (!((bad[j / 32] >> (j % 32)) & 1)) continue;
           const int key = k0 + j, b = key - t.cached;
-          const __nv_bfloat16* v = a.v_cache + (tree_slot(a, t.slots[key]) * a.hkv + h) * D;
+          const __nv_bfloat16* v = a.v_cache + (tree_slot(a, a.page_table[t.table + key]) * a.hkv + h) * D;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             if (b >= 0 && !(((uint32_t)bits[i][b >> 5] >> (b & 31)) & 1)) continue;

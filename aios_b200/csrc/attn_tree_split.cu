@@ -86,8 +86,8 @@ struct Pieces {
   TreeRequest t;
   int64_t w, span;
 
-  __device__ __forceinline__ void request(const TreeAttnArgs& a) {
-    t = tree_request(a, r, false);
+  __device__ __forceinline__ void take(const TreeAttnArgs& a, const TreeRequest& request) {
+    t = request;
     w = unit_weight(t);
     span = w * unit_blocks(a, t) * a.hkv;
   }
@@ -96,7 +96,7 @@ struct Pieces {
       while (pos >= base + span) {
         base += span;
         ++r;
-        request(a);
+        take(a, tree_request(a, r, false));
       }
       const int blocks = unit_blocks(a, t);
       // (64-bit divisions only for what no memory holds)
@@ -285,6 +285,7 @@ struct Shared {
   volatile int abort_flag;
   int r0;
   int64_t pos, end, base;  // this CTA's range, and where the first request of it starts
+  TreeRequest first;
   Cut cut;
   float2 few_state[kSoftWarps][16];  // (reference, sum) of the warps' rows, in a piece of few rows
   uint32_t bad[kBadSlots][AIOSB_TREE_MAX_NODES / 32];  // per piece: tree keys whose V holds an infinity or a NaN
@@ -330,9 +331,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
   }
   pdl_wait();
   if (warp == 0) {  // the weight of all units, and where this CTA's range starts
+    TreeRequest t;  // of the last request that this lane looked at
     auto weight_of = [&](int r, bool tell) {
       if (r >= a.requests) return (int64_t)0;
-      const TreeRequest t = tree_request(a, r, tell);
+      t = tree_request(a, r, tell);
       return unit_weight(t) * unit_blocks(a, t) * a.hkv;
     };
     const int64_t first = weight_of(lane, blockIdx.x == 0);
@@ -348,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
     int64_t base = 0;
     int found = 0;
     for (int r0 = 0; used; r0 += 32) {
-      const int64_t w = r0 == 0 ? first : weight_of(r0 + lane, false);
+      const int64_t w = a.requests <= 32 ? first : weight_of(r0 + lane, false);
       int64_t upto = w;
 #pragma unroll 1
       for (int o = 1; o < 32; o <<= 1) {
@@ -360,6 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
         const int l = __ffs(hit) - 1;
         found = r0 + l;
         base += __shfl_sync(0xffffffffu, upto - w, l);
+        if (lane == l) sh.first = t;
         break;
       }
       base += __shfl_sync(0xffffffffu, upto, 31);
@@ -385,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
   it.end = sh.end;
   it.base = sh.base;
   it.r = sh.r0;
-  if (it.pos < it.end) it.request(a);
+  if (it.pos < it.end) it.take(a, sh.first);
   Piece p = {};
 
   if (warp >= kSoftWarps && warp < kMmaWarp) {
@@ -403,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int key = (chunk + j) * kKeys + lw * 32 + lane;
-        out[j] = key < min(p.t.keys, p.c1 * kKeys) ? p.t.slots[key] : 0;
+        out[j] = key < min(p.t.keys, p.c1 * kKeys) ? a.page_table[p.t.table + key] : 0;
       }
     };
     auto load = [&](bool values, int chunk) {
@@ -775,7 +778,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
           for (int j = 0; j < a.words; ++j) {
             for (uint32_t hit = sh.bad[turn][j] & (uint32_t)own[j]; hit; hit &= hit - 1) {
               const int key = p.t.cached + j * 32 + __ffs(hit) - 1;
-              const __nv_bfloat16* x = a.v_cache + (tree_slot(a, p.t.slots[key]) * a.hkv + p.h) * D + c4 * 4;
+              const __nv_bfloat16* x = a.v_cache + (tree_slot(a, a.page_table[p.t.table + key]) * a.hkv + p.h) * D + c4 * 4;
               float* const e = &v.x;
               for (int z = 0; z < 4; ++z) {
                 const float y = bf16_to_f(x[z]);
@@ -933,7 +936,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
               for (uint32_t hit = sh.bad[turn][w] & (uint32_t)bits[w]; hit; hit &= hit - 1) {
                 const int key = p.t.cached + w * 32 + __ffs(hit) - 1;
                 const __nv_bfloat16* x =
-                    a.v_cache + (tree_slot(a, p.t.slots[key]) * a.hkv + p.h) * D + j * 16;
+                    a.v_cache + (tree_slot(a, a.page_table[p.t.table + key]) * a.hkv + p.h) * D + j * 16;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                   const float y = bf16_to_f(x[e]);

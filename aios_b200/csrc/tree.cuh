@@ -36,7 +36,7 @@ struct TreeAttnArgs {
 struct TreeRequest {
   int start, nodes;  // rows of the flat token arrays
   int cached, keys;  // keys [0, cached) are history, [cached, keys) the tree's
-  const int32_t* slots;
+  int64_t table;  // of its page-table row, in entries
 };
 
 // Request r with its numbers held inside the arrays; `tell`: report what had to be cut.
@@ -49,7 +49,7 @@ __device__ __forceinline__ TreeRequest tree_request(const TreeAttnArgs& a, int r
   const bool row_ok = row >= 0 && row < a.table_rows;
   t.cached = row_ok ? min(max(c, 0), a.table_width) : 0;
   t.keys = row_ok ? t.cached + min(t.nodes, a.table_width - t.cached) : 0;
-  t.slots = a.page_table + (row_ok ? row : 0) * a.table_stride;
+  t.table = (row_ok ? row : 0) * a.table_stride;
   if (tell && (s < 0 || e < s || e > a.tokens || t.nodes != nodes ||
                (nodes > 0 && (t.cached != c || t.keys - t.cached != t.nodes))))
     report(a.status, AIOSB_DEV_TREE_RANGE);
