@@ -34,8 +34,12 @@ constexpr int kLoadWarps = 4;
 constexpr int kMmaWarp = kSoftWarps + kLoadWarps;
 constexpr int kThreads = (kMmaWarp + 2) * 32;
 constexpr int kAtomBytes = kKeys * 128;  // 128 rows of 64 values, 128-byte swizzled
-constexpr int kUnitCost = 1;             // a unit's start and end, in chunks
-constexpr int kMinShare = 3;             // weight below which a range is not worth a CTA
+// Weights of the cut: a chunk of a unit of up to 128 rows, of a wider one, a unit's start and end, and the least range
+// that is worth a CTA (above kWideCost, so that every range inside a unit has a chunk's start). Fitted: 41 ragged requests
+// of up to 264 rows 105 us with chunks and units of equal weight, 100 with 2, 4, 5, 6, 87 with these; 16 x 1900 keys
+// 20.7, 18.2 and 18.3, and 23 with a least range of 8.
+constexpr int kChunkCost = 2, kWideCost = 4, kUnitCost = 12, kMinShare = 5;
+constexpr int kPieceSlots = 8;
 constexpr int kMaxGrid = 256;            // ranges: the join holds a weight for each of a unit's pieces and 32 rows
 constexpr int kBadSlots = 8;
 constexpr float kRescaleAt = 8.f;
@@ -62,7 +66,7 @@ struct Piece {
   int h;
   int row0, rows;  // rows of the unit, in the request's (node, head) pairs
   int c0, c1, chunks;
-  int64_t first_at;  // position of the unit's first chunk
+  int64_t last_at;  // position of the unit's last chunk
   __device__ __forceinline__ bool whole() const { return c0 == 0 && c1 == chunks; }
   __device__ __forceinline__ bool pair() const { return rows > kTile; }
   __device__ __forceinline__ bool few() const { return rows <= kFewRows; }
@@ -72,24 +76,35 @@ struct Piece {
 // fp32 is off by 2^-23 of it.
 __device__ __forceinline__ int node_of(int x, float inv_group) { return (int)(((float)x + 0.5f) * inv_group); }
 
-__device__ __forceinline__ int64_t unit_weight(const TreeRequest& t) {
-  return max(1, (t.keys + kKeys - 1) / kKeys) + kUnitCost;
-}
-__device__ __forceinline__ int unit_blocks(const TreeAttnArgs& a, const TreeRequest& t) {
-  return (t.nodes * a.group + kUnitRows - 1) / kUnitRows;
-}
+// Of a request, for each KV head: `full` units of 256 rows, and one of the rest.
+struct Units {
+  int chunks, full, rest;  // rest: rows of the last unit, 0 if there is none
+  int64_t wide, last;      // weights of a unit of 256 rows and of the last one
+  __device__ __forceinline__ Units() {}
+  __device__ __forceinline__ Units(const TreeAttnArgs& a, const TreeRequest& t) {
+    const int rows = t.nodes * a.group;
+    chunks = max(1, (t.keys + kKeys - 1) / kKeys);
+    full = rows / kUnitRows;
+    rest = rows - full * kUnitRows;
+    wide = (int64_t)chunks * kWideCost + kUnitCost;
+    last = rest > 0 ? (int64_t)chunks * (rest > kTile ? kWideCost : kChunkCost) + kUnitCost : 0;
+  }
+  __device__ __forceinline__ int64_t head() const { return full * wide + last; }
+};
 
-// The pieces of a range, in order. Every warp walks its own: a few loads a piece, ahead of what uses it.
+// The pieces of a range, in order. The gathering warps walk them, ahead of the others, and the first one of them hands
+// them on (sh.pieces).
 struct Pieces {
   int64_t pos, end, base;
   int r;
   TreeRequest t;
-  int64_t w, span;
+  Units u;
+  int64_t span;
 
   __device__ __forceinline__ void take(const TreeAttnArgs& a, const TreeRequest& request) {
     t = request;
-    w = unit_weight(t);
-    span = w * unit_blocks(a, t) * a.hkv;
+    u = Units(a, t);
+    span = u.head() * a.hkv;
   }
   __device__ __forceinline__ bool next(const TreeAttnArgs& a, Piece& p) {
     while (pos < end) {
@@ -98,21 +113,27 @@ struct Pieces {
         ++r;
         take(a, tree_request(a, r, false));
       }
-      const int blocks = unit_blocks(a, t);
       // (64-bit divisions only for what no memory holds)
-      const int64_t unit = span >> 32 ? (pos - base) / w : (int64_t)((uint32_t)(pos - base) / (uint32_t)w);
-      const int64_t at = base + unit * w;
-      const int64_t stop = min(end, at + w);
-      p.c0 = (int)max((int64_t)0, pos - at - kUnitCost);
-      p.c1 = (int)(stop - at - kUnitCost);
+      const int64_t off = pos - base, per_head = u.head();
+      const bool small = span >> 32 == 0;
+      const int h = (int)(small ? (uint32_t)off / (uint32_t)per_head : off / per_head);
+      const int64_t in_head = off - h * per_head;
+      const int block = min(u.full, (int)(small ? (uint32_t)in_head / (uint32_t)u.wide : in_head / u.wide));
+      const bool is_last = block == u.full;
+      const int cost = is_last && u.rest <= kTile ? kChunkCost : kWideCost;
+      const int64_t at = base + h * per_head + block * u.wide, stop = min(end, at + (is_last ? u.last : u.wide));
+      // chunk i starts at at + kUnitCost + i * cost, and belongs to the range with its start
+      const int64_t from = pos - at - kUnitCost, to = stop - at - kUnitCost;
+      p.c0 = from <= 0 ? 0 : (int)((from + cost - 1) / cost);
+      p.c1 = to <= 0 ? 0 : (int)((to + cost - 1) / cost);
       pos = stop;
       if (p.c1 <= p.c0) continue;
       p.t = t;
-      p.h = (int)((uint32_t)unit / (uint32_t)blocks);
-      p.row0 = (int)((uint32_t)unit % (uint32_t)blocks) * kUnitRows;
-      p.rows = min(kUnitRows, t.nodes * a.group - p.row0);
-      p.chunks = (int)w - kUnitCost;
-      p.first_at = at + kUnitCost;
+      p.h = h;
+      p.row0 = block * kUnitRows;
+      p.rows = is_last ? u.rest : kUnitRows;
+      p.chunks = u.chunks;
+      p.last_at = at + kUnitCost + (int64_t)(u.chunks - 1) * cost;
       return true;
     }
     return false;
@@ -280,12 +301,13 @@ __device__ __forceinline__ bool soft_step(uint32_t t_s, uint32_t t_o, const uint
 
 struct Shared {
   uint64_t full[10], empty[10];
-  uint64_t s_full[2][2], p_full[2][2], pv_done[2], q_full, piece_done, met, drained;
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2], q_full, piece_done, met, drained, piece_ready[kPieceSlots], piece_read[kPieceSlots];
   uint32_t tmem_slot;
   volatile int abort_flag;
   int r0;
   int64_t pos, end, base;  // this CTA's range, and where the first request of it starts
   TreeRequest first;
+  Piece pieces[kPieceSlots];  // rows 0: no more
   Cut cut;
   float2 few_state[kSoftWarps][16];  // (reference, sum) of the warps' rows, in a piece of few rows
   uint32_t bad[kBadSlots][AIOSB_TREE_MAX_NODES / 32];  // per piece: tree keys whose V holds an infinity or a NaN
@@ -320,6 +342,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
     mbar_init(&sh.piece_done, 2);
     mbar_init(&sh.met, kSoftWarps);
     mbar_init(&sh.drained, 2);
+    for (int i = 0; i < kPieceSlots; ++i) {
+      mbar_init(&sh.piece_ready[i], 1);
+      mbar_init(&sh.piece_read[i], kSoftWarps + 2);
+    }
     sh.abort_flag = 0;
     fence_mbar_init();
   }
@@ -335,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
     auto weight_of = [&](int r, bool tell) {
       if (r >= a.requests) return (int64_t)0;
       t = tree_request(a, r, tell);
-      return unit_weight(t) * unit_blocks(a, t) * a.hkv;
+      return Units(a, t).head() * a.hkv;
     };
     const int64_t first = weight_of(lane, blockIdx.x == 0);
     int64_t total = first;
@@ -383,13 +409,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
   const int me = blockIdx.x;
   const float inv_group = 1.f / (float)a.group;
 
-  Pieces it;
-  it.pos = sh.pos;
-  it.end = sh.end;
-  it.base = sh.base;
-  it.r = sh.r0;
-  if (it.pos < it.end) it.take(a, sh.first);
   Piece p = {};
+  uint32_t piece_number = 0;
+  auto next_piece = [&](bool& ok) {
+    const uint32_t slot = piece_number % kPieceSlots;
+    ok = __all_sync(0xffffffffu, mbar_wait(&sh.piece_ready[slot], (piece_number / kPieceSlots) & 1));
+    if (!ok) return false;
+    ++piece_number;
+    p = sh.pieces[slot];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.piece_read[slot]);
+    return p.rows > 0;
+  };
 
   if (warp >= kSoftWarps && warp < kMmaWarp) {
     // ---- gather
@@ -479,8 +510,27 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
         phase ^= 1;
       }
     };
+    Pieces it;
+    it.pos = sh.pos;
+    it.end = sh.end;
+    it.base = sh.base;
+    it.r = sh.r0;
+    if (it.pos < it.end) it.take(a, sh.first);
+    auto hand_on = [&] {
+      if (lw != 0) return;
+      const uint32_t slot = piece_number % kPieceSlots;
+      // its last piece has been read by all
+      ok = __all_sync(0xffffffffu, mbar_wait(&sh.piece_read[slot], ((piece_number / kPieceSlots) & 1) ^ 1));
+      if (!ok) return;
+      ++piece_number;
+      if (lane == 0) sh.pieces[slot] = p;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.piece_ready[slot]);
+    };
     // block order of a piece: the order in which the MMAs want them
     while (ok && it.next(a, p)) {
+      hand_on();
+      if (!ok) break;
       window = p.c0;
       ask(window, here);
       ask(window + 4, ahead);
@@ -499,6 +549,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       }
       turn = (turn + 1) % kBadSlots;
     }
+    if (ok) {
+      p.rows = 0;
+      hand_on();
+    }
     cp_async_wait_all();
     if (!ok) {
       report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
@@ -512,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
     const int s = warp - kMmaWarp;
     uint32_t base = 0, q_phase = 0, steps = 0;  // of the stream, in all pieces so far
     bool ok = true;
-    while (ok && it.next(a, p)) {
+    while (ok && next_piece(ok)) {
       const int n = p.c1 - p.c0;
       if (p.few()) {
         base += 2 * n;
@@ -612,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       join.row0 = p.row0;
       join.rows = p.rows;
       join.h = p.h;
-      if (threadIdx.x == 0) join.last = sh.cut.owner(p.first_at + p.chunks - 1);
+      if (threadIdx.x == 0) join.last = sh.cut.owner(p.last_at);
     };
     // Up to 32 rows: 16 to a warp on mma.sync, each warp with its share of every chunk's keys and its own maximum,
     // sum and output, joined at the end. The tensor pipe is idle here, but a TMEM round trip per step (scores out,
@@ -803,7 +857,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       if (warp == 0) sh.bad[(turn + kBadSlots - 1) % kBadSlots][lane] = 0;
       return true;
     };
-    while (ok && it.next(a, p)) {
+    while (ok && next_piece(ok)) {
       const bool pair = p.pair();
       // `tile` of Q's `count` rows, by 128 threads
       auto load_q = [&](int tile, int count) {
