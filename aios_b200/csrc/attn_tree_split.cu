@@ -32,7 +32,10 @@ constexpr int kStep = 64;       // keys of a softmax step, half a chunk
 constexpr int kSoftWarps = 8;
 constexpr int kLoadWarps = 4;
 constexpr int kMmaWarp = kSoftWarps + kLoadWarps;
-constexpr int kThreads = (kMmaWarp + 2) * 32;
+constexpr int kThreads = (kMmaWarp + 4) * 32;  // whole groups of four warps: two idle
+// Registers of a thread, by role: 2 x 176 + 96 + 64 = 4 x 128, what the block is launched with.
+constexpr int kSoftRegs = 176, kLoadRegs = 96, kMmaRegs = 64;
+static_assert(2 * kSoftRegs + kLoadRegs + kMmaRegs <= 65536 / kThreads * 4, "more registers than the block has");
 constexpr int kAtomBytes = kKeys * 128;  // 128 rows of 64 values, 128-byte swizzled
 // Weights of the cut: a chunk of a unit of up to 128 rows, of a wider one, a unit's start and end, and the least range
 // that is worth a CTA (above kWideCost, so that every range inside a unit has a chunk's start). Fitted: 41 ragged requests
@@ -424,6 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
 
   if (warp >= kSoftWarps && warp < kMmaWarp) {
     // ---- gather
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
     const int lw = warp - kSoftWarps;
     const int64_t slot_bytes = (int64_t)a.hkv * D * 2;
     int stage = 0;
@@ -559,6 +563,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       sh.abort_flag = 1;
     }
   } else if (warp >= kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
+    if (warp < kMmaWarp + 2) {
     // ---- MMAs of stream s: O += P V of its last step, then S of the step after next, so that scores are there when
     // the softmax comes to them. A warp for each stream: a wait that is over and the issue behind it take some
     // hundred clocks of a warp, in which the other's MMAs run.
@@ -643,8 +649,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       report(a.status, AIOSB_DEV_WAIT_TIMEOUT);
       sh.abort_flag = 1;
     }
+    }
   } else {
     // ---- softmax of stream s; a thread owns row `row` of the stream's tile
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
     const int s = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t t_o = t_lane + 256 + s * 128;
@@ -1032,7 +1040,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
 
   tc_fence_before();
   __syncthreads();
-  if (sh.abort_flag && warp >= kMmaWarp) {  // MMAs may still run: their end is waited for
+  if (sh.abort_flag && warp >= kMmaWarp && warp < kMmaWarp + 2) {  // MMAs may still run: their end is waited for
     if (elect_one()) tc_commit(&sh.drained);
     __syncwarp();
     mbar_wait(&sh.drained, 0);
