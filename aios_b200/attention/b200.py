@@ -5,7 +5,9 @@ Prefill runs the sm_100a prologue kernel (q/k RMSNorm + bf16 RoPE + KV store) an
 the causal paged prefill kernel; decode runs the cascade decode kernel, which
 reads each shared-prefix KV slot once per KV head for all candidate rows. The
 reference slot API ``forward(q, k, v, ...)`` (already normalised and rotated q/k)
-is served by the KV-store kernel plus the same attention kernels.
+is served by the KV-store kernel plus the same attention kernels. Draft batches
+(trees of drafted tokens, verified after the forward) run the prefill prologue with the
+nodes' positions and the tree attention.
 
 Metadata is device-resident: ``prepare_metadata`` uploads the few per-request
 integers once per batch (no host-side planning step), and the CandidateGroup
@@ -52,6 +54,12 @@ class B200AttentionMetadata(BaseAttentionMetadata):
     # position were written by earlier launches (the CandidateGroup runtime)
     stable_history: bool | int = False  # aiosb_attention_decode's history mode (0, 1 staged, 2 prefix-once)
     staged_prefix: int = 0  # bound on the prefix keys staged before the wait (0: the kernel's default)
+    # draft (row_table as for decode)
+    parents: torch.Tensor | None = None  # int32 [tokens]
+    tree_start: torch.Tensor | None = None  # int32 [bs + 1]
+    tree_mask: torch.Tensor | None = None  # int32 [tokens, words]
+    cached_lens: torch.Tensor | None = None  # int32 [bs]
+    max_cached: int = 0
 
     def get_last_indices(self, bs: int) -> torch.Tensor:
         assert self.cu_seqlens_q is not None, "last indices exist for prefill batches"
@@ -83,9 +91,12 @@ class B200AttentionBackend(BaseAttentionBackend):
     def prepare_metadata(self, batch: Batch) -> B200AttentionMetadata:
         ctx = get_global_ctx()
         device = ctx.page_table.device
-        positions = batch.positions.to(device=device, dtype=torch.int32)
         out_loc = batch.out_loc.to(device=device, dtype=torch.int32).view(-1)
         reqs = batch.reqs
+        if batch.is_draft:
+            batch.attn_metadata = md = self._draft_metadata(batch, out_loc)
+            return md
+        positions = batch.positions.to(device=device, dtype=torch.int32)
         if batch.is_prefill:
             q_lens = [r.extend_len for r in reqs]
             cu = [0]
@@ -118,6 +129,31 @@ class B200AttentionBackend(BaseAttentionBackend):
         batch.attn_metadata = md
         return md
 
+    @staticmethod
+    def _draft_metadata(batch: Batch, out_loc: torch.Tensor) -> B200AttentionMetadata:
+        if batch.trees is None or len(batch.trees) != len(batch.reqs):
+            raise ValueError("a draft batch needs one tree of parents per request")
+        sizes = [len(t) for t in batch.trees]
+        tokens, bs = sum(sizes), len(sizes)
+        if out_loc.numel() != tokens:
+            raise ValueError("a draft batch needs one slot per node")
+        if not tokens or max(sizes) > ops.TREE_MAX_NODES:
+            raise ValueError(f"a drafted tree has 1 to {ops.TREE_MAX_NODES} nodes")
+        for tree in batch.trees:
+            if any(not -1 <= p < i for i, p in enumerate(tree)):
+                raise ValueError("a drafted tree's parents come before their children (-1: a root)")
+        starts = [0]
+        for n in sizes:
+            starts.append(starts[-1] + n)
+        cached = [int(r.cached_len) for r in batch.reqs]
+        packed = _to_device_i32([p for t in batch.trees for p in t] + starts + [int(r.table_idx) for r in batch.reqs]
+                                + cached, out_loc.device)
+        parents, tree_start, row_table, cached_lens = packed.split([tokens, bs + 1, bs, bs])
+        mask, positions = ops.draft_tree(parents, tree_start, max_nodes=max(sizes), cached_lens=cached_lens)
+        return B200AttentionMetadata(phase="draft", positions=positions, out_loc=out_loc, row_table=row_table,
+                                     parents=parents, tree_start=tree_start, tree_mask=mask, cached_lens=cached_lens,
+                                     max_cached=max(cached))
+
     # -- fused path (raw qkv projection in) -------------------------------------
     def forward_qkv(
         self,
@@ -146,14 +182,15 @@ class B200AttentionBackend(BaseAttentionBackend):
                 max_q_len=md.max_q_len, num_qo_heads=self.num_heads, num_kv_heads=self.num_kv_heads,
                 head_dim=self.head_dim, scale=self.sm_scale,
             )
-        if md.phase == "prefill":
+        if md.phase in ("prefill", "draft"):
             qbuf = torch.empty_like(out)
             ops.qk_norm_rope_store(
                 qkv=qkv, num_qo_heads=self.num_heads, num_kv_heads=self.num_kv_heads, head_dim=self.head_dim,
                 q_norm_w=q_norm_w, k_norm_w=k_norm_w, eps=self.eps, cos=cos, sin=sin, positions=md.positions,
                 out_loc=md.out_loc, k_cache=kc, v_cache=vc, q_out=qbuf,
             )
-            return self._prefill(qbuf, out, kc, vc, ctx.page_table, md)
+            run = self._prefill if md.phase == "prefill" else self._tree
+            return run(qbuf, out, kc, vc, ctx.page_table, md)
         return ops.attention_decode(
             out=out, k_cache=kc, v_cache=vc, page_table=ctx.page_table, row_table=md.row_table,
             seq_lens=md.seq_lens, positions=md.positions, num_qo_heads=self.num_heads,
@@ -183,11 +220,20 @@ class B200AttentionBackend(BaseAttentionBackend):
         kc, vc = paged_kv_cache.k_slots(layer_id), paged_kv_cache.v_slots(layer_id)
         if md.phase == "prefill":
             return self._prefill(q2, out, kc, vc, ctx.page_table, md)
+        if md.phase == "draft":
+            return self._tree(q2, out, kc, vc, ctx.page_table, md)
         return ops.attention_decode(
             out=out, k_cache=kc, v_cache=vc, page_table=ctx.page_table, row_table=md.row_table,
             seq_lens=md.seq_lens, positions=md.positions, num_qo_heads=self.num_heads,
             num_kv_heads=self.num_kv_heads, head_dim=self.head_dim, scale=self.sm_scale, q=q2,
             prefix_len=md.prefix_len, active=md.active,
+        )
+
+    def _tree(self, q, out, kc, vc, page_table, md: B200AttentionMetadata) -> torch.Tensor:
+        return ops.attention_tree(
+            q=q, out=out, k_cache=kc, v_cache=vc, page_table=page_table, row_table=md.row_table,
+            cached_lens=md.cached_lens, tree_start=md.tree_start, tree_mask=md.tree_mask, max_cached=md.max_cached,
+            num_qo_heads=self.num_heads, num_kv_heads=self.num_kv_heads, head_dim=self.head_dim, scale=self.sm_scale,
         )
 
     def _prefill(self, q, out, kc, vc, page_table, md: B200AttentionMetadata) -> torch.Tensor:

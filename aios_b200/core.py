@@ -73,7 +73,7 @@ class Batch:
     out_loc, the attention backend fills attn_metadata."""
 
     reqs: List[Req]
-    phase: Literal["prefill", "decode"]
+    phase: Literal["prefill", "decode", "draft"]
     input_ids: torch.Tensor = field(init=False)
     positions: torch.Tensor = field(init=False)
     out_loc: torch.Tensor = field(init=False)
@@ -91,6 +91,11 @@ class Batch:
     # (bf16 rows [rows, hidden], RowStats of them); the trunk then starts at its
     # first linear instead of the embedding
     pre_embedded: tuple | None = None
+    # A draft batch (phase "draft"): per request the parents of its drafted tree, node 0 the
+    # request's last known token (-1), every other node's parent before it. input_ids and
+    # out_loc hold the nodes of all trees; page-table entry cached_len + i of a request holds
+    # node i's slot. The backend derives the nodes' positions; logits come for every node.
+    trees: List[List[int]] | None = None
 
     @property
     def is_prefill(self) -> bool:
@@ -99,6 +104,10 @@ class Batch:
     @property
     def is_decode(self) -> bool:
         return self.phase == "decode"
+
+    @property
+    def is_draft(self) -> bool:
+        return self.phase == "draft"
 
     @property
     def size(self) -> int:

@@ -110,5 +110,41 @@ class Sampler:
             return tok[0], lp[0]
         return tok, lp
 
+    def verify(
+        self,
+        logits: torch.Tensor,
+        draft_tokens: torch.Tensor,
+        parents: torch.Tensor,
+        tree_start: torch.Tensor,
+        *,
+        draft_probs: torch.Tensor | None = None,
+        generator: torch.Generator | None = None,
+        accept_uniforms: torch.Tensor | None = None,
+        sample_uniforms: torch.Tensor | None = None,
+    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """``ops.verify_draft`` with this sampler's parameters: which nodes of drafted trees stay,
+        and each request's next token, drawn as ``sample`` draws from the temperature distribution
+        (top-k and top-p apply to neither: mask the logits with -inf). Uniforms that are not given
+        are drawn from ``generator``."""
+        sp = self.sampling_params
+        if not sp.is_greedy and (sp.top_k > 0 or sp.top_p < 1.0):
+            raise ValueError("verify takes the temperature alone: mask the logits of filtered tokens with -inf")
+        if generator is not None and (accept_uniforms is not None or sample_uniforms is not None):
+            raise ValueError("generator and uniforms are mutually exclusive")
+        if sp.is_greedy:
+            return ops.verify_draft(logits, draft_tokens, parents, tree_start, greedy=True)
+        dev = logits.device
+
+        def uniforms(given: torch.Tensor | None, count: int) -> torch.Tensor:
+            if given is not None:
+                return given
+            return torch.rand(count, generator=generator, dtype=torch.float32,
+                              device=generator.device if generator is not None else dev).to(dev)
+
+        return ops.verify_draft(
+            logits, draft_tokens, parents, tree_start, uniforms(accept_uniforms, logits.shape[0]),
+            uniforms(sample_uniforms, tree_start.shape[0] - 1), temperature=sp.temperature, draft_probs=draft_probs,
+        )
+
     def sample(self, logits: torch.Tensor) -> torch.Tensor:
         return self.sample_with_logprobs(logits)[0]
