@@ -259,7 +259,7 @@ extern "C" int aiosb_attention_tree(const void* q, int64_t q_stride, int64_t tok
                 AIOSB_TREE_MAX_NODES);
   const int64_t group = num_qo_heads / num_kv_heads;
   AIOSB_REQUIRE(group <= AIOSB_TREE_MAX_GROUP && num_kv_heads <= 65535 && requests <= 65535 &&
-                    tokens * group <= INT32_MAX && table_width < INT32_MAX && table_rows < INT32_MAX,
+                    tokens * group <= INT32_MAX && table_width <= (1 << 30) && table_rows < INT32_MAX,
                 AIOSB_ERR_UNSUPPORTED, "attention_tree: too many rows, heads or requests");
   AIOSB_REQUIRE(q_stride >= num_qo_heads * head_dim && out_stride >= num_qo_heads * head_dim && q_stride % 8 == 0 &&
                     out_stride % 8 == 0,

@@ -9,6 +9,7 @@ status word that :func:`check_status` turns into a ``RuntimeError``.
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 
 import torch
 
@@ -1151,8 +1152,9 @@ def attention_tree(
     if tokens and requests:
         work, size = None, 0
         if (max_cached or table_width) > ATTENTION_TREE_WHOLE_KEYS:
-            size = _lib.load().aiosb_attention_tree_work_bytes(tokens, requests, words, max_cached or table_width,
-                                                               num_qo_heads, num_kv_heads, head_dim)
+            with torch.cuda.device(index) if index != torch._C._cuda_getDevice() else nullcontext():
+                size = _lib.load().aiosb_attention_tree_work_bytes(
+                    tokens, requests, words, max_cached or table_width, num_qo_heads, num_kv_heads, head_dim)
             work = _empty_vector(q, size, torch.uint8)
         _launch(index, "aiosb_attention_tree", q.data_ptr(), q_stride, tokens, k_cache.data_ptr(), v_cache.data_ptr(),
                 slots, page_table.data_ptr(), page_table.stride(0) if table_rows > 1 else table_width, table_rows,
@@ -1210,7 +1212,8 @@ def verify_draft(
 
     Returns ``accepted`` (int32 [requests]: nodes behind the root that stay), ``next_token``
     (int64 [requests]; -1 where there is no tree or no distribution) and ``order`` (int32
-    [tokens]: each tree's node numbers, the path from the root first, then the others)."""
+    [tokens]: each tree's node numbers, the path from the root first, then the others; undefined
+    behind the last tree)."""
     if not logits.is_cuda:
         raise ValueError("verify_draft requires CUDA tensors")
     fp32 = logits.dtype is torch.float32

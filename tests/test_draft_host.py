@@ -53,6 +53,7 @@ def test_attention_tree_refuses() -> None:
     call(UNS, "at most 1024", words=0)
     call(UNS, "too many", hq=65 * 4, qs=65 * 256, os=65 * 256)
     call(UNS, "too many", requests=65536)
+    call(UNS, "too many", width=(1 << 30) + 1, ts=1 << 31)
     call(INV, "row strides", qs=760)
     call(INV, "row strides", qs=772)
     call(INV, "row strides", os=760)

@@ -131,9 +131,41 @@ def test_rows_behind_the_last_tree_and_strides(cuda_device) -> None:
     out = torch.full((20, 4 * 64 + 40), 3.0, dtype=torch.bfloat16, device="cuda")
     table = torch.full((4, c.table.shape[1] + 9), -1, dtype=torch.int32, device="cuda")
     table[:, : c.table.shape[1]] = c.table
-    c.run(q=q[:, 8:264], out=out[:, 16:272], page_table=table[:, : c.table.shape[1]])
-    c.check(out[:, 16:272])
-    assert (out[14:] == 3).all() and (out[:, :16] == 3).all() and (out[:, 272:] == 3).all()
+    for bound in (1, 1 << 20):
+        out.fill_(3)
+        c.run(q=q[:, 8:264], out=out[:, 16:272], page_table=table[:, : c.table.shape[1]], max_cached=bound)
+        c.check(out[:, 16:272])
+        assert (out[14:] == 3).all() and (out[:, :16] == 3).all() and (out[:, 272:] == 3).all()
+
+
+@pytest.mark.parametrize("nodes", [5, 20, 100])
+def test_a_query_that_is_no_number_stays_in_its_row(cuda_device, nodes) -> None:
+    c = Case([nodes, nodes], [900, 40], 4, 2, 64, seed=6)
+    for bound in (1, 1 << 20):
+        clean = c.run(max_cached=bound)
+        kept = c.q[3, 64].clone()
+        c.q[3, 64] = float("nan")  # head 1 of node 3
+        got = c.run(max_cached=bound)
+        c.q[3, 64] = kept
+        assert torch.isnan(got[3, 64:128]).all()
+        got[3, 64:128] = clean[3, 64:128]
+        assert torch.equal(got, clean)
+
+
+def test_more_requests_than_a_warp_has_lanes(cuda_device) -> None:
+    """Ranges that start among hundreds of requests of unlike sizes, some of them empty."""
+    sizes = [(7 * i) % 11 for i in range(300)]
+    cached = [(131 * i) % 700 if i % 5 else 0 for i in range(300)]
+    c = Case(sizes, cached, 4, 2, 64, seed=8)
+    c.check_every_way()
+
+
+def test_every_kind_of_unit_in_one_batch(cuda_device) -> None:
+    """Units of up to 16, 32, 128 and 256 rows, and of 256 with a rest of each kind, cut at any place."""
+    sizes = [3, 8, 30, 60, 64 + 3, 64 + 30, 128 + 50]
+    for cached in ([3000] * 7, [100, 5000, 1, 700, 2000, 0, 333]):
+        c = Case(sizes, cached, 8, 2, 128, seed=9, page=16)
+        c.check_every_way()
 
 
 @pytest.mark.parametrize("d", [64, 96, 128])

@@ -139,6 +139,19 @@ def test_verify_large_vocabularies(cuda_device, vocab: int, probs: bool) -> None
     assert _run(case, sizes, temperature=0.8) == [list(w) for w in want]
 
 
+@pytest.mark.parametrize("kind", ["star", "chain", "mixed"])
+@pytest.mark.parametrize("probs", [False, True])
+def test_verify_large_trees(cuda_device, kind: str, probs: bool) -> None:
+    """More children than a warp has lanes, the longest path, as many nodes as a tree may have."""
+    sizes = [1024, 70]
+    case = _case(sizes, 90, kind, torch.float32, probs, seed=4, spread=0.2)
+    case[3].mul_(0.2 if kind == "chain" else 1.0)
+    if kind == "star":
+        case[3][1:60] = 0.9999
+    want = ref.verify(case[1], case[2], case[0], case[3], case[4], probs=case[5])
+    assert _run(case, sizes) == [list(w) for w in want]
+
+
 @pytest.mark.parametrize("requests", [1, 8, 37, 150, 400])
 def test_verify_many_requests(cuda_device, requests: int) -> None:
     sizes = [1 + i % 4 for i in range(requests)]
