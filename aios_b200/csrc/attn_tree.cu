@@ -223,8 +223,12 @@ cudaError_t launch_small(const TreeAttnArgs& a, int64_t max_nodes, cudaStream_t 
   return launch_pdl(kernel, grid, dim3(kThreads), kSmallSmem<D>, stream, a);
 }
 
-// Whether the keys are dealt over the SMs (attn_tree_split.cu).
-bool splits(int64_t max_cached) { return max_cached > 256; }
+// Whether the keys are dealt over the SMs (attn_tree_split.cu): for longer histories, or many rows, which its tensor
+// cores take faster. Measured, whole / dealt, us: 16 requests of 26 nodes, 8/2 heads of 96: 64 keys 10.2 / 13.1, 128
+// 13.2 / 14.3, 256 19.3 / 16.2, 1024 55 / 18.4; 1 of 8 heads of 128, 5 nodes: 64 10.9 / 11.0, 128 15.3 / 14.6; 64 of 60
+// nodes, 32 keys, 8 / 12 / 32 heads (30720, 46080, 122880 rows): 26.3 / 18.8, 25.3 / 21.8, 117 / 47; of 26 nodes, 8 and
+// 12 heads (13312, 19968 rows): 10.1 / 14.6, 14.8 / 17.7.
+bool splits(int64_t max_cached, int64_t tokens, int64_t heads) { return max_cached > 128 || tokens * heads > 24000; }
 
 }  // namespace
 }  // namespace aiosb
@@ -234,7 +238,7 @@ using namespace aiosb;
 extern "C" int64_t aiosb_attention_tree_work_bytes(int64_t tokens, int64_t requests, int64_t mask_words,
                                                    int64_t max_cached, int64_t num_qo_heads, int64_t num_kv_heads,
                                                    int64_t head_dim) {
-  if (tokens <= 0 || requests <= 0 || num_kv_heads <= 0 || !splits(max_cached)) return 0;
+  if (tokens <= 0 || requests <= 0 || num_kv_heads <= 0 || !splits(max_cached, tokens, num_qo_heads)) return 0;
   const int64_t rows = std::min(mask_words * 32, tokens) * (num_qo_heads / num_kv_heads);
   return tree_split_work_bytes(tree_split_grid(), tree_split_unit_rows(rows), (int)head_dim);
 }
@@ -272,7 +276,7 @@ extern "C" int aiosb_attention_tree(const void* q, int64_t q_stride, int64_t tok
                 AIOSB_ERR_INVALID_ARG, "attention_tree: null pointer");
   AIOSB_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out), AIOSB_ERR_MISALIGNED,
                 "attention_tree: q, out and the KV cache must be 16-byte aligned");
-  const bool split = splits(max_cached > 0 ? max_cached : table_width);
+  const bool split = splits(max_cached > 0 ? max_cached : table_width, tokens, num_qo_heads);
   const int64_t max_nodes = std::min<int64_t>(mask_words * 32, tokens);
   const int unit_rows = tree_split_unit_rows(max_nodes * group), grid = tree_split_grid();
   AIOSB_REQUIRE(!split || (work != nullptr && aligned16(work) &&

@@ -1151,21 +1151,18 @@ def attention_tree(
     table_rows, table_width = page_table.shape
     if tokens and requests:
         work, size = None, 0
-        if (max_cached or table_width) > ATTENTION_TREE_WHOLE_KEYS:
+        # the library's rule for whole requests to a CTA, which take no work area
+        if (max_cached or table_width) > 128 or tokens * num_qo_heads > 24000:
             with torch.cuda.device(index) if index != torch._C._cuda_getDevice() else nullcontext():
                 size = _lib.load().aiosb_attention_tree_work_bytes(
                     tokens, requests, words, max_cached or table_width, num_qo_heads, num_kv_heads, head_dim)
-            work = _empty_vector(q, size, torch.uint8)
+            work = _empty_vector(q, size, torch.uint8) if size else None
         _launch(index, "aiosb_attention_tree", q.data_ptr(), q_stride, tokens, k_cache.data_ptr(), v_cache.data_ptr(),
                 slots, page_table.data_ptr(), page_table.stride(0) if table_rows > 1 else table_width, table_rows,
                 table_width, row_table.data_ptr(), cached_lens.data_ptr(), tree_start.data_ptr(), requests,
                 tree_mask.data_ptr(), words, max_cached, num_qo_heads, num_kv_heads, head_dim, scale,
                 out.data_ptr(), out_stride, _ptr(work), size, _status_pointer(index))
     return out
-
-
-# Histories up to here are attended whole by a CTA, without a work area (aiosb_attention_tree_work_bytes gives 0)
-ATTENTION_TREE_WHOLE_KEYS = 256
 
 
 def _refuse_attention_tree(index, tokens, cache, k_cache, v_cache, page_table, row_table, cached_lens, tree_start,

@@ -104,3 +104,11 @@ def test_wrappers_want_cuda_tensors() -> None:
                            tree_mask=f, num_qo_heads=1, num_kv_heads=1, head_dim=8, scale=1.0)
     with pytest.raises(ValueError, match="CUDA"):
         ops.verify_draft(f, i.long(), i, i, greedy=True)
+
+
+@pytest.mark.parametrize("bound", [1, 127, 128, 129, 5000])
+@pytest.mark.parametrize("tokens", [1, 100, 3000, 3001])
+def test_the_work_areas_rule_is_the_wrappers(bound: int, tokens: int) -> None:
+    """attention_tree asks the library for a work area's size only where it needs one."""
+    size = _lib.load().aiosb_attention_tree_work_bytes(tokens, 1, 1, bound, 8, 2, 64)
+    assert (size > 0) == (bound > 128 or tokens * 8 > 24000)

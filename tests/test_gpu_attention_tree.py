@@ -160,6 +160,12 @@ def test_more_requests_than_a_warp_has_lanes(cuda_device) -> None:
     c.check_every_way()
 
 
+def test_many_rows_over_short_histories(cuda_device) -> None:
+    """Enough rows for the tensor cores, whatever the bound on the histories says."""
+    c = Case([60] * 64, [(5 * i) % 40 for i in range(64)], 8, 2, 64, seed=8)
+    c.check_every_way()
+
+
 def test_every_kind_of_unit_in_one_batch(cuda_device) -> None:
     """Units of up to 16, 32, 128 and 256 rows, and of 256 with a rest of each kind, cut at any place."""
     sizes = [3, 8, 30, 60, 64 + 3, 64 + 30, 128 + 50]
