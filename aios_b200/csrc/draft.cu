@@ -104,41 +104,64 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
 }
 __device__ __forceinline__ float load_logit(const __nv_bfloat16* p) { return bf16_to_f(*p); }
 __device__ __forceinline__ float load_logit(const float* p) { return *p; }
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    x[2 * j] = bf16_lo(w[j]);
-    x[2 * j + 1] = bf16_hi(w[j]);
-  }
-}
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
 
-// The eight ids of a lane in the block of kBlockIds from `base` on: consecutive ones where the row lies on 16
-// bytes, else every 32nd.
-struct Ids {
-  int base, end, first, step;
-  __device__ __forceinline__ Ids(int base, int end, bool vec, int lane)
-      : base(base), end(end), first(vec ? base + lane * 8 : base + lane), step(vec ? 1 : 32) {}
-  __device__ __forceinline__ int operator[](int j) const { return first + j * step; }
-  __device__ __forceinline__ bool whole() const { return step == 1 && first + 8 <= end; }
-};
-template <typename V>
-__device__ __forceinline__ void load_ids(const V* row, bool vec, const Ids& ids, float none, float (&x)[8]) {
-  if (vec && ids.whole()) {
-    load8(row + ids.first, x);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = ids[j] < ids.end ? load_logit(row + ids[j]) : none;
+// A row of logits in groups of eight places that lie on 16 bytes: place p holds id p - shift, and the first group's
+// first `shift` places and those from `end` on hold none. 16-byte loads reach up to 15 bytes over a row's ends, but
+// never a 16-byte piece without any of the row.
+template <typename T>
+struct Places {
+  const T* base;
+  int shift, end;
+  __device__ __forceinline__ Places(const T* row, int vocab) {
+    shift = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
+    base = row - shift;
+    end = vocab + shift;
   }
-}
-template <typename V>
-__device__ __forceinline__ bool lies_on_16(const V* row) {
-  return (reinterpret_cast<uintptr_t>(row) & 15u) == 0;
+  __device__ __forceinline__ void load(int p, float (&x)[8]) const {
+    if (p < end) {
+      pieces(base, p, x);
+    }
+    if (p < shift || p + 8 > end) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (p + j < shift || p + j >= end) x[j] = -INFINITY;
+    }
+  }
+  __device__ __forceinline__ void pieces(const __nv_bfloat16* from, int p, float (&x)[8]) const {
+    const uint4 u = *reinterpret_cast<const uint4*>(from + p);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[2 * j] = bf16_lo(w[j]);
+      x[2 * j + 1] = bf16_hi(w[j]);
+    }
+  }
+  __device__ __forceinline__ void pieces(const float* from, int p, float (&x)[8]) const {
+    const float4 a = *reinterpret_cast<const float4*>(from + p);
+    float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p + 4 < end) b = *reinterpret_cast<const float4*>(from + p + 4);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  }
+};
+// The eight values of `row` from index i on (0 outside of it), by 16-byte loads as above. The row's own place on 16
+// bytes is the same for every i that is a multiple of eight apart.
+__device__ __forceinline__ void load_probs(const float* row, int i, int vocab, float (&x)[8]) {
+  const int over = (int)((reinterpret_cast<uintptr_t>(row + i) & 15u) / 4);
+  float y[12];
+#pragma unroll
+  for (int g = 0; g < 3; ++g) {
+    const int at = i - over + 4 * g;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if ((g < 2 || over > 0) && at + 3 >= 0 && at < vocab) v = *reinterpret_cast<const float4*>(row + at);
+    y[4 * g] = v.x, y[4 * g + 1] = v.y, y[4 * g + 2] = v.z, y[4 * g + 3] = v.w;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = over == 0 ? y[j] : over == 1 ? y[j + 1] : over == 2 ? y[j + 2] : y[j + 3];
+  if (i < 0 || i + 8 > vocab) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i + j < 0 || i + j >= vocab) x[j] = 0.f;
+  }
 }
 
 // An fp32 value's bits as an fp64 one: the conversion instruction runs at an eighth of the fp64 rate. 0 and subnormals
@@ -253,7 +276,7 @@ __device__ __forceinline__ bool tree_rows(const VerifyArgs& a, int r, bool first
 
 // Greedy: a node's argmax decides. A cluster per request; each warp looks through every (ranks x warps)th block.
 template <typename T>
-__global__ void __launch_bounds__(kVerifyThreads) verify_greedy_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kVerifyThreads, 1) verify_greedy_kernel(const VerifyArgs a) {
   __shared__ Walk walk;
   __shared__ Exchange ex;
   __shared__ float warp_top[kVerifyWarps];
@@ -272,19 +295,18 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_greedy_kernel(const Ver
   int64_t token = -1;
   for (;;) {
     const T* const row = reinterpret_cast<const T*>(a.logits) + (int64_t)(t.start + cur) * a.logits_stride;
-    const bool vec = lies_on_16(row);
+    const Places<T> places(row, a.vocab);
     float top = -INFINITY;
     int arg = INT32_MAX;
     // ids ascend within a lane, so that the first of equal ones stays
-#pragma unroll 4
-    for (int base = (rank * kVerifyWarps + warp) * kBlockIds; base < a.vocab;
-         base += ranks * kVerifyWarps * kBlockIds) {
-      const Ids ids(base, a.vocab, vec, lane);
+#pragma unroll 2
+    for (int p = (rank * kVerifyWarps + warp) * kBlockIds + lane * 8; p < places.end;
+         p += ranks * kVerifyWarps * kBlockIds) {
       float x[8];
-      load_ids(row, vec, ids, -INFINITY, x);
+      places.load(p, x);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        if (x[j] > top) arg = ids[j];
+        if (x[j] > top) arg = p + j - places.shift;
         top = max_nan(top, x[j]);
       }
     }
@@ -359,7 +381,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_greedy_kernel(const Ver
 constexpr int kGroupPlaces = 10;
 
 template <typename T, bool PROBS>
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyArgs a) {
   extern __shared__ __align__(16) double weights[];
   __shared__ Walk walk;
   __shared__ Exchange ex;
@@ -390,10 +412,9 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
   cluster_sync();  // every CTA runs: its shared memory may be written
 
   const double scale = a.inv_temperature * (1.4426950408889634 * kExpTable);
-  const int per_rank = a.run * kVerifyWarps, rank_lo = rank * per_rank;
-  const int lo = min(rank_lo + warp * a.run, a.vocab), hi = min(rank_lo + (warp + 1) * a.run, a.vocab);
-  auto group_of = [&](int v) { return weights + ((v - rank_lo) >> 3) * kGroupPlaces; };
-  auto at = [&](int v) -> double& { return group_of(v)[(v - rank_lo) & 7]; };
+  // places of the row (Places), not ids
+  const int per_rank = a.run * kVerifyWarps, rank_lo = rank * per_rank, lo = rank_lo + warp * a.run;
+  auto group_of = [&](int p) { return weights + ((p - rank_lo) >> 3) * kGroupPlaces; };
   auto load_group = [](const double* g, double (&w)[8]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -406,8 +427,6 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
 #pragma unroll
     for (int j = 0; j < 4; ++j) reinterpret_cast<double2*>(g)[j] = make_double2(w[2 * j], w[2 * j + 1]);
   };
-  // ids of a lane's group that are none of this warp's hold 0 at all times
-  const int last_block = lo + (hi - lo + kBlockIds - 1) / kBlockIds * kBlockIds;
 
   int turn = 0, cur = 0, depth = 0, last_turn = 0;
   // The sums of the warps' runs within the CTA, then of the CTAs (ex.sum, in rank order); `top` goes along.
@@ -435,7 +454,11 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
   for (;;) {
     const T* const row = reinterpret_cast<const T*>(a.logits) + (int64_t)(t.start + cur) * a.logits_stride;
     const float* const q = PROBS ? a.probs + (int64_t)(t.start + cur) * a.probs_stride : nullptr;
-    const bool vec = lies_on_16(row), vec_q = PROBS && lies_on_16(q);
+    const Places<T> places(row, a.vocab);
+    const int shift = places.shift;
+    // of this warp: [lo, hi), in whole blocks up to `last`; places without an id have weight 0 throughout
+    const int hi = max(lo, min(lo + a.run, places.end));
+    const int last_block = lo + (hi - lo + kBlockIds - 1) / kBlockIds * kBlockIds;
     // the children; their logits and probabilities are asked for ahead of the row's, a lane each
     float child_l = -INFINITY, child_p = 0.f;
     if (warp == 0) {
@@ -452,20 +475,14 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
     // ---- the row, as it is, to its place; its maximum
     float top = -INFINITY;
 #pragma unroll 2
-    for (int base = lo; base < hi; base += kBlockIds) {
-      const Ids ids(base, hi, vec, lane);
+    for (int p = lo + lane * 8; p < last_block; p += kBlockIds) {
       float x[8];
-      load_ids(row, vec, ids, -INFINITY, x);
+      places.load(p, x);
 #pragma unroll
       for (int j = 0; j < 8; ++j) top = max_nan(top, x[j]);
-      if (vec) {
-        float4* const g = reinterpret_cast<float4*>(group_of(ids.first));
-        g[0] = make_float4(x[0], x[1], x[2], x[3]);
-        g[1] = make_float4(x[4], x[5], x[6], x[7]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) reinterpret_cast<float*>(group_of(ids[j]))[(ids[j] - rank_lo) & 7] = x[j];
-      }
+      float4* const g = reinterpret_cast<float4*>(group_of(p));
+      g[0] = make_float4(x[0], x[1], x[2], x[3]);
+      g[1] = make_float4(x[4], x[5], x[6], x[7]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -500,10 +517,10 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
       double e[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) e[j] = exp_table(x[j], scale, mine, table);
-      if (v + 8 > hi) {
+      if (v < shift || v + 8 > places.end) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (v + j >= hi) e[j] = 0;
+          if (v + j < shift || v + j >= places.end) e[j] = 0;
       }
       store_group(g, e);
       part += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
@@ -537,7 +554,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
         const int x = node_x[walk.child[i]];
         double p = 0;
         if (x >= 0) {
-          const int owner = x / per_rank;
+          const int owner = (x + shift) / per_rank;
           const float m = ex.top[last_turn][owner];
           if (m > -INFINITY)
             p = exp_table(*reinterpret_cast<const float*>(&child_r[i]), scale, widen(m) * scale, table) *
@@ -564,11 +581,10 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
         const double inv = 1.0 / total;
         part = 0;
 #pragma unroll 1
-        for (int base = lo; base < last_block; base += kBlockIds) {
-          const Ids ids(base, hi, true, lane);
-          double* const g = group_of(ids.first);
+        for (int p = lo + lane * 8; p < last_block; p += kBlockIds) {
+          double* const g = group_of(p);
           float qv[8];
-          load_ids(q, vec_q, ids, 0.f, qv);
+          load_probs(q, p - shift, a.vocab, qv);
           double w[8], sum = 0;
           load_group(g, w);
 #pragma unroll
@@ -596,7 +612,9 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
         __syncthreads();
         for (int c = threadIdx.x; c < children; c += kVerifyThreads)
           if (node_x[walk.child[c]] == x) child_r[c] = 0;
-        if (threadIdx.x == 0 && x >= rank_lo && x < rank_lo + per_rank) at(x) = 0;
+        const int place = x + shift;
+        if (threadIdx.x == 0 && place >= rank_lo && place < rank_lo + per_rank)
+          group_of(place)[(place - rank_lo) & 7] = 0;
         total -= rx;
         stale = true;
         __syncthreads();
@@ -614,10 +632,10 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
     }
 
     // ---- the next token
-    auto group_weights = [&](const Ids& ids, double (&w)[8]) {  // r of a lane's group
-      load_group(group_of(ids.first), w);
+    auto group_weights = [&](int p, double (&w)[8]) {  // r of the group at p
+      load_group(group_of(p), w);
       float qv[8];
-      if (PROBS && pending != 0) load_ids(q, vec_q, ids, 0.f, qv);
+      if (PROBS && pending != 0) load_probs(q, p - shift, a.vocab, qv);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         w[j] *= mult;
@@ -626,9 +644,9 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
     };
     if (stale) {
       part = 0;
-      for (int base = lo; base < last_block; base += kBlockIds) {
+      for (int p = lo + lane * 8; p < last_block; p += kBlockIds) {
         double w[8];
-        group_weights(Ids(base, hi, true, lane), w);
+        group_weights(p, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) part += w[j];
       }
@@ -667,14 +685,13 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
       if (warp == own_warp) {
         before = warp_before;
         int pick = -1;
-        for (int base = lo; base < last_block; base += kBlockIds) {
-          const Ids ids(base, hi, true, lane);
+        for (int p = lo + lane * 8; p < last_block; p += kBlockIds) {
           double w[8], sum = 0;
-          group_weights(ids, w);
+          group_weights(p, w);
           int last = -1;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            if (w[j] > kNothing) last = ids[j];
+            if (w[j] > kNothing) last = p + j - shift;
             sum += w[j];
           }
           double upto = sum;
@@ -693,7 +710,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
             for (int j = 0; j < 8; ++j) {  // the first one past the target
               c += w[j];
               if (w[j] > kNothing && c > target) {
-                pick = ids[j];
+                pick = p + j - shift;
                 c = -INFINITY;
               }
             }
@@ -715,8 +732,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
   write_order(walk, depth, t.n, t.all, a.order + t.start);
 }
 
-constexpr size_t kWeightBytes = 190 * 1024;  // beside the static shared memory
-constexpr int kMaxSampleVocab = 262144;
+constexpr size_t kWeightBytes = 160 * 1024;  // of 262144 places over 16 CTAs; the static shared memory lies beside it
+constexpr int kMaxSamplePlaces = 262144;
 
 template <typename Kernel>
 cudaError_t launch_cluster(Kernel kernel, const VerifyArgs& a, int requests, size_t smem, bool (&configured)[64],
@@ -740,14 +757,20 @@ cudaError_t launch_cluster(Kernel kernel, const VerifyArgs& a, int requests, siz
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-int warp_run(int vocab, int ranks) {
-  const int blocks = (vocab + kBlockIds - 1) / kBlockIds, warps = ranks * kVerifyWarps;
+int warp_run(int places, int ranks) {
+  const int blocks = (places + kBlockIds - 1) / kBlockIds, warps = ranks * kVerifyWarps;
   return (blocks + warps - 1) / warps * kBlockIds;
 }
 size_t weight_bytes(int run) { return (size_t)run * kVerifyWarps / 8 * kGroupPlaces * sizeof(double); }
 
+// Places of a row (Places): more than its ids where a row may start anywhere on 16 bytes.
+int64_t row_places(const void* logits, int64_t stride, int64_t vocab, int64_t tokens, int value_bytes) {
+  const bool aligned = aligned16(logits) && (tokens <= 1 || stride * value_bytes % 16 == 0);
+  return vocab + (aligned ? 0 : 16 / value_bytes - 1);
+}
+
 template <typename T>
-cudaError_t launch_verify(VerifyArgs a, int requests, bool greedy, cudaStream_t stream) {
+cudaError_t launch_verify(VerifyArgs a, int requests, bool greedy, int places, cudaStream_t stream) {
   a.ranks = 1;
   const int sms = sm_count();
   // more CTAs to a request while they find SMs, and two blocks to each of their warps
@@ -756,8 +779,8 @@ cudaError_t launch_verify(VerifyArgs a, int requests, bool greedy, cudaStream_t 
   static bool configured[3][64] = {};
   if (greedy) return launch_cluster(verify_greedy_kernel<T>, a, requests, 0, configured[0], stream);
   // two CTAs to an SM if the weights allow it
-  while (a.ranks < kMaxRanks && weight_bytes(warp_run(a.vocab, a.ranks)) > kWeightBytes / 2) a.ranks *= 2;
-  a.run = warp_run(a.vocab, a.ranks);
+  while (a.ranks < kMaxRanks && weight_bytes(warp_run(places, a.ranks)) > kWeightBytes / 2) a.ranks *= 2;
+  a.run = warp_run(places, a.ranks);
   const size_t smem = weight_bytes(a.run);
   if (a.probs != nullptr) return launch_cluster(verify_kernel<T, true>, a, requests, smem, configured[1], stream);
   return launch_cluster(verify_kernel<T, false>, a, requests, smem, configured[2], stream);
@@ -795,8 +818,10 @@ extern "C" int aiosb_verify_draft(const void* logits, int logits_fp32, int64_t l
                                   int64_t* next_token, int32_t* order, int32_t* status, void* stream) {
   AIOSB_REQUIRE(tokens >= 0 && requests >= 0 && vocab >= 1 && tokens <= INT32_MAX && requests <= INT32_MAX / kMaxRanks,
                 AIOSB_ERR_INVALID_ARG, "verify_draft: bad sizes");
-  AIOSB_REQUIRE(vocab <= (greedy ? 1 << 30 : kMaxSampleVocab), AIOSB_ERR_UNSUPPORTED,
-                "verify_draft: vocabulary too large (sampling: at most %d)", kMaxSampleVocab);
+  const int64_t places = row_places(logits, logits_stride, vocab, tokens, logits_fp32 ? 4 : 2);
+  AIOSB_REQUIRE((greedy ? vocab : places) <= (greedy ? 1 << 30 : kMaxSamplePlaces), AIOSB_ERR_UNSUPPORTED,
+                "verify_draft: vocabulary too large (sampling: at most %d, less 7 where rows are not on 16 bytes)",
+                kMaxSamplePlaces);
   AIOSB_REQUIRE(logits_stride >= vocab || tokens <= 1, AIOSB_ERR_INVALID_ARG,
                 "verify_draft: logits row stride below the vocabulary");
   AIOSB_REQUIRE(greedy || (temperature >= 1e-6 && temperature <= 1e6), AIOSB_ERR_INVALID_ARG,
@@ -829,6 +854,6 @@ extern "C" int aiosb_verify_draft(const void* logits, int logits_fp32, int64_t l
   a.order = order;
   a.status = status;
   cudaStream_t s = as_stream(stream);
-  return check_launch("verify_draft", logits_fp32 ? launch_verify<float>(a, (int)requests, greedy != 0, s)
-                                                  : launch_verify<__nv_bfloat16>(a, (int)requests, greedy != 0, s));
+  const auto launch = logits_fp32 ? launch_verify<float> : launch_verify<__nv_bfloat16>;
+  return check_launch("verify_draft", launch(a, (int)requests, greedy != 0, (int)places, s));
 }

@@ -77,7 +77,9 @@ def test_verify_draft_refuses() -> None:
     _refused(name, good, INV, "bad sizes", tokens=-1)
     _refused(name, good, INV, "bad sizes", vocab=0)
     _refused(name, good, INV, "bad sizes", requests=1 << 29)
-    _refused(name, good, UNS, "too large", vocab=262145, ls=262145)
+    _refused(name, good, UNS, "too large", vocab=262145, ls=262152)
+    _refused(name, good, UNS, "too large", vocab=262138, ls=262138)  # rows anywhere on 16 bytes
+    _refused(name, good, UNS, "too large", vocab=262144, ls=262144, logits=P + 2)
     _refused(name, good, UNS, "too large", vocab=1 << 31, ls=1 << 31, greedy=1)
     _refused(name, good, INV, "logits row stride", ls=99)
     _refused(name, good, INV, "temperature", temperature=0.0)

@@ -130,13 +130,38 @@ def test_verify(cuda_device, sizes, vocab: int, mode: str) -> None:
     ops.check_status(cuda_device)
 
 
-@pytest.mark.parametrize("vocab", [50021, 131072, 151111, 160001, 262144])
+@pytest.mark.parametrize("vocab", [50021, 131072, 151111, 160001, 262137, 262144])
 @pytest.mark.parametrize("probs", [False, True])
 def test_verify_large_vocabularies(cuda_device, vocab: int, probs: bool) -> None:
     sizes = [12, 7, 1]
     case = _case(sizes, vocab, probs=probs, seed=vocab)
     want = ref.verify(case[1], case[2], case[0], case[3], case[4], temperature=0.8, probs=case[5])
     assert _run(case, sizes, temperature=0.8) == [list(w) for w in want]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("off", range(8))
+@pytest.mark.parametrize("mode", ["greedy", "plain", "probs"])
+def test_rows_anywhere_on_16_bytes(cuda_device, dtype, off: int, mode: str) -> None:
+    """Every place of a row and of its probabilities, NaN around both."""
+    for vocab in (1, 6, 255, 1030):
+        sizes = [3, 6]
+        case = _case(sizes, vocab, dtype=dtype, probs=mode == "probs", seed=off)
+        parents, logits, drafts, accept, sample, q = case
+        kw = {"greedy": True} if mode == "greedy" else {}
+        want = ref.verify(logits, drafts, parents, accept, sample, probs=q, **kw)
+        for stride in (vocab + 16, vocab + 21):
+            wide = torch.full((9, stride), float("nan"), dtype=dtype, device="cuda")
+            wide[:, off : off + vocab] = logits.cuda()
+            wide_q = torch.full((9, stride + 2), float("nan"), device="cuda")
+            at = (3 * off + 1) % 8
+            if q is not None:
+                wide_q[:, at : at + vocab] = q.cuda()
+            got = ops.verify_draft(wide[:, off : off + vocab], drafts.cuda(), _flat(parents), _i32([0, 3, 9]),
+                                   accept.cuda(), sample.cuda(),
+                                   draft_probs=wide_q[:, at : at + vocab] if q is not None else None, **kw)
+            assert [t.tolist() for t in got] == [list(w) for w in want]
+    ops.check_status(cuda_device)
 
 
 @pytest.mark.parametrize("kind", ["star", "chain", "mixed"])
