@@ -376,9 +376,8 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) verify_greedy_kernel(const 
 // tried, so that a row is read once. A pass leaves each warp the sum of its run and each CTA the sum of its warps';
 // a token is found by these sums from the outside in. Sums are taken in a fixed order, in fp64: what is accepted or
 // drawn hangs on comparisons of them.
-// Weights lie in groups of eight ids, ten places to a group: a lane's 16-byte accesses to its group then fall on
-// different banks. A row comes as fp32 into its group's first places.
-constexpr int kGroupPlaces = 10;
+// A warp's run of a row is a multiple of this; a row comes as fp32 into the first half of its groups' places.
+constexpr int kRunIds = 64;
 
 template <typename T, bool PROBS>
 __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyArgs a) {
@@ -414,18 +413,21 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
   const double scale = a.inv_temperature * (1.4426950408889634 * kExpTable);
   // places of the row (Places), not ids
   const int per_rank = a.run * kVerifyWarps, rank_lo = rank * per_rank, lo = rank_lo + warp * a.run;
-  auto group_of = [&](int p) { return weights + ((p - rank_lo) >> 3) * kGroupPlaces; };
-  auto load_group = [](const double* g, double (&w)[8]) {
+  // Groups of eight, a lane each; their 16-byte pieces change places from one pair of groups to the next, so that
+  // eight lanes' pieces lie on different banks (runs are multiples of 64, so a lane's groups all have its order).
+  auto group_of = [&](int p) { return weights + (p - rank_lo); };
+  const int swap = (lane >> 1) & 3;
+  auto load_group = [&](const double* g, double (&w)[8]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const double2 d = reinterpret_cast<const double2*>(g)[j];
+      const double2 d = reinterpret_cast<const double2*>(g)[j ^ swap];
       w[2 * j] = d.x;
       w[2 * j + 1] = d.y;
     }
   };
-  auto store_group = [](double* g, const double (&w)[8]) {
+  auto store_group = [&](double* g, const double (&w)[8]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) reinterpret_cast<double2*>(g)[j] = make_double2(w[2 * j], w[2 * j + 1]);
+    for (int j = 0; j < 4; ++j) reinterpret_cast<double2*>(g)[j ^ swap] = make_double2(w[2 * j], w[2 * j + 1]);
   };
 
   int turn = 0, cur = 0, depth = 0, last_turn = 0;
@@ -456,9 +458,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
     const float* const q = PROBS ? a.probs + (int64_t)(t.start + cur) * a.probs_stride : nullptr;
     const Places<T> places(row, a.vocab);
     const int shift = places.shift;
-    // of this warp: [lo, hi), in whole blocks up to `last`; places without an id have weight 0 throughout
-    const int hi = max(lo, min(lo + a.run, places.end));
-    const int last_block = lo + (hi - lo + kBlockIds - 1) / kBlockIds * kBlockIds;
+    const int hi = max(lo, min(lo + a.run, places.end));  // of this warp: [lo, hi), the last group in full
     // the children; their logits and probabilities are asked for ahead of the row's, a lane each
     float child_l = -INFINITY, child_p = 0.f;
     if (warp == 0) {
@@ -475,14 +475,14 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
     // ---- the row, as it is, to its place; its maximum
     float top = -INFINITY;
 #pragma unroll 2
-    for (int p = lo + lane * 8; p < last_block; p += kBlockIds) {
+    for (int p = lo + lane * 8; p < hi; p += kBlockIds) {
       float x[8];
       places.load(p, x);
 #pragma unroll
       for (int j = 0; j < 8; ++j) top = max_nan(top, x[j]);
       float4* const g = reinterpret_cast<float4*>(group_of(p));
-      g[0] = make_float4(x[0], x[1], x[2], x[3]);
-      g[1] = make_float4(x[4], x[5], x[6], x[7]);
+      g[swap] = make_float4(x[0], x[1], x[2], x[3]);
+      g[1 ^ swap] = make_float4(x[4], x[5], x[6], x[7]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -509,10 +509,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
     double part = 0;
     const double mine = widen(top > -INFINITY ? top : 0.f) * scale;
 #pragma unroll 1
-    for (int base = lo; base < last_block; base += kBlockIds) {
-      const int v = base + lane * 8;
+    for (int v = lo + lane * 8; v < hi; v += kBlockIds) {
       double* const g = group_of(v);
-      const float4 x0 = reinterpret_cast<const float4*>(g)[0], x1 = reinterpret_cast<const float4*>(g)[1];
+      const float4 x0 = reinterpret_cast<const float4*>(g)[swap], x1 = reinterpret_cast<const float4*>(g)[1 ^ swap];
       const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
       double e[8];
 #pragma unroll
@@ -581,7 +580,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
         const double inv = 1.0 / total;
         part = 0;
 #pragma unroll 1
-        for (int p = lo + lane * 8; p < last_block; p += kBlockIds) {
+        for (int p = lo + lane * 8; p < hi; p += kBlockIds) {
           double* const g = group_of(p);
           float qv[8];
           load_probs(q, p - shift, a.vocab, qv);
@@ -613,8 +612,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
         for (int c = threadIdx.x; c < children; c += kVerifyThreads)
           if (node_x[walk.child[c]] == x) child_r[c] = 0;
         const int place = x + shift;
-        if (threadIdx.x == 0 && place >= rank_lo && place < rank_lo + per_rank)
-          group_of(place)[(place - rank_lo) & 7] = 0;
+        if (threadIdx.x == 0 && place >= rank_lo && place < rank_lo + per_rank) {
+          const int i = place - rank_lo;
+          weights[i ^ (((i >> 4) & 3) << 1)] = 0;
+        }
         total -= rx;
         stale = true;
         __syncthreads();
@@ -644,7 +645,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
     };
     if (stale) {
       part = 0;
-      for (int p = lo + lane * 8; p < last_block; p += kBlockIds) {
+      for (int p = lo + lane * 8; p < hi; p += kBlockIds) {
         double w[8];
         group_weights(p, w);
 #pragma unroll
@@ -685,9 +686,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
       if (warp == own_warp) {
         before = warp_before;
         int pick = -1;
-        for (int p = lo + lane * 8; p < last_block; p += kBlockIds) {
-          double w[8], sum = 0;
-          group_weights(p, w);
+        for (int base = lo; base < hi; base += kBlockIds) {
+          const int p = base + lane * 8;
+          double w[8] = {}, sum = 0;
+          if (p < hi) group_weights(p, w);
           int last = -1;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -732,8 +734,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
   write_order(walk, depth, t.n, t.all, a.order + t.start);
 }
 
-constexpr size_t kWeightBytes = 160 * 1024;  // of 262144 places over 16 CTAs; the static shared memory lies beside it
 constexpr int kMaxSamplePlaces = 262144;
+constexpr size_t kWeightBytes = sizeof(double) * kMaxSamplePlaces / kMaxRanks;
+constexpr size_t kSharedBytes = 80 * 1024;  // of two CTAs on an SM, 28 KiB beside it
 
 template <typename Kernel>
 cudaError_t launch_cluster(Kernel kernel, const VerifyArgs& a, int requests, size_t smem, bool (&configured)[64],
@@ -758,10 +761,10 @@ cudaError_t launch_cluster(Kernel kernel, const VerifyArgs& a, int requests, siz
 }
 
 int warp_run(int places, int ranks) {
-  const int blocks = (places + kBlockIds - 1) / kBlockIds, warps = ranks * kVerifyWarps;
-  return (blocks + warps - 1) / warps * kBlockIds;
+  const int runs = (places + kRunIds - 1) / kRunIds, warps = ranks * kVerifyWarps;
+  return (runs + warps - 1) / warps * kRunIds;
 }
-size_t weight_bytes(int run) { return (size_t)run * kVerifyWarps / 8 * kGroupPlaces * sizeof(double); }
+size_t weight_bytes(int run) { return (size_t)run * kVerifyWarps * sizeof(double); }
 
 // Places of a row (Places): more than its ids where a row may start anywhere on 16 bytes.
 int64_t row_places(const void* logits, int64_t stride, int64_t vocab, int64_t tokens, int value_bytes) {
@@ -779,7 +782,7 @@ cudaError_t launch_verify(VerifyArgs a, int requests, bool greedy, int places, c
   static bool configured[3][64] = {};
   if (greedy) return launch_cluster(verify_greedy_kernel<T>, a, requests, 0, configured[0], stream);
   // two CTAs to an SM if the weights allow it
-  while (a.ranks < kMaxRanks && weight_bytes(warp_run(places, a.ranks)) > kWeightBytes / 2) a.ranks *= 2;
+  while (a.ranks < kMaxRanks && weight_bytes(warp_run(places, a.ranks)) > kSharedBytes) a.ranks *= 2;
   a.run = warp_run(places, a.ranks);
   const size_t smem = weight_bytes(a.run);
   if (a.probs != nullptr) return launch_cluster(verify_kernel<T, true>, a, requests, smem, configured[1], stream);
