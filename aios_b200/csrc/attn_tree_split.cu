@@ -1,22 +1,32 @@
-// Attention of drafted trees on tcgen05, the keys of all requests dealt evenly over the SMs.
+// Attention of drafted trees, the keys of all requests dealt evenly over the SMs.
 //
 // A unit is up to 256 rows ((node, query head) pairs) of one KV head of one request; its keys are
-// chunks of 128. The units' chunks laid end to end (a unit weighs its chunks and one more for its
-// start and end) are cut into one range per CTA, so that a CTA takes pieces of units, whatever the
-// requests' lengths. A piece that is a whole unit is written as it is; the pieces of a cut unit leave
-// their rows' maximum, sum and unnormalised output in fp32 in the work area, and a second kernel joins
-// them in the order of the keys.
+// chunks of 128. The units' chunks laid end to end, each weighed by what it costs, are cut into one
+// range per CTA, so that a CTA takes pieces of units, whatever the requests' lengths. A piece that is a
+// whole unit is written as it is; the pieces of a cut unit leave their rows' maximum, sum and
+// unnormalised output in fp32 in the work area, and a second kernel joins them in the order of the keys.
 //
-// In a CTA: four warps gather keys and values into a ring of 128-key blocks with cp.async (the slots of
-// neighbouring keys are anywhere, so there is no box for TMA to fetch), one warp issues the MMAs, and
-// two groups of four warps hold the softmax of one stream each. With more than 128 rows the streams are
-// the two halves of the rows, both on every chunk; with fewer they are the even and the odd chunks of
-// the same rows, each with its own maximum, sum and output, joined at the end. So the MMAs of one stream
-// run while the other's exponentials are taken. S = Q K^T comes from shared memory into TMEM; a thread
-// owns a row (a TMEM lane), takes its maximum and exponentials, and writes the weights back over S as the
-// bf16 A operand of O += P V (V as it lies, the keys as its k: an MN-major B operand).
+// In a CTA: four warps walk the CTA's pieces and gather their keys and values into a ring of 128-key
+// blocks with cp.async (the slots of neighbouring keys are anywhere, so there is no box for TMA to
+// fetch); two warps issue the MMAs, one for each of two streams; and two groups of four warps hold the
+// streams' softmax. With more than 128 rows the streams are the two halves of the rows, both on every
+// chunk; with fewer they are the even and the odd chunks of the same rows, each with its own maximum,
+// sum and output, joined at the end. S = Q K^T goes from shared memory into TMEM, 64 keys at a time into
+// two buffers, so that a stream's next scores are formed while it takes the present exponentials. A
+// thread owns a row (a TMEM lane), takes its maximum and exponentials, and writes the weights back over
+// S as the bf16 A operand of O += P V (V as it lies, the keys as its k: an MN-major B operand). Up to 32
+// rows go on mma.sync instead, with no TMEM round trip (few_rows below).
 // A row's output is rescaled only where its maximum has grown by more than 2^8 over the one that its
-// exponentials refer to: any reference gives the same quotient.
+// exponentials refer to: any reference gives the same quotient. Weights are rounded to bf16 for the
+// second product (each off by 2^-8 of itself at most, of either sign); their sum is of the
+// unrounded ones.
+//
+// What bounds it, with more than 128 rows: a step of 64 keys takes about 2100 clocks, of which the
+// exponentials of 256 rows are 1024 (16 a clock), the softmax threads' whole work 1500 to 1900 while two
+// groups share the issue slots, and the products 1370. 32 requests x 16384 keys, 64 nodes, 32/8 heads of
+// 128: 579 us alone, 697 in a row of calls under the power limit; the products at the dense rate would take
+// 328. With few rows: the gather (64 x 8192 keys, 5 nodes, 12/4 heads of 64: 122 us, 4.4 TB/s). With little
+// work: the start and end of a unit, some 10000 clocks (16 x 1900 keys 17 us).
 #include <algorithm>
 
 #include "tree.cuh"
@@ -678,7 +688,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
     };
     // Up to 32 rows: 16 to a warp on mma.sync, each warp with its share of every chunk's keys and its own maximum,
     // sum and output, joined at the end. The tensor pipe is idle here, but a TMEM round trip per step (scores out,
-    // weights back) took longer than the chunk's bytes: 64 x 8192 keys, 15 rows 148 -> KEEP us.
+    // weights back) took longer than the chunk's bytes: 64 x 8192 keys, 15 rows 148 -> 134 us.
     auto few_rows = [&](auto load_q) {
       const int tiles = p.rows > 16 ? 2 : 1, tile = warp & (tiles - 1), part = warp / tiles;
       if (s == 0) load_q(0, 16 * tiles);
@@ -1052,7 +1062,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
 }
 
 // Joins the pieces of the unit that starts in range blockIdx.x and goes on behind it. A CTA takes 32 rows and D / 4
-// columns: first every piece's maxima and sums, then the pieces' outputs, four loads in flight to a thread.
+// columns: first every piece's maxima and sums, then the pieces' outputs, four loads in flight to a thread. It adds
+// 4.5 us to 16 x 1900 keys (12.6 without it), two of them for a grid that finds little to do, and 11 to 41 ragged
+// requests, whose 33 MB of pieces are read again. More columns to a CTA, and the first two pieces loaded at once with
+// the record, took as long or longer.
 constexpr int kJoinRows = 32, kJoinParts = 4;
 
 template <int D>

@@ -13,7 +13,7 @@ constexpr int kTreeThreads = 256;
 
 // A CTA per tree, by doubling: with every node's bits of its 2^k nearest ancestors (itself among them) and its 2^k-th
 // ancestor known, the ancestor's bits or-ed into its own are those of 2^(k + 1). So a chain of 256 takes eight rounds,
-// where a walk from each node to its root takes 256 dependent loads (63 us; 256 mixed trees of up to 256 nodes 13.5).
+// where a walk from each node to its root takes 256 dependent loads (63 us, so 10; 256 mixed trees of up to 256 nodes 6.4).
 // Bits may be or-ed while their owner adds to them: what it adds are ancestors as well. The ancestors' numbers have
 // two buffers.
 __global__ void __launch_bounds__(kTreeThreads)
@@ -89,7 +89,7 @@ struct VerifyArgs {
   int32_t* order;
   int32_t* status;
   int ranks;  // CTAs of a cluster: they share a request's vocabulary
-  int run;    // ids of a warp, a multiple of kBlockIds
+  int run;    // places of a warp, a multiple of kRunIds
 };
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -274,7 +274,9 @@ __device__ __forceinline__ bool tree_rows(const VerifyArgs& a, int r, bool first
   return t.n > 0;
 }
 
-// Greedy: a node's argmax decides. A cluster per request; each warp looks through every (ranks x warps)th block.
+// Greedy: a node's argmax decides. A cluster per request; each warp looks through every (ranks x warps)th block. Bound
+// by the latency of the visited nodes, one after another (a row's loads, the exchange): 24 trees of 13 at 50021 fp32
+// ids 17.4 us. Four blocks in flight in place of two took 20 to 30% longer: the registers.
 template <typename T>
 __global__ void __launch_bounds__(kVerifyThreads, 1) verify_greedy_kernel(const VerifyArgs a) {
   __shared__ Walk walk;
@@ -376,6 +378,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) verify_greedy_kernel(const 
 // tried, so that a row is read once. A pass leaves each warp the sum of its run and each CTA the sum of its warps';
 // a token is found by these sums from the outside in. Sums are taken in a fixed order, in fp64: what is accepted or
 // drawn hangs on comparisons of them.
+// Bound by the latency of the visited nodes: some 6600 clocks each for the row's loads, eleven fp64 instructions to an
+// exponential, and the cluster's exchange; with many requests by the fp64 pipes and the passes over shared memory. A
+// chain of 5 at 16384 ids 13.5 us, 16 trees of 26 at 32001 ids 18, 64 trees of 24 with probabilities at 131072 ids 128
+// (one CTA to an SM 196).
 // A warp's run of a row is a multiple of this; a row comes as fp32 into the first half of its groups' places.
 constexpr int kRunIds = 64;
 
