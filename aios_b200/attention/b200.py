@@ -152,7 +152,7 @@ class B200AttentionBackend(BaseAttentionBackend):
         mask, positions = ops.draft_tree(parents, tree_start, max_nodes=max(sizes), cached_lens=cached_lens)
         return B200AttentionMetadata(phase="draft", positions=positions, out_loc=out_loc, row_table=row_table,
                                      parents=parents, tree_start=tree_start, tree_mask=mask, cached_lens=cached_lens,
-                                     max_cached=max(cached))
+                                     max_cached=max(1, *cached))
 
     # -- fused path (raw qkv projection in) -------------------------------------
     def forward_qkv(
