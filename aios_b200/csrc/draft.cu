@@ -70,6 +70,7 @@ __global__ void __launch_bounds__(kTreeThreads)
 constexpr int kVerifyThreads = 512;
 constexpr int kVerifyWarps = kVerifyThreads / 32;
 constexpr int kMaxRanks = 16;
+constexpr int kGreedyRanks = 8;
 constexpr int kBlockIds = 256;  // ids that a warp takes at a time, eight to a lane
 
 struct VerifyArgs {
@@ -380,7 +381,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) verify_greedy_kernel(const 
 // drawn hangs on comparisons of them.
 // Bound by the latency of the visited nodes: some 6600 clocks each for the row's loads, eleven fp64 instructions to an
 // exponential, and the cluster's exchange; with many requests by the fp64 pipes and the passes over shared memory. A
-// chain of 5 at 16384 ids 13.5 us, 16 trees of 26 at 32001 ids 18, 64 trees of 24 with probabilities at 131072 ids 128
+// chain of 5 at 16384 ids 13.5 us, 16 trees of 26 at 32001 ids 17, 64 trees of 24 with probabilities at 131072 ids 128
 // (one CTA to an SM 196).
 // A warp's run of a row is a multiple of this; a row comes as fp32 into the first half of its groups' places.
 constexpr int kRunIds = 64;
@@ -782,8 +783,13 @@ template <typename T>
 cudaError_t launch_verify(VerifyArgs a, int requests, bool greedy, int places, cudaStream_t stream) {
   a.ranks = 1;
   const int sms = sm_count();
-  // more CTAs to a request while they find SMs, and two blocks to each of their warps
-  while (a.ranks < 8 && (int64_t)requests * a.ranks * 2 <= sms && a.vocab >= a.ranks * 2 * kVerifyWarps * kBlockIds)
+  // More CTAs to a request while they find SMs, and a block to each of their warps: two for the argmax, which has
+  // little to do with one (1 x 16384 ids 5.7 us with 4 CTAs, 6.2 with 8). Sampling, us: 16 trees of 26, 32001 ids: 4
+  // CTAs 18.4, 8 17.1; 2 of 8, 6400 ids: 1 CTA 15.0, 2 12.0; 8 of 8, 50021 ids: 8 CTAs 13.9, 16 12.8, with
+  // probabilities 37.0 and 30.7.
+  const int64_t each = (int64_t)kVerifyWarps * kBlockIds * (greedy ? 2 : 1);
+  while (a.ranks < (greedy ? kGreedyRanks : kMaxRanks) && (int64_t)requests * a.ranks * 2 <= sms &&
+         a.vocab >= a.ranks * each)
     a.ranks *= 2;
   static bool configured[3][64] = {};
   if (greedy) return launch_cluster(verify_greedy_kernel<T>, a, requests, 0, configured[0], stream);
