@@ -228,7 +228,7 @@ cudaError_t launch_small(const TreeAttnArgs& a, int64_t max_nodes, cudaStream_t 
 // Whether the keys are dealt over the SMs (attn_tree_split.cu): for longer histories, or many rows, which its tensor
 // cores take faster. Measured, whole / dealt, us: 16 requests of 26 nodes, 8/2 heads of 96: 64 keys 10.2 / 13.1, 128
 // 13.2 / 14.3, 256 19.3 / 16.2, 1024 55 / 18.4; 1 of 8 heads of 128, 5 nodes: 64 10.9 / 11.0, 128 15.3 / 14.6; 64 of 60
-// nodes, 32 keys, 8 / 12 / 32 heads (30720, 46080, 122880 rows): 26.3 / 18.8, 25.3 / 21.8, 117 / 47; of 26 nodes, 8 and
+// nodes, 32 keys, 8 / 12 / 32 heads (31, 46, 123 thousand rows): 26.3 / 18.8, 25.3 / 21.8, 117 / 47; of 26 nodes, 8 and
 // 12 heads (13312, 19968 rows): 10.1 / 14.6, 14.8 / 17.7.
 bool splits(int64_t max_cached, int64_t tokens, int64_t heads) { return max_cached > 128 || tokens * heads > 24000; }
 
