@@ -180,11 +180,10 @@ constexpr int kExpTable = 16;
 // P. T. P. Tang, ACM TOMS 15, 1989). Eleven fp64 instructions, where the general function takes some thirty. A sum's
 // borders are off by 2^-42 of it at most, so that a draw among 2^18 tokens differs from the exact one's once in 2^24.
 // scale: 16 / (T ln 2); base: m * scale (its rounding is a factor of all weights). Below m - 600 T, and for x of -inf,
-// it is 2^-865, as nothing against 1: at or below kNothing a weight counts as 0.
-constexpr double kNothing = 0x1p-800;
+// it is 0: a masked token adds nothing to any sum, so that a sum is above 0 exactly where one of its tokens is.
 __device__ __forceinline__ double exp_table(float x, double scale, double base, const double* table) {
-  double t = fma(widen(x), scale, -base);
-  t = __hiloint2double((int)min((uint32_t)__double2hiint(t), 0xC0CB0D00u), __double2loint(t));  // max(t, -13850)
+  const double t = fma(widen(x), scale, -base);
+  const bool none = (uint32_t)__double2hiint(t) >= 0xC0CB0D00u;  // t <= -13850
   const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are round(t)
   const double s = t + magic, f = t - (s - magic);
   const int k = __double2loint(s);
@@ -195,7 +194,7 @@ __device__ __forceinline__ double exp_table(float x, double scale, double base, 
   p = fma(f, p, c);
   const double b = table[k & (kExpTable - 1)];
   const double r = fma(b, f * p, b);
-  return __hiloint2double(__double2hiint(r) + ((k >> 4) << 20), __double2loint(r));
+  return none ? 0.0 : __hiloint2double(__double2hiint(r) + ((k >> 4) << 20), __double2loint(r));
 }
 __device__ __forceinline__ double positive(double x) {  // max(x, 0) of a number
   const int keep = ~(__double2hiint(x) >> 31);
@@ -578,7 +577,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
     for (int i = 0; i < children; ++i) {
       const double rx = child_r[i], qx = PROBS ? widen(child_q[i]) : 1.0;
       const int child = walk.child[i], x = node_x[child];
-      if (rx > kNothing && (double)node_u[child] * qx * total < rx) {
+      if (rx > 0 && (double)node_u[child] * qx * total < rx) {
         found = child;
         break;
       }
@@ -614,7 +613,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
             child_r[c] = positive(fma(child_r[c], inv, -widen(child_q[c])));
           __syncthreads();
         }
-      } else if (rx > kNothing) {
+      } else if (rx > 0) {
         __syncthreads();
         for (int c = threadIdx.x; c < children; c += kVerifyThreads)
           if (node_x[walk.child[c]] == x) child_r[c] = 0;
@@ -640,13 +639,16 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
     }
 
     // ---- the next token
-    auto group_weights = [&](int p, double (&w)[8]) {  // r of the group at p
+    // the first pass's sums and weights are over the ranks' own maxima, later ones are r's
+    const bool direct = stale || pending != 0;
+    const double by = direct ? mult : 1.0;
+    auto group_weights = [&](int p, double (&w)[8]) {  // the group at p, as the sums have it
       load_group(group_of(p), w);
       float qv[8];
       if (PROBS && pending != 0) load_probs(q, p - shift, a.vocab, qv);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        w[j] *= mult;
+        w[j] *= by;
         if (PROBS && pending != 0) w[j] = positive(fma(w[j], pending, -widen(qv[j])));
       }
     };
@@ -660,8 +662,6 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
       }
       exchange(part, 0.f);
     }
-    // the first pass's sums are over the ranks' own maxima, later ones are r's
-    const bool direct = stale || pending != 0;
     auto rank_sum = [&](int c) { return ex.sum[last_turn][c] * (direct ? 1.0 : factor[c]); };
     double target = 0, before = 0, owner_before = 0;
     for (int c = 0; c < ranks; ++c) target += rank_sum(c);
@@ -670,7 +670,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
     int owner = -1;
     for (int c = 0; c < ranks; ++c) {
       const double w = rank_sum(c);
-      if (w > kNothing) {
+      if (w > 0) {
         owner = c;
         owner_before = before;
         if (before + w > target) break;
@@ -678,12 +678,14 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
       before += w;
     }
     if (owner == rank) {
+      // (over the rank's own maximum: far below the others' its weights times their factor may all be 0)
+      if (!direct) target = (target - owner_before) / factor[rank];
       int own_warp = -1;
-      double warp_before = owner_before;
-      before = owner_before;
+      double warp_before = 0;
+      before = direct ? owner_before : 0;
       for (int w = 0; w < kVerifyWarps; ++w) {
-        const double x = warp_sum_of[w] * (direct ? 1.0 : mult);
-        if (x > kNothing) {
+        const double x = warp_sum_of[w];
+        if (x > 0) {
           own_warp = w;
           warp_before = before;
           if (before + x > target) break;
@@ -700,7 +702,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
           int last = -1;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            if (w[j] > kNothing) last = p + j - shift;
+            if (w[j] > 0) last = p + j - shift;
             sum += w[j];
           }
           double upto = sum;
@@ -718,7 +720,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
 #pragma unroll
             for (int j = 0; j < 8; ++j) {  // the first one past the target
               c += w[j];
-              if (w[j] > kNothing && c > target) {
+              if (w[j] > 0 && c > target) {
                 pick = p + j - shift;
                 c = -INFINITY;
               }

@@ -510,7 +510,7 @@ AIOSB_API int aiosb_attention_tree(const void* q, int64_t q_stride, int64_t toke
  * which is the next token; the uniforms may be NULL and the temperature is not read.
  * Logits of -inf take a token out. Everything is computed in fp64 from the inputs.
  * Sampling takes vocabularies of up to 262144 ids (262137 where rows are not on 16 bytes) and temperatures in [1e-6, 1e6]; tokens
- * whose logit lies more than 600 * temperature below the largest one count as masked.
+ * whose logit lies more than 600 * temperature below the largest one may count as masked.
  * Outputs: accepted[r], the accepted nodes behind the root; next_token[r] (int64); order
  * ([tokens]): the tree's node numbers, the path from the root first, the others after it
  * in ascending order (the order in which a caller keeps the page-table entries). An empty
