@@ -181,9 +181,9 @@ constexpr int kExpTable = 16;
 // borders are off by 2^-42 of it at most, so that a draw among 2^18 tokens differs from the exact one's once in 2^24.
 // scale: 16 / (T ln 2); base: m * scale (its rounding is a factor of all weights). Below m - 600 T, and for x of -inf,
 // it is 0: a masked token adds nothing to any sum, so that a sum is above 0 exactly where one of its tokens is.
-__device__ __forceinline__ double exp_table(float x, double scale, double base, const double* table) {
-  const double t = fma(widen(x), scale, -base);
-  const bool none = (uint32_t)__double2hiint(t) >= 0xC0CB0D00u;  // t <= -13850
+constexpr uint32_t kFar = 0xC0CB0D00u;  // upper half of -13850
+// (t above -13850, or anything where the result is not used)
+__device__ __forceinline__ double exp_any(double t, const double* table) {
   const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are round(t)
   const double s = t + magic, f = t - (s - magic);
   const int k = __double2loint(s);
@@ -194,7 +194,11 @@ __device__ __forceinline__ double exp_table(float x, double scale, double base, 
   p = fma(f, p, c);
   const double b = table[k & (kExpTable - 1)];
   const double r = fma(b, f * p, b);
-  return none ? 0.0 : __hiloint2double(__double2hiint(r) + ((k >> 4) << 20), __double2loint(r));
+  return __hiloint2double(__double2hiint(r) + ((k >> 4) << 20), __double2loint(r));
+}
+__device__ __forceinline__ double exp_table(float x, double scale, double base, const double* table) {
+  const double t = fma(widen(x), scale, -base);
+  return (uint32_t)__double2hiint(t) >= kFar ? 0.0 : exp_any(t, table);
 }
 __device__ __forceinline__ double positive(double x) {  // max(x, 0) of a number
   const int keep = ~(__double2hiint(x) >> 31);
@@ -236,6 +240,17 @@ __device__ __forceinline__ void list_children(Walk& w, int cur, int n) {  // one
     count += __popc(some);
   }
   if (lane == 0) w.children = count;
+}
+// Bit i of `repeated`: a child before child i has its token. One warp, behind list_children.
+__device__ __forceinline__ void mark_repeated(const Walk& w, const int32_t* child_x, uint32_t* repeated) {
+  const int lane = threadIdx.x & 31, n = w.children;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const int x = i0 + lane < n ? child_x[i0 + lane] : -2 - lane;
+    bool again = (__match_any_sync(0xffffffffu, x) & ((1u << lane) - 1)) != 0;
+    for (int j = 0; j < i0; ++j) again |= child_x[j] == x;
+    const unsigned some = __ballot_sync(0xffffffffu, again);
+    if (lane == 0) repeated[i0 >> 5] = some;
+  }
 }
 // Writes the path, then the other nodes; one warp.
 __device__ __forceinline__ void write_order(const Walk& w, int depth, int n, int all, int32_t* order) {
@@ -394,10 +409,15 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
   __shared__ double child_r[AIOSB_TREE_MAX_NODES];  // the children's r, and what they were drawn with
   __shared__ float child_q[AIOSB_TREE_MAX_NODES], node_u[AIOSB_TREE_MAX_NODES];
   __shared__ int32_t node_x[AIOSB_TREE_MAX_NODES];  // the nodes' tokens; -1: none of the vocabulary
+  __shared__ int32_t child_x[AIOSB_TREE_MAX_NODES];
   __shared__ double warp_sum_of[kVerifyWarps];
   __shared__ float warp_top[kVerifyWarps];
   __shared__ double factor[kMaxRanks];  // of the ranks' weights: they are stored over the rank's own maximum
   __shared__ double all_weights;
+  // without probabilities: the children's repeated tokens, the child that is accepted (-1: none), and the only token
+  // that is left (-1: there are others)
+  __shared__ uint32_t repeated[AIOSB_TREE_MAX_NODES / 32];
+  __shared__ int accepted_child, only_token;
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int ranks = a.ranks, rank = (int)cluster_ctarank(), r = blockIdx.x / ranks;
@@ -477,6 +497,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
           if (PROBS) child_p = q[x];
         }
       }
+      for (int i = lane; i < walk.children; i += 32) child_x[i] = node_x[walk.child[i]];
+      __syncwarp();
+      if (!PROBS) mark_repeated(walk, child_x, repeated);
     }
     // ---- the row, as it is, to its place; its maximum
     float top = -INFINITY;
@@ -495,7 +518,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
     if (lane == 0) warp_top[warp] = top;
     if (warp == 0) {
       for (int i = lane; i < walk.children; i += 32) {
-        const int x = node_x[walk.child[i]];
+        const int x = child_x[i];
         if (x < 0 && rank == 0) report(a.status, AIOSB_DEV_TOKEN_RANGE);
         if (i >= 32) {
           child_l = x >= 0 ? load_logit(row + x) : -INFINITY;
@@ -511,6 +534,17 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
     for (int o = kVerifyWarps / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     top = __shfl_sync(0xffffffffu, top, 0);
     const int children = walk.children;
+    if (!PROBS) {  // proposals stand beside the others' weights (below): out of the row, whose values are still fp32
+      for (int i = lane; i < children; i += 32) {
+        const int x = child_x[i], place = x + shift;
+        if (x >= 0 && place >= lo && place < hi) {
+          const int at = place - rank_lo;
+          reinterpret_cast<float*>(weights)[(at & ~7) * 2 + ((((at >> 4) & 3) ^ ((at >> 2) & 1)) << 2) + (at & 3)] =
+              -INFINITY;
+        }
+      }
+      __syncwarp();
+    }
     // ---- weights over this CTA's maximum (one that is NaN or +inf ends the walk below; -inf leaves nothing)
     double part = 0;
     const double mine = widen(top > -INFINITY ? top : 0.f) * scale;
@@ -546,43 +580,85 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
       const float m = ex.top[last_turn][c];
       return m > -INFINITY ? exp_table(m, scale, all, table) : 0.0;
     };
-    if (warp == 0) {
+    auto child_weight = [&](int i) {
+      const int x = child_x[i];
+      if (x < 0) return 0.0;
+      const int owner = (x + shift) / per_rank;
+      const float m = ex.top[last_turn][owner];
+      if (!(m > -INFINITY)) return 0.0;
+      return exp_table(*reinterpret_cast<const float*>(&child_r[i]), scale, widen(m) * scale, table) * factor_of(owner);
+    };
+    if (PROBS && warp == 1) {
+      for (int i = lane; i < children; i += 32) child_r[i] = child_weight(i);
+    } else if (warp < 2) {
       const int c = lane & (kMaxRanks - 1);
       const double f = c < ranks ? factor_of(c) : 0.0;
       double z = c < ranks ? f * ex.sum[last_turn][c] : 0.0;
 #pragma unroll
       for (int o = kMaxRanks / 2; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-      if (lane < ranks) factor[lane] = f;
-      if (lane == 0) all_weights = z;
-    } else if (warp == 1) {
-      for (int i = lane; i < children; i += 32) {
-        const int x = node_x[walk.child[i]];
-        double p = 0;
-        if (x >= 0) {
-          const int owner = (x + shift) / per_rank;
-          const float m = ex.top[last_turn][owner];
-          if (m > -INFINITY)
-            p = exp_table(*reinterpret_cast<const float*>(&child_r[i]), scale, widen(m) * scale, table) *
-                factor_of(owner);
+      if (warp == 0) {
+        if (lane < ranks) factor[lane] = f;
+        if (lane == 0) all_weights = z;
+      } else if (!PROBS) {
+        // Where child i is tried, what is left is z, the weights of the tokens that nobody proposed, and those of the
+        // proposals from i on: a sum from the last one back, never a difference, which would lose its digits when a
+        // rejected token had most of the weight.
+        double behind = z;
+        int found = -1, last = -1;
+        for (int i0 = (children - 1) & ~31; i0 >= 0; i0 -= 32) {
+          const int i = i0 + lane;
+          const bool tried = i < children && !((repeated[i0 >> 5] >> lane) & 1);
+          const double w = tried ? child_weight(i) : 0.0;
+          double from = w;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const double y = __shfl_down_sync(0xffffffffu, from, o);
+            if (lane + o < 32) from += y;
+          }
+          from += behind;
+          const unsigned yes =
+              __ballot_sync(0xffffffffu, w > 0 && (double)node_u[walk.child[min(i, children - 1)]] * from < w);
+          const unsigned some = __ballot_sync(0xffffffffu, w > 0);
+          if (yes) found = i0 + __ffs(yes) - 1;
+          if (some && last < 0) last = i0 + 31 - __clz(some);
+          behind = __shfl_sync(0xffffffffu, from, 0);
         }
-        child_r[i] = p;
+        int only = -1;
+        if (found < 0 && !(z > 0) && last >= 0) {
+          // rejecting the last proposal would leave nothing: r stays as it was, that token alone, and a later child
+          // with the same token may still be accepted
+          only = child_x[last];
+          int again = INT32_MAX;
+          for (int i = last + 1 + lane; i < children; i += 32)
+            if (child_x[i] == only && node_u[walk.child[i]] < 1.f) again = min(again, i);
+          again = __reduce_min_sync(0xffffffffu, again);
+          if (again < INT32_MAX) found = again;
+        }
+        if (lane == 0) {
+          accepted_child = found;
+          only_token = only;
+        }
       }
     }
     __syncthreads();
 
-    // ---- the children, in ascending order. r(v) is weights(v) * mult, behind `pending`, the last subtraction
-    double mult = factor[rank], pending = 0, total = all_weights;
+    // ---- with probabilities: the children, in ascending order. r(v) is weights(v) * mult, behind `pending`, the last
+    // subtraction
+    double mult = factor[rank], pending = 0;
     bool stale = false;  // the runs' sums are not r's
     int found = -1;
-    for (int i = 0; i < children; ++i) {
-      const double rx = child_r[i], qx = PROBS ? widen(child_q[i]) : 1.0;
-      const int child = walk.child[i], x = node_x[child];
-      if (rx > 0 && (double)node_u[child] * qx * total < rx) {
-        found = child;
-        break;
-      }
-      if (x < 0) continue;
-      if (PROBS) {
+    if (!PROBS) {
+      if (accepted_child >= 0) found = walk.child[accepted_child];
+    } else {
+      double total = all_weights;
+      for (int i = 0; i < children; ++i) {
+        const double rx = child_r[i], qx = widen(child_q[i]);
+        const int child = walk.child[i];
+        if (rx > 0 && (double)node_u[child] * qx * total < rx) {
+          found = child;
+          break;
+        }
+        if (child_x[i] < 0) continue;
         const double inv = 1.0 / total;
         part = 0;
 #pragma unroll 1
@@ -613,18 +689,6 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
             child_r[c] = positive(fma(child_r[c], inv, -widen(child_q[c])));
           __syncthreads();
         }
-      } else if (rx > 0) {
-        __syncthreads();
-        for (int c = threadIdx.x; c < children; c += kVerifyThreads)
-          if (node_x[walk.child[c]] == x) child_r[c] = 0;
-        const int place = x + shift;
-        if (threadIdx.x == 0 && place >= rank_lo && place < rank_lo + per_rank) {
-          const int i = place - rank_lo;
-          weights[i ^ (((i >> 4) & 3) << 1)] = 0;
-        }
-        total -= rx;
-        stale = true;
-        __syncthreads();
       }
     }
     if (found >= 0) {
@@ -639,7 +703,12 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
     }
 
     // ---- the next token
-    // the first pass's sums and weights are over the ranks' own maxima, later ones are r's
+    if (!PROBS && only_token >= 0) {
+      if (first) a.next_token[r] = only_token;
+      break;
+    }
+    // the first pass's sums and weights are over the ranks' own maxima, later ones are r's (without probabilities
+    // there are none: the row's weights have no proposal's)
     const bool direct = stale || pending != 0;
     const double by = direct ? mult : 1.0;
     auto group_weights = [&](int p, double (&w)[8]) {  // the group at p, as the sums have it
@@ -676,6 +745,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
         if (before + w > target) break;
       }
       before += w;
+    }
+    if (owner < 0 && first) {  // no token has any weight
+      report(a.status, AIOSB_DEV_NO_DISTRIBUTION);
+      a.next_token[r] = -1;
     }
     if (owner == rank) {
       // (over the rank's own maximum: far below the others' its weights times their factor may all be 0)

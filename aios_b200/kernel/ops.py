@@ -1201,7 +1201,8 @@ def verify_draft(
     on, a node's children are tried in order: child c stays if ``accept_uniforms[c] * q(x) *
     sum(r) < r(x)``, where r is softmax(logits / temperature) less what the rejected ones took,
     and q is ``draft_probs`` (fp32 [tokens, vocab]; row i: the distribution that i's children were
-    drawn from, independently) or 1 without it (distinct proposals). With no child left the next
+    drawn from, independently) or 1 without it (distinct proposals). A rejection that would leave
+    nothing (a certain token, a uniform of 1) leaves r as it was. With no child left the next
     token is drawn from r by inverse CDF with ``sample_uniforms``. What is kept has the target's
     distribution. ``greedy``: children and next token by argmax (the lowest id of equal ones).
     A sampler's filters (top-k, forbidden ids) go in as logits of -inf. Sampling takes up to 262144

@@ -500,12 +500,13 @@ AIOSB_API int aiosb_attention_tree(const void* q, int64_t q_stride, int64_t toke
  *   p = softmax(logits[node] / temperature), r = p;
  *   the node's children c in ascending order: c is accepted if
  *     accept_uniforms[c] * q(x_c) * sum(r) < r(x_c),   x_c = draft_tokens[c];
- *   rejected, r becomes max(r / sum(r) - q, 0) with draft_probs (kept as it is where
- *   that is 0 for every token), and r with r(x_c) = 0 without;
+ *   rejected, r becomes max(r / sum(r) - q, 0) with draft_probs, and r with r(x_c) = 0
+ *   without; where that is 0 for every token, r stays as it was;
  *   an accepted child is the next node; with none, the next token is the first v with
  *     r(0) + ... + r(v) > sample_uniforms[r] * sum(r).
  * draft_probs ([tokens, vocab] fp32 or NULL): row `node` is the distribution q that the
  * node's children were drawn from, independently; without it q = 1 (distinct proposals).
+ * The uniforms may be any numbers; one of 1 or more rejects, even a certain token.
  * greedy: a child is accepted if it is the logits' argmax (the lowest id of equal ones),
  * which is the next token; the uniforms may be NULL and the temperature is not read.
  * Logits of -inf take a token out. Everything is computed in fp64 from the inputs.

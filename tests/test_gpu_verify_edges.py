@@ -50,3 +50,53 @@ def test_tokens_up_to_600_temperatures_below_the_largest(cuda_device, vocab: int
             assert want[1][0] == at[1 if sample < 0.6 else 2]  # 1 / (1 + e^-0.5) = 0.62
             assert got == want
     ops.check_status(cuda_device)
+
+
+@pytest.mark.parametrize("vocab", [1, 8, 70000])
+@pytest.mark.parametrize("u", [1.0, 1.5])
+def test_a_rejection_that_would_leave_nothing(cuda_device, vocab: int, u: float) -> None:
+    """Without probabilities: a forced token, rejected by a uniform of 1 (splitmix uniforms round up to it), stays the
+    only one, for later children and as the next token."""
+    logits = [-INF] * vocab
+    x = vocab - 1
+    logits[x] = 3.0
+    for parents, drafts, accept, accepted, token in [
+        ([-1, 0], [0, x], [0.0, u], 0, x),
+        ([-1, 0, 0, 0], [0, x, 0, x], [0.0, u, u, 0.5], 1 if vocab > 1 else None, x),
+        ([-1, 0, 0, 0], [0, x, 0, x], [0.0, u, u, u], 0, x),
+        ([-1] + [0] * 70, [0] + [x] * 70, [0.0] + [u] * 66 + [0.9] * 4, 1, x),
+        ([-1] + [0] * 70, [0] * 36 + [x] * 35, [0.0] + [u] * 70, 0, x),
+    ]:
+        got, want = _verify(logits, drafts, parents, accept, 0.4)
+        assert got == want and got[1] == [token] and accepted in (None, got[0][0])
+    ops.check_status(cuda_device)
+
+
+@pytest.mark.parametrize("vocab", [24, 70000])
+@pytest.mark.parametrize("step", [15.7, 16.2])
+def test_what_near_certain_rejections_leave(cuda_device, vocab: int, step: float) -> None:
+    """Children that have all but e^-16 of what is left, one after another, each rejected by a uniform next to 1: the
+    last one is tried against its share of a sum that is 2^-69 of the first."""
+    logits = _spread([0.0, -step, -2 * step, -3 * step, -3 * step - 0.7, -3 * step - 0.9], vocab)
+    at = [i for i, x in enumerate(logits) if x > -INF]
+    share = 1 / (1 + 2.718281828459045**-0.7 + 2.718281828459045**-0.9)
+    below = 1 - 2.0**-24
+    for u in (share - 0.1, share - 1e-4, share + 1e-4, share + 0.1, below):
+        for sample in (0.3, 0.5, 0.6):
+            got, want = _verify(logits, [0] + at[:4], [-1] + [0] * 4, [0.0] + [below] * 3 + [u], sample)
+            assert want[0] == [1 if u < share else 0]
+            assert got == want
+    ops.check_status(cuda_device)
+
+
+def test_many_proposals_of_few_tokens(cuda_device) -> None:
+    """Tokens repeated among up to 200 children, within and across groups of 32: each counts once."""
+    g = torch.Generator().manual_seed(9)
+    for n in (2, 31, 33, 64, 65, 200):
+        for vocab in (5, 40, 300):
+            logits = (2 * torch.randn(vocab, generator=g)).tolist()
+            for top in (1.0, 0.99999):
+                drafts = [0] + torch.randint(0, vocab, (n,), generator=g).tolist()
+                accept = [0.0] + (1 - torch.rand(n, generator=g) ** 4 * top).tolist()
+                got, want = _verify(logits, drafts, [-1] + [0] * n, accept, 0.5)
+                assert got == want
