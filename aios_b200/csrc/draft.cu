@@ -1,6 +1,7 @@
 // Drafted token trees around the forward: the ancestors' bits and positions of the nodes, and the
 // verification of a tree against the target model's distributions.
 #include <algorithm>
+#include <type_traits>
 
 #include "abi_util.h"
 #include "common.cuh"
@@ -182,8 +183,10 @@ constexpr int kExpTable = 16;
 // scale: 16 / (T ln 2); base: m * scale (its rounding is a factor of all weights). Below m - 600 T, and for x of -inf,
 // it is 0: a masked token adds nothing to any sum, so that a sum is above 0 exactly where one of its tokens is.
 constexpr uint32_t kFar = 0xC0CB0D00u;  // upper half of -13850
-// (t above -13850, or anything where the result is not used)
-__device__ __forceinline__ double exp_any(double t, const double* table) {
+// FAR false: t is above -13850, or the result is not used.
+template <bool FAR = true>
+__device__ __forceinline__ double exp_table(float x, double scale, double base, const double* table) {
+  const double t = fma(widen(x), scale, -base);
   const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are round(t)
   const double s = t + magic, f = t - (s - magic);
   const int k = __double2loint(s);
@@ -194,11 +197,8 @@ __device__ __forceinline__ double exp_any(double t, const double* table) {
   p = fma(f, p, c);
   const double b = table[k & (kExpTable - 1)];
   const double r = fma(b, f * p, b);
+  if (FAR && (uint32_t)__double2hiint(t) >= kFar) return 0.0;
   return __hiloint2double(__double2hiint(r) + ((k >> 4) << 20), __double2loint(r));
-}
-__device__ __forceinline__ double exp_table(float x, double scale, double base, const double* table) {
-  const double t = fma(widen(x), scale, -base);
-  return (uint32_t)__double2hiint(t) >= kFar ? 0.0 : exp_any(t, table);
 }
 __device__ __forceinline__ double positive(double x) {  // max(x, 0) of a number
   const int keep = ~(__double2hiint(x) >> 31);
@@ -502,13 +502,16 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
       if (!PROBS) mark_repeated(walk, child_x, repeated);
     }
     // ---- the row, as it is, to its place; its maximum
-    float top = -INFINITY;
+    float top = -INFINITY, low = INFINITY;
 #pragma unroll 2
     for (int p = lo + lane * 8; p < hi; p += kBlockIds) {
       float x[8];
       places.load(p, x);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = max_nan(top, x[j]);
+      for (int j = 0; j < 8; ++j) {
+        top = max_nan(top, x[j]);
+        low = fminf(low, x[j]);
+      }
       float4* const g = reinterpret_cast<float4*>(group_of(p));
       g[swap] = make_float4(x[0], x[1], x[2], x[3]);
       g[1 ^ swap] = make_float4(x[4], x[5], x[6], x[7]);
@@ -541,6 +544,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
           const int at = place - rank_lo;
           reinterpret_cast<float*>(weights)[(at & ~7) * 2 + ((((at >> 4) & 3) ^ ((at >> 2) & 1)) << 2) + (at & 3)] =
               -INFINITY;
+          low = -INFINITY;
         }
       }
       __syncwarp();
@@ -548,22 +552,27 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
     // ---- weights over this CTA's maximum (one that is NaN or +inf ends the walk below; -inf leaves nothing)
     double part = 0;
     const double mine = widen(top > -INFINITY ? top : 0.f) * scale;
+    auto weigh = [&](auto any) {
 #pragma unroll 1
-    for (int v = lo + lane * 8; v < hi; v += kBlockIds) {
-      double* const g = group_of(v);
-      const float4 x0 = reinterpret_cast<const float4*>(g)[swap], x1 = reinterpret_cast<const float4*>(g)[1 ^ swap];
-      const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-      double e[8];
+      for (int v = lo + lane * 8; v < hi; v += kBlockIds) {
+        double* const g = group_of(v);
+        const float4 x0 = reinterpret_cast<const float4*>(g)[swap], x1 = reinterpret_cast<const float4*>(g)[1 ^ swap];
+        const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+        double e[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) e[j] = exp_table(x[j], scale, mine, table);
-      if (v < shift || v + 8 > places.end) {
+        for (int j = 0; j < 8; ++j) e[j] = exp_table<any.value>(x[j], scale, mine, table);
+        if (v < shift || v + 8 > places.end) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (v + j < shift || v + j >= places.end) e[j] = 0;
+          for (int j = 0; j < 8; ++j)
+            if (v + j < shift || v + j >= places.end) e[j] = 0;
+        }
+        store_group(g, e);
+        part += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
       }
-      store_group(g, e);
-      part += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-    }
+    };
+    // 0 for a far value takes three instructions of a thread: only where the warp has one
+    if (__any_sync(0xffffffffu, (uint32_t)__double2hiint(fma(widen(low), scale, -mine)) >= kFar)) weigh(std::true_type());
+    else weigh(std::false_type());
     exchange(part, top);
     float most = -INFINITY;
     for (int c = 0; c < ranks; ++c) most = max_nan(most, ex.top[last_turn][c]);
