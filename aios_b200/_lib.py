@@ -36,7 +36,7 @@ DEVICE_STATUS_NAMES = {
     DEV_POOL_EMPTY: "free-slot FIFO exhausted",
     DEV_POSITION_RANGE: "position outside the RoPE table",
     DEV_TREE_RANGE: "drafted tree or its history outside its arrays",
-    DEV_NO_DISTRIBUTION: "logits row that no token can be drawn from",
+    DEV_NO_DISTRIBUTION: "row of logits or draft probabilities that no token can be drawn from",
 }
 
 EPI_STORE = 0

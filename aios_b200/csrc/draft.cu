@@ -1,5 +1,7 @@
 // Drafted token trees around the forward: the ancestors' bits and positions of the nodes, and the
 // verification of a tree against the target model's distributions.
+#include <math_constants.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -171,6 +173,14 @@ __device__ __forceinline__ void load_probs(const float* row, int i, int vocab, f
 __device__ __forceinline__ double widen(float x) {
   const uint32_t u = __float_as_uint(x);
   return __hiloint2double((int)((((u >> 3) & 0x0FFFFFFFu) + 0x38000000u) | (u & 0x80000000u)), (int)(u << 29));
+}
+
+// A probability in fp64; 0 and what lies below 2^-126 as 0 (the subtrahend of a token that was never proposed, which
+// may have next to no weight itself). nan becomes NaN where a value is infinite or NaN.
+__device__ __forceinline__ double probability(float x, float& nan) {
+  nan = fmaf(x, 0.f, nan);
+  const double d = widen(x);
+  return __hiloint2double(fabsf(x) < 0x1p-126f ? 0 : __double2hiint(d), __double2loint(d));
 }
 
 // 2^(i / 16) for the exponential below: sixteen doubles are all of the banks once, so that no two lanes' entries
@@ -656,13 +666,15 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
     double mult = factor[rank], pending = 0;
     bool stale = false;  // the runs' sums are not r's
     int found = -1;
+    float nan = 0.f;  // NaN: one of the probabilities that were read is no number
     if (!PROBS) {
       if (accepted_child >= 0) found = walk.child[accepted_child];
     } else {
       double total = all_weights;
       for (int i = 0; i < children; ++i) {
-        const double rx = child_r[i], qx = widen(child_q[i]);
+        const double rx = child_r[i], qx = probability(child_q[i], nan);
         const int child = walk.child[i];
+        if (isnan(nan)) break;
         if (rx > 0 && (double)node_u[child] * qx * total < rx) {
           found = child;
           break;
@@ -679,7 +691,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
           load_group(g, w);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const double qj = widen(qv[j]);
+            const double qj = probability(qv[j], nan);
             w[j] *= mult;
             if (pending != 0) w[j] = positive(fma(w[j], pending, -qj));
             sum += positive(fma(w[j], inv, -qj));
@@ -688,17 +700,26 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
           part += sum;
         }
         mult = 1;
-        exchange(part, 0.f);
+        exchange(part + nan, 0.f);
         const double left = total_sum();
+        nan = isnan(left) ? CUDART_NAN_F : 0.f;  // in all threads
+        if (isnan(left)) break;
         pending = left > 0 ? inv : 0;  // where nothing is left r stays
         stale = !(left > 0);
         if (left > 0) {
           total = left;
           for (int c = threadIdx.x; c < children; c += kVerifyThreads)
-            child_r[c] = positive(fma(child_r[c], inv, -widen(child_q[c])));
+            child_r[c] = positive(fma(child_r[c], inv, -probability(child_q[c], nan)));
           __syncthreads();
         }
       }
+    }
+    if (PROBS && isnan(nan)) {
+      if (first) {
+        report(a.status, AIOSB_DEV_NO_DISTRIBUTION);
+        a.next_token[r] = -1;
+      }
+      break;
     }
     if (found >= 0) {
       cur = found;
@@ -727,7 +748,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         w[j] *= by;
-        if (PROBS && pending != 0) w[j] = positive(fma(w[j], pending, -widen(qv[j])));
+        if (PROBS && pending != 0) w[j] = positive(fma(w[j], pending, -probability(qv[j], nan)));
       }
     };
     if (stale) {

@@ -1209,7 +1209,8 @@ def verify_draft(
     ids and temperatures in [1e-6, 1e6].
 
     Returns ``accepted`` (int32 [requests]: nodes behind the root that stay), ``next_token``
-    (int64 [requests]; -1 where there is no tree or no distribution) and ``order`` (int32
+    (int64 [requests]; -1 where there is no tree, or a row of logits or probabilities that was read
+    is no distribution) and ``order`` (int32
     [tokens]: each tree's node numbers, the path from the root first, then the others; undefined
     behind the last tree)."""
     if not logits.is_cuda:

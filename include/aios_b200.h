@@ -53,7 +53,7 @@ extern "C" {
 #define AIOSB_DEV_POOL_EMPTY 4    /* free-slot FIFO had fewer entries than asked    */
 #define AIOSB_DEV_POSITION_RANGE 5 /* RoPE position outside the cos/sin table      */
 #define AIOSB_DEV_TREE_RANGE 6    /* a drafted tree or its history outside its arrays */
-#define AIOSB_DEV_NO_DISTRIBUTION 7 /* a logits row that no token can be drawn from  */
+#define AIOSB_DEV_NO_DISTRIBUTION 7 /* logits or probabilities that no token can be drawn from */
 
 /* GEMM epilogues for aiosb_linear. */
 #define AIOSB_EPI_STORE 0    /* y = x W^T, bf16                                         */
@@ -506,7 +506,8 @@ AIOSB_API int aiosb_attention_tree(const void* q, int64_t q_stride, int64_t toke
  *     r(0) + ... + r(v) > sample_uniforms[r] * sum(r).
  * draft_probs ([tokens, vocab] fp32 or NULL): row `node` is the distribution q that the
  * node's children were drawn from, independently; without it q = 1 (distinct proposals).
- * The uniforms may be any numbers; one of 1 or more rejects, even a certain token.
+ * The uniforms may be any numbers: without draft_probs, one of 1 or more rejects even a
+ * certain token.
  * greedy: a child is accepted if it is the logits' argmax (the lowest id of equal ones),
  * which is the next token; the uniforms may be NULL and the temperature is not read.
  * Logits of -inf take a token out. Everything is computed in fp64 from the inputs.
@@ -516,7 +517,9 @@ AIOSB_API int aiosb_attention_tree(const void* q, int64_t q_stride, int64_t toke
  * ([tokens]): the tree's node numbers, the path from the root first, the others after it
  * in ascending order (the order in which a caller keeps the page-table entries). An empty
  * tree gets 0 and -1. A row with a NaN, with +inf (unless greedy) or with -inf only ends
- * the path with next_token -1 and AIOSB_DEV_NO_DISTRIBUTION; a draft token outside the
+ * the path with next_token -1 and AIOSB_DEV_NO_DISTRIBUTION, and so does a probability
+ * that is infinite or NaN, where one is read (at a tried child's token, and anywhere in
+ * the row that a rejection takes off r; below 2^-126 it counts as 0); a draft token outside the
  * vocabulary is rejected (AIOSB_DEV_TOKEN_RANGE). */
 AIOSB_API int aiosb_verify_draft(const void* logits, int logits_fp32, int64_t logits_stride, int64_t tokens,
                                  int64_t vocab, const int64_t* draft_tokens, const int32_t* parents,

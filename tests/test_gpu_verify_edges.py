@@ -100,3 +100,62 @@ def test_many_proposals_of_few_tokens(cuda_device) -> None:
                 accept = [0.0] + (1 - torch.rand(n, generator=g) ** 4 * top).tolist()
                 got, want = _verify(logits, drafts, [-1] + [0] * n, accept, 0.5)
                 assert got == want
+
+
+@pytest.mark.parametrize("vocab", [8, 9000, 70000])
+@pytest.mark.parametrize("below", [60.0, 95.0, 400.0, 599.0])
+def test_what_the_drafting_model_never_proposes_loses_nothing(cuda_device, vocab: int, below: float) -> None:
+    """Probabilities of 0 take nothing, not even from the smallest of weights."""
+    logits = _spread([0.0, -below, -below - 0.5], vocab)
+    at = [i for i, x in enumerate(logits) if x > -INF]
+    for zero in (0.0, -0.0):
+        q = [zero] * vocab
+        q[at[0]] = 1.0
+        for sample in (0.3, 0.7):
+            got, want = _verify(logits, [0, at[0]], [-1, 0], [0.0, 1.5], sample, q)
+            assert want[1][0] == at[1 if sample < 0.6 else 2]  # 1 / (1 + e^-0.5) = 0.62
+            assert got == want
+    ops.check_status(cuda_device)
+
+
+@pytest.mark.parametrize("zero", [0.0, -0.0, 1e-39])
+def test_a_masked_token_gains_nothing(cuda_device, zero: float) -> None:
+    """q = p but for the sign of a masked token's 0 (or a probability that is none of the normal numbers): nothing is
+    left, so the distribution stays."""
+    for sample, token in ((0.2, 0), (0.6, 1), (0.99, 1)):
+        got, want = _verify([0.0, 0.0, -INF], [0, 0], [-1, 0], [0.0, 1.5], sample, [0.5, 0.5, zero])
+        assert got == want and got[1] == [token]
+    ops.check_status(cuda_device)
+
+
+@pytest.mark.parametrize("vocab", [6, 70000])
+@pytest.mark.parametrize("value", [float("nan"), -float("nan"), INF, -INF])
+def test_probabilities_that_are_none(cuda_device, vocab: int, value: float) -> None:
+    """Seen where they are read: at a child's own token, and in the row that a rejection takes off. The path ends there
+    without a next token, as it does at a row of logits that is no distribution."""
+    x = vocab - 2
+    logits = [0.0] * vocab
+    q = [1.0 / vocab] * vocab
+    q[x] = value
+    for drafts, accept, stays in (([0, x], [0.0, 0.1], 0), ([0, 1], [0.0, 5.0 * vocab], 0),
+                                  ([0, 1, x], [0.0, 5.0 * vocab, 0.1], 0)):
+        got, _ = _verify(logits, drafts, [-1] + [0] * (len(drafts) - 1), accept, 0.5, q)
+        assert got[0] == [stays] and got[1] == [-1] and got[2] == list(range(len(drafts)))
+        with pytest.raises(RuntimeError, match="no token"):
+            ops.check_status(cuda_device)
+    # not read: the first child stays, and its own row has no children
+    got, _ = _verify(logits, [0, 1], [-1, 0], [0.0, 0.5], 0.5, q)
+    assert got[0] == [1] and 0 <= got[1][0] < vocab
+    ops.check_status(cuda_device)
+
+
+def test_probabilities_are_taken_as_they_are(cuda_device) -> None:
+    """Above 1 or below 0, they go into the formula all the same."""
+    for x, value in ((2, -0.25), (2, 7.0), (3, -1e-30)):
+        q = [0.2, 0.3, 0.1, 0.4]
+        q[x] = value
+        for sample in (0.1, 0.4, 0.7, 0.95):
+            for accept in (0.1, 3.0):
+                got, want = _verify([0.5, 0.1, 0.2, -0.3], [0, 1, 2], [-1, 0, 0], [0.0, 3.0, accept], sample, q)
+                assert got == want
+    ops.check_status(cuda_device)
