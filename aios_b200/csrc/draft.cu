@@ -190,13 +190,12 @@ constexpr int kExpTable = 16;
 // from the table and k's upper bits, and 2^(f / 16) by its series to the fifth power (table-driven exponentials:
 // P. T. P. Tang, ACM TOMS 15, 1989). Eleven fp64 instructions, where the general function takes some thirty. A sum's
 // borders are off by 2^-42 of it at most, so that a draw among 2^18 tokens differs from the exact one's once in 2^24.
-// scale: 16 / (T ln 2); base: m * scale (its rounding is a factor of all weights). Below m - 600 T, and for x of -inf,
+// scale: 16 / (T ln 2); base: m * scale (its rounding is a factor of the weights over it). Below m - 600 T, and for x of -inf,
 // it is 0: a masked token adds nothing to any sum, so that a sum is above 0 exactly where one of its tokens is.
 constexpr uint32_t kFar = 0xC0CB0D00u;  // upper half of -13850
-// FAR false: t is above -13850, or the result is not used.
+// 2^(t / 16). FAR false: t is above -13850, or the result is not used.
 template <bool FAR = true>
-__device__ __forceinline__ double exp_table(float x, double scale, double base, const double* table) {
-  const double t = fma(widen(x), scale, -base);
+__device__ __forceinline__ double exp_table(double t, const double* table) {
   const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are round(t)
   const double s = t + magic, f = t - (s - magic);
   const int k = __double2loint(s);
@@ -209,6 +208,10 @@ __device__ __forceinline__ double exp_table(float x, double scale, double base, 
   const double r = fma(b, f * p, b);
   if (FAR && (uint32_t)__double2hiint(t) >= kFar) return 0.0;
   return __hiloint2double(__double2hiint(r) + ((k >> 4) << 20), __double2loint(r));
+}
+template <bool FAR = true>
+__device__ __forceinline__ double exp_table(float x, double scale, double base, const double* table) {
+  return exp_table<FAR>(fma(widen(x), scale, -base), table);
 }
 __device__ __forceinline__ double positive(double x) {  // max(x, 0) of a number
   const int keep = ~(__double2hiint(x) >> 31);
@@ -595,9 +598,11 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
     }
     // ---- what the ranks' weights count, and the children's r
     const double all = widen(most) * scale;
+    // from the rounded base that the rank's weights are over: its rounding is up to 2^-54 of m / T, and would stand
+    // between one rank's weights and another's
     auto factor_of = [&](int c) {
       const float m = ex.top[last_turn][c];
-      return m > -INFINITY ? exp_table(m, scale, all, table) : 0.0;
+      return m > -INFINITY ? exp_table(__dmul_rn(widen(m), scale) - all, table) : 0.0;
     };
     auto child_weight = [&](int i) {
       const int x = child_x[i];

@@ -2,6 +2,9 @@
 
 from __future__ import annotations
 
+import math
+from fractions import Fraction
+
 import pytest
 import torch
 
@@ -159,3 +162,35 @@ def test_probabilities_are_taken_as_they_are(cuda_device) -> None:
                 got, want = _verify([0.5, 0.1, 0.2, -0.3], [0, 1, 2], [-1, 0, 0], [0.0, 3.0, accept], sample, q)
                 assert got == want
     ops.check_status(cuda_device)
+
+
+def _temperature_for(u: float, lower: float, nudge: float) -> float:
+    """Where a token 0 has the share u * (1 + nudge) beside one of logit -lower."""
+    share = u * (1 + nudge)
+    return lower / math.log(share / (1 - share))
+
+
+def test_borders_between_ctas(cuda_device) -> None:
+    """The likeliest two tokens in different CTAs of a request, |logit| / T about 10^7: fp64's rounding of logit / T must
+    not come between them. The draws lie 5e-11 to 1e-10 of the sum from the border; the temperatures are those where
+    twice the roundings (of 16 logit / (T ln 2), exact by fractions) would carry the border across."""
+    vocab, found = 70000, 0
+    for m1 in (20.0, -20.0, 300.0):
+        m2 = float(torch.nextafter(torch.tensor(m1), torch.tensor(-INF)))
+        row = [-INF] * vocab
+        row[3], row[60003] = m1, m2
+        for i in range(400):
+            nudge = (5e-11 + 5e-11 * i / 400) * (1 if i % 2 else -1)
+            t = _temperature_for(0.75, m1 - m2, nudge)
+            scale = (1 / t) * (1.4426950408889634 * 16)
+            e1, e2 = (float(Fraction(m) * Fraction(scale) - Fraction(m * scale)) for m in (m1, m2))
+            crossed = 0.25 * (e1 - e2) * math.log(2) / 16 * (1 if nudge < 0 else -1)
+            if crossed < 1.5 * abs(nudge):
+                continue
+            found += 1
+            got, want = _verify(row, [0], [-1], [0.0], 0.75, temperature=t)
+            assert want[1] == [3 if nudge > 0 else 60003]
+            assert got == want
+            if found % 8 == 0:
+                break
+    assert found >= 16
