@@ -186,10 +186,10 @@ __device__ __forceinline__ double probability(float x, float& nan) {
 // 2^(i / 16) for the exponential below: sixteen doubles are all of the banks once, so that no two lanes' entries
 // conflict (a table of 128 cost as much as the arithmetic).
 constexpr int kExpTable = 16;
-// e^((x - m) / T) in fp64 for x <= m, off by about 2^-42: (x - m) / (T ln 2) = (k + f) / 16 with |f| <= 1/2, 2^(k / 16)
-// from the table and k's upper bits, and 2^(f / 16) by its series to the fifth power (table-driven exponentials:
-// P. T. P. Tang, ACM TOMS 15, 1989). Eleven fp64 instructions, where the general function takes some thirty. A sum's
-// borders are off by 2^-42 of it at most, so that a draw among 2^18 tokens differs from the exact one's once in 2^24.
+// e^((x - m) / T) in fp64 for x <= m: (x - m) / (T ln 2) = (k + f) / 16 with |f| <= 1/2, 2^(k / 16) from the table and
+// k's upper bits, and 2^(f / 16) by its series to the sixth power (table-driven exponentials: P. T. P. Tang, ACM TOMS
+// 15, 1989), whose rest is 2^-51. Twelve fp64 instructions, where the general function takes some thirty. Off by 2^-50,
+// and by 2^-51 of (x - m) / T for the rounding of what it is taken of.
 // scale: 16 / (T ln 2); base: m * scale (its rounding is a factor of the weights over it). Below m - 600 T, and for x of -inf,
 // it is 0: a masked token adds nothing to any sum, so that a sum is above 0 exactly where one of its tokens is.
 constexpr uint32_t kFar = 0xC0CB0D00u;  // upper half of -13850
@@ -200,7 +200,8 @@ __device__ __forceinline__ double exp_table(double t, const double* table) {
   const double s = t + magic, f = t - (s - magic);
   const int k = __double2loint(s);
   constexpr double c = 0.043321698784996581;  // ln 2 / 16
-  double p = fma(f, c * c * c * c * c / 120, c * c * c * c / 24);
+  double p = fma(f, c * c * c * c * c * c / 720, c * c * c * c * c / 120);
+  p = fma(f, p, c * c * c * c / 24);
   p = fma(f, p, c * c * c / 6);
   p = fma(f, p, c * c / 2);
   p = fma(f, p, c);

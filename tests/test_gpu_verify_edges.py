@@ -194,3 +194,17 @@ def test_borders_between_ctas(cuda_device) -> None:
             if found % 8 == 0:
                 break
     assert found >= 16
+
+
+@pytest.mark.parametrize("probs", [False, True])
+def test_borders_within_fp64(cuda_device, probs: bool) -> None:
+    """Draws 2e-14 of the sum from a border, for weights anywhere between the table's entries: those in the middle are
+    where an exponential of less than fp64's digits is off by most."""
+    for eighth in range(100, 125):
+        z = eighth / 4 * math.log(2) / 16 + 1e-4
+        u = float(torch.tensor(1 / (1 + math.exp(-z))))
+        for nudge in (-2e-14, 2e-14):
+            t = _temperature_for(u, 1.0, nudge)
+            got, want = _verify([0.0, -1.0], [0], [-1], [0.0], u, [0.5, 0.5] if probs else None, temperature=t)
+            assert want[1] == [0 if nudge > 0 else 1]
+            assert got == want, (eighth, nudge)
