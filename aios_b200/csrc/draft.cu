@@ -280,10 +280,12 @@ __device__ __forceinline__ void write_order(const Walk& w, int depth, int n, int
   }
 }
 
-// (-1 for what is no node's number)
-__device__ __forceinline__ int16_t parent_of(const VerifyArgs& a, int row) {
-  const int p = a.parents[row];
-  return (int16_t)(p >= 0 && p < AIOSB_TREE_MAX_NODES ? p : -1);
+// Of node i; -1 for what is not the number of a node before it.
+__device__ __forceinline__ int16_t parent_of(const VerifyArgs& a, int start, int i, bool tell) {
+  const int p = a.parents[start + i];
+  if (p >= -1 && p < i) return (int16_t)p;
+  if (tell) report(a.status, AIOSB_DEV_TREE_RANGE);
+  return -1;
 }
 
 struct TreeRows {
@@ -317,7 +319,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) verify_greedy_kernel(const 
   pdl_enter();
   TreeRows t;
   if (!tree_rows(a, r, rank == 0 && threadIdx.x == 0, t)) return;  // the whole cluster leaves
-  for (int i = threadIdx.x; i < t.n; i += kVerifyThreads) walk.up[i] = parent_of(a, t.start + i);
+  for (int i = threadIdx.x; i < t.n; i += kVerifyThreads) walk.up[i] = parent_of(a, t.start, i, rank == 0);
   if (threadIdx.x < AIOSB_TREE_MAX_NODES / 32) walk.on_path[threadIdx.x] = threadIdx.x == 0 ? 1u : 0u;
   if (threadIdx.x == 0) walk.path[0] = 0;
   cluster_sync();  // every CTA runs: its shared memory may be written
@@ -442,7 +444,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
   if (!tree_rows(a, r, first, t)) return;  // the whole cluster leaves
   for (int i = threadIdx.x; i < t.n; i += kVerifyThreads) {
     const int64_t x = a.draft_tokens[t.start + i];
-    walk.up[i] = parent_of(a, t.start + i);
+    walk.up[i] = parent_of(a, t.start, i, rank == 0);
     node_x[i] = x >= 0 && x < a.vocab ? (int32_t)x : -1;
     node_u[i] = a.accept_u[t.start + i];
   }

@@ -208,3 +208,21 @@ def test_borders_within_fp64(cuda_device, probs: bool) -> None:
             got, want = _verify([0.0, -1.0], [0], [-1], [0.0], u, [0.5, 0.5] if probs else None, temperature=t)
             assert want[1] == [0 if nudge > 0 else 1]
             assert got == want, (eighth, nudge)
+
+
+@pytest.mark.parametrize("mode", ["greedy", "plain", "probs"])
+@pytest.mark.parametrize("node,parent", [(2, 2), (1, 3), (3, -2), (2, 1 << 20), (0, 0), (1, -(1 << 31))])
+def test_parents_that_are_no_earlier_node_are_reported(cuda_device, mode: str, node: int, parent: int) -> None:
+    """As by draft_tree: the node counts as a root, so nothing leads to it."""
+    parents, drafts = [-1, 0, 0, 1], [0, 3, 4, 2]
+    logits = [0.0, 0.1, 0.3, 0.9, 0.2]
+    q = [0.2] * 5 if mode == "probs" else None
+    kw = {"greedy": True} if mode == "greedy" else {}
+    as_root = [-1 if i == node else p for i, p in enumerate(parents)]
+    want, _ = _verify(logits, drafts, as_root, [0.0, 0.3, 0.3, 0.3], 0.5, q, **kw)
+    ops.check_status(cuda_device)
+    got, _ = _verify(logits, drafts, [parent if i == node else p for i, p in enumerate(parents)],
+                     [0.0, 0.3, 0.3, 0.3], 0.5, q, **kw)
+    assert got == want
+    with pytest.raises(RuntimeError, match="tree"):
+        ops.check_status(cuda_device)
