@@ -937,6 +937,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
               const uint32_t all[2] = {};
               ok = soft_step<D, false>(t_s, t_o, all, a.scale_log2, fresh, ref, sum, settled);
             }
+            if (!ok) break;  // the output is still at the old reference: nothing may follow it
           }
           fresh = false;
           tc_fence_before();
