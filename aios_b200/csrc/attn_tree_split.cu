@@ -616,6 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full, q_phase));
       q_phase ^= 1;
       if (!ok) break;
+      tc_fence_after();  // the softmax warps have read the last piece's scores' place
       if (chunk_of(0) < n) {
         ok = __all_sync(0xffffffffu, wait_block(k_block(chunk_of(0))));
         if (ok && elect_one()) {
