@@ -95,6 +95,7 @@ class B200AttentionBackend(BaseAttentionBackend):
         reqs = batch.reqs
         if batch.is_draft:
             batch.attn_metadata = md = self._draft_metadata(batch, out_loc)
+            batch.positions = md.positions  # what a model rotates by where it is not this backend that does
             return md
         positions = batch.positions.to(device=device, dtype=torch.int32)
         if batch.is_prefill:
