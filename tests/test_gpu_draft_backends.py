@@ -1,7 +1,9 @@
-"""Draft batches of models on other roads than the fused bf16 one: an attention backend behind another."""
+"""Draft batches of models on other roads than the fused bf16 one: an attention backend behind another, and 8-bit
+linears."""
 
 from __future__ import annotations
 
+import math
 import random
 
 import pytest
@@ -12,6 +14,7 @@ from aios_b200.core import Batch, Req
 from aios_b200.kernel import ops
 from tests import draft_reference as ref
 from tests.test_gpu_draft_model import GREEDY, MODELS, IDS, Server, _prompts
+from tests.test_gpu_fp8_model import _attnres_by_hand, _standard_by_hand
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +76,26 @@ def test_a_draft_batch_holds_its_positions(cuda_device) -> None:
             b.positions = given
         s.llm.model.attn_backend.prepare_metadata(b)
         assert b.positions.tolist() == ref.tree_bits(trees, 1, s.cached)[1].tolist()
+
+
+@pytest.mark.parametrize("cfg", MODELS, ids=IDS)
+def test_8_bit_linears(cuda_device, cfg) -> None:
+    """A draft forward's logits are those of its operators one by one in a layer's order, bit for bit, and as far from
+    the bf16 model's as 8-bit prefills may be."""
+    s = _serve(cfg, "fp8")
+    caught = []
+
+    def forward():
+        out = LLMModel.forward(s.llm.model)
+        batch = s.llm.ctx.batch
+        caught.append((_attnres_by_hand if cfg is MODELS[2] else _standard_by_hand)(s.llm, batch))
+        return out
+
+    LLMModel = type(s.llm.model)
+    s.llm.model.forward = forward
+    _, got = _draft(s, cfg)
+    assert torch.equal(got, caught[0])
+    del s.llm.model.forward
+    exact = _draft(_serve(cfg, "bf16"), cfg)[1].double()
+    assert float((got.double() - exact).norm() / exact.norm()) < 0.051 * math.sqrt(7 * cfg.num_layers)
+    ops.check_status(cuda_device)
