@@ -240,7 +240,8 @@ using namespace aiosb;
 extern "C" int64_t aiosb_attention_tree_work_bytes(int64_t tokens, int64_t requests, int64_t mask_words,
                                                    int64_t max_cached, int64_t num_qo_heads, int64_t num_kv_heads,
                                                    int64_t head_dim) {
-  if (tokens <= 0 || requests <= 0 || num_kv_heads <= 0 || !splits(max_cached, tokens, num_qo_heads)) return 0;
+  if (tokens <= 0 || requests <= 0 || num_kv_heads <= 0) return 0;
+  if (max_cached > 0 && !splits(max_cached, tokens, num_qo_heads)) return 0;  // 0: the page table's width, any
   const int64_t rows = std::min(mask_words * 32, tokens) * (num_qo_heads / num_kv_heads);
   return tree_split_work_bytes(tree_split_grid(), tree_split_unit_rows(rows), (int)head_dim);
 }

@@ -480,8 +480,9 @@ AIOSB_API int aiosb_draft_tree(const int32_t* parents, int64_t tokens, const int
  * head; mask_words up to AIOSB_TREE_MAX_NODES / 32. max_cached: a bound on cached_lens
  * from which the split over the GPU is chosen (0: the page table's width); longer
  * histories are read all the same.
- * work: aiosb_attention_tree_work_bytes() bytes, 16-byte aligned, of any content;
- * launches that may overlap need one each. */
+ * work: aiosb_attention_tree_work_bytes() bytes for the same arguments, 16-byte aligned,
+ * of any content (with max_cached 0, what any width may need); launches that may overlap
+ * need one each. */
 AIOSB_API int64_t aiosb_attention_tree_work_bytes(int64_t tokens, int64_t requests, int64_t mask_words,
                                                   int64_t max_cached, int64_t num_qo_heads, int64_t num_kv_heads,
                                                   int64_t head_dim);

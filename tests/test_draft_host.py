@@ -114,3 +114,16 @@ def test_the_work_areas_rule_is_the_wrappers(bound: int, tokens: int) -> None:
     """attention_tree asks the library for a work area's size only where it needs one."""
     size = _lib.load().aiosb_attention_tree_work_bytes(tokens, 1, 1, bound, 8, 2, 64)
     assert (size > 0) == (bound > 128 or tokens * 8 > 24000)
+
+
+@pytest.mark.parametrize("tokens", [1, 3000, 3001])
+@pytest.mark.parametrize("width", [64, 128, 129, 4096])
+def test_without_a_bound_the_work_area_is_enough_for_any_width(tokens: int, width: int) -> None:
+    """max_cached 0 stands for the page table's width, which the query does not have: it names what the widest needs."""
+    lib = _lib.load()
+    size = lib.aiosb_attention_tree_work_bytes(tokens, 1, 1, 0, 12, 4, 64)
+    assert size >= lib.aiosb_attention_tree_work_bytes(tokens, 1, 1, width, 12, 4, 64) and size > 0
+    good = {**ATTENTION, "tokens": tokens, "width": width, "ts": width}
+    if width > 128 or tokens * 12 > 24000:
+        _refused("aiosb_attention_tree", good, INV, "work area", work_bytes=size - 1)
+        _refused("aiosb_attention_tree", good, INV, "work area", work=P + 8, work_bytes=size)
