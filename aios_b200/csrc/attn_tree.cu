@@ -165,16 +165,19 @@ __global__ void __launch_bounds__(kThreads) attn_tree_small_kernel(const TreeAtt
       }
 #pragma unroll
       for (int k = 0; k < kChunk / 16; ++k) {
-        // the weights as the A operand, to bf16: off by 2^-8 of each at most, as the result is by its own
-        const uint32_t p[4] = {pack_bf16x2(s[2 * k][0], s[2 * k][1]), pack_bf16x2(s[2 * k][2], s[2 * k][3]),
-                               pack_bf16x2(s[2 * k + 1][0], s[2 * k + 1][1]),
-                               pack_bf16x2(s[2 * k + 1][2], s[2 * k + 1][3])};
+        uint32_t p[2][4];  // the weights as the A operand, upper and lower halves
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          split_bf16x2(make_float2(s[2 * k + i / 2][i % 2 * 2], s[2 * k + i / 2][i % 2 * 2 + 1]), p[0][i], p[1][i]);
 #pragma unroll
         for (int n = 0; n < D / 16; ++n) {
           uint32_t b[4];
           ldmatrix4_trans(b, smem_u32(vs + (k * 16 + (lane & 15)) * kPitch<D> + n * 16 + (lane & 16 ? 8 : 0)));
-          mma_16816(o[2 * n], p, b[0], b[1]);
-          mma_16816(o[2 * n + 1], p, b[2], b[3]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            mma_16816(o[2 * n], p[i], b[0], b[1]);
+            mma_16816(o[2 * n + 1], p[i], b[2], b[3]);
+          }
         }
       }
       if (tree && (bad[0] | bad[1])) {

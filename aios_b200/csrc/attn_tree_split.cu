@@ -14,18 +14,18 @@
 // sum and output, joined at the end. S = Q K^T goes from shared memory into TMEM, 64 keys at a time into
 // two buffers, so that a stream's next scores are formed while it takes the present exponentials. A
 // thread owns a row (a TMEM lane), takes its maximum and exponentials, and writes the weights back over
-// S as the bf16 A operand of O += P V (V as it lies, the keys as its k: an MN-major B operand). Up to 32
+// S as bf16 A operands of O += P V (V as it lies, the keys as its k: an MN-major B operand), one of their
+// upper and one of their lower halves, which together fill S's place (split_bf16x2). Up to 32
 // rows go on mma.sync instead, with no TMEM round trip (few_rows below).
 // A row's output is rescaled only where its maximum has grown by more than 2^8 over the one that its
-// exponentials refer to: any reference gives the same quotient. Weights are rounded to bf16 for the
-// second product (each off by 2^-8 of itself at most, of either sign); their sum is of the
-// unrounded ones.
+// exponentials refer to: any reference gives the same quotient.
 //
-// What bounds it, with more than 128 rows: a step of 64 keys takes about 2100 clocks, of which the
-// exponentials of 256 rows are 1024 (16 a clock), the softmax threads' whole work 1500 to 1900 while two
-// groups share the issue slots, and the products 1370. 32 requests x 16384 keys, 64 nodes, 32/8 heads of
-// 128: 579 us alone, 697 in a row of calls under the power limit; the products at the dense rate would take
-// 328. With few rows: the gather (64 x 8192 keys, 5 nodes, 12/4 heads of 64: 122 us, 4.4 TB/s). With little
+// What bounds it, with more than 128 rows: a step of 64 keys takes about 2560 clocks, of which the
+// exponentials of 256 rows are 1024 (16 a clock), the softmax threads' whole work some 1900 to 2200 while two
+// groups share the issue slots, and the products 1880. Without the weights' lower halves it took 2100: 131071
+// keys, 64 nodes, 32/8 heads of 128 150 us, 182 with them (164 without their products, 169 without their
+// arithmetic). Their upper halves' products begun ahead of the lower ones took 196. 32 requests x 16384 keys
+// at the same rows: 705 to 750 us; its products at the dense rate, with one half, would take 328. With few rows: the gather (64 x 8192 keys, 5 nodes, 12/4 heads of 64: 122 us, 4.4 TB/s). With little
 // work: the start and end of a unit, some 10000 clocks (16 x 1900 keys 17 us).
 #include <algorithm>
 
@@ -244,9 +244,9 @@ __device__ __forceinline__ uint32_t seen32(const int32_t* bits, int words, int k
   return left >= 32 ? m : m & ((1u << left) - 1u);
 }
 
-// One step of a row: its 64 scores at t_s to weights in bf16 over them; the row's reference and sum, and its output
-// at t_o where the reference moves (behind `settled`: the products so far are in it). `seen`: bits of the keys, if
-// some are hidden. False: a wait ran out.
+// One step of a row: its 64 scores at t_s to weights over them, 32 columns of upper halves and 32 of lower ones; the
+// row's reference and sum, and its output at t_o where the reference moves (behind `settled`: the products so far are
+// in it). `seen`: bits of the keys, if some are hidden. False: a wait ran out.
 template <int D, bool MASKED, typename Settled>
 __device__ __forceinline__ bool soft_step(uint32_t t_s, uint32_t t_o, const uint32_t (&seen)[2], float scale, bool fresh,
                                           float& ref, float& sum, Settled settled) {
@@ -297,15 +297,16 @@ __device__ __forceinline__ bool soft_step(uint32_t t_s, uint32_t t_o, const uint
   float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    uint32_t w[16];
+    uint32_t w[2][16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       float2 x = __ffma2_rn(make_float2(__uint_as_float(v[j][2 * e]), __uint_as_float(v[j][2 * e + 1])), s2, m2);
       x = make_float2(exp2_fast(x.x), exp2_fast(x.y));
       part[e & 1] = __fadd2_rn(part[e & 1], x);
-      w[e] = pack_bf16x2(x.x, x.y);  // off by 2^-8 of each at most, as the result is by its own
+      split_bf16x2(x, w[0][e], w[1][e]);
     }
-    tmem_st16(t_s + j * 16, w);  // over columns that have been read
+#pragma unroll
+    for (int i = 0; i < 2; ++i) tmem_st16(t_s + i * (kStep / 2) + j * 16, w[i]);  // over columns that have been read
   }
   sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
   tmem_wait_st();
@@ -642,8 +643,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
           const uint32_t v = ring + stage * S::kBlockBytes + (h & 1) * (kStep * 128);
 #pragma unroll
           for (int k = 0; k < kStep / 16; ++k)
-            tc_mma_bf16_ts(tmem + 256 + s * 128, tmem + s * 128 + buffer * kStep + k * 8, umma_desc_mn(v + k * 2048),
-                           idesc_o, h > 0 || k > 0);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)  // the weights' upper and lower halves
+              tc_mma_bf16_ts(tmem + 256 + s * 128, tmem + s * 128 + buffer * kStep + i * (kStep / 2) + k * 8,
+                             umma_desc_mn(v + k * 2048), idesc_o, h > 0 || k > 0 || i > 0);
           tc_commit(&sh.pv_done[s]);
           if (h & 1) release(stage);
           if (next < n) score(h + 2);
@@ -715,7 +718,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
         const uint32_t ks = kb % S::kStages, vs = vb % S::kStages;
         const uint32_t k_mem = ring + ks * S::kBlockBytes, v_mem = ring + vs * S::kBlockBytes;
         if (!__all_sync(0xffffffffu, mbar_wait(&sh.full[ks], (kb / S::kStages) & 1))) return false;
-        uint32_t w[2][4];  // weights as A operands, 16 keys each
+        uint32_t w[2][2][4];  // weights as A operands, 16 keys each: upper and lower halves
         if (works) {
           float x[2][2][4];  // scores: 16 keys, 8 keys, the accumulator's values
 #pragma unroll
@@ -782,7 +785,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
                 const float y = exp2_fast(fmaf(x[g][n][2 * i], a.scale_log2, minus)),
                             z = exp2_fast(fmaf(x[g][n][2 * i + 1], a.scale_log2, minus));
                 sum[i] += y + z;
-                w[g][2 * n + i] = pack_bf16x2(y, z);  // off by 2^-8 of each at most, as the result is by its own
+                split_bf16x2(make_float2(y, z), w[g][0][2 * n + i], w[g][1][2 * n + i]);
               }
             }
           }
@@ -798,8 +801,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
           for (int n = 0; n < D / 16; ++n) {
             uint32_t b[4];
             ldmatrix4_trans(b, piece_at(v_mem, key + (lane & 15), 2 * n + (lane >> 4)));
-            mma_16816(o[2 * n], w[g], b[0], b[1]);
-            mma_16816(o[2 * n + 1], w[g], b[2], b[3]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              mma_16816(o[2 * n], w[g][i], b[0], b[1]);
+              mma_16816(o[2 * n + 1], w[g][i], b[2], b[3]);
+            }
           }
         }
         __syncwarp();

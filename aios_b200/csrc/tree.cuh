@@ -69,6 +69,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// Two weights as bf16 and what is left of them as bf16 again: both halves go through the second product, as in the
+// prefill attention, so that its weights are off by 2^-16 of each at most, where one bf16 would be off by 2^-8.
+__device__ __forceinline__ void split_bf16x2(float2 x, uint32_t& upper, uint32_t& lower) {
+  upper = pack_bf16x2(x.x, x.y);
+  lower = pack_bf16x2(x.x - bf16_lo(upper), x.y - bf16_hi(upper));
+}
+
 __device__ __forceinline__ bool finite_bf16x2(uint32_t v) {
   return (v & 0x7F800000u) != 0x7F800000u && (v & 0x7F80u) != 0x7F80u;
 }
