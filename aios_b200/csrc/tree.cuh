@@ -69,11 +69,14 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// Two weights as bf16 and what is left of them as bf16 again: both halves go through the second product, as in the
-// prefill attention, so that its weights are off by 2^-16 of each at most, where one bf16 would be off by 2^-8.
+// Two weights as bf16, cut off, and what is left of them as bf16 again: both halves go through the second product, as in
+// the prefill attention. The rest is below 2^-7 of a weight and rounded by 2^-8 of itself, so that the weights of the
+// product are off by 2^-15 of each at most, where one bf16 would be off by 2^-8. A rest of a weight above 0 is above 0 as
+// well (the factor's 2^-20 of the weight): beside an infinite value a product with 0, or a negative one, would be NaN.
 __device__ __forceinline__ void split_bf16x2(float2 x, uint32_t& upper, uint32_t& lower) {
-  upper = pack_bf16x2(x.x, x.y);
-  lower = pack_bf16x2(x.x - bf16_lo(upper), x.y - bf16_hi(upper));
+  constexpr float c = 1.f + 0x1p-20f;
+  upper = __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);
+  lower = pack_bf16x2(fmaf(x.x, c, -bf16_lo(upper)), fmaf(x.y, c, -bf16_hi(upper)));
 }
 
 __device__ __forceinline__ bool finite_bf16x2(uint32_t v) {
