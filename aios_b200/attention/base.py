@@ -40,7 +40,7 @@ class BaseAttentionBackend(ABC):
 
 
 class HybridAttentionBackend(BaseAttentionBackend):
-    """Dispatch to separate prefill/decode backends by batch phase."""
+    """Dispatch to separate prefill/decode backends by batch phase (draft batches: the decode one)."""
 
     def __init__(self, prefill_backend: BaseAttentionBackend, decode_backend: BaseAttentionBackend) -> None:
         self.prefill_backend = prefill_backend

@@ -94,7 +94,7 @@ class Batch:
     # A draft batch (phase "draft"): per request the parents of its drafted tree, node 0 the
     # request's last known token (-1), every other node's parent before it. input_ids and
     # out_loc hold the nodes of all trees; page-table entry cached_len + i of a request holds
-    # node i's slot. The backend derives the nodes' positions; logits come for every node.
+    # node i's slot. The backend derives the nodes' positions and sets them; logits come for every node.
     trees: List[List[int]] | None = None
 
     @property

@@ -961,7 +961,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
       // ---- a narrow unit's streams are joined here: each group writes half of the columns
       float weight[2] = {1.f, 0.f};
       float m_all = ref, l_all = sum;
-      bool use[2] = {s == 0 || !pair, !pair && p.c1 - p.c0 > 1};
+      const bool both = !pair && p.c1 - p.c0 > 1;  // streams of a narrow unit that have seen keys
       if (!pair) {
         // through TMEM, where S was: the two warps with this row reach the same lane
         tmem_st2(t_lane + s * 128, __float_as_uint(ref), __float_as_uint(sum));
@@ -973,11 +973,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
         float2 x, y;
         tmem_ld2(t_lane, x);
         tmem_ld2(t_lane + 128, y);
-        m_all = fmaxf(x.x, use[1] ? y.x : -INFINITY);
+        m_all = fmaxf(x.x, both ? y.x : -INFINITY);
         const float m = m_all == -INFINITY ? 0.f : m_all;
         weight[0] = exp2_fast(x.x - m);
-        weight[1] = use[1] ? exp2_fast(y.x - m) : 0.f;
-        l_all = x.y * weight[0] + (use[1] ? y.y * weight[1] : 0.f);
+        weight[1] = both ? exp2_fast(y.x - m) : 0.f;
+        l_all = x.y * weight[0] + (both ? y.y * weight[1] : 0.f);
       }
       const bool whole = p.whole();
       const bool none = m_all == -INFINITY && l_all == 0.f;  // the row sees none of these keys
@@ -1003,7 +1003,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_split_kernel(const Tree
           tmem_wait(v);
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[e] = __uint_as_float(v[e]) * weight[0];
-          if (use[1]) {
+          if (both) {
             tmem_ld(t_lane + 384 + j * 16, v);
             tmem_wait(v);
 #pragma unroll
