@@ -23,7 +23,7 @@ constexpr size_t kSmallSmem = 2 * 2 * (size_t)kChunk * kPitch<D> * 2;  // K and 
 
 // Whole requests: a CTA takes 64 rows of one KV head through all of their keys, on mma.sync from two staged chunks in
 // turn: with few keys there is nothing to deal out, and a TMEM round trip is longer than a chunk's products. Bound by
-// launch and two dependent loads (slots, then keys): 1 request, 32 + 8 keys, 8 nodes, 12/4 heads of 64 in 5.4 us.
+// launch and two dependent loads (slots, then keys): 1 request, 32 + 8 keys, 8 nodes, 12/4 heads of 64 in 5.7 us.
 template <int D>
 __global__ void __launch_bounds__(kThreads) attn_tree_small_kernel(const TreeAttnArgs a) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -229,10 +229,10 @@ cudaError_t launch_small(const TreeAttnArgs& a, int64_t max_nodes, cudaStream_t 
 }
 
 // Whether the keys are dealt over the SMs (attn_tree_split.cu): for longer histories, or many rows, which its tensor
-// cores take faster. Measured, whole / dealt, us: 16 requests of 26 nodes, 8/2 heads of 96: 64 keys 10.2 / 13.1, 128
-// 13.2 / 14.3, 256 19.3 / 16.2, 1024 55 / 18.4; 1 of 8 heads of 128, 5 nodes: 64 10.9 / 11.0, 128 15.3 / 14.6; 64 of 60
-// nodes, 32 keys, 8 / 12 / 32 heads (31, 46, 123 thousand rows): 26.3 / 18.8, 25.3 / 21.8, 117 / 47; of 26 nodes, 8 and
-// 12 heads (13312, 19968 rows): 10.1 / 14.6, 14.8 / 17.7.
+// cores take faster. Measured, whole / dealt, us: 16 requests of 26 nodes, 8/2 heads of 96: 64 keys 10.9 / 13.5, 128
+// 14.6 / 14.9, 256 20.8 / 16.9, 1024 60 / 19.5; 1 of 5 nodes, 32/8 heads of 128: 64 11.7 / 11.5, 128 16.7 / 15.1. 64
+// requests, 32 keys, 8/2 heads of 96: 15872 rows 11.1 / 15.3, 20480 16.1 / 18.7, 30720 27.6 / 19.3; 12/4 of 64: 19968
+// 15.6 / 18.9, 23808 15.7 / 19.1, 30720 22.5 / 21.0; 32/8 of 128: 53248 41.6 / 37.5, 122880 126 / 50.
 bool splits(int64_t max_cached, int64_t tokens, int64_t heads) { return max_cached > 128 || tokens * heads > 24000; }
 
 }  // namespace

@@ -21,12 +21,13 @@
 // exponentials refer to: any reference gives the same quotient.
 //
 // What bounds it, with more than 128 rows: a step of 64 keys takes about 2560 clocks, of which the
-// exponentials of 256 rows are 1024 (16 a clock), the softmax threads' whole work some 1900 to 2200 while two
-// groups share the issue slots, and the products 1880. Without the weights' lower halves it took 2100: 131071
-// keys, 64 nodes, 32/8 heads of 128 150 us, 182 with them (164 without their products, 169 without their
-// arithmetic). Their upper halves' products begun ahead of the lower ones took 196. 32 requests x 16384 keys
-// at the same rows: 705 to 750 us; its products at the dense rate, with one half, would take 328. With few rows: the gather (64 x 8192 keys, 5 nodes, 12/4 heads of 64: 122 us, 4.4 TB/s). With little
-// work: the start and end of a unit, some 10000 clocks (16 x 1900 keys 17 us).
+// exponentials of 256 rows are 1024 (16 a clock) and the products 1880 (1370 without the weights' lower
+// halves). Without those a step took 2100: 131071 keys, 64 nodes, 32/8 heads of 128 150 us, 182 with them
+// (164 without their products, 169 without their arithmetic; the upper halves' products begun ahead of the
+// lower ones 196). 32 requests x 16384 keys with the same trees: 705 to 835 us alone, 845 in a row of calls
+// under the power limit; one product of each kind at the dense rate would take 328. With few rows: the
+// gather (64 x 8192 keys, 5 nodes, 12/4 heads of 64: 125 us, 4.3 TB/s). With little work: the start and end
+// of a unit, some 10000 clocks (16 x 1900 keys 17.8 us).
 #include <algorithm>
 
 #include "tree.cuh"
@@ -48,9 +49,9 @@ constexpr int kSoftRegs = 176, kLoadRegs = 96, kMmaRegs = 64;
 static_assert(2 * kSoftRegs + kLoadRegs + kMmaRegs <= 65536 / kThreads * 4, "more registers than the block has");
 constexpr int kAtomBytes = kKeys * 128;  // 128 rows of 64 values, 128-byte swizzled
 // Weights of the cut: a chunk of a unit of up to 128 rows, of a wider one, a unit's start and end, and the least range
-// that is worth a CTA (above kWideCost, so that every range inside a unit has a chunk's start). Fitted: 41 ragged requests
-// of up to 264 rows 105 us with chunks and units of equal weight, 100 with 2, 4, 5, 6, 87 with these; 16 x 1900 keys
-// 20.7, 18.2 and 18.3, and 23 with a least range of 8.
+// that is worth a CTA (above kWideCost, so that every range inside a unit has a chunk's start). Fitted, with one product
+// of the weights: 41 ragged requests of up to 264 rows 105 us with chunks and units of equal weight, 100 with 2, 4, 5,
+// 6, 87 with these; 16 x 1900 keys 20.7, 18.2 and 18.3, and 23 with a least range of 8.
 constexpr int kChunkCost = 2, kWideCost = 4, kUnitCost = 12, kMinShare = 5;
 constexpr int kPieceSlots = 8;
 constexpr int kMaxGrid = 256;            // ranges: the join holds a weight for each of a unit's pieces and 32 rows

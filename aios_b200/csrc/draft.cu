@@ -406,13 +406,14 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) verify_greedy_kernel(const 
 
 // Sampling. A cluster per request walks its tree from the root. The vocabulary is cut into one run of ids per warp
 // of the cluster, in ascending order, and a node's weights r stay in shared memory in fp64 while its children are
-// tried, so that a row is read once. A pass leaves each warp the sum of its run and each CTA the sum of its warps';
+// tried, so that a row is read once. (Without probabilities the proposals are taken out of it and stand beside it: a
+// rejection changes no other weight.) A pass leaves each warp the sum of its run and each CTA the sum of its warps';
 // a token is found by these sums from the outside in. Sums are taken in a fixed order, in fp64: what is accepted or
 // drawn hangs on comparisons of them.
-// Bound by the latency of the visited nodes: some 6600 clocks each for the row's loads, eleven fp64 instructions to an
+// Bound by the latency of the visited nodes: some 7000 clocks each for the row's loads, twelve fp64 instructions to an
 // exponential, and the cluster's exchange; with many requests by the fp64 pipes and the passes over shared memory. A
-// chain of 5 at 16384 ids 13.5 us, 16 trees of 26 at 32001 ids 17, 64 trees of 24 with probabilities at 131072 ids 128
-// (one CTA to an SM 196).
+// chain of 5 at 16384 ids with probabilities 14.1 us, 16 trees of 26 at 32001 ids without 18.4, 64 trees of 24 with
+// them at 131072 ids 136 (with one CTA to an SM it was 196 to 128).
 // A warp's run of a row is a multiple of this; a row comes as fp32 into the first half of its groups' places.
 constexpr int kRunIds = 64;
 
@@ -856,7 +857,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
 
 constexpr int kMaxSamplePlaces = 262144;
 constexpr size_t kWeightBytes = sizeof(double) * kMaxSamplePlaces / kMaxRanks;
-constexpr size_t kSharedBytes = 80 * 1024;  // of two CTAs on an SM, 28 KiB beside it
+constexpr size_t kSharedBytes = 80 * 1024;  // of two CTAs on an SM, 32 KiB beside it
 
 template <typename Kernel>
 cudaError_t launch_cluster(Kernel kernel, const VerifyArgs& a, int requests, size_t smem, bool (&configured)[64],
@@ -898,8 +899,8 @@ cudaError_t launch_verify(VerifyArgs a, int requests, bool greedy, int places, c
   const int sms = sm_count();
   // More CTAs to a request while they find SMs, and a block to each of their warps: two for the argmax, which has
   // little to do with one (1 x 16384 ids 5.7 us with 4 CTAs, 6.2 with 8). Sampling, us: 16 trees of 26, 32001 ids: 4
-  // CTAs 18.4, 8 17.1; 2 of 8, 6400 ids: 1 CTA 15.0, 2 12.0; 8 of 8, 50021 ids: 8 CTAs 13.9, 16 12.8, with
-  // probabilities 37.0 and 30.7.
+  // CTAs 26.2, 8 22.9; 2 of 8, 6400 ids: 1 CTA 15.2, 2 12.5; 8 of 8, 50021 ids: 8 CTAs 14.0, 16 12.9, with
+  // probabilities 19.6 and 18.5.
   const int64_t each = (int64_t)kVerifyWarps * kBlockIds * (greedy ? 2 : 1);
   while (a.ranks < (greedy ? kGreedyRanks : kMaxRanks) && (int64_t)requests * a.ranks * 2 <= sms &&
          a.vocab >= a.ranks * each)
