@@ -175,13 +175,19 @@ __device__ __forceinline__ double widen(float x) {
   return __hiloint2double((int)((((u >> 3) & 0x0FFFFFFFu) + 0x38000000u) | (u & 0x80000000u)), (int)(u << 29));
 }
 
-// A probability in fp64; 0 and what lies below 2^-126 as 0 (the subtrahend of a token that was never proposed, which
-// may have next to no weight itself). nan becomes NaN where a value is infinite or NaN.
+__device__ __forceinline__ double positive(double x) {  // max(x, 0) of a number
+  const int keep = ~(__double2hiint(x) >> 31);
+  return __hiloint2double(__double2hiint(x) & keep, __double2loint(x) & keep);
+}
+// A probability times 2^-896 in fp64: its bits where an fp64 value has them, exact for 0 and subnormals too. nan becomes
+// NaN where a value is infinite or NaN.
 __device__ __forceinline__ double probability(float x, float& nan) {
   nan = fmaf(x, 0.f, nan);
-  const double d = widen(x);
-  return __hiloint2double(fabsf(x) < 0x1p-126f ? 0 : __double2hiint(d), __double2loint(d));
+  const uint32_t u = __float_as_uint(x);
+  return __hiloint2double((int)((u >> 3 & 0x0FFFFFFFu) | (u & 0x80000000u)), (int)(u << 29));
 }
+// max(r - q, 0) for q as above. r comes rounded: a product's rest beside q would be left over where both are the same.
+__device__ __forceinline__ double less(double r, double q) { return positive(fma(q, -0x1p896, r)); }
 
 // 2^(i / 16) for the exponential below: sixteen doubles are all of the banks once, so that no two lanes' entries
 // conflict (a table of 128 cost as much as the arithmetic).
@@ -213,10 +219,6 @@ __device__ __forceinline__ double exp_table(double t, const double* table) {
 template <bool FAR = true>
 __device__ __forceinline__ double exp_table(float x, double scale, double base, const double* table) {
   return exp_table<FAR>(fma(widen(x), scale, -base), table);
-}
-__device__ __forceinline__ double positive(double x) {  // max(x, 0) of a number
-  const int keep = ~(__double2hiint(x) >> 31);
-  return __hiloint2double(__double2hiint(x) & keep, __double2loint(x) & keep);
 }
 
 // Values that the CTAs of a cluster hand to one another; the buffers take turns, so that one barrier an exchange is
@@ -681,7 +683,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
     } else {
       double total = all_weights;
       for (int i = 0; i < children; ++i) {
-        const double rx = child_r[i], qx = probability(child_q[i], nan);
+        const double rx = child_r[i], qx = probability(child_q[i], nan) * 0x1p896;
         const int child = walk.child[i];
         if (isnan(nan)) break;
         if (rx > 0 && (double)node_u[child] * qx * total < rx) {
@@ -702,8 +704,8 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
           for (int j = 0; j < 8; ++j) {
             const double qj = probability(qv[j], nan);
             w[j] *= mult;
-            if (pending != 0) w[j] = positive(fma(w[j], pending, -qj));
-            sum += positive(fma(w[j], inv, -qj));
+            if (pending != 0) w[j] = less(w[j] * pending, qj);
+            sum += less(w[j] * inv, qj);
           }
           store_group(g, w);
           part += sum;
@@ -718,7 +720,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
         if (left > 0) {
           total = left;
           for (int c = threadIdx.x; c < children; c += kVerifyThreads)
-            child_r[c] = positive(fma(child_r[c], inv, -probability(child_q[c], nan)));
+            child_r[c] = less(child_r[c] * inv, probability(child_q[c], nan));
           __syncthreads();
         }
       }
@@ -757,7 +759,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         w[j] *= by;
-        if (PROBS && pending != 0) w[j] = positive(fma(w[j], pending, -probability(qv[j], nan)));
+        if (PROBS && pending != 0) w[j] = less(w[j] * pending, probability(qv[j], nan));
       }
     };
     if (stale) {

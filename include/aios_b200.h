@@ -520,7 +520,7 @@ AIOSB_API int aiosb_attention_tree(const void* q, int64_t q_stride, int64_t toke
  * tree gets 0 and -1. A row with a NaN, with +inf (unless greedy) or with -inf only ends
  * the path with next_token -1 and AIOSB_DEV_NO_DISTRIBUTION, and so does a probability
  * that is infinite or NaN, where one is read (at a tried child's token, and anywhere in
- * the row that a rejection takes off r; below 2^-126 it counts as 0); a draft token outside the
+ * the row that a rejection takes off r); a draft token outside the
  * vocabulary is rejected (AIOSB_DEV_TOKEN_RANGE). */
 AIOSB_API int aiosb_verify_draft(const void* logits, int logits_fp32, int64_t logits_stride, int64_t tokens,
                                  int64_t vocab, const int64_t* draft_tokens, const int32_t* parents,

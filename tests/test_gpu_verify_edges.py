@@ -226,3 +226,33 @@ def test_parents_that_are_no_earlier_node_are_reported(cuda_device, mode: str, n
     assert got == want
     with pytest.raises(RuntimeError, match="tree"):
         ops.check_status(cuda_device)
+
+
+@pytest.mark.parametrize("vocab", [8, 70000])
+def test_the_smallest_probabilities(cuda_device, vocab: int) -> None:
+    """Subnormal ones count as they are: e^-150 less 2^-147 is nothing, e^-95 less 2^-140 is not."""
+    for lower, q1, left in ((150.0, 2.0**-147, False), (95.0, 2.0**-140, True), (101.0, 2.0**-149, True),
+                            (101.0, 2.0**-145, False), (101.0, 0.0, True)):
+        logits = _spread([0.0, -lower], vocab)
+        at = [i for i, x in enumerate(logits) if x > -INF]
+        q = [0.0] * vocab
+        q[at[0]], q[at[1]] = 1.0, q1
+        got, want = _verify(logits, [0, at[0]], [-1, 0], [0.0, 1.5], 0.5, q)
+        assert got == want and got[1] == [at[1] if left else at[0]]
+    ops.check_status(cuda_device)
+
+
+@pytest.mark.parametrize("vocab", [16, 70000])
+def test_what_a_certain_drafting_model_leaves(cuda_device, vocab: int) -> None:
+    """A drafting model that is certain of the token that the target is all but certain of: a rejection (of a masked
+    token) takes all of it, whatever the logit's size, and the rest is left."""
+    for largest in (0.1, 20.3, -47.7, 301.0):
+        for temperature in (1.0, 0.05, 0.3):
+            logits = _spread([largest, largest - 100 * temperature, largest - 100.5 * temperature, -INF], vocab)
+            at = [i * (vocab // 4) + 3 for i in range(4)]
+            q = [0.0] * vocab
+            q[at[0]] = 1.0
+            for sample in (0.3, 0.7):
+                got, want = _verify(logits, [0, at[3]], [-1, 0], [0.0, 0.5], sample, q, temperature=temperature)
+                assert got == want and got[1] == [at[1 if sample < 0.6 else 2]]  # 1 / (1 + e^-0.5) = 0.62
+    ops.check_status(cuda_device)
