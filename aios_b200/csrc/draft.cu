@@ -196,8 +196,8 @@ constexpr int kExpTable = 16;
 // k's upper bits, and 2^(f / 16) by its series to the sixth power (table-driven exponentials: P. T. P. Tang, ACM TOMS
 // 15, 1989), whose rest is 2^-51. Twelve fp64 instructions, where the general function takes some thirty. Off by 2^-50,
 // and by 2^-51 of (x - m) / T for the rounding of what it is taken of.
-// scale: 16 / (T ln 2); base: m * scale (its rounding is a factor of the weights over it). Below m - 600 T, and for x of -inf,
-// it is 0: a masked token adds nothing to any sum, so that a sum is above 0 exactly where one of its tokens is.
+// scale: 16 / (T ln 2); base: m * scale (its rounding is a factor of the weights over it). Below m - 600 T, and for x
+// of -inf, it is 0: a masked token adds nothing to any sum, so that a sum is above 0 exactly where one of its tokens is.
 constexpr uint32_t kFar = 0xC0CB0D00u;  // upper half of -13850
 // 2^(t / 16). FAR false: t is above -13850, or the result is not used.
 template <bool FAR = true>
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) verify_greedy_kernel(const 
 // Bound by the latency of the visited nodes: some 7000 clocks each for the row's loads, twelve fp64 instructions to an
 // exponential, and the cluster's exchange; with many requests by the fp64 pipes and the passes over shared memory. A
 // chain of 5 at 16384 ids with probabilities 14.1 us, 16 trees of 26 at 32001 ids without 18.4, 64 trees of 24 with
-// them at 131072 ids 136 (with one CTA to an SM it was 196 to 128).
+// them at 131072 ids 135 (with one CTA to an SM it was 196 to 128).
 // A warp's run of a row is a multiple of this; a row comes as fp32 into the first half of its groups' places.
 constexpr int kRunIds = 64;
 
@@ -751,14 +751,12 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
     // the first pass's sums and weights are over the ranks' own maxima, later ones are r's (without probabilities
     // there are none: the row's weights have no proposal's)
     const bool direct = stale || pending != 0;
-    const double by = direct ? mult : 1.0;
     auto group_weights = [&](int p, double (&w)[8]) {  // the group at p, as the sums have it
       load_group(group_of(p), w);
       float qv[8];
       if (PROBS && pending != 0) load_probs(q, p - shift, a.vocab, qv);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        w[j] *= by;
         if (PROBS && pending != 0) w[j] = less(w[j] * pending, probability(qv[j], nan));
       }
     };
