@@ -231,8 +231,8 @@ cudaError_t launch_small(const TreeAttnArgs& a, int64_t max_nodes, cudaStream_t 
 // Whether the keys are dealt over the SMs (attn_tree_split.cu): for longer histories, or many rows, which its tensor
 // cores take faster. Measured, whole / dealt, us: 16 requests of 26 nodes, 8/2 heads of 96: 64 keys 10.9 / 13.5, 128
 // 14.6 / 14.9, 256 20.8 / 16.9, 1024 60 / 19.5; 1 of 5 nodes, 32/8 heads of 128: 64 11.7 / 11.5, 128 16.7 / 15.1. 64
-// requests, 32 keys, 8/2 heads of 96: 15872 rows 11.1 / 15.3, 20480 16.1 / 18.7, 30720 27.6 / 19.3; 12/4 of 64: 19968
-// 15.6 / 18.9, 23808 15.7 / 19.1, 30720 22.5 / 21.0; 32/8 of 128: 53248 41.6 / 37.5, 122880 126 / 50.
+// requests, 32 keys, thousands of rows, 8/2 heads of 96: 15.9 11.1 / 15.3, 20.5 16.1 / 18.7, 30.7 27.6 / 19.3; 12/4 of
+// 64: 20.0 15.6 / 18.9, 23.8 15.7 / 19.1, 30.7 22.5 / 21.0; 32/8 of 128: 53 41.6 / 37.5, 123 126 / 50.
 bool splits(int64_t max_cached, int64_t tokens, int64_t heads) { return max_cached > 128 || tokens * heads > 24000; }
 
 }  // namespace
